@@ -31,6 +31,9 @@ GS_MAX_SLICES = 8
 GS_MAX_RANK = 512
 GS_RANK_CLASS_SPLIT = 64
 GS_NOALLOC_SCRATCH_BYTES = 64 << 20
+GS_GATE_NONE = 0
+GS_GATE_SIGMOID = 1
+GS_GATE_TANH = 2
 
 # name -> (restype, argtypes); mirrors include/granite_switch_amd.h
 SIGNATURES = {
@@ -91,6 +94,25 @@ SIGNATURES = {
                                              c_i32, c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_i32,
                                              c_i32, c_i32, c_void_p]),
     "gs_gemm_bf16_tn": (c_i32, [c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64, c_void_p]),
+    "gs_append_kv": (c_i32, [c_i32] + [c_void_p, c_i64, c_i64] * 3 + [c_i64, c_i32, c_i32, c_i32, c_void_p, c_void_p,
+                             c_i64, c_i32, c_i32, c_void_p] + [c_void_p, c_i64, c_i64, c_i64] * 2
+                     + [c_i64, c_i32, c_void_p, c_i64, c_i64, c_void_p]),
+    "gs_cache_slots": (c_i32, [c_void_p, c_i64, c_i32, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_void_p,
+                               c_void_p, c_void_p]),
+    "gs_paged_attention_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "gs_paged_attention": (c_i32, [c_i32, c_void_p, c_i64, c_i64] + [c_void_p, c_i64, c_i64, c_i64] * 2
+                           + [c_i64, c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_i32, c_i32,
+                              c_i32, c_i32, ctypes.c_float, c_i32, c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64,
+                              c_void_p]),
+    "gs_check_paged_addresses": (c_i64, [c_i32] + [c_i64] * 9 + [c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p,
+                                         c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32,
+                                         ctypes.c_char_p, c_i64, c_void_p]),
+    "gs_check_append_addresses": (c_i64, [c_i32, c_i32] + [c_i64] * 5 + [c_i32, c_i32, c_i32, c_void_p, c_i64, c_i32,
+                                          c_i32, c_void_p] + [c_i64] * 4 + [c_i32, c_i32, ctypes.c_char_p, c_i64,
+                                          c_void_p]),
+    "gs_residual_norm": (c_i32, [c_i32, c_void_p, c_i64, c_void_p, c_i64, c_i32, c_void_p, c_i64, c_i64, c_i32,
+                                 c_void_p, c_void_p, c_i32, ctypes.c_float, ctypes.c_float, c_i64, c_i32, c_void_p,
+                                 c_i64, c_void_p, c_i64, c_void_p]),
     "gs_gemm_form": (c_i32, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i32, c_void_p]),
 }
 

@@ -246,5 +246,99 @@ GS_HD int64_t small_part(int64_t region, int g, int ks, int cap, int slot, int z
   return static_cast<int64_t>(g - 1) * region + (static_cast<int64_t>(ks) * cap + slot) * zw + col;
 }
 
+// ---- paged cache: append and attention (gs_paged.hip) -----------------------
+// n / d and n % d for d >= 1 with magic = floor((2^32 - 1) / d): the product's
+// high word is at most one short of the quotient.
+GS_HD uint32_t div_magic(uint32_t d) { return 0xffffffffu / d; }
+GS_HD void div_by(uint32_t n, uint32_t d, uint32_t magic, uint32_t& quot, uint32_t& rem) {
+  uint32_t q = static_cast<uint32_t>((static_cast<uint64_t>(n) * magic) >> 32);
+  uint32_t r = n - q * d;
+  while (r >= d) {                       // at most twice
+    r -= d;
+    ++q;
+  }
+  quot = q;
+  rem = r;
+}
+// Append: the columns [c0, + VE) and [c1, + VE) (c1 < 0: none) of unit u of a
+// head; rot: they are partners of a rotation by pairs append_pair(u) on.
+struct AppendCols {
+  int c0, c1;
+  bool rot;
+};
+GS_HD int append_units(int VE, int D, int R) { return R / (2 * VE) + (D - R + 2 * VE - 1) / (2 * VE); }
+GS_HD AppendCols append_cols(int u, int VE, int D, int R, bool pairs) {
+  const int nrot = R / (2 * VE);
+  AppendCols c;
+  c.rot = u < nrot;
+  if (c.rot) {
+    c.c0 = pairs ? 2 * VE * u : VE * u;
+    c.c1 = pairs ? c.c0 + VE : R / 2 + VE * u;
+  } else {
+    c.c0 = R + 2 * VE * (u - nrot);
+    c.c1 = c.c0 + VE < D ? c.c0 + VE : -1;
+  }
+  return c;
+}
+GS_HD int append_pair(int u, int VE) { return VE * u; }
+// The table row of a position (those outside the table: its first or last).
+GS_HD int64_t append_pos(int64_t pos, int64_t max_pos) { return pos < 0 ? 0 : lmin(pos, max_pos - 1); }
+GS_HD bool append_stored(int64_t slot, int64_t num_slots) { return slot >= 0 && slot < num_slots; }
+// A sequence of a batch: its first query row and number of query rows within
+// the T rows given, and its cached tokens within what its table row addresses.
+struct PagedSeq {
+  int q0, n, len;
+};
+GS_HD PagedSeq paged_seq(int lo, int hi, int len, int T, int64_t max_len) {
+  PagedSeq s;
+  s.q0 = lo < 0 ? 0 : imin(lo, T);
+  const int e = imin(hi, T);
+  s.n = e > s.q0 ? e - s.q0 : 0;
+  s.len = len < 0 ? 0 : static_cast<int>(lmin(len, max_len));
+  return s;
+}
+// Tile j of 16 (query, head) rows of a sequence, row r = query * G + head: the
+// queries i0 .. i1 it holds and the tokens [vs, ve) that some row of it sees
+// (none: ve = vs); first = vs rounded down to a multiple of 8.
+struct PagedTile {
+  int i0, i1, vs, ve, first;
+};
+GS_HD PagedTile paged_tile(const PagedSeq& s, int G, int window, int j) {
+  PagedTile t;
+  const int64_t rows = static_cast<int64_t>(s.n) * G;
+  const int64_t r0 = static_cast<int64_t>(j) * 16;
+  t.i0 = static_cast<int>(r0 / G);
+  t.i1 = static_cast<int>(lmin(r0 + 15, rows - 1) / G);
+  const int p0 = s.len - s.n + t.i0, p1 = s.len - s.n + t.i1;   // positions: may be negative
+  t.ve = p1 + 1 > 0 ? p1 + 1 : 0;
+  t.vs = window > 0 && p0 - window + 1 > 0 ? p0 - window + 1 : 0;
+  if (t.vs > t.ve) t.vs = t.ve;
+  t.first = t.vs & ~7;
+  return t;
+}
+GS_HD int64_t paged_tiles(const PagedSeq& s, int G) { return (static_cast<int64_t>(s.n) * G + 15) / 16; }
+// Units of `unit` tokens that cover what any tile of the sequence sees (one at least).
+GS_HD int paged_tile_units(const PagedSeq& s, int G, int window, int unit) {
+  int64_t span = s.len;
+  if (window > 0) span = lmin(span, static_cast<int64_t>(window) + 16 / G + 1 + 7);
+  return span <= unit ? 1 : static_cast<int>((span + unit - 1) / unit);
+}
+GS_HD int64_t paged_seq_units(const PagedSeq& s, int G, int window, int unit) {
+  return s.n == 0 ? 0 : paged_tiles(s, G) * paged_tile_units(s, G, window, unit);
+}
+// First unit of part p of P; the part that holds unit u of U.
+GS_HD int64_t paged_part_lo(int64_t U, int P, int p) { return U * p / P; }
+GS_HD int paged_part_of(int64_t U, int P, int64_t u) { return static_cast<int>(((u + 1) * P - 1) / U); }
+// The first token of the 8 that a lane reads from tok on (a multiple of 8):
+// 8 tokens are always of one page; past the last seen ones re-read those.
+GS_HD int paged_octet(int tok, int ve) { return imin(tok, (ve - 1) & ~7); }
+GS_HD int paged_page(int id, int num_pages) {
+  return static_cast<uint32_t>(id) < static_cast<uint32_t>(num_pages) ? id : 0;
+}
+// Parts that have work: one unit at least each.
+GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin(U, parts)); }
+// Floats of one partial result: 16 rows of DT sums, their maxima and totals.
+GS_HD int64_t paged_partial_floats(int DT) { return 16 * DT + 32; }
+
 }  // namespace addr
 }  // namespace gs

@@ -1,0 +1,318 @@
+"""Paged key/value cache: rotated append, and attention over it.
+
+The steps of a decoder layer between the switched QKV projection and the
+switched output projection:
+
+    slots, positions = cache_slots(page_table, kv_lens, page_size, num_pages, cu_seqlens)   # once per step
+    q = append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin)                    # per layer
+    o = paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens)
+
+A cache is [num_pages, kv_heads, page_size, head_dim] with any order of its first
+three dimensions in memory (``allocate_cache`` keeps a head's rows of a page
+side by side).  Sequence s has its token j in row j % page_size of page
+page_table[s, j // page_size]; kv_lens[s] counts its tokens, those of the call
+among them.  An aLoRA adapter that switches on mid-sequence attends over the
+base model's cached prefix this way: its few invocation tokens are a chunk of
+queries (``cu_seqlens``) over a long cache.
+
+Everything is launched on torch's current stream without host synchronisation;
+bfloat16 or float32; no gradients are computed.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_FP32}
+
+
+def allocate_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+                   device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """A key and a value cache [num_pages, kv_heads, page_size, head_dim].
+
+    A head's rows of a page lie side by side, so a page of 16 rows of 128 bf16
+    values is one run of 4 KB.  The contents are not initialised: rows are read
+    only once they were stored.
+    """
+    shape = (num_pages, kv_heads, page_size, head_dim)
+    return torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+
+
+def rope_table(max_pos: int, rot_dim: int, theta: float = 10000.0, device="cuda",
+               inv_freq: torch.Tensor | None = None, scaling: float = 1.0) -> torch.Tensor:
+    """The rotation table [max_pos, rot_dim] fp32: per position rot_dim/2 cosines, then rot_dim/2 sines.
+
+    Angles are position * theta^(-2j / rot_dim) (or * ``inv_freq`` [rot_dim/2]),
+    computed in 64 bits: a 32-bit product at position 10^6 is off by 0.06.
+    ``scaling`` multiplies cosines and sines (an attention factor).
+    """
+    if rot_dim % 2 or rot_dim <= 0:
+        raise ValueError(f"rope_table: rot_dim={rot_dim} must be even and positive")
+    if inv_freq is None:
+        inv_freq = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    elif inv_freq.numel() != rot_dim // 2:
+        raise ValueError(f"rope_table: inv_freq has {inv_freq.numel()} entries, rot_dim={rot_dim} needs {rot_dim // 2}")
+    angle = torch.arange(max_pos, dtype=torch.float64, device=device)[:, None] * inv_freq.to(device, torch.float64)[None, :]
+    return (torch.cat([angle.cos(), angle.sin()], dim=1) * scaling).float()
+
+
+# ---------------------------------------------------------------------------
+# Checks
+# ---------------------------------------------------------------------------
+def _heads3(who: str, name: str, t: torch.Tensor, tokens: int | None, dtype) -> torch.Tensor:
+    if t.dim() != 3 or t.dtype != dtype or (tokens is not None and t.shape[0] != tokens):
+        raise ValueError(f"{who}: {name} must be a {dtype} tensor [{'tokens' if tokens is None else tokens}, heads, "
+                         f"head_dim], got {t.dtype} {tuple(t.shape)}")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        raise ValueError(f"{who}: {name}'s head dimension must be contiguous (strides {t.stride()})")
+    return t
+
+
+def _caches(who: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_heads, head_dim: int):
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c.dim() != 4 or c.dtype != dtype or c.shape != k_cache.shape or c.shape[3] != head_dim or \
+                (kv_heads is not None and c.shape[1] != kv_heads):
+            raise ValueError(f"{who}: {name} must be a {dtype} tensor [pages, kv_heads, page_size, {head_dim}], "
+                             f"both caches alike, got {c.dtype} {tuple(c.shape)}")
+        if c.stride(3) != 1 and head_dim > 1:
+            raise ValueError(f"{who}: {name}'s head dimension must be contiguous (strides {c.stride()})")
+    if k_cache.shape[0] == 0 or k_cache.shape[2] == 0:
+        raise ValueError(f"{who}: the caches hold no rows ({tuple(k_cache.shape)})")
+
+
+def _on_gpu(who: str, device: torch.device, *ts) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"{who}: tensors must live on the GPU")
+    for t in ts:
+        if t is not None and t.device != device:
+            raise ValueError(f"{who}: tensors must live on one GPU ({t.device} beside {device})")
+
+
+def _ints(who: str, name: str, t: torch.Tensor, dtype, shape=None) -> torch.Tensor:
+    if t.dtype != dtype or (shape is not None and tuple(t.shape) != tuple(shape)) or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be a contiguous {dtype} tensor"
+                         f"{'' if shape is None else ' ' + str(tuple(shape))}, got {t.dtype} {tuple(t.shape)}")
+    return t
+
+
+def _table(who: str, page_table: torch.Tensor, seqs: int) -> torch.Tensor:
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[0] != seqs or \
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{who}: page_table must be an int32 tensor [{seqs}, max_pages] with contiguous rows, got "
+                         f"{page_table.dtype} {tuple(page_table.shape)}")
+    return page_table
+
+
+def _table_ld(page_table: torch.Tensor) -> int:
+    return page_table.stride(0) if page_table.shape[0] > 1 else max(page_table.stride(0), page_table.shape[1])
+
+
+# ---------------------------------------------------------------------------
+# Append
+# ---------------------------------------------------------------------------
+def cache_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, num_pages: int,
+                cu_seqlens: torch.Tensor | None = None,
+                num_tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(slots, positions)`` int64 [num_tokens] of a batch's tokens, once per step for every layer.
+
+    Row i of sequence s's n rows is its token p = kv_lens[s] - n + i: the slot is
+    page_table[s, p // page_size] * page_size + p % page_size, -1 where there is
+    none (p < 0: a padding row).  ``cu_seqlens`` None: one row per sequence;
+    otherwise ``num_tokens`` is the packed batch's row count.
+    """
+    who = "cache_slots"
+    B = kv_lens.shape[0]
+    _on_gpu(who, kv_lens.device, page_table, cu_seqlens)
+    _ints(who, "kv_lens", kv_lens, torch.int32, (B,))
+    _table(who, page_table, B)
+    if cu_seqlens is not None:
+        _ints(who, "cu_seqlens", cu_seqlens, torch.int32, (B + 1,))
+        if num_tokens is None:
+            raise ValueError("cache_slots: cu_seqlens needs num_tokens (reading it would synchronise)")
+    elif num_tokens is None:
+        num_tokens = B
+    elif num_tokens != B:
+        raise ValueError(f"cache_slots: num_tokens={num_tokens} of {B} sequences without cu_seqlens")
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device)
+    positions = torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device)
+    _lib.call("gs_cache_slots", page_table.data_ptr(), _table_ld(page_table), page_table.shape[1], int(num_pages),
+              int(page_size), kv_lens.data_ptr(), _lib.ptr(cu_seqlens), B, int(num_tokens), slots.data_ptr(),
+              positions.data_ptr(), _lib.stream_ptr(kv_lens.device))
+    return slots, positions
+
+
+def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+               slots: torch.Tensor, positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+    """Rotate q and k by their positions, store k and v into the cache; returns the rotated q.
+
+    q [T, heads, D], k and v [T, kv_heads, D]: views with contiguous head rows,
+    such as slices of the QKV projection's output
+    slots     [T] int64: page * page_size + row; one outside the pool (-1) stores
+              nothing (padding rows).  No two tokens may share a slot.
+    positions [T] int64 and cos_sin [max_pos, R] fp32 (``rope_table``): the first R
+              columns of a head are rotated as pairs (j, j + R/2), or (2j, 2j + 1)
+              with ``interleaved``, the others copied.  cos_sin None: no rotation.
+    q_out     receives q (allocated when None; q itself: in place).  q None: only
+              k and v are handled, and None is returned.
+    """
+    who = "append_kv_"
+    dtype = k.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"{who}: unsupported dtype {dtype}; expected bfloat16 or float32")
+    if k.dim() != 3:
+        raise ValueError(f"{who}: k must be [tokens, kv_heads, head_dim], got {tuple(k.shape)}")
+    T, HK, D = k.shape
+    _on_gpu(who, k.device, q, v, k_cache, v_cache, slots, positions, cos_sin, q_out)
+    _heads3(who, "k", k, T, dtype)
+    _heads3(who, "v", v, T, dtype)
+    if v.shape != k.shape:
+        raise ValueError(f"{who}: v is {tuple(v.shape)}, k {tuple(k.shape)}")
+    _caches(who, k_cache, v_cache, dtype, HK, D)
+    _ints(who, "slots", slots, torch.int64, (T,))
+    R = 0
+    if cos_sin is not None:
+        if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.shape[0] == 0:
+            raise ValueError(f"{who}: cos_sin must be a contiguous float32 tensor [max_pos, rot_dim], got "
+                             f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
+        R = cos_sin.shape[1]
+        if R % 2 or R > D:
+            raise ValueError(f"{who}: cos_sin rotates {R} columns of {D}")
+        if positions is None:
+            raise ValueError(f"{who}: cos_sin needs positions")
+        _ints(who, "positions", positions, torch.int64, (T,))
+    H = 0
+    if q is not None:
+        _heads3(who, "q", q, T, dtype)
+        H = q.shape[1]
+        if q.shape[2] != D:
+            raise ValueError(f"{who}: q has heads of {q.shape[2]}, k of {D}")
+        if q_out is None:
+            q_out = torch.empty(T, H, D, dtype=dtype, device=k.device)
+        else:
+            _heads3(who, "q_out", q_out, T, dtype)
+            if q_out.shape != q.shape:
+                raise ValueError(f"{who}: q_out is {tuple(q_out.shape)}, q {tuple(q.shape)}")
+    elif q_out is not None:
+        raise ValueError(f"{who}: q_out without q")
+    if T == 0:
+        return q_out
+    qs = (None, 0, 0) if q is None else (q.data_ptr(), q.stride(0), q.stride(1))
+    qo = (None, 0, 0) if q is None else (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+    _lib.call("gs_append_kv", _DTYPES[dtype], *qs, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+              v.stride(1), T, H, HK, D, _lib.ptr(positions if R else None), _lib.ptr(cos_sin if R else None),
+              cos_sin.shape[0] if R else 0, R, int(bool(interleaved)), slots.data_ptr(), k_cache.data_ptr(),
+              k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(), v_cache.stride(0),
+              v_cache.stride(1), v_cache.stride(2), k_cache.shape[0], k_cache.shape[2], *qo, _lib.stream_ptr(k.device))
+    return q_out
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+# One workspace for each stream: calls on one stream follow each other, calls on
+# different streams may overlap.  A replaced buffer is kept (``_retired``): a
+# captured graph may still hold its address.
+_workspaces: dict = {}
+_retired: list = []
+
+
+def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
+    key = (device.index, stream)
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < need:
+        if torch.cuda.is_current_stream_capturing():
+            # a buffer of the graph's own: it lives as long as the graph's pool does
+            return torch.empty(need, dtype=torch.uint8, device=device)
+        if buf is not None:
+            _retired.append(buf)
+        buf = _workspaces[key] = torch.empty(need, dtype=torch.uint8, device=device)
+    return buf
+
+
+_need: dict = {}
+
+
+def workspace_bytes(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Workspace of one ``paged_attention`` call (for ``workspace=``); does not depend on the batch."""
+    key = (dtype, heads, kv_heads, head_dim, torch.cuda.current_device())
+    n = _need.get(key)
+    if n is None:
+        n = int(_lib.load().gs_paged_attention_workspace_bytes(_DTYPES[dtype], heads, kv_heads, head_dim))
+        if n < 0:
+            raise _lib.GraniteSwitchError("gs_paged_attention_workspace_bytes", -n, _lib.last_error())
+        _need[key] = n
+    return n
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    kv_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None, scale: float | None = None,
+                    window: int = 0, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                    max_q: int | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the batch's query rows over the paged cache; returns ``out`` [T, heads, D].
+
+    q          [T, heads, D]; heads a multiple of the cache's kv_heads
+    page_table [B, max_pages] int32, kv_lens [B] int32: the sequences' pages and
+               lengths, the call's own tokens (already appended) counted
+    cu_seqlens [B + 1] int32: sequence s has query rows cu_seqlens[s] ..
+               cu_seqlens[s + 1], its last tokens; None: one row per sequence
+    scale      of the scores (1 / sqrt(D) when None)
+    window     > 0: a row sees the last ``window`` tokens up to its own
+    lse        [T, heads] float32: receives the log of each softmax's total
+    max_q      the most query rows of a sequence where the caller knows it
+    workspace  uint8, ``workspace_bytes`` long (one per stream is kept when None)
+
+    A row that sees nothing (an empty sequence) gives zeros.
+    """
+    who = "paged_attention"
+    dtype = q.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"{who}: unsupported dtype {dtype}; expected bfloat16 or float32")
+    _heads3(who, "q", q, None, dtype)
+    T, H, D = q.shape
+    dev = q.device
+    _on_gpu(who, dev, k_cache, v_cache, page_table, kv_lens, cu_seqlens, out, lse, workspace)
+    _caches(who, k_cache, v_cache, dtype, None, D)
+    HK = k_cache.shape[1]
+    B = kv_lens.shape[0]
+    if HK == 0 or H % HK or H == 0:
+        raise ValueError(f"{who}: {H} query heads over {HK} key/value heads")
+    _ints(who, "kv_lens", kv_lens, torch.int32, (B,))
+    _table(who, page_table, B)
+    if cu_seqlens is not None:
+        _ints(who, "cu_seqlens", cu_seqlens, torch.int32, (B + 1,))
+    elif T != B:
+        raise ValueError(f"{who}: {T} query rows of {B} sequences without cu_seqlens")
+    if window < 0 or (max_q is not None and max_q < 0):
+        raise ValueError(f"{who}: window={window} max_q={max_q}")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=dtype, device=dev)
+    else:
+        _heads3(who, "out", out, T, dtype)
+        if out.shape != q.shape:
+            raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    if lse is not None:
+        _ints(who, "lse", lse, torch.float32, (T, H))
+    if T == 0 or B == 0:
+        return out
+    stream = _lib.stream_ptr(dev)
+    need = workspace_bytes(dtype, H, HK, D)
+    if workspace is None:
+        workspace = _workspace(dev, stream, need)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"{who}: workspace must be a contiguous uint8 tensor")
+    _lib.call("gs_paged_attention", _DTYPES[dtype], q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
+              k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(), v_cache.stride(0),
+              v_cache.stride(1), v_cache.stride(2), k_cache.shape[0], k_cache.shape[2], page_table.data_ptr(),
+              _table_ld(page_table), page_table.shape[1], kv_lens.data_ptr(), _lib.ptr(cu_seqlens), B, T,
+              1 if cu_seqlens is None else int(max_q or 0), H, HK, D, 1.0 / math.sqrt(D) if scale is None else scale,
+              int(window), out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(lse), workspace.data_ptr(),
+              workspace.numel(), stream)
+    return out
+
+
+__all__ = ["allocate_cache", "append_kv_", "cache_slots", "paged_attention", "rope_table", "workspace_bytes"]

@@ -512,6 +512,123 @@ int gs_gemm_form(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int3
 int64_t gs_check_gemm_addresses(int64_t M, int64_t N, int64_t K, int64_t lda, int64_t ldb, int64_t ldc, char* msg,
                                 int64_t msg_len, int64_t* checked);
 
+/* ------------------------------------------------------------------------
+ * Paged key/value cache.  No counterpart in the reference, whose serving
+ * engine brings its own cache and attention; these are the layer's steps
+ * between the switched QKV and output projections.
+ *
+ * A cache is [num_pages, kv_heads, page_size, head_dim] in any order of its
+ * first three dimensions (page, head and row strides in elements, the head
+ * dimension contiguous).  Sequence s keeps its token j in row j % page_size of
+ * page page_table[s * ld_table + j / page_size]; a slot is page * page_size +
+ * row.  kv_lens[s] counts the tokens in the cache, the call's own among them.
+ * cu_seqlens [num_seqs + 1] bounds the sequences' rows in the packed batch;
+ * NULL: one row per sequence.
+ * ---------------------------------------------------------------------- */
+
+/* Rotates q and k by their positions and stores k and v into their slots.
+ * Per head, with R = rot_dim, c and s the pair's cosine and sine from row
+ * positions[t] of cos_sin [max_pos, R] (R/2 cosines, then R/2 sines; fp32):
+ *   (a, b) -> (a c - b s, b c + a s)
+ * for the pairs (j, j + R/2), or (2j, 2j + 1) with interleaved != 0; columns
+ * from R on are copied (R = 0: no rotation, positions and cos_sin NULL).
+ * Computed in fp32, rounded once.  q [num_tokens, heads, head_dim], k and v
+ * [num_tokens, kv_heads, head_dim] with token and head strides; q_out may be q.
+ * heads = 0: q and q_out are not used.  A slot outside [0, num_pages *
+ * page_size) stores nothing (padding rows: -1); two tokens of a call must not
+ * have the same slot.  Positions outside the table take its first or last row.
+ * Any head_dim up to 512 and any alignment; 16-byte accesses where pointers,
+ * strides and rot_dim allow them. */
+int gs_append_kv(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                 int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                 int64_t v_head_stride, int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                 const int64_t* positions, const float* cos_sin, int64_t max_pos, int32_t rot_dim,
+                 int32_t interleaved, const int64_t* slots, void* k_cache, int64_t kc_page_stride,
+                 int64_t kc_head_stride, int64_t kc_row_stride, void* v_cache, int64_t vc_page_stride,
+                 int64_t vc_head_stride, int64_t vc_row_stride, int64_t num_pages, int32_t page_size, void* q_out,
+                 int64_t qo_token_stride, int64_t qo_head_stride, void* stream);
+
+/* The slot and the position of each of a batch's tokens (once per step, for
+ * every layer): token t, row i of sequence s with n rows, is the sequence's
+ * token p = kv_lens[s] - n + i.  slots[t] = -1 where p < 0, past the page
+ * table, on a page id outside the pool, or t in no sequence; positions[t] =
+ * max(p, 0). */
+int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_pages, int64_t num_pages,
+                   int32_t page_size, const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                   int64_t num_tokens, int64_t* slots, int64_t* positions, void* stream);
+
+/* Attention of the batch's rows over the paged cache:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h / G]) v[j, h / G]
+ * with G = heads / kv_heads, over the tokens j <= p of the row's sequence (p =
+ * kv_lens[s] - n + i as above), and j > p - window where window > 0.  A row
+ * that sees nothing (an empty sequence, p < 0) gets zeros.  lse [num_tokens,
+ * heads] fp32 or NULL: the natural logarithm of the softmax's total, -inf for
+ * such a row.  Cache rows that no row of a call sees may hold anything (NaN
+ * too).  Rows of tokens that are in no sequence are not written.
+ * Limits: head_dim a multiple of 8 (fp32: 4) up to 256, page_size a multiple
+ * of 8; q, caches and out 16-byte aligned, strides multiples of 16 bytes.
+ * kv_lens past the page table's reach are cut to it; page ids outside the
+ * pool are read as page 0.  max_q: the most rows of a sequence where the caller
+ * knows it (0: unknown); a smaller value than the batch has is an error of the
+ * caller's that leaves those rows unwritten.
+ * workspace: gs_paged_attention_workspace_bytes, 16-byte aligned, no
+ * initialisation; calls that may overlap in time must not share one. */
+int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim);
+int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* k_cache, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                       const void* v_cache, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
+                       int64_t num_pages, int32_t page_size, const int32_t* page_table, int64_t ld_table,
+                       int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                       int64_t num_tokens, int32_t max_q, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                       float scale, int32_t window, void* out, int64_t o_token_stride, int64_t o_head_stride,
+                       float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Test support (no counterpart in the reference; makes no HIP call).  The
+ * accesses of gs_paged_attention (every part, wave, lane and block, with `cus`
+ * compute units), or of gs_append_kv, replayed on the host for host copies of
+ * the tables; k and v strides and cache strides shared where one set is given.
+ * Also that every output row is written once and every partial result joined
+ * once, and that every column is taken once.  Returns the number of violations
+ * (0: clean), the first described in msg, *checked the number of accesses
+ * checked; a negated GS_* status on bad arguments. */
+int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t k_page_stride,
+                                 int64_t k_head_stride, int64_t k_row_stride, int64_t v_page_stride,
+                                 int64_t v_head_stride, int64_t v_row_stride, int64_t num_pages, int32_t page_size,
+                                 const int32_t* page_table, int64_t ld_table, int32_t max_pages,
+                                 const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                                 int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                 int32_t window, int64_t o_token_stride, int64_t o_head_stride, int32_t cus, char* msg,
+                                 int64_t msg_len, int64_t* checked);
+int64_t gs_check_append_addresses(int32_t dtype, int32_t vec, int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t k_token_stride, int64_t k_head_stride, int64_t num_tokens, int32_t heads,
+                                  int32_t kv_heads, int32_t head_dim, const int64_t* positions, int64_t max_pos,
+                                  int32_t rot_dim, int32_t interleaved, const int64_t* slots, int64_t cache_page_stride,
+                                  int64_t cache_head_stride, int64_t cache_row_stride, int64_t num_pages,
+                                  int32_t page_size, int32_t cus, char* msg, int64_t msg_len, int64_t* checked);
+
+/* ------------------------------------------------------------------------
+ * The residual add between two blocks with the norms around it, one pass:
+ *   b  = x, times rsqrt(mean(x^2) + eps) * post_weight if that is given,
+ *        times act(gate) if that is given
+ *   r' = residual + scale * b                      -> residual_out
+ *   y  = r' * rsqrt(mean(r'^2) + eps) * weight     -> y
+ * x, gate and y in dtype; residual and residual_out in residual_dtype, weight
+ * and post_weight [hidden] in weight_dtype (each dtype or fp32).  y comes from
+ * the unrounded r'.  gate: row stride 0 (one row for all) or gate_col_stride 0
+ * (one value per row) broadcast.  x NULL: y is the norm of the residual alone,
+ * residual_out is not used.  residual_out may be residual and y may be x;
+ * outputs overlap nothing else.  Any hidden size, stride and alignment;
+ * 16-byte accesses where they allow them.
+ * ---------------------------------------------------------------------- */
+#define GS_GATE_NONE 0
+#define GS_GATE_SIGMOID 1
+#define GS_GATE_TANH 2
+int gs_residual_norm(int32_t dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                     int32_t residual_dtype, const void* gate, int64_t gate_row_stride, int64_t gate_col_stride,
+                     int32_t gate_act, const void* post_weight, const void* weight, int32_t weight_dtype, float eps,
+                     float scale, int64_t rows, int32_t hidden, void* residual_out, int64_t ldro, void* y, int64_t ldy,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,7 +99,7 @@ SIGNATURES = {
                      + [c_i64, c_i32, c_void_p, c_i64, c_i64, c_void_p]),
     "gs_cache_slots": (c_i32, [c_void_p, c_i64, c_i32, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_void_p,
                                c_void_p, c_void_p]),
-    "gs_paged_attention_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "gs_paged_attention_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32, c_i32]),
     "gs_paged_attention": (c_i32, [c_i32, c_void_p, c_i64, c_i64] + [c_void_p, c_i64, c_i64, c_i64] * 2
                            + [c_i64, c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_i32, c_i32,
                               c_i32, c_i32, ctypes.c_float, c_i32, c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64,

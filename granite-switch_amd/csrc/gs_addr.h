@@ -337,6 +337,51 @@ GS_HD int paged_page(int id, int num_pages) {
 }
 // Parts that have work: one unit at least each.
 GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin(U, parts)); }
+
+// Chunk form: tiles of `tq` whole queries (tq * G rows), key tiles of 64.
+// Queries of a tile, with R rows in a tile.
+GS_HD int chunk_tq(int R, int G) { return R / G; }
+GS_HD int chunk_tiles(const PagedSeq& s, int tq) { return (s.n + tq - 1) / tq; }
+GS_HD PagedTile chunk_tile(const PagedSeq& s, int tq, int window, int j) {
+  PagedTile t;
+  t.i0 = j * tq;
+  t.i1 = imin(t.i0 + tq, s.n) - 1;
+  const int p0 = s.len - s.n + t.i0, p1 = s.len - s.n + t.i1;
+  t.ve = p1 + 1 > 0 ? p1 + 1 : 0;
+  t.vs = window > 0 && p0 - window + 1 > 0 ? p0 - window + 1 : 0;
+  if (t.vs > t.ve) t.vs = t.ve;
+  t.first = t.vs & ~7;
+  return t;
+}
+GS_HD int chunk_key_tiles(const PagedTile& t) { return (t.ve - t.first + 63) / 64; }
+// The work of a sequence's tiles, taken as the mean of its first and its last
+// one's key tiles (half a tile at least), doubled: an integer.
+GS_HD int64_t chunk_work2(const PagedSeq& s, int tq, int window) {
+  const int nt = chunk_tiles(s, tq);
+  if (nt == 0) return 0;
+  return static_cast<int64_t>(nt) * (chunk_key_tiles(chunk_tile(s, tq, window, 0)) + chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) + 1);
+}
+// Key tiles of a part for a batch of doubled work U2 a head: 3/4 of an equal
+// share of `slots` workgroups, and some at least.
+GS_HD int chunk_part_tiles(int64_t U2, int HK, int slots, int least) {
+  const int64_t c = (U2 * HK * 3 + 8 * slots - 1) / (8 * static_cast<int64_t>(slots));
+  return c < least ? least : static_cast<int>(c);
+}
+// Parts of each of a sequence's tiles: those whose last tile has two parts' key tiles or more are split.
+GS_HD int chunk_parts(const PagedSeq& s, int tq, int window, int part_tiles) {
+  const int nt = chunk_tiles(s, tq);
+  if (nt == 0) return 0;
+  const int p = chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) / part_tiles;
+  return p < 1 ? 1 : p;
+}
+// Partial results a head can have: 2 U2 / 2 / part_tiles of them at most.
+GS_HD int64_t chunk_slots_per_head(int HK, int slots) { return (8 * static_cast<int64_t>(slots) + 3 * HK - 1) / (3 * static_cast<int64_t>(HK)) + 1; }
+GS_HD int64_t chunk_partial_floats(int R, int DT) { return static_cast<int64_t>(R) * (DT + 2); }
+// Where the 16-byte piece p of key row r is kept in LDS (rows of DT * 2 bytes).
+// K is read 16 rows at a time at one piece, V 4 rows at a time over 64 bytes;
+// either way a read's pieces fall on different banks.
+GS_HD int chunk_k_pos(int DT, int r, int p) { return DT == 128 ? p ^ (r & 15) : p ^ ((r >> 1) & 7); }
+GS_HD int chunk_v_pos(int DT, int r, int p) { return DT == 128 ? p ^ ((r & 3) << 2) : p ^ ((r & 2) << 1); }
 // Floats of one partial result: 16 rows of DT sums, their maxima and totals.
 GS_HD int64_t paged_partial_floats(int DT) { return 16 * DT + 32; }
 

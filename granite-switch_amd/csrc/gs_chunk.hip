@@ -1,0 +1,436 @@
+// Attention of query chunks over a paged cache (bf16, head widths up to 128):
+// the form of gs_paged_attention for sequences of many rows.
+//
+// A workgroup of 8 waves takes 256 (query, head) rows of one sequence and
+// key/value head -- 64 queries where 4 query heads share it, so the group's
+// heads read K and V once -- and walks the keys in tiles of 64.  Keys and values
+// go from the pages straight into LDS (three stages: a tile is two tiles' work
+// on its way), 16 bytes a lane, permuted so that every operand read falls on
+// different banks.
+//
+// Per wave, 32 rows: S^T = K Q^T with 32 x 32 x 16 products, the keys as rows.  A
+// lane then has one query row: the running maximum and total are its own, and its
+// 16 scores of 32 keys are, packed in order, the operand that O^T = V^T P^T takes
+// (its keys permuted alike: V^T is read transposed from LDS, 4 keys at a time).
+#include <algorithm>
+
+#include "gs_paged.h"
+
+namespace gs {
+namespace {
+
+constexpr int kCWaves = 8;
+constexpr int kCKeys = 64;
+constexpr int kCStages = 3;
+
+// V rows that no query of a tile sees are zero in LDS: the cache may hold
+// anything there, and 0 * NaN is not 0.
+__device__ const u32x4 g_zero16 = {0, 0, 0, 0};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// 4 x 16 elements, transposed: lane i of 16 gives the address of 4 elements of
+// row i / 4 and gets column i of the 4 rows.
+__device__ __forceinline__ uint64_t read_tr(const char* p) {
+  return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
+}
+
+// As dma16, with the wait state that M0 needs.
+__device__ __forceinline__ void dma16_row(const char* src, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_dst) : "memory", "m0");
+}
+constexpr int wait_vm_lds0(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
+
+struct ChunkItem {
+  int s, j, part, nparts, slot;      // slot: its partial result's, or -1
+};
+
+// Workgroup-wide sums of two values a thread, and their exclusive prefixes.
+struct Scan2 {
+  int64_t before0, total0;
+  int64_t before1, total1;
+};
+__device__ __forceinline__ Scan2 scan2(int64_t a, int64_t b, int64_t (*red)[2]) {
+  const int l = lane_id(), wave = threadIdx.x >> 6;
+  int64_t ia = a, ib = b;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t ua = __shfl_up(ia, d, 64), ub = __shfl_up(ib, d, 64);
+    if (l >= d) {
+      ia += ua;
+      ib += ub;
+    }
+  }
+  if (l == 63) {
+    red[wave][0] = ia;
+    red[wave][1] = ib;
+  }
+  __syncthreads();
+  Scan2 s{ia - a, 0, ib - b, 0};
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
+    if (w < wave) {
+      s.before0 += red[w][0];
+      s.before1 += red[w][1];
+    }
+    s.total0 += red[w][0];
+    s.total1 += red[w][1];
+  }
+  __syncthreads();
+  return s;
+}
+
+// The r-th part (JOIN: the r-th tile that was split) of the batch's tiles for one
+// head, in order of sequences, tiles and parts; r counts from the last where
+// `reverse`.  Every thread of the workgroup calls it.
+template <bool JOIN>
+__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, int64_t r, bool by_xcd, int& h, int64_t (*red)[2], int* found) {
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  const int threads = blockDim.x;
+  const int run = (a.B + threads - 1) / threads;
+  const int s0 = min(static_cast<int>(threadIdx.x) * run, a.B), s1 = min(s0 + run, a.B);
+  int64_t work = 0;
+  for (int s = s0; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
+  const Scan2 w = scan2(work, 0, red);
+  const int pt = addr::chunk_part_tiles(w.total0, a.HK, a.chunk_slots, kChunkLeast);
+  int64_t items = 0, split = 0;                      // items: parts (JOIN: split tiles); split: partial results
+  for (int s = s0; s < s1; ++s) {
+    const addr::PagedSeq sq = seq_of_form<true>(a, s);
+    const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
+    items += JOIN ? (np > 1 ? nt : 0) : static_cast<int64_t>(nt) * np;
+    split += np > 1 ? static_cast<int64_t>(nt) * np : 0;
+  }
+  const Scan2 c = scan2(items, split, red);
+  const int64_t n = c.total0;
+  if (by_xcd) {
+    // consecutive workgroups go to the XCDs in turn: each XCD takes a contiguous
+    // range of (head, part), so a sequence's tiles share one L2's keys
+    const int64_t total = n * a.HK, per = (total + 7) >> 3;
+    const int64_t t = (r & 7) * per + (r >> 3);
+    if ((r >> 3) >= per || t >= total) r = -1;
+    else {
+      h = static_cast<int>(t / n);
+      r = n - 1 - (t - h * n);                       // a sequence's last tiles, the longest, first
+    }
+  }
+  if (threadIdx.x == 0) found[0] = -1;
+  __syncthreads();
+  if (r >= 0 && r < n && r >= c.before0 && r < c.before0 + items) {
+    int64_t at = c.before0, sl = c.before1;
+    for (int s = s0; s < s1; ++s) {
+      const addr::PagedSeq sq = seq_of_form<true>(a, s);
+      const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
+      const int64_t here = JOIN ? (np > 1 ? nt : 0) : static_cast<int64_t>(nt) * np;
+      if (r < at + here) {
+        const int k = static_cast<int>(r - at);
+        found[0] = s;
+        found[1] = JOIN ? k : k / np;
+        found[2] = JOIN ? 0 : k % np;
+        found[3] = np;
+        found[4] = np > 1 ? static_cast<int>(sl + (JOIN ? static_cast<int64_t>(k) * np : k)) : -1;
+        break;
+      }
+      at += here;
+      sl += np > 1 ? static_cast<int64_t>(nt) * np : 0;
+    }
+  }
+  __syncthreads();
+  return ChunkItem{found[0], found[1], found[2], found[3], found[4]};
+}
+
+__device__ __forceinline__ void store4(const PagedArgs& a, int64_t e, f32x4 x) {
+  uint32_t* p = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + e);
+  const uint64_t w = pack_bf16x2(x[0], x[1]) | (static_cast<uint64_t>(pack_bf16x2(x[2], x[3])) << 32);
+  *reinterpret_cast<uint64_t*>(p) = w;
+}
+
+template <int DT>
+__global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs a) {
+  constexpr int kRowB = DT * 2;                     // bytes of a key row in LDS
+  constexpr int kTileB = kCKeys * kRowB;            // of a stage's keys, and of its values
+  constexpr int kStageB = 2 * kTileB;
+  constexpr int kRowsPer = 1024 / kRowB;            // rows a wave transfer moves
+  constexpr int kMoves = 8 / kRowsPer;              // transfers of a wave for its 8 keys (as many for the values)
+  constexpr int kSteps = DT / 16;
+  constexpr int kDT = DT / 32;                      // O^T tiles of 32 columns
+  __shared__ __attribute__((aligned(1024))) char lds[kCStages * kStageB];
+  __shared__ int64_t s_red[kCWaves][2];
+  __shared__ int s_found[5];
+
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
+  const int lq = l & 31, hl = l >> 5;
+  int h = 0;
+  const ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, s_red, s_found);
+  if (it.s < 0) return;
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  const int s = __builtin_amdgcn_readfirstlane(it.s);
+  const addr::PagedSeq sq = seq_of_form<true>(a, s);
+  const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
+  const int nkt = addr::chunk_key_tiles(tile);
+  const int kt0 = static_cast<int>(static_cast<int64_t>(nkt) * it.part / it.nparts);
+  const int kt1 = static_cast<int>(static_cast<int64_t>(nkt) * (it.part + 1) / it.nparts);
+
+  // ---- the lane's query row ---------------------------------------------------
+  const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
+  const int r = wave * 32 + lq;
+  const bool live = r < nrow;
+  const int qi = tile.i0 + (live ? r / a.G : 0);
+  const int qh = h * a.G + (live ? r % a.G : 0);
+  const int hi = live ? sq.len - sq.n + qi + 1 : 0;                // sees [lo, hi)
+  const int lo = a.window > 0 ? hi - a.window : 0;
+  const int64_t tok = sq.q0 + qi;
+  u32x4 qf[kSteps];
+  {
+    const char* qp = static_cast<const char*>(a.q) + (tok * a.q_ts + static_cast<int64_t>(qh) * a.q_hs) * 2;
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st) {
+      const int d = 16 * st + 8 * hl;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(qp + (d < a.D ? d : 0) * 2);
+      qf[st] = live && d < a.D ? x : u32x4{0, 0, 0, 0};
+    }
+  }
+  // what the wave's rows see between them: [any_lo, any_hi); all of them: [all_lo, all_hi)
+  const int w0 = wave * 32, w1 = min(w0 + 31, nrow - 1);
+  const bool wave_live = w0 < nrow;
+  const int base_pos = sq.len - sq.n + tile.i0 + 1;
+  const int all_hi = __builtin_amdgcn_readfirstlane(base_pos + w0 / a.G);
+  const int any_hi = __builtin_amdgcn_readfirstlane(wave_live ? base_pos + w1 / a.G : 0);
+  const int any_lo = a.window > 0 ? all_hi - a.window : 0, all_lo = a.window > 0 ? any_hi - a.window : 0;
+
+  // ---- transfers ------------------------------------------------------------------
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
+  const int32_t* trow = a.table + static_cast<int64_t>(s) * a.ld_table;
+  const int t_row = l / (64 / kRowsPer), t_pos = l % (64 / kRowsPer);   // the lane's row and LDS position in a transfer
+  struct Id {
+    int id;
+    uint32_t row;
+  };
+  const auto id_of = [&](int kt) {
+    uint32_t pg, row;
+    const int oct = addr::paged_octet(tile.first + kt * kCKeys + 8 * __builtin_amdgcn_readfirstlane(wave), tile.ve);
+    addr::div_by(static_cast<uint32_t>(oct) >> 3, a.page_octets, a.page_magic, pg, row);
+    return Id{trow[pg], row * 8};
+  };
+  const auto issue = [&](int kt, int stage, const Id& id) {
+    const int64_t page = addr::paged_page(id.id, a.num_pages);
+    const int64_t kb = page * a.k_ps + h * a.k_hs + static_cast<int64_t>(id.row) * a.k_rs;
+    const int64_t vb = page * a.v_ps + h * a.v_hs + static_cast<int64_t>(id.row) * a.v_rs;
+    const int t0 = tile.first + kt * kCKeys + 8 * wave;
+#pragma unroll
+    for (int x = 0; x < kMoves; ++x) {
+      const int row = x * kRowsPer + t_row;                        // of the wave's 8
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + stage * kStageB + (8 * wave + x * kRowsPer) * kRowB);
+      const int kp = addr::chunk_k_pos(DT, 8 * wave + row, t_pos), vp = addr::chunk_v_pos(DT, 8 * wave + row, t_pos);
+      const char* zero = reinterpret_cast<const char*>(&g_zero16);
+      const char* ks = static_cast<const char*>(a.k) + (kb + row * a.k_rs + kp * 8) * 2;
+      const char* vs = static_cast<const char*>(a.v) + (vb + row * a.v_rs + vp * 8) * 2;
+      const bool seen = t0 + row >= tile.vs && t0 + row < tile.ve;
+      dma16_row(kp * 8 < a.D ? ks : zero, dst);
+      dma16_row(seen && vp * 8 < a.D ? vs : zero, dst + kTileB);
+    }
+  };
+
+  f32x16 o[kDT];
+#pragma unroll
+  for (int d = 0; d < kDT; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
+  float m = -INFINITY, lsum = 0.f;
+
+  // LDS addresses of the lane's operand rows, per K step and per column tile
+  uint32_t k_at[kSteps], v_at[kDT];
+#pragma unroll
+  for (int st = 0; st < kSteps; ++st) k_at[st] = lq * kRowB + addr::chunk_k_pos(DT, lq, 2 * st + hl) * 16;
+  const int v_row = 4 * hl + ((l & 15) >> 2);
+#pragma unroll
+  for (int d = 0; d < kDT; ++d)
+    v_at[d] = kTileB + v_row * kRowB + addr::chunk_v_pos(DT, v_row, 4 * d + 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
+
+  const auto compute = [&](int kt, int stage) {
+    const int tb = tile.first + kt * kCKeys;
+    if (!wave_live || tb >= any_hi || tb + kCKeys <= any_lo) return;
+    const char* base = lds + stage * kStageB;
+    f32x16 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sc[u][v] = 0.f;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) sc[u] = mfma32_bf16(ld16(base + k_at[st] + u * 32 * kRowB), qf[st], sc[u]);
+    }
+    if (tb + kCKeys > all_hi || tb < all_lo) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int t = tb + 32 * u + mfma32_row(v, l);
+          if (t >= hi || t < lo) sc[u][v] = -INFINITY;
+        }
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[u][v]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
+    // the reference point follows the maximum once it has grown by 2^8: the sums
+    // stay far from their limits, and o is rarely scaled
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      lsum *= f;
+#pragma unroll
+      for (int d = 0; d < kDT; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    u32x4 pf[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(sc[g >> 1][8 * (g & 1) + i], a.scale_log2, -ms));
+        lsum += p[i];
+      }
+      // bf16 probabilities (relative error 2^-8, as the values and the result have); the total stays in fp32
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+    }
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint64_t x0 = read_tr(base + v_at[d] + g * 16 * kRowB), x1 = read_tr(base + v_at[d] + (g * 16 + 8) * kRowB);
+        const u32x4 vf = {static_cast<uint32_t>(x0), static_cast<uint32_t>(x0 >> 32), static_cast<uint32_t>(x1),
+                          static_cast<uint32_t>(x1 >> 32)};
+        o[d] = mfma32_bf16(vf, pf[g], o[d]);
+      }
+  };
+
+  // ---- the walk over the keys ---------------------------------------------------
+  const int n = kt1 - kt0;
+  if (n > 0) {
+    Id id = id_of(kt0);
+    issue(kt0, 0, id);
+    id = id_of(kt0 + 1);
+    if (n > 1) issue(kt0 + 1, 1, id);
+    id = id_of(kt0 + 2);
+    int stage = 0;
+    for (int i = 0; i < n; ++i) {
+      mem_fence_compiler();
+      if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm_lds0(2 * kMoves));
+      else __builtin_amdgcn_s_waitcnt(wait_vm_lds0(0));
+      __builtin_amdgcn_s_barrier();
+      mem_fence_compiler();
+      if (i + 2 < n) {
+        issue(kt0 + i + 2, stage == 0 ? 2 : stage - 1, id);       // the stage of tile i - 1, which every wave is past
+        id = id_of(kt0 + i + 3);
+      }
+      compute(kt0 + i, stage);
+      stage = stage == kCStages - 1 ? 0 : stage + 1;
+    }
+  }
+
+  // ---- results --------------------------------------------------------------------
+  lsum += __shfl_xor(lsum, 32, 64);
+  if (!live) return;
+  if (it.slot < 0) {
+    const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+    const int64_t e = tok * a.o_ts + static_cast<int64_t>(qh) * a.o_hs;
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4) {
+        const int col = 32 * d + mfma32_row(v, l);
+        f32x4 x = {o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+        x = lsum == 0.f ? f32x4{0, 0, 0, 0} : x * inv;
+        if (col < a.D) store4(a, e + col, x);
+      }
+    if (a.lse != nullptr && hl == 0) a.lse[tok * a.H + qh] = lsum == 0.f ? -INFINITY : (m + log2f(lsum)) * 0.6931471805599453f;
+  } else {
+    float* p = a.chunk_ws + (h * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * addr::chunk_partial_floats(kChunkRows, DT);
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<f32x4*>(p + r * DT + 32 * d + mfma32_row(v, l)) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+    if (hl == 0) {
+      p[kChunkRows * DT + r] = m;
+      p[kChunkRows * (DT + 1) + r] = lsum;
+    }
+  }
+}
+
+// The parts of a tile joined, in the order of their keys: grid (split tiles x row groups, heads).
+constexpr int kJoinRows = 32;
+template <int DT>
+__global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
+  __shared__ int64_t s_red[4][2];
+  __shared__ int s_found[5];
+  int h = blockIdx.y;
+  const ChunkItem it = find_chunk<true>(a, blockIdx.x / (kChunkRows / kJoinRows), false, h, s_red, s_found);
+  if (it.s < 0) return;
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  const addr::PagedSeq sq = seq_of_form<true>(a, it.s);
+  const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
+  const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
+  const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
+  const float* first = a.chunk_ws + (h * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * size;
+  const int r0 = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
+  for (int x = threadIdx.x; x < kJoinRows * (DT / 4); x += 256) {
+    const int r = r0 + x / (DT / 4), d = (x % (DT / 4)) * 4;
+    if (r >= nrow) break;
+    float M = -INFINITY;
+    for (int p = 0; p < it.nparts; ++p) M = fmaxf(M, first[p * size + kChunkRows * DT + r]);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int p = 0; p < it.nparts; ++p) {
+      const float f = exp2f(first[p * size + kChunkRows * DT + r] - ms);
+      L += f * first[p * size + kChunkRows * (DT + 1) + r];
+      acc += f * *reinterpret_cast<const f32x4*>(first + p * size + r * DT + d);
+    }
+    if (d >= a.D) continue;
+    const int64_t tok = sq.q0 + tile.i0 + r / a.G;
+    const int head = h * a.G + r % a.G;
+    store4(a, tok * a.o_ts + static_cast<int64_t>(head) * a.o_hs + d, L == 0.f ? f32x4{0, 0, 0, 0} : acc * (1.0f / L));
+    if (a.lse != nullptr && d == 0) a.lse[tok * a.H + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+  }
+}
+
+}  // namespace
+
+int64_t chunk_workspace_bytes(int HK, int DT, int cus) {
+  return HK * addr::chunk_slots_per_head(HK, cus) * addr::chunk_partial_floats(kChunkRows, DT) * 4;
+}
+
+// Tiles of a head at most: each sequence may end with a partial one.
+static int64_t chunk_most_tiles(const PagedArgs& a) {
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  return a.T / tq + std::min(a.B, a.T);
+}
+
+// Parts at most: tiles, and the split tiles' parts.
+int64_t chunk_grid(const PagedArgs& a) {
+  const int64_t per_head = chunk_most_tiles(a) + addr::chunk_slots_per_head(a.HK, a.chunk_slots);
+  return 8 * ((per_head * a.HK + 7) / 8);
+}
+
+void launch_chunk(const PagedArgs& a, int DT, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(chunk_grid(a)));
+  // split tiles at most: half the partial results, as each has two or more
+  const int64_t split = std::min(chunk_most_tiles(a), addr::chunk_slots_per_head(a.HK, a.chunk_slots) / 2);
+  const dim3 join(static_cast<unsigned>(split * (kChunkRows / kJoinRows)), static_cast<unsigned>(a.HK));
+  if (DT == 64) {
+    hipLaunchKernelGGL((chunk_attention_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);
+    hipLaunchKernelGGL((chunk_join_kernel<64>), join, dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((chunk_attention_kernel<128>), grid, dim3(64 * kCWaves), 0, st, a);
+    hipLaunchKernelGGL((chunk_join_kernel<128>), join, dim3(256), 0, st, a);
+  }
+}
+
+}  // namespace gs

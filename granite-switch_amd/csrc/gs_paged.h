@@ -1,0 +1,53 @@
+// What the kernels over a paged cache share (gs_paged.hip, gs_chunk.hip).
+#pragma once
+
+#include "gs_addr.h"
+#include "gs_common.h"
+
+namespace gs {
+
+struct PagedArgs {
+  const void* q;
+  int64_t q_ts, q_hs;               // token and head strides, elements
+  void* out;
+  int64_t o_ts, o_hs;
+  const void* k;
+  int64_t k_ps, k_hs, k_rs;         // page, head and row strides
+  const void* v;
+  int64_t v_ps, v_hs, v_rs;
+  const int32_t* table;
+  int64_t ld_table;
+  const int32_t* lens;
+  const int32_t* cu;
+  float* lse;                       // [T, H] or NULL
+  float* ws;                        // row form: partial results, then join
+  int4* join;                       // [parts * HK]: the item a part completes, or none
+  float* chunk_ws;                  // chunk form: partial results
+  int64_t max_len;
+  uint32_t page_octets, page_magic;
+  int num_pages;
+  int B, T, H, HK, G, D;
+  int window, parts;
+  int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
+  int chunk_slots;                  // workgroups that the chunk form fills
+  float scale_log2;
+};
+
+// Sequences of a batch that a form takes: of at most `limit` rows, or of more.
+template <bool CHUNK>
+__device__ __host__ __forceinline__ addr::PagedSeq seq_of_form(const PagedArgs& a, int s) {
+  addr::PagedSeq q = a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], a.lens[s], a.T, a.max_len)
+                                     : addr::paged_seq(s, s + 1, a.lens[s], a.T, a.max_len);
+  const bool few = static_cast<int64_t>(q.n) * a.G <= a.row_limit;
+  if (few == CHUNK) q.n = 0;
+  return q;
+}
+
+// The chunk form for the batch (bf16, head widths up to 128): true if launched.
+constexpr int kChunkRows = 256;
+constexpr int kChunkLeast = 8;      // key tiles of a part, at least
+int64_t chunk_workspace_bytes(int HK, int DT, int cus);
+int64_t chunk_grid(const PagedArgs& a);
+void launch_chunk(const PagedArgs& a, int DT, hipStream_t st);
+
+}  // namespace gs

@@ -9,15 +9,16 @@
 // gs_append_kv (append_kv_kernel): the QKV projection's rows in, the rotated
 // query rows out, the rotated keys and the values into their slots.
 //
-// gs_paged_attention (paged_attention_kernel, paged_join_kernel): per query row
-// one pass over the keys it sees with the running maximum and total of its
-// softmax; the passes of one sequence are split over workgroups by length and
-// joined.
+// gs_paged_attention: per query row one pass over the keys it sees with the
+// running maximum and total of its softmax.  The row form here
+// (paged_attention_kernel, paged_join_kernel) takes 16 rows at a time, straight
+// from the pages into registers, a sequence's length split over workgroups and
+// joined: one new token of a sequence.  Sequences of many rows take the chunk
+// form (gs_chunk.hip).
 #include <algorithm>
 #include <vector>
 
-#include "gs_addr.h"
-#include "gs_common.h"
+#include "gs_paged.h"
 
 namespace gs {
 namespace {
@@ -204,30 +205,6 @@ __global__ __launch_bounds__(256) void cache_slots_kernel(const int32_t* table, 
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
-struct PagedArgs {
-  const void* q;
-  int64_t q_ts, q_hs;
-  void* out;
-  int64_t o_ts, o_hs;
-  const void* k;
-  int64_t k_ps, k_hs, k_rs;
-  const void* v;
-  int64_t v_ps, v_hs, v_rs;
-  const int32_t* table;
-  int64_t ld_table;
-  const int32_t* lens;
-  const int32_t* cu;
-  float* lse;                       // [T, H] or NULL
-  float* ws;
-  int4* join;                       // [parts * HK]: the item a part completes, or none
-  int64_t max_len;
-  uint32_t page_octets, page_magic;
-  int num_pages;
-  int B, T, H, HK, G, D;
-  int window, parts;
-  float scale_log2;
-};
-
 // What the two element types differ in.  Both use 16 x 16 products: S^T = K Q^T
 // with the keys as rows, so a lane has one query row's scores of consecutive
 // keys, which is the operand that O^T = V^T P^T takes them as.
@@ -302,10 +279,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 15, lg = l >> 4;
   const int part = blockIdx.x, h = blockIdx.y;
-  const auto seq_at = [&](int s) {
-    return a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], a.lens[s], a.T, a.max_len)
-                           : addr::paged_seq(s, s + 1, a.lens[s], a.T, a.max_len);
-  };
+  const auto seq_at = [&](int s) { return seq_of_form<false>(a, s); };
 
   // ---- the part's share: every part takes an equal run of the batch's units --
   const int run = (a.B + 255) / 256;
@@ -649,6 +623,26 @@ int64_t paged_ws_bytes(int HK, int D, int cus) {
   return n * (2 * addr::paged_partial_floats(paged_width(D)) * 4 + static_cast<int64_t>(sizeof(int4)));
 }
 
+// Whether ragged calls of these sizes have a chunk form, and the rows up to
+// which a sequence stays with the row form.
+bool chunk_form(bool bf16, int G, int D) { return bf16 && D <= 128 && G <= kChunkRows; }
+constexpr int kRowFormRows = 16;
+
+int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus) {
+  return paged_ws_bytes(HK, D, cus) + (ragged && chunk_form(bf16, G, D) ? chunk_workspace_bytes(HK, paged_width(D), cus) : 0);
+}
+
+// What follows from the sizes alone.
+void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, float scale) {
+  a.parts = paged_parts_for(a.HK, cus);
+  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - 4096);
+  a.page_octets = static_cast<uint32_t>(page_size / 8);
+  a.page_magic = addr::div_magic(a.page_octets);
+  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) ? kRowFormRows : INT32_MAX;
+  a.chunk_slots = cus;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+}
+
 template <bool BF16, int DT>
 void launch_paged(const PagedArgs& a, hipStream_t st) {
   const dim3 grid(a.parts, a.HK);
@@ -672,6 +666,7 @@ bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 && a % n 
 // ---------------------------------------------------------------------------
 struct PagedModel {
   int64_t bad = 0, checked = 0;
+  std::vector<char> rows;                           // output rows written
   char msg[256] = "";
   void fail(const char* what, int64_t at, int64_t n, int64_t cap) {
     if (bad++ == 0) snprintf(msg, sizeof(msg), "%s: elements [%lld, %lld) of %lld", what, (long long)at, (long long)(at + n), (long long)cap);
@@ -697,16 +692,13 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
   const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D);
   const int64_t o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
-  const auto seq_at = [&](int s) {
-    return a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], a.lens[s], a.T, a.max_len)
-                           : addr::paged_seq(s, s + 1, a.lens[s], a.T, a.max_len);
-  };
+  const auto seq_at = [&](int s) { return seq_of_form<false>(a, s); };
   std::vector<int64_t> start(a.B + 1, 0);
   for (int s = 0; s < a.B; ++s) start[s + 1] = start[s] + addr::paged_seq_units(seq_at(s), a.G, a.window, kUnit);
   const int64_t U = start[a.B];
   const int parts = addr::paged_parts(U, a.parts);
   std::vector<char> slots(static_cast<size_t>(a.parts) * a.HK * 2, 0);
-  std::vector<char> rows(static_cast<size_t>(a.T) * a.H, 0);
+  std::vector<char>& rows = m.rows;
   const auto written = [&](const addr::PagedSeq& sq, int j, int h, int nrow) {
     for (int q = 0; q < nrow; ++q) {
       const int64_t rr = static_cast<int64_t>(j) * 16 + q;
@@ -804,11 +796,99 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   }
   for (char c : slots)
     if (c == 1 && !m.bad) m.fail("a partial result that no join reads", 0, 1, 0);
+}
+
+// The chunk form.
+template <int DT>
+void model_chunk(PagedModel& m, const PagedArgs& a) {
+  constexpr int kWaves = 8, kRowB = DT * 2, kTileB = 64 * kRowB, kRowsPer = 1024 / kRowB;
+  // what the transfers leave in LDS, and what the operand reads take from it
+  std::vector<int> k_lds(kTileB / 16, -1), v_lds(kTileB / 16, -1);
+  for (int w = 0; w < kWaves; ++w)
+    for (int x = 0; x < 8 / kRowsPer; ++x)
+      for (int l = 0; l < 64; ++l) {
+        const int row = 8 * w + x * kRowsPer + l / (64 / kRowsPer), pos = l % (64 / kRowsPer);
+        const int at = ((8 * w + x * kRowsPer) * kRowB + l * 16) / 16;
+        k_lds[at] = row * 64 + addr::chunk_k_pos(DT, row, pos);
+        v_lds[at] = row * 64 + addr::chunk_v_pos(DT, row, pos);
+      }
+  for (int l = 0; l < 64; ++l) {
+    const int lq = l & 31, hl = l >> 5, v_row = 4 * hl + ((l & 15) >> 2);
+    for (int u = 0; u < 2; ++u)
+      for (int st = 0; st < DT / 16; ++st) {
+        const int at = lq * kRowB + addr::chunk_k_pos(DT, lq, 2 * st + hl) * 16 + u * 32 * kRowB;
+        m.in("K operand (LDS)", at, 16, kTileB);
+        if (k_lds[at / 16] != (32 * u + lq) * 64 + 2 * st + hl) m.fail("K operand of another piece", at, 16, kTileB);
+      }
+    for (int d = 0; d < DT / 32; ++d)
+      for (int g = 0; g < 4; ++g)
+        for (int x = 0; x < 2; ++x) {
+          const int piece = 4 * d + 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
+          const int at = v_row * kRowB + addr::chunk_v_pos(DT, v_row, piece) * 16 + (l & 1) * 8 + (g * 16 + 8 * x) * kRowB;
+          m.in("V operand (LDS)", at, 8, kTileB);
+          if (v_lds[at / 16] != (g * 16 + 8 * x + v_row) * 64 + piece) m.fail("V operand of another piece", at, 8, kTileB);
+        }
+  }
+  const int max_pages = static_cast<int>(a.max_len / (8 * a.page_octets));
+  const int64_t page_rows = 8 * a.page_octets;
+  const int64_t k_elems = extent3(a.num_pages, a.k_ps, a.HK, a.k_hs, page_rows, a.k_rs, a.D);
+  const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
+  const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D), o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  int64_t U2 = 0, n = 0, slots = 0, split = 0;
+  for (int s = 0; s < a.B; ++s) U2 += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
+  const int pt = addr::chunk_part_tiles(U2, a.HK, a.chunk_slots, kChunkLeast);
   for (int s = 0; s < a.B && !m.bad; ++s) {
-    const addr::PagedSeq sq = seq_at(s);
+    const addr::PagedSeq sq = seq_of_form<true>(a, s);
+    const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
+    n += static_cast<int64_t>(nt) * np;
+    if (np > 1) {
+      slots += static_cast<int64_t>(nt) * np;
+      split += nt;
+    }
+    for (int j = 0; j < nt && !m.bad; ++j) {
+      const addr::PagedTile t = addr::chunk_tile(sq, tq, a.window, j);
+      const int nkt = addr::chunk_key_tiles(t);
+      const int nrow = (t.i1 - t.i0 + 1) * a.G;
+      if (nrow < 1 || nrow > kChunkRows) m.fail("rows of a tile", 0, nrow, kChunkRows);
+      for (int h = 0; h < a.HK && !m.bad; ++h) {
+        for (int r = 0; r < nrow; ++r) {
+          const int64_t tok = sq.q0 + t.i0 + r / a.G, head = h * a.G + r % a.G;
+          m.in("output row", tok * a.H + head, 1, static_cast<int64_t>(a.T) * a.H);
+          if (m.bad) return;
+          if (m.rows[tok * a.H + head]++) m.fail("output row written twice", tok, 1, a.T);
+          m.in("q", tok * a.q_ts + head * a.q_hs, a.D, q_elems);
+          m.in("out", tok * a.o_ts + head * a.o_hs, a.D, o_elems);
+        }
+        for (int kt = 0; kt < nkt + 2 && nkt > 0; ++kt)       // ids are read up to two tiles past the last
+          for (int w = 0; w < kWaves; ++w) {
+            uint32_t pg, row;
+            addr::div_by(static_cast<uint32_t>(addr::paged_octet(t.first + kt * 64 + 8 * w, t.ve)) >> 3, a.page_octets, a.page_magic, pg, row);
+            m.in("page table row", pg, 1, max_pages);
+            if (m.bad) return;
+            if (kt >= nkt) continue;
+            const int64_t page = addr::paged_page(a.table[s * a.ld_table + pg], a.num_pages);
+            for (int rr = 0; rr < 8; ++rr) {
+              m.in("page row", row * 8 + rr, 1, page_rows);
+              m.in("k cache", page * a.k_ps + h * a.k_hs + (row * 8 + rr) * a.k_rs, a.D, k_elems);
+              m.in("v cache", page * a.v_ps + h * a.v_hs + (row * 8 + rr) * a.v_rs, a.D, v_elems);
+            }
+          }
+      }
+    }
+  }
+  m.in("partial results", 0, slots, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
+  m.in("split tiles", 0, 2 * split, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
+  const int64_t per = (n * a.HK + 7) >> 3;
+  m.in("workgroups", 0, 8 * per, chunk_grid(a));
+}
+
+void model_rows(PagedModel& m, const PagedArgs& a) {
+  for (int s = 0; s < a.B && !m.bad; ++s) {
+    const addr::PagedSeq sq = a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], 0, a.T, 0) : addr::PagedSeq{s, 1, 0};
     for (int i = 0; i < sq.n; ++i)
       for (int h = 0; h < a.H; ++h)
-        if (!rows[static_cast<int64_t>(sq.q0 + i) * a.H + h] && !m.bad) m.fail("output row never written", sq.q0 + i, 1, a.T);
+        if (!m.rows[static_cast<int64_t>(sq.q0 + i) * a.H + h] && !m.bad) m.fail("output row never written", sq.q0 + i, 1, a.T);
   }
 }
 
@@ -949,13 +1029,13 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
   return GS_OK;
 }
 
-int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim) {
+int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t ragged) {
   if ((dtype != GS_DTYPE_BF16 && dtype != GS_DTYPE_FP32) || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 ||
       head_dim <= 0 || head_dim > 256) {
     set_error("gs_paged_attention_workspace_bytes: dtype=%d heads=%d kv_heads=%d head_dim=%d", dtype, heads, kv_heads, head_dim);
     return -GS_ERR_INVALID;
   }
-  return paged_ws_bytes(kv_heads, head_dim, device_cus());
+  return attention_ws_bytes(dtype == GS_DTYPE_BF16, ragged != 0, heads / kv_heads, kv_heads, head_dim, device_cus());
 }
 
 int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs, const void* k_cache, int64_t k_ps,
@@ -993,7 +1073,7 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
                    strides_ok(o_ts, o_hs, ve),
                "%s: q, the caches and out must be 16-byte aligned with strides that are multiples of %d elements", who, ve);
   const int cus = device_cus();
-  const int64_t need = paged_ws_bytes(kv_heads, head_dim, cus);
+  const int64_t need = attention_ws_bytes(bf16, cu_seqlens != nullptr, heads / kv_heads, kv_heads, head_dim, cus);
   if (workspace == nullptr || workspace_bytes < need) {
     set_error("%s: workspace of %lld bytes needed (got %lld)", who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
     return GS_ERR_WORKSPACE;
@@ -1006,19 +1086,22 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   a.v = v_cache; a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
   a.table = page_table; a.ld_table = ld_table;
   a.lens = kv_lens; a.cu = cu_seqlens; a.lse = lse;
-  a.parts = paged_parts_for(kv_heads, cus);
-  a.ws = static_cast<float*>(workspace);
-  a.join = reinterpret_cast<int4*>(a.ws + static_cast<int64_t>(a.parts) * kv_heads * 2 * addr::paged_partial_floats(paged_width(head_dim)));
-  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - 4096);
-  a.page_octets = static_cast<uint32_t>(page_size / 8);
-  a.page_magic = addr::div_magic(a.page_octets);
   a.num_pages = static_cast<int>(num_pages);
   a.B = num_seqs; a.T = static_cast<int>(num_tokens);
   a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
   a.window = window;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  plan_paged(a, bf16, cus, max_pages, page_size, scale);
+  const int DT = paged_width(head_dim);
+  a.ws = static_cast<float*>(workspace);
+  const int64_t partials = static_cast<int64_t>(a.parts) * kv_heads * 2 * addr::paged_partial_floats(DT);
+  a.join = reinterpret_cast<int4*>(a.ws + partials);
+  a.chunk_ws = reinterpret_cast<float*>(a.join + static_cast<int64_t>(a.parts) * kv_heads);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (paged_width(head_dim)) {
+  if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
+    GS_CHECK_ARG(chunk_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
+    launch_chunk(a, DT, st);
+  }
+  switch (DT) {
     case 64: bf16 ? launch_paged<true, 64>(a, st) : launch_paged<false, 64>(a, st); break;
     case 128: bf16 ? launch_paged<true, 128>(a, st) : launch_paged<false, 128>(a, st); break;
     default: bf16 ? launch_paged<true, 256>(a, st) : launch_paged<false, 256>(a, st); break;
@@ -1046,20 +1129,20 @@ int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int6
   a.k_ps = k_ps; a.k_hs = k_hs; a.k_rs = k_rs;
   a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
   a.table = page_table; a.ld_table = ld_table; a.lens = kv_lens; a.cu = cu_seqlens;
-  a.parts = paged_parts_for(kv_heads, cus);
-  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - 4096);
-  a.page_octets = static_cast<uint32_t>(page_size / 8);
-  a.page_magic = addr::div_magic(a.page_octets);
   a.num_pages = static_cast<int>(num_pages);
   a.B = num_seqs; a.T = static_cast<int>(num_tokens);
   a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
   a.window = window;
+  plan_paged(a, bf16, cus, max_pages, page_size, 1.f);
   PagedModel m;
+  m.rows.assign(static_cast<size_t>(a.T) * a.H, 0);
+  if (a.row_limit != INT32_MAX) paged_width(head_dim) == 64 ? model_chunk<64>(m, a) : model_chunk<128>(m, a);
   switch (paged_width(head_dim)) {
     case 64: bf16 ? model_attention<true, 64>(m, a) : model_attention<false, 64>(m, a); break;
     case 128: bf16 ? model_attention<true, 128>(m, a) : model_attention<false, 128>(m, a); break;
     default: bf16 ? model_attention<true, 256>(m, a) : model_attention<false, 256>(m, a); break;
   }
+  model_rows(m, a);
   if (checked) *checked = m.checked;
   if (msg && msg_len > 0) snprintf(msg, static_cast<size_t>(msg_len), "%s", m.msg);
   return m.bad;

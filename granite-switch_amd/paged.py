@@ -237,12 +237,12 @@ def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
 _need: dict = {}
 
 
-def workspace_bytes(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int) -> int:
-    """Workspace of one ``paged_attention`` call (for ``workspace=``); does not depend on the batch."""
-    key = (dtype, heads, kv_heads, head_dim, torch.cuda.current_device())
+def workspace_bytes(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int, ragged: bool = False) -> int:
+    """Workspace of one ``paged_attention`` call (for ``workspace=``), with ``cu_seqlens`` or without; whatever the batch."""
+    key = (dtype, heads, kv_heads, head_dim, ragged, torch.cuda.current_device())
     n = _need.get(key)
     if n is None:
-        n = int(_lib.load().gs_paged_attention_workspace_bytes(_DTYPES[dtype], heads, kv_heads, head_dim))
+        n = int(_lib.load().gs_paged_attention_workspace_bytes(_DTYPES[dtype], heads, kv_heads, head_dim, int(ragged)))
         if n < 0:
             raise _lib.GraniteSwitchError("gs_paged_attention_workspace_bytes", -n, _lib.last_error())
         _need[key] = n
@@ -300,7 +300,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if T == 0 or B == 0:
         return out
     stream = _lib.stream_ptr(dev)
-    need = workspace_bytes(dtype, H, HK, D)
+    need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None)
     if workspace is None:
         workspace = _workspace(dev, stream, need)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():

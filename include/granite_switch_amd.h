@@ -571,9 +571,10 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * pool are read as page 0.  max_q: the most rows of a sequence where the caller
  * knows it (0: unknown); a smaller value than the batch has is an error of the
  * caller's that leaves those rows unwritten.
- * workspace: gs_paged_attention_workspace_bytes, 16-byte aligned, no
- * initialisation; calls that may overlap in time must not share one. */
-int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim);
+ * workspace: gs_paged_attention_workspace_bytes (ragged: for calls with
+ * cu_seqlens) whatever the batch, 16-byte aligned, no initialisation; calls that may overlap in time must not share one. */
+int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                           int32_t ragged);
 int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                        const void* k_cache, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
                        const void* v_cache, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,

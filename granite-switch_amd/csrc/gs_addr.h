@@ -247,13 +247,13 @@ GS_HD int64_t small_part(int64_t region, int g, int ks, int cap, int slot, int z
 }
 
 // ---- paged cache: append and attention (gs_paged.hip) -----------------------
-// n / d and n % d for d >= 1 with magic = floor((2^32 - 1) / d): the product's
-// high word is at most one short of the quotient.
+// n / d and n % d for d >= 1 and n < 2^31 with magic = floor((2^32 - 1) / d):
+// n magic / 2^32 is short of n / d by n (2^32 / d - magic) / 2^32 <= n / 2^32 (1 + 1/d) < 1.
 GS_HD uint32_t div_magic(uint32_t d) { return 0xffffffffu / d; }
 GS_HD void div_by(uint32_t n, uint32_t d, uint32_t magic, uint32_t& quot, uint32_t& rem) {
   uint32_t q = static_cast<uint32_t>((static_cast<uint64_t>(n) * magic) >> 32);
   uint32_t r = n - q * d;
-  while (r >= d) {                       // at most twice
+  if (r >= d) {
     r -= d;
     ++q;
   }
@@ -361,11 +361,11 @@ GS_HD int64_t chunk_work2(const PagedSeq& s, int tq, int window) {
   if (nt == 0) return 0;
   return static_cast<int64_t>(nt) * (chunk_key_tiles(chunk_tile(s, tq, window, 0)) + chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) + 1);
 }
-// Key tiles of a part for a batch of doubled work U2 a head: 3/4 of an equal
-// share of `slots` workgroups, and some at least.
-GS_HD int chunk_part_tiles(int64_t U2, int HK, int slots, int least) {
-  const int64_t c = (U2 * HK * 3 + 8 * slots - 1) / (8 * static_cast<int64_t>(slots));
-  return c < least ? least : static_cast<int>(c);
+// Key tiles of a part for a batch of doubled work U2 a head: an equal share of
+// `slots` workgroups, and some at least.  share = HK / (2 slots).
+GS_HD int chunk_part_tiles(int64_t U2, double share, int least) {
+  const double c = static_cast<double>(U2) * share;
+  return c < least ? least : static_cast<int>(c) + 1;
 }
 // Parts of each of a sequence's tiles: those whose last tile has two parts' key tiles or more are split.
 GS_HD int chunk_parts(const PagedSeq& s, int tq, int window, int part_tiles) {
@@ -374,8 +374,9 @@ GS_HD int chunk_parts(const PagedSeq& s, int tq, int window, int part_tiles) {
   const int p = chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) / part_tiles;
   return p < 1 ? 1 : p;
 }
-// Partial results a head can have: 2 U2 / 2 / part_tiles of them at most.
-GS_HD int64_t chunk_slots_per_head(int HK, int slots) { return (8 * static_cast<int64_t>(slots) + 3 * HK - 1) / (3 * static_cast<int64_t>(HK)) + 1; }
+// Partial results a head can have: U2 / part_tiles < 2 slots / HK of them at most,
+// as a split tile has part_tiles key tiles or more for each of its parts.
+GS_HD int chunk_slots_per_head(int HK, int slots) { return (2 * slots + HK - 1) / HK + 1; }
 GS_HD int64_t chunk_partial_floats(int R, int DT) { return static_cast<int64_t>(R) * (DT + 2); }
 // Where the 16-byte piece p of key row r is kept in LDS (rows of DT * 2 bytes).
 // K is read 16 rows at a time at one piece, V 4 rows at a time over 64 bytes;

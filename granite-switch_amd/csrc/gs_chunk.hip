@@ -1,12 +1,13 @@
 // Attention of query chunks over a paged cache (bf16, head widths up to 128):
 // the form of gs_paged_attention for sequences of many rows.
 //
-// A workgroup of 8 waves takes 256 (query, head) rows of one sequence and
-// key/value head -- 64 queries where 4 query heads share it, so the group's
+// A workgroup of 4 waves takes 128 (query, head) rows of one sequence and
+// key/value head -- 32 queries where 4 query heads share it, so the group's
 // heads read K and V once -- and walks the keys in tiles of 64.  Keys and values
-// go from the pages straight into LDS (three stages: a tile is two tiles' work
-// on its way), 16 bytes a lane, permuted so that every operand read falls on
-// different banks.
+// go from the pages straight into LDS (two stages), 16 bytes a lane, permuted so
+// that every operand read falls on different banks.  Two workgroups share a
+// compute unit: one multiplies while the other is in its softmax, its start or
+// its end.
 //
 // Per wave, 32 rows: S^T = K Q^T with 32 x 32 x 16 products, the keys as rows.  A
 // lane then has one query row: the running maximum and total are its own, and its
@@ -19,9 +20,9 @@
 namespace gs {
 namespace {
 
-constexpr int kCWaves = 8;
+constexpr int kCWaves = 4;
 constexpr int kCKeys = 64;
-constexpr int kCStages = 3;
+constexpr int kCStages = 2;
 
 // V rows that no query of a tile sees are zero in LDS: the cache may hold
 // anything there, and 0 * NaN is not 0.
@@ -39,6 +40,10 @@ __device__ __forceinline__ uint64_t read_tr(const char* p) {
 // As dma16, with the wait state that M0 needs.
 __device__ __forceinline__ void dma16_row(const char* src, uint32_t lds_dst) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_dst) : "memory", "m0");
+}
+// As above from a uniform base and the lane's byte offset.
+__device__ __forceinline__ void dma16_off(const char* base, uint32_t off, uint32_t lds_dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_dst) : "memory", "m0");
 }
 constexpr int wait_vm_lds0(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
 
@@ -92,7 +97,7 @@ __device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, int64_t r, b
   int64_t work = 0;
   for (int s = s0; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
   const Scan2 w = scan2(work, 0, red);
-  const int pt = addr::chunk_part_tiles(w.total0, a.HK, a.chunk_slots, kChunkLeast);
+  const int pt = addr::chunk_part_tiles(w.total0, a.chunk_share, kChunkLeast);
   int64_t items = 0, split = 0;                      // items: parts (JOIN: split tiles); split: partial results
   for (int s = s0; s < s1; ++s) {
     const addr::PagedSeq sq = seq_of_form<true>(a, s);
@@ -145,12 +150,12 @@ __device__ __forceinline__ void store4(const PagedArgs& a, int64_t e, f32x4 x) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedArgs a) {
   constexpr int kRowB = DT * 2;                     // bytes of a key row in LDS
   constexpr int kTileB = kCKeys * kRowB;            // of a stage's keys, and of its values
   constexpr int kStageB = 2 * kTileB;
   constexpr int kRowsPer = 1024 / kRowB;            // rows a wave transfer moves
-  constexpr int kMoves = 8 / kRowsPer;              // transfers of a wave for its 8 keys (as many for the values)
+  constexpr int kMoves = 8 / kRowsPer;              // transfers for 8 keys (as many for the values); a wave moves 16 keys
   constexpr int kSteps = DT / 16;
   constexpr int kDT = DT / 32;                      // O^T tiles of 32 columns
   __shared__ __attribute__((aligned(1024))) char lds[kCStages * kStageB];
@@ -160,10 +165,15 @@ __global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 31, hl = l >> 5;
   int h = 0;
-  const ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, s_red, s_found);
+  ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, s_red, s_found);
   if (it.s < 0) return;
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  h = __builtin_amdgcn_readfirstlane(h);             // uniform, and known to be from here on
   const int s = __builtin_amdgcn_readfirstlane(it.s);
+  it.j = __builtin_amdgcn_readfirstlane(it.j);
+  it.part = __builtin_amdgcn_readfirstlane(it.part);
+  it.nparts = __builtin_amdgcn_readfirstlane(it.nparts);
+  it.slot = __builtin_amdgcn_readfirstlane(it.slot);
+  const int tq = addr::chunk_tq(kChunkRows, a.G);
   const addr::PagedSeq sq = seq_of_form<true>(a, s);
   const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
   const int nkt = addr::chunk_key_tiles(tile);
@@ -201,32 +211,62 @@ __global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
   const int32_t* trow = a.table + static_cast<int64_t>(s) * a.ld_table;
   const int t_row = l / (64 / kRowsPer), t_pos = l % (64 / kRowsPer);   // the lane's row and LDS position in a transfer
-  struct Id {
-    int id;
-    uint32_t row;
+  // Page ids: lanes 2 i and 2 i + 1 hold those of the wave's 16 keys in tile i of
+  // 32, one load for 32 tiles (a load a tile would wait for the transfers issued
+  // before it).
+  const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+  const auto octet_of = [&](int kt, int o) {
+    return addr::paged_octet(tile.first + kt * kCKeys + 16 * wave_u + 8 * o, tile.ve);
   };
-  const auto id_of = [&](int kt) {
+  int ids = 0;
+  const auto load_ids = [&](int kt) {
     uint32_t pg, row;
-    const int oct = addr::paged_octet(tile.first + kt * kCKeys + 8 * __builtin_amdgcn_readfirstlane(wave), tile.ve);
-    addr::div_by(static_cast<uint32_t>(oct) >> 3, a.page_octets, a.page_magic, pg, row);
-    return Id{trow[pg], row * 8};
+    addr::div_by(static_cast<uint32_t>(octet_of(kt + (l >> 1), l & 1)) >> 3, a.page_octets, a.page_magic, pg, row);
+    ids = trow[pg];
   };
-  const auto issue = [&](int kt, int stage, const Id& id) {
-    const int64_t page = addr::paged_page(id.id, a.num_pages);
-    const int64_t kb = page * a.k_ps + h * a.k_hs + static_cast<int64_t>(id.row) * a.k_rs;
-    const int64_t vb = page * a.v_ps + h * a.v_hs + static_cast<int64_t>(id.row) * a.v_rs;
-    const int t0 = tile.first + kt * kCKeys + 8 * wave;
+  // Whole rows within 32-bit offsets: a transfer is a uniform base and these.
+  const bool plain = a.D == DT && a.k_rs < (1 << 26) && a.v_rs < (1 << 26);
+  uint32_t k_off[kMoves], v_off[kMoves];
 #pragma unroll
-    for (int x = 0; x < kMoves; ++x) {
-      const int row = x * kRowsPer + t_row;                        // of the wave's 8
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + stage * kStageB + (8 * wave + x * kRowsPer) * kRowB);
-      const int kp = addr::chunk_k_pos(DT, 8 * wave + row, t_pos), vp = addr::chunk_v_pos(DT, 8 * wave + row, t_pos);
-      const char* zero = reinterpret_cast<const char*>(&g_zero16);
-      const char* ks = static_cast<const char*>(a.k) + (kb + row * a.k_rs + kp * 8) * 2;
-      const char* vs = static_cast<const char*>(a.v) + (vb + row * a.v_rs + vp * 8) * 2;
-      const bool seen = t0 + row >= tile.vs && t0 + row < tile.ve;
-      dma16_row(kp * 8 < a.D ? ks : zero, dst);
-      dma16_row(seen && vp * 8 < a.D ? vs : zero, dst + kTileB);
+  for (int x = 0; x < kMoves; ++x) {
+    const int row = x * kRowsPer + t_row;              // of 8: the permutation is the same for each 8 rows or repeats in 16
+    k_off[x] = static_cast<uint32_t>(row * a.k_rs) * 2;
+    v_off[x] = static_cast<uint32_t>(row * a.v_rs + addr::chunk_v_pos(DT, row, t_pos) * 8) * 2;
+  }
+  uint32_t k_pos[2][kMoves];
+#pragma unroll
+  for (int oc = 0; oc < 2; ++oc)
+#pragma unroll
+    for (int x = 0; x < kMoves; ++x) k_pos[oc][x] = k_off[x] + addr::chunk_k_pos(DT, 8 * oc + x * kRowsPer + t_row, t_pos) * 16;
+  const auto issue = [&](int kt, int stage) {
+    const int i32 = (kt - kt0) & 31;
+    if (i32 == 0) load_ids(kt);
+#pragma unroll
+    for (int oc = 0; oc < 2; ++oc) {
+      uint32_t pg, row8;
+      addr::div_by(static_cast<uint32_t>(octet_of(kt, oc)) >> 3, a.page_octets, a.page_magic, pg, row8);
+      const int64_t page = addr::paged_page(__builtin_amdgcn_readlane(ids, 2 * i32 + oc), a.num_pages);
+      const char* kbase = static_cast<const char*>(a.k) + (page * a.k_ps + h * a.k_hs + static_cast<int64_t>(row8 * 8) * a.k_rs) * 2;
+      const char* vbase = static_cast<const char*>(a.v) + (page * a.v_ps + h * a.v_hs + static_cast<int64_t>(row8 * 8) * a.v_rs) * 2;
+      const uint32_t dst = lds0 + stage * kStageB + (16 * wave_u + 8 * oc) * kRowB;
+      const int t0 = tile.first + kt * kCKeys + 16 * wave_u + 8 * oc;
+      if (plain && t0 >= tile.vs && t0 + 8 <= tile.ve) {
+#pragma unroll
+        for (int x = 0; x < kMoves; ++x) {
+          dma16_off(kbase, k_pos[oc][x], dst + x * 1024);
+          dma16_off(vbase, v_off[x], dst + x * 1024 + kTileB);
+        }
+      } else {
+        const char* zero = reinterpret_cast<const char*>(&g_zero16);
+#pragma unroll
+        for (int x = 0; x < kMoves; ++x) {
+          const int row = x * kRowsPer + t_row;
+          const int kp = addr::chunk_k_pos(DT, 8 * oc + row, t_pos), vp = addr::chunk_v_pos(DT, row, t_pos);
+          const bool seen = t0 + row >= tile.vs && t0 + row < tile.ve;
+          dma16_row(kp * 8 < a.D ? kbase + (row * a.k_rs + kp * 8) * 2 : zero, dst + x * 1024);
+          dma16_row(seen && vp * 8 < a.D ? vbase + (row * a.v_rs + vp * 8) * 2 : zero, dst + x * 1024 + kTileB);
+        }
+      }
     }
   };
 
@@ -250,14 +290,33 @@ __global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs
     const int tb = tile.first + kt * kCKeys;
     if (!wave_live || tb >= any_hi || tb + kCKeys <= any_lo) return;
     const char* base = lds + stage * kStageB;
+    // every read of K on its way before the first product
+    u32x4 kf[kSteps][2];
+#pragma unroll
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) kf[st][u] = ld16(base + k_at[st] + u * 32 * kRowB);
+    __builtin_amdgcn_sched_barrier(0);
     f32x16 sc[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int v = 0; v < 16; ++v) sc[u][v] = 0.f;
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) sc[u] = mfma32_bf16(ld16(base + k_at[st] + u * 32 * kRowB), qf[st], sc[u]);
-    }
+    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sc[u] = mfma32_bf16(kf[st][u], qf[st], sc[u]);
+    // the first half of V under the softmax
+    uint64_t vf[kDT][4][2];
+    const auto read_v = [&](int d) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) vf[d][g][x] = read_tr(base + v_at[d] + (g * 16 + 8 * x) * kRowB);
+    };
+#pragma unroll
+    for (int d = 0; d < kDT / 2; ++d) read_v(d);
+    __builtin_amdgcn_sched_barrier(0);
     if (tb + kCKeys > all_hi || tb < all_lo) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -300,37 +359,31 @@ __global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs
       for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
     }
 #pragma unroll
+    for (int d = kDT / 2; d < kDT; ++d) read_v(d);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
     for (int d = 0; d < kDT; ++d)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const uint64_t x0 = read_tr(base + v_at[d] + g * 16 * kRowB), x1 = read_tr(base + v_at[d] + (g * 16 + 8) * kRowB);
-        const u32x4 vf = {static_cast<uint32_t>(x0), static_cast<uint32_t>(x0 >> 32), static_cast<uint32_t>(x1),
-                          static_cast<uint32_t>(x1 >> 32)};
-        o[d] = mfma32_bf16(vf, pf[g], o[d]);
+        const u32x4 x = {static_cast<uint32_t>(vf[d][g][0]), static_cast<uint32_t>(vf[d][g][0] >> 32),
+                         static_cast<uint32_t>(vf[d][g][1]), static_cast<uint32_t>(vf[d][g][1] >> 32)};
+        o[d] = mfma32_bf16(x, pf[g], o[d]);
       }
   };
 
   // ---- the walk over the keys ---------------------------------------------------
   const int n = kt1 - kt0;
   if (n > 0) {
-    Id id = id_of(kt0);
-    issue(kt0, 0, id);
-    id = id_of(kt0 + 1);
-    if (n > 1) issue(kt0 + 1, 1, id);
-    id = id_of(kt0 + 2);
+    issue(kt0, 0);
     int stage = 0;
     for (int i = 0; i < n; ++i) {
       mem_fence_compiler();
-      if (i + 1 < n) __builtin_amdgcn_s_waitcnt(wait_vm_lds0(2 * kMoves));
-      else __builtin_amdgcn_s_waitcnt(wait_vm_lds0(0));
+      __builtin_amdgcn_s_waitcnt(wait_vm_lds0(0));                 // own transfers landed, own reads done
       __builtin_amdgcn_s_barrier();
       mem_fence_compiler();
-      if (i + 2 < n) {
-        issue(kt0 + i + 2, stage == 0 ? 2 : stage - 1, id);       // the stage of tile i - 1, which every wave is past
-        id = id_of(kt0 + i + 3);
-      }
+      if (i + 1 < n) issue(kt0 + i + 1, stage ^ 1);                // the stage of tile i - 1, which every wave is past
       compute(kt0 + i, stage);
-      stage = stage == kCStages - 1 ? 0 : stage + 1;
+      stage ^= 1;
     }
   }
 
@@ -351,7 +404,7 @@ __global__ __launch_bounds__(64 * kCWaves) void chunk_attention_kernel(PagedArgs
       }
     if (a.lse != nullptr && hl == 0) a.lse[tok * a.H + qh] = lsum == 0.f ? -INFINITY : (m + log2f(lsum)) * 0.6931471805599453f;
   } else {
-    float* p = a.chunk_ws + (h * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * addr::chunk_partial_floats(kChunkRows, DT);
+    float* p = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * addr::chunk_partial_floats(kChunkRows, DT);
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
 #pragma unroll
@@ -378,7 +431,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
   const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
   const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
   const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
-  const float* first = a.chunk_ws + (h * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * size;
+  const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * size;
   const int r0 = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
   for (int x = threadIdx.x; x < kJoinRows * (DT / 4); x += 256) {
     const int r = r0 + x / (DT / 4), d = (x % (DT / 4)) * 4;
@@ -403,8 +456,10 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
 
 }  // namespace
 
+int chunk_slots_for(int cus) { return 2 * cus; }
+
 int64_t chunk_workspace_bytes(int HK, int DT, int cus) {
-  return HK * addr::chunk_slots_per_head(HK, cus) * addr::chunk_partial_floats(kChunkRows, DT) * 4;
+  return static_cast<int64_t>(HK) * addr::chunk_slots_per_head(HK, chunk_slots_for(cus)) * addr::chunk_partial_floats(kChunkRows, DT) * 4;
 }
 
 // Tiles of a head at most: each sequence may end with a partial one.
@@ -422,7 +477,7 @@ int64_t chunk_grid(const PagedArgs& a) {
 void launch_chunk(const PagedArgs& a, int DT, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(chunk_grid(a)));
   // split tiles at most: half the partial results, as each has two or more
-  const int64_t split = std::min(chunk_most_tiles(a), addr::chunk_slots_per_head(a.HK, a.chunk_slots) / 2);
+  const int64_t split = std::min<int64_t>(chunk_most_tiles(a), addr::chunk_slots_per_head(a.HK, a.chunk_slots) / 2);
   const dim3 join(static_cast<unsigned>(split * (kChunkRows / kJoinRows)), static_cast<unsigned>(a.HK));
   if (DT == 64) {
     hipLaunchKernelGGL((chunk_attention_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);

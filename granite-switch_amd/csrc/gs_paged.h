@@ -30,6 +30,7 @@ struct PagedArgs {
   int window, parts;
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
   int chunk_slots;                  // workgroups that the chunk form fills
+  double chunk_share;               // HK / (2 chunk_slots)
   float scale_log2;
 };
 
@@ -44,8 +45,9 @@ __device__ __host__ __forceinline__ addr::PagedSeq seq_of_form(const PagedArgs& 
 }
 
 // The chunk form for the batch (bf16, head widths up to 128): true if launched.
-constexpr int kChunkRows = 256;
-constexpr int kChunkLeast = 8;      // key tiles of a part, at least
+constexpr int kChunkRows = 128;
+constexpr int kChunkLeast = 4;      // key tiles of a part, at least
+int chunk_slots_for(int cus);
 int64_t chunk_workspace_bytes(int HK, int DT, int cus);
 int64_t chunk_grid(const PagedArgs& a);
 void launch_chunk(const PagedArgs& a, int DT, hipStream_t st);

@@ -265,7 +265,7 @@ struct PagedBlock {
 constexpr int kPWaves = 4;
 
 template <bool BF16, int DT>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
   using F = PagedForm<BF16, DT>;
   constexpr int kUnit = F::kBlock * kPWaves;
   constexpr int kOC = F::kVN * F::kVW;              // O^T tiles of 16 columns
@@ -635,11 +635,12 @@ int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus
 // What follows from the sizes alone.
 void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, float scale) {
   a.parts = paged_parts_for(a.HK, cus);
-  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - 4096);
+  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
   a.page_octets = static_cast<uint32_t>(page_size / 8);
   a.page_magic = addr::div_magic(a.page_octets);
   a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) ? kRowFormRows : INT32_MAX;
-  a.chunk_slots = cus;
+  a.chunk_slots = chunk_slots_for(cus);
+  a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
   a.scale_log2 = scale * 1.44269504088896340736f;
 }
 
@@ -801,14 +802,14 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
 // The chunk form.
 template <int DT>
 void model_chunk(PagedModel& m, const PagedArgs& a) {
-  constexpr int kWaves = 8, kRowB = DT * 2, kTileB = 64 * kRowB, kRowsPer = 1024 / kRowB;
+  constexpr int kWaves = 4, kRowB = DT * 2, kTileB = 64 * kRowB, kRowsPer = 1024 / kRowB;
   // what the transfers leave in LDS, and what the operand reads take from it
   std::vector<int> k_lds(kTileB / 16, -1), v_lds(kTileB / 16, -1);
   for (int w = 0; w < kWaves; ++w)
-    for (int x = 0; x < 8 / kRowsPer; ++x)
+    for (int x = 0; x < 16 / kRowsPer; ++x)
       for (int l = 0; l < 64; ++l) {
-        const int row = 8 * w + x * kRowsPer + l / (64 / kRowsPer), pos = l % (64 / kRowsPer);
-        const int at = ((8 * w + x * kRowsPer) * kRowB + l * 16) / 16;
+        const int row = 16 * w + x * kRowsPer + l / (64 / kRowsPer), pos = l % (64 / kRowsPer);
+        const int at = ((16 * w + x * kRowsPer) * kRowB + l * 16) / 16;
         k_lds[at] = row * 64 + addr::chunk_k_pos(DT, row, pos);
         v_lds[at] = row * 64 + addr::chunk_v_pos(DT, row, pos);
       }
@@ -837,7 +838,7 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
   const int tq = addr::chunk_tq(kChunkRows, a.G);
   int64_t U2 = 0, n = 0, slots = 0, split = 0;
   for (int s = 0; s < a.B; ++s) U2 += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
-  const int pt = addr::chunk_part_tiles(U2, a.HK, a.chunk_slots, kChunkLeast);
+  const int pt = addr::chunk_part_tiles(U2, a.chunk_share, kChunkLeast);
   for (int s = 0; s < a.B && !m.bad; ++s) {
     const addr::PagedSeq sq = seq_of_form<true>(a, s);
     const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
@@ -860,8 +861,8 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
           m.in("q", tok * a.q_ts + head * a.q_hs, a.D, q_elems);
           m.in("out", tok * a.o_ts + head * a.o_hs, a.D, o_elems);
         }
-        for (int kt = 0; kt < nkt + 2 && nkt > 0; ++kt)       // ids are read up to two tiles past the last
-          for (int w = 0; w < kWaves; ++w) {
+        for (int kt = 0; kt < nkt + 2 && nkt > 0; ++kt)       // ids are read past the last tile, too
+          for (int w = 0; w < 8; ++w) {
             uint32_t pg, row;
             addr::div_by(static_cast<uint32_t>(addr::paged_octet(t.first + kt * 64 + 8 * w, t.ve)) >> 3, a.page_octets, a.page_magic, pg, row);
             m.in("page table row", pg, 1, max_pages);

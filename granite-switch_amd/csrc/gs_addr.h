@@ -341,7 +341,15 @@ GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin(U, pa
 // Chunk form: tiles of `tq` whole queries (tq * G rows), key tiles of 64.
 // Queries of a tile, with R rows in a tile.
 GS_HD int chunk_tq(int R, int G) { return R / G; }
-GS_HD int chunk_tiles(const PagedSeq& s, int tq) { return (s.n + tq - 1) / tq; }
+struct ChunkTq {
+  int tq;
+  uint32_t magic;                    // div_magic(tq)
+};
+GS_HD int chunk_tiles(const PagedSeq& s, const ChunkTq& q) {
+  uint32_t n, r;
+  div_by(static_cast<uint32_t>(s.n + q.tq - 1), static_cast<uint32_t>(q.tq), q.magic, n, r);
+  return static_cast<int>(n);
+}
 GS_HD PagedTile chunk_tile(const PagedSeq& s, int tq, int window, int j) {
   PagedTile t;
   t.i0 = j * tq;
@@ -356,10 +364,10 @@ GS_HD PagedTile chunk_tile(const PagedSeq& s, int tq, int window, int j) {
 GS_HD int chunk_key_tiles(const PagedTile& t) { return (t.ve - t.first + 63) / 64; }
 // The work of a sequence's tiles, taken as the mean of its first and its last
 // one's key tiles (half a tile at least), doubled: an integer.
-GS_HD int64_t chunk_work2(const PagedSeq& s, int tq, int window) {
-  const int nt = chunk_tiles(s, tq);
+GS_HD int64_t chunk_work2(const PagedSeq& s, const ChunkTq& q, int window) {
+  const int nt = chunk_tiles(s, q);
   if (nt == 0) return 0;
-  return static_cast<int64_t>(nt) * (chunk_key_tiles(chunk_tile(s, tq, window, 0)) + chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) + 1);
+  return static_cast<int64_t>(nt) * (chunk_key_tiles(chunk_tile(s, q.tq, window, 0)) + chunk_key_tiles(chunk_tile(s, q.tq, window, nt - 1)) + 1);
 }
 // Key tiles of a part for a batch of doubled work U2 a head: an equal share of
 // `slots` workgroups, and some at least.  share = HK / (2 slots).
@@ -368,11 +376,17 @@ GS_HD int chunk_part_tiles(int64_t U2, double share, int least) {
   return c < least ? least : static_cast<int>(c) + 1;
 }
 // Parts of each of a sequence's tiles: those whose last tile has two parts' key tiles or more are split.
-GS_HD int chunk_parts(const PagedSeq& s, int tq, int window, int part_tiles) {
-  const int nt = chunk_tiles(s, tq);
+GS_HD int chunk_parts(const PagedSeq& s, const ChunkTq& q, int window, int part_tiles, uint32_t part_magic) {
+  const int nt = chunk_tiles(s, q);
   if (nt == 0) return 0;
-  const int p = chunk_key_tiles(chunk_tile(s, tq, window, nt - 1)) / part_tiles;
-  return p < 1 ? 1 : p;
+  uint32_t p, r;
+  div_by(static_cast<uint32_t>(chunk_key_tiles(chunk_tile(s, q.tq, window, nt - 1))), static_cast<uint32_t>(part_tiles), part_magic, p, r);
+  return p < 1 ? 1 : static_cast<int>(p);
+}
+// Key tiles [k0, k1) of part p of n of a tile of nkt.
+GS_HD void chunk_part_range(int nkt, int p, int n, int& k0, int& k1) {
+  k0 = static_cast<int>(static_cast<int64_t>(nkt) * p / n);
+  k1 = static_cast<int>(static_cast<int64_t>(nkt) * (p + 1) / n);
 }
 // Partial results a head can have: U2 / part_tiles < 2 slots / HK of them at most,
 // as a split tile has part_tiles key tiles or more for each of its parts.

@@ -49,98 +49,116 @@ constexpr int wait_vm_lds0(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14
 
 struct ChunkItem {
   int s, j, part, nparts, slot;      // slot: its partial result's, or -1
+  addr::PagedSeq sq;
+};
+struct ChunkShared {
+  int64_t work[4];
+  int items[4], split[4];
+  int found[8];
 };
 
-// Workgroup-wide sums of two values a thread, and their exclusive prefixes.
-struct Scan2 {
-  int64_t before0, total0;
-  int64_t before1, total1;
-};
-__device__ __forceinline__ Scan2 scan2(int64_t a, int64_t b, int64_t (*red)[2]) {
-  const int l = lane_id(), wave = threadIdx.x >> 6;
-  int64_t ia = a, ib = b;
+__device__ __forceinline__ int wave_scan(int v) {
+  const int l = lane_id();
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t ua = __shfl_up(ia, d, 64), ub = __shfl_up(ib, d, 64);
-    if (l >= d) {
-      ia += ua;
-      ib += ub;
-    }
+    const int u = __shfl_up(v, d, 64);
+    if (l >= d) v += u;
   }
-  if (l == 63) {
-    red[wave][0] = ia;
-    red[wave][1] = ib;
-  }
-  __syncthreads();
-  Scan2 s{ia - a, 0, ib - b, 0};
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
-    if (w < wave) {
-      s.before0 += red[w][0];
-      s.before1 += red[w][1];
-    }
-    s.total0 += red[w][0];
-    s.total1 += red[w][1];
-  }
-  __syncthreads();
-  return s;
+  return v;
 }
 
 // The r-th part (JOIN: the r-th tile that was split) of the batch's tiles for one
-// head, in order of sequences, tiles and parts; r counts from the last where
-// `reverse`.  Every thread of the workgroup calls it.
+// head, in order of sequences, tiles and parts.  by_xcd: r is a workgroup of
+// (part, head) pairs.  Every thread of a workgroup of 256 calls it.
 template <bool JOIN>
-__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, int64_t r, bool by_xcd, int& h, int64_t (*red)[2], int* found) {
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
-  const int threads = blockDim.x;
-  const int run = (a.B + threads - 1) / threads;
-  const int s0 = min(static_cast<int>(threadIdx.x) * run, a.B), s1 = min(s0 + run, a.B);
-  int64_t work = 0;
-  for (int s = s0; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
-  const Scan2 w = scan2(work, 0, red);
-  const int pt = addr::chunk_part_tiles(w.total0, a.chunk_share, kChunkLeast);
-  int64_t items = 0, split = 0;                      // items: parts (JOIN: split tiles); split: partial results
-  for (int s = s0; s < s1; ++s) {
-    const addr::PagedSeq sq = seq_of_form<true>(a, s);
-    const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
-    items += JOIN ? (np > 1 ? nt : 0) : static_cast<int64_t>(nt) * np;
-    split += np > 1 ? static_cast<int64_t>(nt) * np : 0;
+__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, int r, bool by_xcd, int& h, ChunkShared& sh) {
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
+  const int run = (a.B + 255) >> 8;
+  const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
+  addr::PagedSeq first{0, 0, 0};                     // the thread's first sequence: its only one up to 256
+  if (s0 < s1) first = seq_of_form<true>(a, s0);
+  int64_t work = addr::chunk_work2(first, a.tq, a.window);
+  for (int s = s0 + 1; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), a.tq, a.window);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
+  if (l == 0) sh.work[wave] = work;
+  if (tid == 0) sh.found[0] = -1;
+  __syncthreads();
+  const int pt = addr::chunk_part_tiles(sh.work[0] + sh.work[1] + sh.work[2] + sh.work[3], a.chunk_share, kChunkLeast);
+  const uint32_t pm = addr::div_magic(pt);
+  struct Count {
+    int nt, np, items, split;                        // items: parts (JOIN: split tiles); split: partial results
+  };
+  const auto count = [&](const addr::PagedSeq& sq) {
+    Count c;
+    c.nt = addr::chunk_tiles(sq, a.tq);
+    c.np = addr::chunk_parts(sq, a.tq, a.window, pt, pm);
+    c.split = c.np > 1 ? c.nt * c.np : 0;
+    c.items = JOIN ? (c.np > 1 ? c.nt : 0) : c.nt * c.np;
+    return c;
+  };
+  const Count c0 = count(first);
+  int items = c0.items, split = c0.split;
+  for (int s = s0 + 1; s < s1; ++s) {
+    const Count c = count(seq_of_form<true>(a, s));
+    items += c.items;
+    split += c.split;
   }
-  const Scan2 c = scan2(items, split, red);
-  const int64_t n = c.total0;
+  int at = wave_scan(items), sl = wave_scan(split);
+  if (l == 63) {
+    sh.items[wave] = at;
+    sh.split[wave] = sl;
+  }
+  __syncthreads();
+  int n = 0;
+  at -= items;
+  sl -= split;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) {
+      at += sh.items[w];
+      sl += sh.split[w];
+    }
+    n += sh.items[w];
+  }
   if (by_xcd) {
     // consecutive workgroups go to the XCDs in turn: each XCD takes a contiguous
     // range of (head, part), so a sequence's tiles share one L2's keys
-    const int64_t total = n * a.HK, per = (total + 7) >> 3;
-    const int64_t t = (r & 7) * per + (r >> 3);
-    if ((r >> 3) >= per || t >= total) r = -1;
-    else {
-      h = static_cast<int>(t / n);
+    const int total = n * a.HK, per = (total + 7) >> 3;
+    const int t = (r & 7) * per + (r >> 3);
+    if ((r >> 3) >= per || t >= total) {
+      r = -1;
+    } else {
+      h = t / n;
       r = n - 1 - (t - h * n);                       // a sequence's last tiles, the longest, first
     }
   }
-  if (threadIdx.x == 0) found[0] = -1;
-  __syncthreads();
-  if (r >= 0 && r < n && r >= c.before0 && r < c.before0 + items) {
-    int64_t at = c.before0, sl = c.before1;
-    for (int s = s0; s < s1; ++s) {
-      const addr::PagedSeq sq = seq_of_form<true>(a, s);
-      const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
-      const int64_t here = JOIN ? (np > 1 ? nt : 0) : static_cast<int64_t>(nt) * np;
-      if (r < at + here) {
-        const int k = static_cast<int>(r - at);
-        found[0] = s;
-        found[1] = JOIN ? k : k / np;
-        found[2] = JOIN ? 0 : k % np;
-        found[3] = np;
-        found[4] = np > 1 ? static_cast<int>(sl + (JOIN ? static_cast<int64_t>(k) * np : k)) : -1;
+  if (r >= at && r < at + items) {
+    addr::PagedSeq sq = first;
+    for (int s = s0;; ++s) {
+      if (s > s0) sq = seq_of_form<true>(a, s);
+      const Count c = count(sq);
+      if (r < at + c.items) {
+        const int k = r - at;
+        sh.found[0] = s;
+        sh.found[1] = JOIN ? k : k / c.np;
+        sh.found[2] = JOIN ? 0 : k % c.np;
+        sh.found[3] = c.np;
+        sh.found[4] = c.np > 1 ? sl + (JOIN ? k * c.np : k) : -1;
+        sh.found[5] = sq.q0;
+        sh.found[6] = sq.n;
+        sh.found[7] = sq.len;
         break;
       }
-      at += here;
-      sl += np > 1 ? static_cast<int64_t>(nt) * np : 0;
+      at += c.items;
+      sl += c.split;
     }
   }
   __syncthreads();
-  return ChunkItem{found[0], found[1], found[2], found[3], found[4]};
+  const int* f = sh.found;
+  const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
+  h = u(h);
+  return ChunkItem{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), {u(f[5]), u(f[6]), u(f[7])}};
 }
 
 __device__ __forceinline__ void store4(const PagedArgs& a, int64_t e, f32x4 x) {
@@ -159,33 +177,28 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
   constexpr int kSteps = DT / 16;
   constexpr int kDT = DT / 32;                      // O^T tiles of 32 columns
   __shared__ __attribute__((aligned(1024))) char lds[kCStages * kStageB];
-  __shared__ int64_t s_red[kCWaves][2];
-  __shared__ int s_found[5];
+  __shared__ ChunkShared sh;
 
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 31, hl = l >> 5;
   int h = 0;
-  ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, s_red, s_found);
+  const ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, sh);
   if (it.s < 0) return;
-  h = __builtin_amdgcn_readfirstlane(h);             // uniform, and known to be from here on
-  const int s = __builtin_amdgcn_readfirstlane(it.s);
-  it.j = __builtin_amdgcn_readfirstlane(it.j);
-  it.part = __builtin_amdgcn_readfirstlane(it.part);
-  it.nparts = __builtin_amdgcn_readfirstlane(it.nparts);
-  it.slot = __builtin_amdgcn_readfirstlane(it.slot);
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
-  const addr::PagedSeq sq = seq_of_form<true>(a, s);
-  const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
+  const int s = it.s;
+  const addr::PagedSeq& sq = it.sq;
+  const addr::PagedTile tile = addr::chunk_tile(sq, a.tq.tq, a.window, it.j);
   const int nkt = addr::chunk_key_tiles(tile);
-  const int kt0 = static_cast<int>(static_cast<int64_t>(nkt) * it.part / it.nparts);
-  const int kt1 = static_cast<int>(static_cast<int64_t>(nkt) * (it.part + 1) / it.nparts);
+  int kt0 = 0, kt1 = nkt;
+  if (it.nparts > 1) addr::chunk_part_range(nkt, it.part, it.nparts, kt0, kt1);
 
   // ---- the lane's query row ---------------------------------------------------
   const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
   const int r = wave * 32 + lq;
   const bool live = r < nrow;
-  const int qi = tile.i0 + (live ? r / a.G : 0);
-  const int qh = h * a.G + (live ? r % a.G : 0);
+  uint32_t r_q, r_h;
+  addr::div_by(live ? r : 0, a.G, a.g_magic, r_q, r_h);
+  const int qi = tile.i0 + static_cast<int>(r_q);
+  const int qh = h * a.G + static_cast<int>(r_h);
   const int hi = live ? sq.len - sq.n + qi + 1 : 0;                // sees [lo, hi)
   const int lo = a.window > 0 ? hi - a.window : 0;
   const int64_t tok = sq.q0 + qi;
@@ -211,18 +224,25 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
   const int32_t* trow = a.table + static_cast<int64_t>(s) * a.ld_table;
   const int t_row = l / (64 / kRowsPer), t_pos = l % (64 / kRowsPer);   // the lane's row and LDS position in a transfer
-  // Page ids: lanes 2 i and 2 i + 1 hold those of the wave's 16 keys in tile i of
-  // 32, one load for 32 tiles (a load a tile would wait for the transfers issued
-  // before it).
+  // Where the wave's keys are: lanes 2 i and 2 i + 1 hold the byte offsets of the
+  // wave's 16 keys in tile i of 32 (its first 8 and its last 8), one load of page
+  // ids and one division for 32 tiles.
   const int wave_u = __builtin_amdgcn_readfirstlane(wave);
-  const auto octet_of = [&](int kt, int o) {
-    return addr::paged_octet(tile.first + kt * kCKeys + 16 * wave_u + 8 * o, tile.ve);
-  };
-  int ids = 0;
+  const char* k_head = static_cast<const char*>(a.k) + static_cast<int64_t>(h) * a.k_hs * 2;
+  const char* v_head = static_cast<const char*>(a.v) + static_cast<int64_t>(h) * a.v_hs * 2;
+  int64_t k_from = 0, v_from = 0;
   const auto load_ids = [&](int kt) {
-    uint32_t pg, row;
-    addr::div_by(static_cast<uint32_t>(octet_of(kt + (l >> 1), l & 1)) >> 3, a.page_octets, a.page_magic, pg, row);
-    ids = trow[pg];
+    uint32_t pg, row8;
+    const int oct = addr::paged_octet(tile.first + (kt + (l >> 1)) * kCKeys + 16 * wave + 8 * (l & 1), tile.ve);
+    addr::div_by(static_cast<uint32_t>(oct) >> 3, a.page_octets, a.page_magic, pg, row8);
+    const int64_t page = addr::paged_page(trow[pg], a.num_pages);
+    k_from = (page * a.k_ps + static_cast<int64_t>(row8 * 8) * a.k_rs) * 2;
+    v_from = (page * a.v_ps + static_cast<int64_t>(row8 * 8) * a.v_rs) * 2;
+  };
+  const auto lane64 = [](int64_t x, int i) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), i);
+    const uint32_t up = __builtin_amdgcn_readlane(static_cast<uint32_t>(static_cast<uint64_t>(x) >> 32), i);
+    return static_cast<int64_t>(lo | (static_cast<uint64_t>(up) << 32));
   };
   // Whole rows within 32-bit offsets: a transfer is a uniform base and these.
   const bool plain = a.D == DT && a.k_rs < (1 << 26) && a.v_rs < (1 << 26);
@@ -243,11 +263,8 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
     if (i32 == 0) load_ids(kt);
 #pragma unroll
     for (int oc = 0; oc < 2; ++oc) {
-      uint32_t pg, row8;
-      addr::div_by(static_cast<uint32_t>(octet_of(kt, oc)) >> 3, a.page_octets, a.page_magic, pg, row8);
-      const int64_t page = addr::paged_page(__builtin_amdgcn_readlane(ids, 2 * i32 + oc), a.num_pages);
-      const char* kbase = static_cast<const char*>(a.k) + (page * a.k_ps + h * a.k_hs + static_cast<int64_t>(row8 * 8) * a.k_rs) * 2;
-      const char* vbase = static_cast<const char*>(a.v) + (page * a.v_ps + h * a.v_hs + static_cast<int64_t>(row8 * 8) * a.v_rs) * 2;
+      const char* kbase = k_head + lane64(k_from, 2 * i32 + oc);
+      const char* vbase = v_head + lane64(v_from, 2 * i32 + oc);
       const uint32_t dst = lds0 + stage * kStageB + (16 * wave_u + 8 * oc) * kRowB;
       const int t0 = tile.first + kt * kCKeys + 16 * wave_u + 8 * oc;
       if (plain && t0 >= tile.vs && t0 + 8 <= tile.ve) {
@@ -286,17 +303,22 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
   for (int d = 0; d < kDT; ++d)
     v_at[d] = kTileB + v_row * kRowB + addr::chunk_v_pos(DT, v_row, 4 * d + 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
 
-  const auto compute = [&](int kt, int stage) {
+  // Tile kt, in `stage`; `next` tells whether tile kt + 1 is moved to the other one.
+  const auto compute = [&](int kt, int stage, bool next) {
     const int tb = tile.first + kt * kCKeys;
-    if (!wave_live || tb >= any_hi || tb + kCKeys <= any_lo) return;
     const char* base = lds + stage * kStageB;
-    // every read of K on its way before the first product
+    const bool active = wave_live && tb < any_hi && tb + kCKeys > any_lo;
+    // every read of K on its way before the first product, the transfers' addresses made meanwhile
     u32x4 kf[kSteps][2];
+    if (active) {
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st)
+      for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) kf[st][u] = ld16(base + k_at[st] + u * 32 * kRowB);
+        for (int u = 0; u < 2; ++u) kf[st][u] = ld16(base + k_at[st] + u * 32 * kRowB);
+    }
     __builtin_amdgcn_sched_barrier(0);
+    if (next) issue(kt + 1, stage ^ 1);              // the stage of tile kt - 1, which every wave is past
+    if (!active) return;
     f32x16 sc[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -381,8 +403,7 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
       __builtin_amdgcn_s_waitcnt(wait_vm_lds0(0));                 // own transfers landed, own reads done
       __builtin_amdgcn_s_barrier();
       mem_fence_compiler();
-      if (i + 1 < n) issue(kt0 + i + 1, stage ^ 1);                // the stage of tile i - 1, which every wave is past
-      compute(kt0 + i, stage);
+      compute(kt0 + i, stage, i + 1 < n);
       stage ^= 1;
     }
   }
@@ -421,14 +442,12 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
 constexpr int kJoinRows = 32;
 template <int DT>
 __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
-  __shared__ int64_t s_red[4][2];
-  __shared__ int s_found[5];
+  __shared__ ChunkShared sh;
   int h = blockIdx.y;
-  const ChunkItem it = find_chunk<true>(a, blockIdx.x / (kChunkRows / kJoinRows), false, h, s_red, s_found);
+  const ChunkItem it = find_chunk<true>(a, blockIdx.x / (kChunkRows / kJoinRows), false, h, sh);
   if (it.s < 0) return;
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
-  const addr::PagedSeq sq = seq_of_form<true>(a, it.s);
-  const addr::PagedTile tile = addr::chunk_tile(sq, tq, a.window, it.j);
+  const addr::PagedSeq& sq = it.sq;
+  const addr::PagedTile tile = addr::chunk_tile(sq, a.tq.tq, a.window, it.j);
   const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
   const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
   const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * size;

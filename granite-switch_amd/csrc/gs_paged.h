@@ -31,6 +31,8 @@ struct PagedArgs {
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
   int chunk_slots;                  // workgroups that the chunk form fills
   double chunk_share;               // HK / (2 chunk_slots)
+  addr::ChunkTq tq;                 // queries of a chunk tile
+  uint32_t g_magic;                 // div_magic(G)
   float scale_log2;
 };
 

@@ -641,6 +641,9 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
   a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
+  a.tq.tq = std::max(1, addr::chunk_tq(kChunkRows, a.G));
+  a.tq.magic = addr::div_magic(a.tq.tq);
+  a.g_magic = addr::div_magic(a.G);
   a.scale_log2 = scale * 1.44269504088896340736f;
 }
 
@@ -835,20 +838,20 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
   const int64_t k_elems = extent3(a.num_pages, a.k_ps, a.HK, a.k_hs, page_rows, a.k_rs, a.D);
   const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
   const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D), o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
+  const addr::ChunkTq& tq = a.tq;
   int64_t U2 = 0, n = 0, slots = 0, split = 0;
   for (int s = 0; s < a.B; ++s) U2 += addr::chunk_work2(seq_of_form<true>(a, s), tq, a.window);
   const int pt = addr::chunk_part_tiles(U2, a.chunk_share, kChunkLeast);
   for (int s = 0; s < a.B && !m.bad; ++s) {
     const addr::PagedSeq sq = seq_of_form<true>(a, s);
-    const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt);
+    const int nt = addr::chunk_tiles(sq, tq), np = addr::chunk_parts(sq, tq, a.window, pt, addr::div_magic(pt));
     n += static_cast<int64_t>(nt) * np;
     if (np > 1) {
       slots += static_cast<int64_t>(nt) * np;
       split += nt;
     }
     for (int j = 0; j < nt && !m.bad; ++j) {
-      const addr::PagedTile t = addr::chunk_tile(sq, tq, a.window, j);
+      const addr::PagedTile t = addr::chunk_tile(sq, tq.tq, a.window, j);
       const int nkt = addr::chunk_key_tiles(t);
       const int nrow = (t.i1 - t.i0 + 1) * a.G;
       if (nrow < 1 || nrow > kChunkRows) m.fail("rows of a tile", 0, nrow, kChunkRows);

@@ -335,8 +335,9 @@ GS_HD int paged_octet(int tok, int ve) { return imin(tok, (ve - 1) & ~7); }
 GS_HD int paged_page(int id, int num_pages) {
   return static_cast<uint32_t>(id) < static_cast<uint32_t>(num_pages) ? id : 0;
 }
-// Parts that have work: one unit at least each.
-GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin(U, parts)); }
+// Parts that have work: kLeastUnits units at least each, or all in one.
+constexpr int kLeastUnits = 2;
+GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin((U + kLeastUnits - 1) / kLeastUnits, parts)); }
 
 // Chunk form: tiles of `tq` whole queries (tq * G rows), key tiles of 64.
 // Queries of a tile, with R rows in a tile.

@@ -1,6 +1,8 @@
 // What the kernels over a paged cache share (gs_paged.hip, gs_chunk.hip).
 #pragma once
 
+#include <vector>
+
 #include "gs_addr.h"
 #include "gs_common.h"
 
@@ -20,9 +22,11 @@ struct PagedArgs {
   const int32_t* lens;
   const int32_t* cu;
   float* lse;                       // [T, H] or NULL
-  float* ws;                        // row form: partial results, then join
-  int4* join;                       // [parts * HK]: the item a part completes, or none
+  float* ws;                        // row form: partial results
   float* chunk_ws;                  // chunk form: partial results
+  int* tickets;                     // zero between calls, as the two below
+  int* chunk_count;                 // one for each of the chunk form's partial results: done with the tile that starts there
+  int* row_count;                   // [parts * HK]: workgroups that are done with the item that a part ends
   int64_t max_len;
   uint32_t page_octets, page_magic;
   int num_pages;
@@ -47,11 +51,35 @@ __device__ __host__ __forceinline__ addr::PagedSeq seq_of_form(const PagedArgs& 
 }
 
 // The chunk form for the batch (bf16, head widths up to 128): true if launched.
+constexpr int kMostParts = 512;     // of a batch for one head, row form
 constexpr int kChunkRows = 128;
 constexpr int kChunkLeast = 4;      // key tiles of a part, at least
 int chunk_slots_for(int cus);
 int64_t chunk_workspace_bytes(int HK, int DT, int cus);
 int64_t chunk_grid(const PagedArgs& a);
 void launch_chunk(const PagedArgs& a, int DT, hipStream_t st);
+
+// Strides that keep rows on 16-byte boundaries.
+inline bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 && a % n == 0 && b % n == 0; }
+
+// ---------------------------------------------------------------------------
+// Address model: the kernels' global accesses for given tables, replayed with
+// the kernels' own arithmetic.
+// ---------------------------------------------------------------------------
+struct PagedModel {
+  int64_t bad = 0, checked = 0;
+  std::vector<char> rows;                           // output rows written
+  char msg[256] = "";
+  void fail(const char* what, int64_t at, int64_t n, int64_t cap) {
+    if (bad++ == 0) snprintf(msg, sizeof(msg), "%s: elements [%lld, %lld) of %lld", what, (long long)at, (long long)(at + n), (long long)cap);
+  }
+  void in(const char* what, int64_t at, int64_t n, int64_t cap) {
+    ++checked;
+    if (at < 0 || at + n > cap) fail(what, at, n, cap);
+  }
+};
+inline int64_t extent3(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t cols) {
+  return (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + cols;
+}
 
 }  // namespace gs

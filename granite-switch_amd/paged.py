@@ -215,8 +215,9 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
 # Attention
 # ---------------------------------------------------------------------------
 # One workspace for each stream: calls on one stream follow each other, calls on
-# different streams may overlap.  A replaced buffer is kept (``_retired``): a
-# captured graph may still hold its address.
+# different streams may overlap.  Its counters start at zero and every call leaves
+# them so.  A replaced buffer is kept (``_retired``): a captured graph may still
+# hold its address.
 _workspaces: dict = {}
 _retired: list = []
 
@@ -227,10 +228,10 @@ def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
     if buf is None or buf.numel() < need:
         if torch.cuda.is_current_stream_capturing():
             # a buffer of the graph's own: it lives as long as the graph's pool does
-            return torch.empty(need, dtype=torch.uint8, device=device)
+            return torch.zeros(need, dtype=torch.uint8, device=device)
         if buf is not None:
             _retired.append(buf)
-        buf = _workspaces[key] = torch.empty(need, dtype=torch.uint8, device=device)
+        buf = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
     return buf
 
 
@@ -264,7 +265,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     window     > 0: a row sees the last ``window`` tokens up to its own
     lse        [T, heads] float32: receives the log of each softmax's total
     max_q      the most query rows of a sequence where the caller knows it
-    workspace  uint8, ``workspace_bytes`` long (one per stream is kept when None)
+    workspace  uint8, ``workspace_bytes`` long, zeroed before its first call and used
+               by nothing else (one per stream is kept when None)
 
     A row that sees nothing (an empty sequence) gives zeros.
     """

@@ -389,6 +389,21 @@ GS_HD void chunk_part_range(int nkt, int p, int n, int& k0, int& k1) {
   k0 = static_cast<int>(static_cast<int64_t>(nkt) * p / n);
   k1 = static_cast<int>(static_cast<int64_t>(nkt) * (p + 1) / n);
 }
+// Parts for each head of the row form on `wgs` workgroups.
+GS_HD int ragged_row_parts(int wgs, int HK, int most) { return imin(wgs / HK, most); }
+// XCD x's tickets: a contiguous eighth of the (head, part) pairs.
+struct Tickets {
+  int first, n;
+};
+GS_HD Tickets tickets_of(int x, int pairs) {
+  Tickets t;
+  const int per = (pairs + 7) >> 3;
+  t.first = x * per;
+  const int left = pairs - t.first;
+  t.n = left < 0 ? 0 : imin(left, per);
+  return t;
+}
+constexpr int cmax(int a, int b) { return a > b ? a : b; }
 // Partial results a head can have: U2 / part_tiles < 2 slots / HK of them at most,
 // as a split tile has part_tiles key tiles or more for each of its parts.
 GS_HD int chunk_slots_per_head(int HK, int slots) { return (2 * slots + HK - 1) / HK + 1; }

@@ -1,6 +1,13 @@
-// Attention of query chunks over a paged cache (bf16, head widths up to 128):
-// the form of gs_paged_attention for sequences of many rows.
+// Attention of a ragged bf16 batch over a paged cache (head widths up to 128): one
+// launch in which sequences of many rows take the chunk form here and those of few
+// (a decode row among prompts) the row form (gs_paged_rows.h).
 //
+// Two workgroups share a compute unit: at the start one has a part of the row form,
+// which streams the cache, and one multiplies.  The chunk form's parts are tickets
+// that its workgroups take until none are left, a sequence's last tiles, the
+// longest, first.
+//
+// The chunk form.
 // A workgroup of 4 waves takes 128 (query, head) rows of one sequence and
 // key/value head -- 32 queries where 4 query heads share it, so the group's
 // heads read K and V once -- and walks the keys in tiles of 64.  Keys and values
@@ -15,7 +22,7 @@
 // (its keys permuted alike: V^T is read transposed from LDS, 4 keys at a time).
 #include <algorithm>
 
-#include "gs_paged.h"
+#include "gs_paged_rows.h"
 
 namespace gs {
 namespace {
@@ -48,13 +55,15 @@ __device__ __forceinline__ void dma16_off(const char* base, uint32_t off, uint32
 constexpr int wait_vm_lds0(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
 
 struct ChunkItem {
-  int s, j, part, nparts, slot;      // slot: its partial result's, or -1
+  int s, j, part, nparts, slot;      // slot: of the tile's first partial result, or -1
+  int order;                         // of the tile among the split ones
   addr::PagedSeq sq;
 };
 struct ChunkShared {
-  int64_t work[4];
-  int items[4], split[4];
-  int found[8];
+  int at[257], split_at[256], tile_at[256];   // parts, partial results and split tiles before a thread's sequences
+  int64_t work[kCWaves];
+  int items[kCWaves], split[kCWaves], tiles[kCWaves];
+  int found[9];
 };
 
 __device__ __forceinline__ int wave_scan(int v) {
@@ -67,108 +76,123 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The r-th part (JOIN: the r-th tile that was split) of the batch's tiles for one
-// head, in order of sequences, tiles and parts.  by_xcd: r is a workgroup of
-// (part, head) pairs.  Every thread of a workgroup of 256 calls it.
-template <bool JOIN>
-__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, int r, bool by_xcd, int& h, ChunkShared& sh) {
+// How many key tiles a part of a split tile has.
+struct ChunkSplit {
+  int tiles;
+  uint32_t magic;
+};
+struct ChunkCount {
+  int nt, np, items, split, tiles;   // tiles, parts of each; parts, partial results and split tiles
+};
+__device__ __forceinline__ ChunkCount chunk_count(const PagedArgs& a, const ChunkSplit& c, const addr::PagedSeq& sq) {
+  ChunkCount k;
+  k.nt = addr::chunk_tiles(sq, a.tq);
+  k.np = addr::chunk_parts(sq, a.tq, a.window, c.tiles, c.magic);
+  k.items = k.nt * k.np;
+  k.split = k.np > 1 ? k.items : 0;
+  k.tiles = k.np > 1 ? k.nt : 0;
+  return k;
+}
+// The batch's parts (a tile of a sequence, or one of those it is split into) for
+// one head, in order of sequences, tiles and parts; after row_scan.
+__device__ __forceinline__ ChunkSplit chunk_scan(const PagedArgs& a, const Schedule& sd, ChunkShared& sh) {
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int run = (a.B + 255) >> 8;
   const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
-  addr::PagedSeq first{0, 0, 0};                     // the thread's first sequence: its only one up to 256
-  if (s0 < s1) first = seq_of_form<true>(a, s0);
+  const addr::PagedSeq first = first_seq<true>(a, sd);
   int64_t work = addr::chunk_work2(first, a.tq, a.window);
   for (int s = s0 + 1; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), a.tq, a.window);
 #pragma unroll
   for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
   if (l == 0) sh.work[wave] = work;
-  if (tid == 0) sh.found[0] = -1;
   __syncthreads();
-  const int pt = addr::chunk_part_tiles(sh.work[0] + sh.work[1] + sh.work[2] + sh.work[3], a.chunk_share, kChunkLeast);
-  const uint32_t pm = addr::div_magic(pt);
-  struct Count {
-    int nt, np, items, split;                        // items: parts (JOIN: split tiles); split: partial results
-  };
-  const auto count = [&](const addr::PagedSeq& sq) {
-    Count c;
-    c.nt = addr::chunk_tiles(sq, a.tq);
-    c.np = addr::chunk_parts(sq, a.tq, a.window, pt, pm);
-    c.split = c.np > 1 ? c.nt * c.np : 0;
-    c.items = JOIN ? (c.np > 1 ? c.nt : 0) : c.nt * c.np;
-    return c;
-  };
-  const Count c0 = count(first);
-  int items = c0.items, split = c0.split;
+  work = 0;
+#pragma unroll
+  for (int w = 0; w < kCWaves; ++w) work += sh.work[w];
+  ChunkSplit c;
+  c.tiles = addr::chunk_part_tiles(work, a.chunk_share, kChunkLeast);
+  c.magic = addr::div_magic(c.tiles);
+  const ChunkCount k0 = chunk_count(a, c, first);
+  int items = k0.items, split = k0.split, tiles = k0.tiles;
   for (int s = s0 + 1; s < s1; ++s) {
-    const Count c = count(seq_of_form<true>(a, s));
-    items += c.items;
-    split += c.split;
+    const ChunkCount k = chunk_count(a, c, seq_of_form<true>(a, s));
+    items += k.items;
+    split += k.split;
+    tiles += k.tiles;
   }
-  int at = wave_scan(items), sl = wave_scan(split);
+  int at = wave_scan(items), sl = wave_scan(split), tl = wave_scan(tiles);
   if (l == 63) {
     sh.items[wave] = at;
     sh.split[wave] = sl;
+    sh.tiles[wave] = tl;
   }
   __syncthreads();
-  int n = 0;
-  at -= items;
-  sl -= split;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kCWaves; ++w)
     if (w < wave) {
       at += sh.items[w];
       sl += sh.split[w];
+      tl += sh.tiles[w];
     }
-    n += sh.items[w];
+  sh.at[tid] = at - items;
+  sh.split_at[tid] = sl - split;
+  sh.tile_at[tid] = tl - tiles;
+  if (tid == 255) {
+    sh.at[256] = at;
+    if (blockIdx.x == 0) a.chunk_list[0].x = tl;      // for the join, with the entries that the tiles' first parts write
   }
-  if (by_xcd) {
-    // consecutive workgroups go to the XCDs in turn: each XCD takes a contiguous
-    // range of (head, part), so a sequence's tiles share one L2's keys
-    const int total = n * a.HK, per = (total + 7) >> 3;
-    const int t = (r & 7) * per + (r >> 3);
-    if ((r >> 3) >= per || t >= total) {
-      r = -1;
-    } else {
-      h = t / n;
-      r = n - 1 - (t - h * n);                       // a sequence's last tiles, the longest, first
-    }
-  }
-  if (r >= at && r < at + items) {
-    addr::PagedSeq sq = first;
-    for (int s = s0;; ++s) {
-      if (s > s0) sq = seq_of_form<true>(a, s);
-      const Count c = count(sq);
-      if (r < at + c.items) {
-        const int k = r - at;
+  __syncthreads();
+  return c;
+}
+
+// Part r (0 <= r < sh.at[256]) of the batch.  Every thread of the workgroup calls it.
+__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, const ChunkSplit& c, int r, const Schedule& sd, ChunkShared& sh) {
+  const int tid = threadIdx.x;
+  if (r >= sh.at[tid] && r < sh.at[tid + 1]) {
+    const int run = (a.B + 255) >> 8;
+    int at = sh.at[tid], sl = sh.split_at[tid], tl = sh.tile_at[tid], s = tid * run;
+    addr::PagedSeq sq = first_seq<true>(a, sd);
+    for (;;) {
+      const ChunkCount k = chunk_count(a, c, sq);
+      if (r < at + k.items) {
+        const int x = r - at;
+        const int j = k.np > 1 ? x / k.np : x;
         sh.found[0] = s;
-        sh.found[1] = JOIN ? k : k / c.np;
-        sh.found[2] = JOIN ? 0 : k % c.np;
-        sh.found[3] = c.np;
-        sh.found[4] = c.np > 1 ? sl + (JOIN ? k * c.np : k) : -1;
+        sh.found[1] = j;
+        sh.found[2] = x - j * k.np;
+        sh.found[3] = k.np;
+        sh.found[4] = k.np > 1 ? sl + j * k.np : -1;
         sh.found[5] = sq.q0;
         sh.found[6] = sq.n;
         sh.found[7] = sq.len;
+        sh.found[8] = tl + j;
         break;
       }
-      at += c.items;
-      sl += c.split;
+      at += k.items;
+      sl += k.split;
+      tl += k.tiles;
+      sq = seq_of_form<true>(a, ++s);
     }
   }
   __syncthreads();
   const int* f = sh.found;
   const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
-  h = u(h);
-  return ChunkItem{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), {u(f[5]), u(f[6]), u(f[7])}};
+  return ChunkItem{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), u(f[8]), {u(f[5]), u(f[6]), u(f[7])}};
 }
 
-__device__ __forceinline__ void store4(const PagedArgs& a, int64_t e, f32x4 x) {
-  uint32_t* p = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + e);
-  const uint64_t w = pack_bf16x2(x[0], x[1]) | (static_cast<uint64_t>(pack_bf16x2(x[2], x[3])) << 32);
-  *reinterpret_cast<uint64_t*>(p) = w;
+// The maximum, or the sum, over a lane and the one 32 lanes away.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// One part: 128 rows of a sequence and head h over its key tiles.
 template <int DT>
-__global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedArgs a) {
+__device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& it, int h, char* lds) {
   constexpr int kRowB = DT * 2;                     // bytes of a key row in LDS
   constexpr int kTileB = kCKeys * kRowB;            // of a stage's keys, and of its values
   constexpr int kStageB = 2 * kTileB;
@@ -176,14 +200,9 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
   constexpr int kMoves = 8 / kRowsPer;              // transfers for 8 keys (as many for the values); a wave moves 16 keys
   constexpr int kSteps = DT / 16;
   constexpr int kDT = DT / 32;                      // O^T tiles of 32 columns
-  __shared__ __attribute__((aligned(1024))) char lds[kCStages * kStageB];
-  __shared__ ChunkShared sh;
 
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 31, hl = l >> 5;
-  int h = 0;
-  const ChunkItem it = find_chunk<false>(a, blockIdx.x, true, h, sh);
-  if (it.s < 0) return;
   const int s = it.s;
   const addr::PagedSeq& sq = it.sq;
   const addr::PagedTile tile = addr::chunk_tile(sq, a.tq.tq, a.window, it.j);
@@ -353,7 +372,7 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[u][v]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * a.scale_log2;
+    mx = max_halves(mx) * a.scale_log2;
     // the reference point follows the maximum once it has grown by 2^8: the sums
     // stay far from their limits, and o is rarely scaled
     if (__any(mx > m + 8.f)) {
@@ -409,23 +428,33 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
   }
 
   // ---- results --------------------------------------------------------------------
-  lsum += __shfl_xor(lsum, 32, 64);
-  if (!live) return;
+  lsum = sum_halves(lsum);
   if (it.slot < 0) {
     const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
-    const int64_t e = tok * a.o_ts + static_cast<int64_t>(qh) * a.o_hs;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + tok * a.o_ts + static_cast<int64_t>(qh) * a.o_hs;
+    // A lane has columns 8 k + 4 hl .. + 3 of its row for every k: swapped between the
+    // two halves of the wave, 8 consecutive ones of every other k.
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
 #pragma unroll
-      for (int v = 0; v < 16; v += 4) {
-        const int col = 32 * d + mfma32_row(v, l);
-        f32x4 x = {o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
-        x = lsum == 0.f ? f32x4{0, 0, 0, 0} : x * inv;
-        if (col < a.D) store4(a, e + col, x);
+      for (int v = 0; v < 16; v += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = lsum == 0.f ? 0.f : o[d][v + 2 * i] * inv, y = lsum == 0.f ? 0.f : o[d][v + 2 * i + 1] * inv;
+          w[i] = pack_bf16x2(x, y);
+        }
+        const auto p0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto p1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        const int col = 32 * d + 2 * v + 8 * hl;
+        if (live && col < a.D) *reinterpret_cast<u32x4*>(out + col) = u32x4{p0[0], p1[0], p0[1], p1[1]};
       }
-    if (a.lse != nullptr && hl == 0) a.lse[tok * a.H + qh] = lsum == 0.f ? -INFINITY : (m + log2f(lsum)) * 0.6931471805599453f;
-  } else {
-    float* p = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * addr::chunk_partial_floats(kChunkRows, DT);
+    if (a.lse != nullptr && hl == 0 && live) a.lse[tok * a.H + qh] = lsum == 0.f ? -INFINITY : (m + log2f(lsum)) * 0.6931471805599453f;
+    return;
+  }
+  float* p = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot + it.part) *
+                              addr::chunk_partial_floats(kChunkRows, DT);
+  if (live) {
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
 #pragma unroll
@@ -436,40 +465,87 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void chunk_attention_kernel(PagedA
       p[kChunkRows * (DT + 1) + r] = lsum;
     }
   }
+  if (it.part == 0 && h == 0 && tid == 0) a.chunk_list[1 + it.order] = make_int4(sq.q0 + tile.i0, nrow, it.nparts, it.slot);
 }
 
-// The parts of a tile joined, in the order of their keys: grid (split tiles x row groups, heads).
-constexpr int kJoinRows = 32;
+// The split tiles' parts, joined in the order of their keys: workgroups take (tile,
+// 16 rows, head) in turn, a thread 4 columns of a row, 8 parts' loads in flight.  (A
+// workgroup that joined its tile at the end of the launch above would read all its
+// parts alone: 14 parts of 128 rows took it 50 us.)
+constexpr int kJoinRows = 16;
 template <int DT>
 __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
-  __shared__ ChunkShared sh;
-  int h = blockIdx.y;
-  const ChunkItem it = find_chunk<true>(a, blockIdx.x / (kChunkRows / kJoinRows), false, h, sh);
-  if (it.s < 0) return;
-  const addr::PagedSeq& sq = it.sq;
-  const addr::PagedTile tile = addr::chunk_tile(sq, a.tq.tq, a.window, it.j);
-  const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
+  constexpr int kBatch = 8;
+  constexpr int kGroups = kChunkRows / kJoinRows;
   const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
-  const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot) * size;
-  const int r0 = (blockIdx.x % (kChunkRows / kJoinRows)) * kJoinRows;
-  for (int x = threadIdx.x; x < kJoinRows * (DT / 4); x += 256) {
-    const int r = r0 + x / (DT / 4), d = (x % (DT / 4)) * 4;
-    if (r >= nrow) break;
-    float M = -INFINITY;
-    for (int p = 0; p < it.nparts; ++p) M = fmaxf(M, first[p * size + kChunkRows * DT + r]);
-    const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    f32x4 acc = {0, 0, 0, 0};
-    for (int p = 0; p < it.nparts; ++p) {
-      const float f = exp2f(first[p * size + kChunkRows * DT + r] - ms);
-      L += f * first[p * size + kChunkRows * (DT + 1) + r];
-      acc += f * *reinterpret_cast<const f32x4*>(first + p * size + r * DT + d);
+  const int total = a.chunk_list[0].x * kGroups * a.HK;
+  for (int w = blockIdx.x; w < total; w += gridDim.x) {
+    const int h = w % a.HK, g = (w / a.HK) % kGroups;
+    const int4 e = a.chunk_list[1 + w / (a.HK * kGroups)];
+    const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + e.w) * size;
+    for (int x = threadIdx.x; x < kJoinRows * (DT / 4); x += 256) {
+      const int jr = g * kJoinRows + x / (DT / 4), d = (x % (DT / 4)) * 4;
+      if (jr >= e.y) break;
+      float M = -INFINITY, L = 0.f;
+      f32x4 acc = {0, 0, 0, 0};
+      for (int p0 = 0; p0 < e.z; p0 += kBatch) {
+        f32x4 px[kBatch];
+        float pm[kBatch], pl[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float* p = first + min(p0 + k, e.z - 1) * size;
+          px[k] = *reinterpret_cast<const f32x4*>(p + jr * DT + d);
+          pm[k] = p[kChunkRows * DT + jr];
+          pl[k] = p[kChunkRows * (DT + 1) + jr];
+        }
+        float Mn = M;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) Mn = fmaxf(Mn, pm[k]);
+        const float ms = Mn == -INFINITY ? 0.f : Mn;
+        const float f0 = __builtin_amdgcn_exp2f(M - ms);           // M = -inf: nothing summed yet
+        L *= f0;
+        acc *= f0;
+        M = Mn;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const float f = p0 + k < e.z ? __builtin_amdgcn_exp2f(pm[k] - ms) : 0.f;
+          L += f * pl[k];
+          acc += f * px[k];
+        }
+      }
+      uint32_t jq, jh;
+      addr::div_by(jr, a.G, a.g_magic, jq, jh);
+      row_store<true>(a, e.x + static_cast<int>(jq), h * a.G + static_cast<int>(jh), d, acc, M, L);
     }
-    if (d >= a.D) continue;
-    const int64_t tok = sq.q0 + tile.i0 + r / a.G;
-    const int head = h * a.G + r % a.G;
-    store4(a, tok * a.o_ts + static_cast<int64_t>(head) * a.o_hs + d, L == 0.f ? f32x4{0, 0, 0, 0} : acc * (1.0f / L));
-    if (a.lse != nullptr && d == 0) a.lse[tok * a.H + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+  }
+}
+
+// Grid: `third` workgroups with a chunk part each, `third` with one of the row form,
+// then the rest of the chunk parts.
+template <int DT>
+__global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_kernel(PagedArgs) {
+  __shared__ __attribute__((aligned(1024))) char lds[addr::cmax(kCStages * 2 * kCKeys * DT * 2, static_cast<int>(sizeof(RowShared<DT>)))];
+  __shared__ ChunkShared sh;
+  __shared__ Schedule sd;
+  load_schedule(fresh_args(), sd);
+  const int w = blockIdx.x;
+  const int third = fresh_args().ragged_third;
+  if (w >= third && w < 2 * third) {
+    const PagedArgs& a = fresh_args();
+    row_scan<true, DT>(a, sd);
+    const int parts = addr::paged_parts(sd.row_at[256], addr::ragged_row_parts(third, a.HK, a.parts));
+    if (w - third < parts * a.HK) row_part<true, DT>(a, sd, (w - third) / a.HK, parts, (w - third) % a.HK, *reinterpret_cast<RowShared<DT>*>(lds));
+  } else {
+    const PagedArgs& a = fresh_args();
+    const ChunkSplit cs = chunk_scan(a, sd, sh);
+    const int n = __builtin_amdgcn_readfirstlane(sh.at[256]);
+    const addr::Tickets t = addr::tickets_of(w & 7, n * a.HK);
+    const int i = (w < third ? w : w - third) >> 3;
+    if (i >= t.n) return;
+    const int c = t.first + i;
+    const int h = c / n;
+    const ChunkItem it = find_chunk(a, cs, n - 1 - (c - h * n), sd, sh);
+    chunk_part<DT>(fresh_args(), it, h, lds);
   }
 }
 
@@ -477,32 +553,30 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
 
 int chunk_slots_for(int cus) { return 2 * cus; }
 
+int64_t chunk_list_floats(int HK, int cus) { return 4 * (1 + static_cast<int64_t>(addr::chunk_slots_per_head(HK, chunk_slots_for(cus))) / 2); }
+
 int64_t chunk_workspace_bytes(int HK, int DT, int cus) {
   return static_cast<int64_t>(HK) * addr::chunk_slots_per_head(HK, chunk_slots_for(cus)) * addr::chunk_partial_floats(kChunkRows, DT) * 4;
 }
 
 // Tiles of a head at most: each sequence may end with a partial one.
 static int64_t chunk_most_tiles(const PagedArgs& a) {
-  const int tq = addr::chunk_tq(kChunkRows, a.G);
-  return a.T / tq + std::min(a.B, a.T);
+  return a.T / a.tq.tq + std::min(a.B, a.T);
 }
 
 // Parts at most: tiles, and the split tiles' parts.
-int64_t chunk_grid(const PagedArgs& a) {
-  const int64_t per_head = chunk_most_tiles(a) + addr::chunk_slots_per_head(a.HK, a.chunk_slots);
-  return 8 * ((per_head * a.HK + 7) / 8);
+int64_t chunk_most_parts(const PagedArgs& a) {
+  return chunk_most_tiles(a) + addr::chunk_slots_per_head(a.HK, a.chunk_slots);
 }
 
-void launch_chunk(const PagedArgs& a, int DT, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(chunk_grid(a)));
-  // split tiles at most: half the partial results, as each has two or more
-  const int64_t split = std::min<int64_t>(chunk_most_tiles(a), addr::chunk_slots_per_head(a.HK, a.chunk_slots) / 2);
-  const dim3 join(static_cast<unsigned>(split * (kChunkRows / kJoinRows)), static_cast<unsigned>(a.HK));
+void launch_ragged(const PagedArgs& a, int DT, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.ragged_third + std::max<int64_t>(a.ragged_third, (chunk_most_parts(a) * a.HK + 7) & ~int64_t(7))));
+  const dim3 join(static_cast<unsigned>(a.chunk_slots));
   if (DT == 64) {
-    hipLaunchKernelGGL((chunk_attention_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);
+    hipLaunchKernelGGL((ragged_attention_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);
     hipLaunchKernelGGL((chunk_join_kernel<64>), join, dim3(256), 0, st, a);
   } else {
-    hipLaunchKernelGGL((chunk_attention_kernel<128>), grid, dim3(64 * kCWaves), 0, st, a);
+    hipLaunchKernelGGL((ragged_attention_kernel<128>), grid, dim3(64 * kCWaves), 0, st, a);
     hipLaunchKernelGGL((chunk_join_kernel<128>), join, dim3(256), 0, st, a);
   }
 }

@@ -24,9 +24,8 @@ struct PagedArgs {
   float* lse;                       // [T, H] or NULL
   float* ws;                        // row form: partial results
   float* chunk_ws;                  // chunk form: partial results
-  int* tickets;                     // zero between calls, as the two below
-  int* chunk_count;                 // one for each of the chunk form's partial results: done with the tile that starts there
-  int* row_count;                   // [parts * HK]: workgroups that are done with the item that a part ends
+  int4* chunk_list;                 // the split tiles: their number, then first query, rows, parts and first partial result of each
+  int* row_count;                   // [parts * HK]: workgroups done with the item that a part ends; zero between calls
   int64_t max_len;
   uint32_t page_octets, page_magic;
   int num_pages;
@@ -34,30 +33,48 @@ struct PagedArgs {
   int window, parts;
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
   int chunk_slots;                  // workgroups that the chunk form fills
+  int ragged_third;                 // workgroups of a third of a ragged launch, a multiple of 8
   double chunk_share;               // HK / (2 chunk_slots)
   addr::ChunkTq tq;                 // queries of a chunk tile
   uint32_t g_magic;                 // div_magic(G)
   float scale_log2;
 };
 
-// Sequences of a batch that a form takes: of at most `limit` rows, or of more.
+__device__ __host__ __forceinline__ addr::PagedSeq any_seq(const PagedArgs& a, int s) {
+  return a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], a.lens[s], a.T, a.max_len)
+                         : addr::paged_seq(s, s + 1, a.lens[s], a.T, a.max_len);
+}
+// A sequence as a form sees it: the row form has those of at most row_limit rows,
+// the chunk form the others.
 template <bool CHUNK>
-__device__ __host__ __forceinline__ addr::PagedSeq seq_of_form(const PagedArgs& a, int s) {
-  addr::PagedSeq q = a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], a.lens[s], a.T, a.max_len)
-                                     : addr::paged_seq(s, s + 1, a.lens[s], a.T, a.max_len);
+__device__ __host__ __forceinline__ addr::PagedSeq only_form(const PagedArgs& a, addr::PagedSeq q) {
   const bool few = static_cast<int64_t>(q.n) * a.G <= a.row_limit;
   if (few == CHUNK) q.n = 0;
   return q;
 }
+template <bool CHUNK>
+__device__ __host__ __forceinline__ addr::PagedSeq seq_of_form(const PagedArgs& a, int s) {
+  return only_form<CHUNK>(a, any_seq(a, s));
+}
 
-// The chunk form for the batch (bf16, head widths up to 128): true if launched.
+// The kernel's only argument, to be loaded where it is used: a kernel of several
+// forms would keep all its fields in registers throughout.
+__device__ __forceinline__ const PagedArgs& fresh_args() {
+  typedef const __attribute__((address_space(4))) PagedArgs* Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const PagedArgs*)(p);
+}
+
+// Ragged bf16 batches, head widths up to 128 (gs_chunk.hip).
 constexpr int kMostParts = 512;     // of a batch for one head, row form
 constexpr int kChunkRows = 128;
 constexpr int kChunkLeast = 4;      // key tiles of a part, at least
 int chunk_slots_for(int cus);
+int64_t chunk_list_floats(int HK, int cus);
 int64_t chunk_workspace_bytes(int HK, int DT, int cus);
-int64_t chunk_grid(const PagedArgs& a);
-void launch_chunk(const PagedArgs& a, int DT, hipStream_t st);
+int64_t chunk_most_parts(const PagedArgs& a);
+void launch_ragged(const PagedArgs& a, int DT, hipStream_t st);
 
 // Strides that keep rows on 16-byte boundaries.
 inline bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 && a % n == 0 && b % n == 0; }
@@ -67,7 +84,7 @@ inline bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 &&
 // the kernels' own arithmetic.
 // ---------------------------------------------------------------------------
 struct PagedModel {
-  int64_t bad = 0, checked = 0;
+  int64_t bad = 0, checked = 0, chunk_parts = 0;
   std::vector<char> rows;                           // output rows written
   char msg[256] = "";
   void fail(const char* what, int64_t at, int64_t n, int64_t cap) {

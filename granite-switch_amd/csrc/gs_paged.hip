@@ -20,9 +20,11 @@ namespace {
 template <bool BF16, int DT>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
   __shared__ RowShared<DT> sh;
-  const RowScan sc = row_scan<BF16, DT>(a, sh);
-  const int parts = addr::paged_parts(sc.U, a.parts);
-  if (static_cast<int>(blockIdx.x) < parts) row_part<BF16, DT>(a, sc, blockIdx.x, parts, blockIdx.y, sh);
+  __shared__ Schedule sd;
+  load_schedule(a, sd);
+  row_scan<BF16, DT>(a, sd);
+  const int parts = addr::paged_parts(sd.row_at[256], a.parts);
+  if (static_cast<int>(blockIdx.x) < parts) row_part<BF16, DT>(a, sd, blockIdx.x, parts, blockIdx.y, sh);
 }
 
 // ---------------------------------------------------------------------------
@@ -36,7 +38,6 @@ int paged_parts_for(int HK, int cus) { return std::max(1, std::min(kMostParts, 2
 // The workspace: counters that are zero between calls, at the same place for
 // every call whatever its sizes, then the partial results.
 constexpr int64_t kHeadInts = GS_PAGED_HEAD_BYTES / 4;
-constexpr int64_t kRowCount = 64, kChunkCount = 64 + 4096;
 
 int64_t row_partial_floats(int HK, int D, int cus) {
   return static_cast<int64_t>(paged_parts_for(HK, cus)) * HK * 2 * addr::paged_partial_floats(paged_width(D));
@@ -44,12 +45,15 @@ int64_t row_partial_floats(int HK, int D, int cus) {
 
 // Whether ragged calls of these sizes have a chunk form, and the rows up to
 // which a sequence stays with the row form.
-bool chunk_form(bool bf16, int G, int HK, int D) { return bf16 && D <= 128 && G <= kChunkRows && HK <= 4096; }
+int ragged_third_for(int cus) { return (chunk_slots_for(cus) / 2 + 7) & ~7; }
+bool chunk_form(bool bf16, int G, int HK, int D, int cus) {
+  return bf16 && D <= 128 && G <= kChunkRows && HK <= ragged_third_for(cus);
+}
 constexpr int kRowFormRows = 16;
 
 int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus) {
   return (kHeadInts + row_partial_floats(HK, D, cus)) * 4 +
-         (ragged && chunk_form(bf16, G, HK, D) ? chunk_workspace_bytes(HK, paged_width(D), cus) : 0);
+         (ragged && chunk_form(bf16, G, HK, D, cus) ? chunk_list_floats(HK, cus) * 4 + chunk_workspace_bytes(HK, paged_width(D), cus) : 0);
 }
 
 // What follows from the sizes alone.
@@ -58,8 +62,9 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
   a.page_octets = static_cast<uint32_t>(page_size / 8);
   a.page_magic = addr::div_magic(a.page_octets);
-  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.HK, a.D) ? kRowFormRows : INT32_MAX;
+  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.HK, a.D, cus) ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
+  a.ragged_third = ragged_third_for(cus);
   a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
   a.tq.tq = std::max(1, addr::chunk_tq(kChunkRows, a.G));
   a.tq.magic = addr::div_magic(a.tq.tq);
@@ -90,7 +95,22 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   std::vector<int64_t> start(a.B + 1, 0);
   for (int s = 0; s < a.B; ++s) start[s + 1] = start[s] + addr::paged_seq_units(seq_at(s), a.G, a.window, kUnit);
   const int64_t U = start[a.B];
-  const int parts = addr::paged_parts(U, a.parts);
+  const int most = a.row_limit == INT32_MAX ? a.parts : addr::ragged_row_parts(a.ragged_third, a.HK, a.parts);
+  const int parts = addr::paged_parts(U, most);
+  m.in("parts", 0, parts, a.parts);
+  if (a.row_limit != INT32_MAX) {                    // every ticket once
+    m.in("row parts", 0, static_cast<int64_t>(parts) * a.HK, a.ragged_third);
+    std::vector<char> pair(static_cast<size_t>(m.chunk_parts) * a.HK, 0);
+    for (int x = 0; x < 8; ++x) {
+      const addr::Tickets t = addr::tickets_of(x, static_cast<int>(pair.size()));
+      for (int i = 0; i < t.n; ++i) {
+        m.in("ticket", t.first + i, 1, static_cast<int64_t>(pair.size()));
+        if (!m.bad) ++pair[t.first + i];
+      }
+    }
+    for (char c : pair)
+      if (c != 1 && !m.bad) m.fail("a chunk part taken other than once", 0, 1, m.chunk_parts);
+  }
   std::vector<char> slots(static_cast<size_t>(a.parts) * a.HK * 2, 0);
   std::vector<char>& rows = m.rows;
   const auto written = [&](const addr::PagedSeq& sq, int j, int h, int nrow) {
@@ -175,7 +195,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
           if (w0 > 0 && w1 == nu) {
             joins.push_back({part, h, s, j, addr::paged_part_of(U, parts, item), nrow});
             if (addr::paged_part_of(U, parts, item + nu - 1) != part) m.fail("the part an item ends in", part, 0, parts);
-            m.in("counter", kRowCount + static_cast<int64_t>(part) * a.HK + h, 1, kChunkCount);
+            m.in("counter", static_cast<int64_t>(part) * a.HK + h, 1, kHeadInts);
           }
         }
       }
@@ -275,11 +295,11 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
       }
     }
   }
-  m.in("counters", kChunkCount, static_cast<int64_t>(a.HK) * addr::chunk_slots_per_head(a.HK, a.chunk_slots), kHeadInts);
+  m.in("list of split tiles", 4, 4 * split, chunk_list_floats(a.HK, a.chunk_slots / 2));
   m.in("partial results", 0, slots, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
   m.in("split tiles", 0, 2 * split, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
-  const int64_t per = (n * a.HK + 7) >> 3;
-  m.in("workgroups", 0, 8 * per, chunk_grid(a));
+  m.in("parts", 0, n, chunk_most_parts(a));
+  m.chunk_parts = n;
 }
 
 void model_rows(PagedModel& m, const PagedArgs& a) {
@@ -362,15 +382,16 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   plan_paged(a, bf16, cus, max_pages, page_size, scale);
   const int DT = paged_width(head_dim);
   int* head = static_cast<int*>(workspace);
-  a.tickets = head;
-  a.row_count = head + kRowCount;
-  a.chunk_count = head + kChunkCount;
+  a.row_count = head;
   a.ws = reinterpret_cast<float*>(head + kHeadInts);
-  a.chunk_ws = a.ws + row_partial_floats(kv_heads, head_dim, cus);
+  a.chunk_list = reinterpret_cast<int4*>(a.ws + row_partial_floats(kv_heads, head_dim, cus));
+  a.chunk_ws = reinterpret_cast<float*>(a.chunk_list) + chunk_list_floats(kv_heads, cus);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
-    GS_CHECK_ARG(chunk_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
-    launch_chunk(a, DT, st);
+    GS_CHECK_ARG(chunk_most_parts(a) * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
+    launch_ragged(a, DT, st);
+    GS_CHECK_LAUNCH(who);
+    return GS_OK;
   }
   switch (DT) {
     case 64: bf16 ? launch_paged<true, 64>(a, st) : launch_paged<false, 64>(a, st); break;

@@ -78,43 +78,58 @@ struct RowShared {
   float o[kPWaves][16][DT + 4];
   float m[kPWaves][16], l[kPWaves][16];
   float red[256][5];
-  int64_t scan[kPWaves];
   int64_t first;
   int seq, q0, n, len;
   int last;
 };
 
-// The batch's units, and the thread's run of sequences among them.
-struct RowScan {
-  int64_t mine, before, U;
-  addr::PagedSeq first;              // the thread's first sequence
+// The batch's schedule, kept in LDS so that a part is found without the registers
+// or the loads: thread t has the sequences from t * run on, run = ceil(B / 256).
+struct Schedule {
+  int64_t row_at[257];               // row form: units before a thread's sequences; of the batch
+  int q0[256], n[256], len[256];     // a thread's first sequence: its only one up to 256
+  int64_t sum[kPWaves];
 };
+// One of a form's sequences from the schedule.
+template <bool CHUNK>
+__device__ __forceinline__ addr::PagedSeq first_seq(const PagedArgs& a, const Schedule& sd) {
+  const int t = threadIdx.x;
+  return only_form<CHUNK>(a, addr::PagedSeq{sd.q0[t], sd.n[t], sd.len[t]});
+}
+
+// Each thread's own entries: no barrier between writing and reading them.
+__device__ __forceinline__ void load_schedule(const PagedArgs& a, Schedule& sd) {
+  const int tid = threadIdx.x;
+  const int run = (a.B + 255) >> 8;
+  addr::PagedSeq sq{0, 0, 0};
+  if (tid * run < a.B) sq = any_seq(a, tid * run);
+  sd.q0[tid] = sq.q0;
+  sd.n[tid] = sq.n;
+  sd.len[tid] = sq.len;
+}
 
 template <bool BF16, int DT>
-__device__ __forceinline__ RowScan row_scan(const PagedArgs& a, RowShared<DT>& sh) {
+__device__ __forceinline__ void row_scan(const PagedArgs& a, Schedule& sd) {
   constexpr int kUnit = PagedForm<BF16, DT>::kBlock * kPWaves;
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int run = (a.B + 255) >> 8;
   const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
-  RowScan r{0, 0, 0, {0, 0, 0}};
-  if (s0 < s1) r.first = seq_of_form<false>(a, s0);
-  r.mine = addr::paged_seq_units(r.first, a.G, a.window, kUnit);
-  for (int s = s0 + 1; s < s1; ++s) r.mine += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
-  int64_t incl = r.mine;
+  int64_t mine = addr::paged_seq_units(first_seq<false>(a, sd), a.G, a.window, kUnit);
+  for (int s = s0 + 1; s < s1; ++s) mine += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
+  int64_t incl = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int64_t up = __shfl_up(incl, d, 64);
     if (l >= d) incl += up;
   }
-  if (l == 63) sh.scan[wave] = incl;
+  if (l == 63) sd.sum[wave] = incl;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kPWaves; ++w) {
-    if (w < wave) incl += sh.scan[w];
-    r.U += sh.scan[w];
-  }
-  r.before = incl - r.mine;
-  return r;
+  for (int w = 0; w < kPWaves; ++w)
+    if (w < wave) incl += sd.sum[w];
+  sd.row_at[tid] = incl - mine;
+  if (tid == 255) sd.row_at[256] = incl;
+  __syncthreads();
 }
 
 // A row of the result from its sums.
@@ -249,21 +264,21 @@ __device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSe
 
 // Part `part` of `parts` of the batch, for key/value head h.
 template <bool BF16, int DT>
-__device__ __forceinline__ void row_part(const PagedArgs& a, const RowScan& sc_, int part, int parts, int h, RowShared<DT>& sh) {
+__device__ __forceinline__ void row_part(const PagedArgs& a, const Schedule& sd, int part, int parts, int h, RowShared<DT>& sh) {
   using F = PagedForm<BF16, DT>;
   constexpr int kUnit = F::kBlock * kPWaves;
   constexpr int kOC = F::kVN * F::kVW;               // O^T tiles of 16 columns
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 15, lg = l >> 4;
-  const int64_t U = sc_.U;
+  const int64_t U = sd.row_at[256];
   const int64_t u0 = addr::paged_part_lo(U, parts, part), u1 = addr::paged_part_lo(U, parts, part + 1);
   __syncthreads();
-  if (sc_.mine > 0 && sc_.before <= u0 && u0 < sc_.before + sc_.mine) {
+  if (sd.row_at[tid] <= u0 && u0 < sd.row_at[tid + 1]) {
     // the sequence that unit u0 is of
     const int run = (a.B + 255) >> 8;
     int s = tid * run;
-    int64_t at = sc_.before;
-    addr::PagedSeq sq = sc_.first;
+    int64_t at = sd.row_at[tid];
+    addr::PagedSeq sq = first_seq<false>(a, sd);
     for (;;) {
       const int64_t n = addr::paged_seq_units(sq, a.G, a.window, kUnit);
       if (u0 < at + n) break;

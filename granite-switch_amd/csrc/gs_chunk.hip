@@ -60,21 +60,11 @@ struct ChunkItem {
   addr::PagedSeq sq;
 };
 struct ChunkShared {
-  int at[257], split_at[256], tile_at[256];   // parts, partial results and split tiles before a thread's sequences
+  int at[256], split_at[256], tile_at[256];   // parts, partial results and split tiles before a thread's sequences
+  int4 count[256];                   // and of them; the key tiles of its longest part
   int64_t work[kCWaves];
-  int items[kCWaves], split[kCWaves], tiles[kCWaves];
   int found[9];
 };
-
-__device__ __forceinline__ int wave_scan(int v) {
-  const int l = lane_id();
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d, 64);
-    if (l >= d) v += u;
-  }
-  return v;
-}
 
 // How many key tiles a part of a split tile has.
 struct ChunkSplit {
@@ -83,6 +73,7 @@ struct ChunkSplit {
 };
 struct ChunkCount {
   int nt, np, items, split, tiles;   // tiles, parts of each; parts, partial results and split tiles
+  int longest;                       // key tiles of its longest part
 };
 __device__ __forceinline__ ChunkCount chunk_count(const PagedArgs& a, const ChunkSplit& c, const addr::PagedSeq& sq) {
   ChunkCount k;
@@ -91,11 +82,17 @@ __device__ __forceinline__ ChunkCount chunk_count(const PagedArgs& a, const Chun
   k.items = k.nt * k.np;
   k.split = k.np > 1 ? k.items : 0;
   k.tiles = k.np > 1 ? k.nt : 0;
+  k.longest = 0;
+  if (k.nt > 0) {
+    k.longest = addr::chunk_key_tiles(addr::chunk_tile(sq, a.tq.tq, a.window, k.nt - 1));
+    if (k.np > 1) k.longest = min(k.longest, 2 * c.tiles);
+  }
   return k;
 }
 // The batch's parts (a tile of a sequence, or one of those it is split into) for
-// one head, in order of sequences, tiles and parts; after row_scan.
-__device__ __forceinline__ ChunkSplit chunk_scan(const PagedArgs& a, const Schedule& sd, ChunkShared& sh) {
+// one head: the sequences with the longest parts first (past 256 sequences, runs of
+// them), their tiles and parts in order from the last; n is their number.
+__device__ __forceinline__ ChunkSplit chunk_scan(const PagedArgs& a, const Schedule& sd, ChunkShared& sh, int& n) {
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int run = (a.B + 255) >> 8;
   const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
@@ -112,50 +109,66 @@ __device__ __forceinline__ ChunkSplit chunk_scan(const PagedArgs& a, const Sched
   ChunkSplit c;
   c.tiles = addr::chunk_part_tiles(work, a.chunk_share, kChunkLeast);
   c.magic = addr::div_magic(c.tiles);
-  const ChunkCount k0 = chunk_count(a, c, first);
-  int items = k0.items, split = k0.split, tiles = k0.tiles;
-  for (int s = s0 + 1; s < s1; ++s) {
-    const ChunkCount k = chunk_count(a, c, seq_of_form<true>(a, s));
-    items += k.items;
-    split += k.split;
-    tiles += k.tiles;
+  int4 mine = make_int4(0, 0, 0, 0);
+  addr::PagedSeq sq = first;
+  for (int s = s0; s < s1; ++s) {
+    if (s > s0) sq = seq_of_form<true>(a, s);
+    const ChunkCount k = chunk_count(a, c, sq);
+    mine.x += k.items;
+    mine.y += k.split;
+    mine.z += k.tiles;
+    mine.w = max(mine.w, k.longest);
   }
-  int at = wave_scan(items), sl = wave_scan(split), tl = wave_scan(tiles);
-  if (l == 63) {
-    sh.items[wave] = at;
-    sh.split[wave] = sl;
-    sh.tiles[wave] = tl;
+  sh.count[tid] = mine;
+  __syncthreads();
+  // Where each run's parts begin: per lanes of a wave compare one run with every
+  // per-th of the others.
+  const int used = min(a.B, 256);                    // runs
+  int lg = 0;
+  while (lg < 6 && (used << (lg + 1)) <= 256) ++lg;
+  const int per = 1 << lg, me = tid >> lg, sub = tid & (per - 1);
+  const int w = sh.count[me].w;
+  int at = 0, sl = 0, tl = 0, all = 0, all_tiles = 0;
+#pragma unroll 4
+  for (int t = sub; t < used; t += per) {
+    const int4 o = sh.count[t];
+    const bool before = o.w > w || (o.w == w && t < me);
+    at += before ? o.x : 0;
+    sl += before ? o.y : 0;
+    tl += before ? o.z : 0;
+    all += o.x;
+    all_tiles += o.z;
+  }
+  for (int d = 1; d < per; d <<= 1) {
+    at += __shfl_xor(at, d, 64);
+    sl += __shfl_xor(sl, d, 64);
+    tl += __shfl_xor(tl, d, 64);
+    all += __shfl_xor(all, d, 64);
+    all_tiles += __shfl_xor(all_tiles, d, 64);
+  }
+  if (sub == 0) {
+    sh.at[me] = at;
+    sh.split_at[me] = sl;
+    sh.tile_at[me] = tl;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kCWaves; ++w)
-    if (w < wave) {
-      at += sh.items[w];
-      sl += sh.split[w];
-      tl += sh.tiles[w];
-    }
-  sh.at[tid] = at - items;
-  sh.split_at[tid] = sl - split;
-  sh.tile_at[tid] = tl - tiles;
-  if (tid == 255) {
-    sh.at[256] = at;
-    if (blockIdx.x == 0) a.chunk_list[0].x = tl;      // for the join, with the entries that the tiles' first parts write
-  }
-  __syncthreads();
+  n = __builtin_amdgcn_readfirstlane(all);
+  // for the join, with the entries that the tiles' first parts write
+  if (tid == 0 && blockIdx.x == 0) a.chunk_list[0].x = all_tiles;
   return c;
 }
 
-// Part r (0 <= r < sh.at[256]) of the batch.  Every thread of the workgroup calls it.
+// Part r (0 <= r < n) of the batch.  Every thread of the workgroup calls it.
 __device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, const ChunkSplit& c, int r, const Schedule& sd, ChunkShared& sh) {
   const int tid = threadIdx.x;
-  if (r >= sh.at[tid] && r < sh.at[tid + 1]) {
+  if (tid < a.B && r >= sh.at[tid] && r < sh.at[tid] + sh.count[tid].x) {
     const int run = (a.B + 255) >> 8;
     int at = sh.at[tid], sl = sh.split_at[tid], tl = sh.tile_at[tid], s = tid * run;
     addr::PagedSeq sq = first_seq<true>(a, sd);
     for (;;) {
       const ChunkCount k = chunk_count(a, c, sq);
       if (r < at + k.items) {
-        const int x = r - at;
+        const int x = at + k.items - 1 - r;          // a sequence's last tiles, the longest, first
         const int j = k.np > 1 ? x / k.np : x;
         sh.found[0] = s;
         sh.found[1] = j;
@@ -537,14 +550,14 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_kernel(Paged
     if (w - third < parts * a.HK) row_part<true, DT>(a, sd, (w - third) / a.HK, parts, (w - third) % a.HK, *reinterpret_cast<RowShared<DT>*>(lds));
   } else {
     const PagedArgs& a = fresh_args();
-    const ChunkSplit cs = chunk_scan(a, sd, sh);
-    const int n = __builtin_amdgcn_readfirstlane(sh.at[256]);
+    int n = 0;
+    const ChunkSplit cs = chunk_scan(a, sd, sh, n);
     const addr::Tickets t = addr::tickets_of(w & 7, n * a.HK);
     const int i = (w < third ? w : w - third) >> 3;
     if (i >= t.n) return;
     const int c = t.first + i;
     const int h = c / n;
-    const ChunkItem it = find_chunk(a, cs, n - 1 - (c - h * n), sd, sh);
+    const ChunkItem it = find_chunk(a, cs, c - h * n, sd, sh);
     chunk_part<DT>(fresh_args(), it, h, lds);
   }
 }

@@ -326,19 +326,15 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
     for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
   float m = -INFINITY, lsum = 0.f;
 
-  // LDS addresses of the lane's operand rows, per K step and per column tile
-  uint32_t k_at[kSteps], v_at[kDT];
-#pragma unroll
-  for (int st = 0; st < kSteps; ++st) k_at[st] = lq * kRowB + addr::chunk_k_pos(DT, lq, 2 * st + hl) * 16;
+  // LDS addresses of the lane's operand rows: the permutations are exclusive ors, so
+  // a K step or a column tile is one more on the address of the first.
+  const uint32_t k_at = lq * kRowB + addr::chunk_k_pos(DT, lq, hl) * 16;
   const int v_row = 4 * hl + ((l & 15) >> 2);
-#pragma unroll
-  for (int d = 0; d < kDT; ++d)
-    v_at[d] = kTileB + v_row * kRowB + addr::chunk_v_pos(DT, v_row, 4 * d + 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
+  const uint32_t v_at = kTileB + v_row * kRowB + addr::chunk_v_pos(DT, v_row, 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
 
   // Tile kt, in `stage`; `next` tells whether tile kt + 1 is moved to the other one.
   const auto compute = [&](int kt, int stage, bool next) {
     const int tb = tile.first + kt * kCKeys;
-    const char* base = lds + stage * kStageB;
     const bool active = wave_live && tb < any_hi && tb + kCKeys > any_lo;
     // every read of K on its way before the first product, the transfers' addresses made meanwhile
     u32x4 kf[kSteps][2];
@@ -346,7 +342,7 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
 #pragma unroll
       for (int st = 0; st < kSteps; ++st)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) kf[st][u] = ld16(base + k_at[st] + u * 32 * kRowB);
+        for (int u = 0; u < 2; ++u) kf[st][u] = ld16(lds + ((k_at + stage * kStageB) ^ (st * 32)) + u * 32 * kRowB);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (next) issue(kt + 1, stage ^ 1);              // the stage of tile kt - 1, which every wave is past
@@ -366,7 +362,7 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) vf[d][g][x] = read_tr(base + v_at[d] + (g * 16 + 8 * x) * kRowB);
+        for (int x = 0; x < 2; ++x) vf[d][g][x] = read_tr(lds + ((v_at + stage * kStageB) ^ (d * 64)) + (g * 16 + 8 * x) * kRowB);
     };
 #pragma unroll
     for (int d = 0; d < kDT / 2; ++d) read_v(d);

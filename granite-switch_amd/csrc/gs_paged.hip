@@ -234,7 +234,7 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
     const int lq = l & 31, hl = l >> 5, v_row = 4 * hl + ((l & 15) >> 2);
     for (int u = 0; u < 2; ++u)
       for (int st = 0; st < DT / 16; ++st) {
-        const int at = lq * kRowB + addr::chunk_k_pos(DT, lq, 2 * st + hl) * 16 + u * 32 * kRowB;
+        const int at = ((lq * kRowB + addr::chunk_k_pos(DT, lq, hl) * 16) ^ (st * 32)) + u * 32 * kRowB;
         m.in("K operand (LDS)", at, 16, kTileB);
         if (k_lds[at / 16] != (32 * u + lq) * 64 + 2 * st + hl) m.fail("K operand of another piece", at, 16, kTileB);
       }
@@ -242,7 +242,7 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
       for (int g = 0; g < 4; ++g)
         for (int x = 0; x < 2; ++x) {
           const int piece = 4 * d + 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
-          const int at = v_row * kRowB + addr::chunk_v_pos(DT, v_row, piece) * 16 + (l & 1) * 8 + (g * 16 + 8 * x) * kRowB;
+          const int at = ((v_row * kRowB + addr::chunk_v_pos(DT, v_row, piece - 4 * d) * 16 + (l & 1) * 8) ^ (d * 64)) + (g * 16 + 8 * x) * kRowB;
           m.in("V operand (LDS)", at, 8, kTileB);
           if (v_lds[at / 16] != (g * 16 + 8 * x + v_row) * 64 + piece) m.fail("V operand of another piece", at, 8, kTileB);
         }

@@ -21,6 +21,13 @@ _DTYPES = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_FP32
 _ACTS = {None: _lib.GS_GATE_NONE, "sigmoid": _lib.GS_GATE_SIGMOID, "tanh": _lib.GS_GATE_TANH}
 
 
+# What a call's checks found, by the shapes, strides, types and devices of its
+# tensors (never by their addresses): a serving loop's calls repeat a few, and the
+# checks take longer than a small call's kernel.
+_plans: dict = {}
+_PLAN_CAP = 4096
+
+
 def _rows(name: str, t: torch.Tensor, shape, dtype) -> torch.Tensor:
     if t.shape != shape or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
         raise ValueError(f"residual_norm: {name} is {t.dtype} {tuple(t.shape)}, expected {dtype} {tuple(shape)}")
@@ -49,6 +56,28 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
     out, residual_out: results (allocated when None); ``residual_out=residual``
               updates the stream in place, ``out=x`` reuses x
     """
+    if x is not None and x.dim() == 2 and residual.dim() == 2:
+        key = (x.shape, x.stride(), x.dtype, x.device, residual.shape, residual.stride(), residual.dtype, residual.device,
+               weight.shape, weight.stride(), weight.dtype, weight.device,
+               None if gate is None else (gate.shape, gate.stride(), gate.dtype, gate.device), gate_act,
+               None if post_weight is None else (post_weight.shape, post_weight.stride(), post_weight.dtype, post_weight.device),
+               None if out is None else (out.shape, out.stride(), out.dtype, out.device),
+               None if residual_out is None else (residual_out.shape, residual_out.stride(), residual_out.dtype,
+                                                  residual_out.device))
+        plan = _plans.get(key)
+        if plan is not None:
+            code, r_code, w_code, act, g_st, ldx, ldr, ldro, ldy, rows, hidden = plan
+            dev = x.device
+            y = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out
+            r = torch.empty(x.shape, dtype=residual.dtype, device=dev) if residual_out is None else residual_out
+            if rows:
+                _lib.call("gs_residual_norm", code, x.data_ptr(), ldx, residual.data_ptr(), ldr, r_code,
+                          None if gate is None else gate.data_ptr(), *g_st, act,
+                          None if post_weight is None else post_weight.data_ptr(), weight.data_ptr(), w_code, eps, scale,
+                          rows, hidden, r.data_ptr(), ldro, y.data_ptr(), ldy, _lib.stream_ptr(dev))
+            return y, r
+    else:
+        key = None
     act = _ACTS.get(gate_act, -1) if gate_act is None or isinstance(gate_act, str) else -1
     if act < 0:
         raise ValueError(f"residual_norm: gate_act={gate_act!r} (None, 'sigmoid' or 'tanh')")
@@ -108,6 +137,7 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
         else:
             _rows("residual_out", ro2, r2.shape, residual.dtype)
     g_row = g_col = 0
+    given_gate = gate
     if gate is not None:
         if gate.dtype != dtype:
             raise TypeError(f"residual_norm: gate is {gate.dtype}, expected {dtype}")
@@ -120,6 +150,11 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
             g = g.contiguous()
             g_row, g_col = hidden, 1
         gate = g
+    if key is not None and (gate is None or gate.data_ptr() == given_gate.data_ptr()):
+        if len(_plans) >= _PLAN_CAP:
+            _plans.clear()
+        _plans[key] = (_DTYPES[dtype], _DTYPES[residual.dtype], _DTYPES[weight.dtype], act, (g_row, g_col), _ld(x2), _ld(r2),
+                       _ld(ro2), _ld(y2), rows, hidden)
     if rows and hidden:
         _lib.call("gs_residual_norm", _DTYPES[dtype], _lib.ptr(x2), 0 if x2 is None else _ld(x2), r2.data_ptr(), _ld(r2),
                   _DTYPES[residual.dtype], _lib.ptr(gate), g_row, g_col, act, _lib.ptr(post_weight), weight.data_ptr(),
@@ -131,4 +166,3 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
     return y, residual_out if residual_out is not None else (ro2 if residual.dim() == 2 else ro2.view(shape))
 
 
-__all__ = ["residual_norm"]

@@ -111,6 +111,21 @@ def _table_ld(page_table: torch.Tensor) -> int:
     return page_table.stride(0) if page_table.shape[0] > 1 else max(page_table.stride(0), page_table.shape[1])
 
 
+# What a call's checks found, by the shapes, strides, types and devices of its
+# tensors (never by their addresses): a serving loop's calls repeat a few, and the
+# checks take longer than a small call's kernel (9 of 15 us).
+_append_plans: dict = {}
+_attention_plans: dict = {}
+_PLAN_CAP = 4096
+
+
+def _keep(plans: dict, key, plan):
+    if len(plans) >= _PLAN_CAP:            # batch sizes vary per step: keep it bounded
+        plans.clear()
+    plans[key] = plan
+    return plan
+
+
 # ---------------------------------------------------------------------------
 # Append
 # ---------------------------------------------------------------------------
@@ -160,6 +175,30 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
     q_out     receives q (allocated when None; q itself: in place).  q None: only
               k and v are handled, and None is returned.
     """
+    dev = k.device
+    key = (None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype, dev, v.shape,
+           v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape,
+           v_cache.stride(), v_cache.dtype, v_cache.device, slots.shape, slots.stride(), slots.dtype, slots.device,
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device),
+           None if cos_sin is None else (cos_sin.shape, cos_sin.stride(), cos_sin.dtype, cos_sin.device),
+           None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.device))
+    plan = _append_plans.get(key)
+    if plan is None:
+        plan = _keep(_append_plans, key, _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out))
+    code, T, H, HK, D, R, q_st, k_st, v_st, kc_st, vc_st, o_st, max_pos, pages, page = plan
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if T == 0:
+        return q_out
+    _lib.call("gs_append_kv", code, None if q is None else q.data_ptr(), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st,
+              T, H, HK, D, positions.data_ptr() if R else None, cos_sin.data_ptr() if R else None, max_pos, R,
+              1 if interleaved else 0, slots.data_ptr(), k_cache.data_ptr(), *kc_st, v_cache.data_ptr(), *vc_st, pages,
+              page, None if q is None else q_out.data_ptr(), *o_st, _lib.stream_ptr(dev))
+    return q_out
+
+
+def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out) -> tuple:
+    """The checks of an ``append_kv_`` call, and its arguments that are not addresses."""
     who = "append_kv_"
     dtype = k.dtype
     if dtype not in _DTYPES:
@@ -191,24 +230,16 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
         H = q.shape[1]
         if q.shape[2] != D:
             raise ValueError(f"{who}: q has heads of {q.shape[2]}, k of {D}")
-        if q_out is None:
-            q_out = torch.empty(T, H, D, dtype=dtype, device=k.device)
-        else:
+        if q_out is not None:
             _heads3(who, "q_out", q_out, T, dtype)
             if q_out.shape != q.shape:
                 raise ValueError(f"{who}: q_out is {tuple(q_out.shape)}, q {tuple(q.shape)}")
     elif q_out is not None:
         raise ValueError(f"{who}: q_out without q")
-    if T == 0:
-        return q_out
-    qs = (None, 0, 0) if q is None else (q.data_ptr(), q.stride(0), q.stride(1))
-    qo = (None, 0, 0) if q is None else (q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
-    _lib.call("gs_append_kv", _DTYPES[dtype], *qs, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-              v.stride(1), T, H, HK, D, _lib.ptr(positions if R else None), _lib.ptr(cos_sin if R else None),
-              cos_sin.shape[0] if R else 0, R, int(bool(interleaved)), slots.data_ptr(), k_cache.data_ptr(),
-              k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(), v_cache.stride(0),
-              v_cache.stride(1), v_cache.stride(2), k_cache.shape[0], k_cache.shape[2], *qo, _lib.stream_ptr(k.device))
-    return q_out
+    o_st = (0, 0) if q is None else (H * D, D) if q_out is None else q_out.stride()[:2]
+    return (_DTYPES[dtype], T, H, HK, D, R, (0, 0) if q is None else q.stride()[:2], k.stride()[:2], v.stride()[:2],
+            k_cache.stride()[:3], v_cache.stride()[:3], o_st, cos_sin.shape[0] if R else 0, k_cache.shape[0],
+            k_cache.shape[2])
 
 
 # ---------------------------------------------------------------------------
@@ -270,6 +301,35 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     A row that sees nothing (an empty sequence) gives zeros.
     """
+    dev = q.device
+    key = (q.shape, q.stride(), q.dtype, dev, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+           v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, page_table.shape, page_table.stride(),
+           page_table.dtype, page_table.device, kv_lens.shape, kv_lens.stride(), kv_lens.dtype, kv_lens.device,
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device),
+           window, max_q, None if out is None else (out.shape, out.stride(), out.dtype, out.device),
+           None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
+           None if workspace is None else (workspace.shape, workspace.stride(), workspace.dtype, workspace.device))
+    plan = _attention_plans.get(key)
+    if plan is None:
+        plan = _keep(_attention_plans, key, _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window,
+                                                            out, lse, max_q, workspace))
+    code, T, B, H, HK, D, q_st, k_st, v_st, pages, page, table, o_st, most, need, default_scale = plan
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if T == 0 or B == 0:
+        return out
+    stream = _lib.stream_ptr(dev)
+    if workspace is None:
+        workspace = _workspace(dev, stream, need)
+    _lib.call("gs_paged_attention", code, q.data_ptr(), *q_st, k_cache.data_ptr(), *k_st, v_cache.data_ptr(), *v_st, pages,
+              page, page_table.data_ptr(), *table, kv_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+              B, T, most, H, HK, D, default_scale if scale is None else scale, window, out.data_ptr(), *o_st,
+              None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
+    return out
+
+
+def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window, out, lse, max_q, workspace) -> tuple:
+    """The checks of a ``paged_attention`` call, and its arguments that are not addresses."""
     who = "paged_attention"
     dtype = q.dtype
     if dtype not in _DTYPES:
@@ -291,30 +351,20 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{who}: {T} query rows of {B} sequences without cu_seqlens")
     if window < 0 or (max_q is not None and max_q < 0):
         raise ValueError(f"{who}: window={window} max_q={max_q}")
-    if out is None:
-        out = torch.empty(T, H, D, dtype=dtype, device=dev)
-    else:
+    if out is not None:
         _heads3(who, "out", out, T, dtype)
         if out.shape != q.shape:
             raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
     if lse is not None:
         _ints(who, "lse", lse, torch.float32, (T, H))
-    if T == 0 or B == 0:
-        return out
-    stream = _lib.stream_ptr(dev)
-    need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None)
-    if workspace is None:
-        workspace = _workspace(dev, stream, need)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
         raise ValueError(f"{who}: workspace must be a contiguous uint8 tensor")
-    _lib.call("gs_paged_attention", _DTYPES[dtype], q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-              k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(), v_cache.stride(0),
-              v_cache.stride(1), v_cache.stride(2), k_cache.shape[0], k_cache.shape[2], page_table.data_ptr(),
-              _table_ld(page_table), page_table.shape[1], kv_lens.data_ptr(), _lib.ptr(cu_seqlens), B, T,
-              1 if cu_seqlens is None else int(max_q or 0), H, HK, D, 1.0 / math.sqrt(D) if scale is None else scale,
-              int(window), out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(lse), workspace.data_ptr(),
-              workspace.numel(), stream)
-    return out
+    with torch.cuda.device(dev):
+        need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None) if T and B else 0
+    return (_DTYPES[dtype], T, B, H, HK, D, q.stride()[:2], k_cache.stride()[:3], v_cache.stride()[:3], k_cache.shape[0],
+            k_cache.shape[2], (_table_ld(page_table), page_table.shape[1]),
+            (H * D, D) if out is None else out.stride()[:2], 1 if cu_seqlens is None else int(max_q or 0), need,
+            1.0 / math.sqrt(D))
 
 
 __all__ = ["allocate_cache", "append_kv_", "cache_slots", "paged_attention", "rope_table", "workspace_bytes"]

@@ -316,7 +316,7 @@ GS_HD PagedTile paged_tile(const PagedSeq& s, int G, int window, int j) {
   t.first = t.vs & ~7;
   return t;
 }
-GS_HD int64_t paged_tiles(const PagedSeq& s, int G) { return (static_cast<int64_t>(s.n) * G + 15) / 16; }
+GS_HD int paged_tiles(const PagedSeq& s, int G) { return static_cast<int>((static_cast<int64_t>(s.n) * G + 15) / 16); }
 // Units of `unit` tokens that cover what any tile of the sequence sees (one at least).
 GS_HD int paged_tile_units(const PagedSeq& s, int G, int window, int unit) {
   int64_t span = s.len;
@@ -324,20 +324,53 @@ GS_HD int paged_tile_units(const PagedSeq& s, int G, int window, int unit) {
   return span <= unit ? 1 : static_cast<int>((span + unit - 1) / unit);
 }
 GS_HD int64_t paged_seq_units(const PagedSeq& s, int G, int window, int unit) {
-  return s.n == 0 ? 0 : paged_tiles(s, G) * paged_tile_units(s, G, window, unit);
+  return s.n == 0 ? 0 : static_cast<int64_t>(paged_tiles(s, G)) * paged_tile_units(s, G, window, unit);
 }
-// First unit of part p of P; the part that holds unit u of U.
-GS_HD int64_t paged_part_lo(int64_t U, int P, int p) { return U * p / P; }
-GS_HD int paged_part_of(int64_t U, int P, int64_t u) { return static_cast<int>(((u + 1) * P - 1) / U); }
+// Times the workgroups are filled by `items` items a head: up to four.
+GS_HD int row_rounds(int64_t items, int HK, int wgs) {
+  const int64_t r = items * HK / wgs;
+  return r >= 4 ? 4 : r < 1 ? 1 : static_cast<int>(r);
+}
+// Units of a part at most, for `items` items of U units in all a head, on `wgs`
+// workgroups: an equal share of them, or of up to four times as many where there are
+// that many items, and four units at least.
+GS_HD int row_part_units(int64_t U, int items, int HK, int wgs) {
+  const int64_t n = static_cast<int64_t>(wgs) * row_rounds(items, HK, wgs);
+  const int64_t u = (U * HK + n - 1) / n;
+  return u < 4 ? 4 : static_cast<int>(u);
+}
+constexpr int kMostParts = 512;      // of an item
+GS_HD int row_parts(int units, int most, uint32_t magic) {
+  uint32_t q, r;
+  div_by(static_cast<uint32_t>(units + most - 1), static_cast<uint32_t>(most), magic, q, r);
+  return q < kMostParts ? static_cast<int>(q) : kMostParts;
+}
+// Partial results of a head at most: an item of u > part units has u / part + 1 < 2 u /
+// part of them, and U / part <= 4 wgs / HK.
+GS_HD int row_slots_per_head(int HK, int wgs) { return (8 * wgs + HK - 1) / HK + 1; }
+// Parts of a head at most, for that many items: each one, and U / part more.
+GS_HD int64_t row_most_parts(int64_t items, int HK, int wgs) {
+  return items + (static_cast<int64_t>(wgs) * row_rounds(items, HK, wgs) + HK - 1) / HK;
+}
+// Workgroup w of a ragged launch: blocks of `block` (a multiple of 8) chunk parts and
+// row parts in turn while there are row_blocks of these, then chunk parts.  True: row
+// part i; false: chunk part i.
+GS_HD bool ragged_role(int w, int block, int row_blocks, int& i) {
+  const int b = w / block;
+  if (b >= 2 * row_blocks) {
+    i = w - row_blocks * block;
+    return false;
+  }
+  i = (b >> 1) * block + (w - b * block);
+  return (b & 1) != 0;
+}
 // The first token of the 8 that a lane reads from tok on (a multiple of 8):
 // 8 tokens are always of one page; past the last seen ones re-read those.
 GS_HD int paged_octet(int tok, int ve) { return imin(tok, (ve - 1) & ~7); }
 GS_HD int paged_page(int id, int num_pages) {
   return static_cast<uint32_t>(id) < static_cast<uint32_t>(num_pages) ? id : 0;
 }
-// Parts that have work: kLeastUnits units at least each, or all in one.
-constexpr int kLeastUnits = 2;
-GS_HD int paged_parts(int64_t U, int parts) { return static_cast<int>(lmin((U + kLeastUnits - 1) / kLeastUnits, parts)); }
+
 
 // Chunk form: tiles of `tq` whole queries (tq * G rows), key tiles of 64.
 // Queries of a tile, with R rows in a tile.
@@ -389,8 +422,6 @@ GS_HD void chunk_part_range(int nkt, int p, int n, int& k0, int& k1) {
   k0 = static_cast<int>(static_cast<int64_t>(nkt) * p / n);
   k1 = static_cast<int>(static_cast<int64_t>(nkt) * (p + 1) / n);
 }
-// Parts for each head of the row form on `wgs` workgroups.
-GS_HD int ragged_row_parts(int wgs, int HK, int most) { return imin(wgs / HK, most); }
 // XCD x's tickets: a contiguous eighth of the (head, part) pairs.
 struct Tickets {
   int first, n;

@@ -2,10 +2,8 @@
 // launch in which sequences of many rows take the chunk form here and those of few
 // (a decode row among prompts) the row form (gs_paged_rows.h).
 //
-// Two workgroups share a compute unit: at the start one has a part of the row form,
-// which streams the cache, and one multiplies.  The chunk form's parts are tickets
-// that its workgroups take until none are left, a sequence's last tiles, the
-// longest, first.
+// Two workgroups share a compute unit: parts of the row form, which stream the cache,
+// and of the chunk form, which multiply, are launched in turn.
 //
 // The chunk form.
 // A workgroup of 4 waves takes 128 (query, head) rows of one sequence and
@@ -529,29 +527,26 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
   }
 }
 
-// Grid: `third` workgroups with a chunk part each, `third` with one of the row form,
-// then the rest of the chunk parts.
+// Grid: addr::ragged_role.
 template <int DT>
 __global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_kernel(PagedArgs) {
   __shared__ __attribute__((aligned(1024))) char lds[addr::cmax(kCStages * 2 * kCKeys * DT * 2, static_cast<int>(sizeof(RowShared<DT>)))];
   __shared__ ChunkShared sh;
   __shared__ Schedule sd;
   load_schedule(fresh_args(), sd);
-  const int w = blockIdx.x;
-  const int third = fresh_args().ragged_third;
-  if (w >= third && w < 2 * third) {
+  int i;
+  if (addr::ragged_role(blockIdx.x, fresh_args().ragged_block, fresh_args().row_blocks, i)) {
     const PagedArgs& a = fresh_args();
-    row_scan<true, DT>(a, sd);
-    const int parts = addr::paged_parts(sd.row_at[256], addr::ragged_row_parts(third, a.HK, a.parts));
-    if (w - third < parts * a.HK) row_part<true, DT>(a, sd, (w - third) / a.HK, parts, (w - third) % a.HK, *reinterpret_cast<RowShared<DT>*>(lds));
+    const int h = i % a.HK;
+    const RowItem it = find_row<true, DT>(a, sd, i / a.HK);
+    if (it.s >= 0) row_part<true, DT>(fresh_args(), it, h, *reinterpret_cast<RowShared<DT>*>(lds));
   } else {
     const PagedArgs& a = fresh_args();
     int n = 0;
     const ChunkSplit cs = chunk_scan(a, sd, sh, n);
-    const addr::Tickets t = addr::tickets_of(w & 7, n * a.HK);
-    const int i = (w < third ? w : w - third) >> 3;
-    if (i >= t.n) return;
-    const int c = t.first + i;
+    const addr::Tickets t = addr::tickets_of(i & 7, n * a.HK);
+    if ((i >> 3) >= t.n) return;
+    const int c = t.first + (i >> 3);
     const int h = c / n;
     const ChunkItem it = find_chunk(a, cs, c - h * n, sd, sh);
     chunk_part<DT>(fresh_args(), it, h, lds);
@@ -578,8 +573,13 @@ int64_t chunk_most_parts(const PagedArgs& a) {
   return chunk_most_tiles(a) + addr::chunk_slots_per_head(a.HK, a.chunk_slots);
 }
 
+int64_t ragged_grid(const PagedArgs& a) {
+  return static_cast<int64_t>(a.row_blocks) * a.ragged_block +
+         std::max<int64_t>(static_cast<int64_t>(a.row_blocks) * a.ragged_block, (chunk_most_parts(a) * a.HK + 7) & ~int64_t(7));
+}
+
 void launch_ragged(const PagedArgs& a, int DT, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.ragged_third + std::max<int64_t>(a.ragged_third, (chunk_most_parts(a) * a.HK + 7) & ~int64_t(7))));
+  const dim3 grid(static_cast<unsigned>(ragged_grid(a)));
   const dim3 join(static_cast<unsigned>(a.chunk_slots));
   if (DT == 64) {
     hipLaunchKernelGGL((ragged_attention_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);

@@ -25,15 +25,17 @@ struct PagedArgs {
   float* ws;                        // row form: partial results
   float* chunk_ws;                  // chunk form: partial results
   int4* chunk_list;                 // the split tiles: their number, then first query, rows, parts and first partial result of each
-  int* row_count;                   // [parts * HK]: workgroups done with the item that a part ends; zero between calls
+  int* row_count;                   // by an item's first partial result: its workgroups that are done; zero between calls
   int64_t max_len;
   uint32_t page_octets, page_magic;
   int num_pages;
   int B, T, H, HK, G, D;
-  int window, parts;
+  int window;
+  int row_wgs;                      // workgroups that the row form fills
+  int row_slots;                    // its partial results for each head
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
   int chunk_slots;                  // workgroups that the chunk form fills
-  int ragged_third;                 // workgroups of a third of a ragged launch, a multiple of 8
+  int ragged_block, row_blocks;     // a ragged launch's order (addr::ragged_role)
   double chunk_share;               // HK / (2 chunk_slots)
   addr::ChunkTq tq;                 // queries of a chunk tile
   uint32_t g_magic;                 // div_magic(G)
@@ -67,13 +69,13 @@ __device__ __forceinline__ const PagedArgs& fresh_args() {
 }
 
 // Ragged bf16 batches, head widths up to 128 (gs_chunk.hip).
-constexpr int kMostParts = 512;     // of a batch for one head, row form
 constexpr int kChunkRows = 128;
 constexpr int kChunkLeast = 4;      // key tiles of a part, at least
 int chunk_slots_for(int cus);
 int64_t chunk_list_floats(int HK, int cus);
 int64_t chunk_workspace_bytes(int HK, int DT, int cus);
 int64_t chunk_most_parts(const PagedArgs& a);
+int64_t ragged_grid(const PagedArgs& a);
 void launch_ragged(const PagedArgs& a, int DT, hipStream_t st);
 
 // Strides that keep rows on 16-byte boundaries.

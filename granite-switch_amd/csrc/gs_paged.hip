@@ -17,14 +17,15 @@
 namespace gs {
 namespace {
 
+// Grid: parts x key/value heads, the heads of a part side by side.
 template <bool BF16, int DT>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
   __shared__ RowShared<DT> sh;
   __shared__ Schedule sd;
   load_schedule(a, sd);
-  row_scan<BF16, DT>(a, sd);
-  const int parts = addr::paged_parts(sd.row_at[256], a.parts);
-  if (static_cast<int>(blockIdx.x) < parts) row_part<BF16, DT>(a, sd, blockIdx.x, parts, blockIdx.y, sh);
+  const int r = blockIdx.x / a.HK;
+  const RowItem it = find_row<BF16, DT>(a, sd, r);
+  if (it.s >= 0) row_part<BF16, DT>(a, it, blockIdx.x - r * a.HK, sh);
 }
 
 // ---------------------------------------------------------------------------
@@ -32,39 +33,51 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel
 // ---------------------------------------------------------------------------
 int paged_width(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 
-// Parts of the batch for each key/value head: two workgroups to a compute unit.
-int paged_parts_for(int HK, int cus) { return std::max(1, std::min(kMostParts, 2 * cus / HK)); }
+// Workgroups of the row form that run at a time: two to a compute unit, one at
+// widths past 128.
+int row_wgs_for(int D, int cus) { return paged_width(D) == 256 ? cus : 2 * cus; }
 
 // The workspace: counters that are zero between calls, at the same place for
 // every call whatever its sizes, then the partial results.
 constexpr int64_t kHeadInts = GS_PAGED_HEAD_BYTES / 4;
 
 int64_t row_partial_floats(int HK, int D, int cus) {
-  return static_cast<int64_t>(paged_parts_for(HK, cus)) * HK * 2 * addr::paged_partial_floats(paged_width(D));
+  return static_cast<int64_t>(HK) * addr::row_slots_per_head(HK, 2 * cus) * addr::paged_partial_floats(paged_width(D));
 }
 
 // Whether ragged calls of these sizes have a chunk form, and the rows up to
 // which a sequence stays with the row form.
-int ragged_third_for(int cus) { return (chunk_slots_for(cus) / 2 + 7) & ~7; }
-bool chunk_form(bool bf16, int G, int HK, int D, int cus) {
-  return bf16 && D <= 128 && G <= kChunkRows && HK <= ragged_third_for(cus);
-}
+bool chunk_form(bool bf16, int G, int D) { return bf16 && D <= 128 && G <= kChunkRows; }
 constexpr int kRowFormRows = 16;
 
 int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus) {
   return (kHeadInts + row_partial_floats(HK, D, cus)) * 4 +
-         (ragged && chunk_form(bf16, G, HK, D, cus) ? chunk_list_floats(HK, cus) * 4 + chunk_workspace_bytes(HK, paged_width(D), cus) : 0);
+         (ragged && chunk_form(bf16, G, D) ? chunk_list_floats(HK, cus) * 4 + chunk_workspace_bytes(HK, paged_width(D), cus) : 0);
+}
+
+// Parts of the row form for each head, at most.
+int64_t row_most_parts(const PagedArgs& a) {
+  // one tile to a sequence where sequences of more take the chunk form
+  const int64_t items = a.row_limit != INT32_MAX ? std::min(a.B, a.T)
+                                                 : std::min<int64_t>(a.B, a.T) + static_cast<int64_t>(a.T) * a.G / 16;
+  return addr::row_most_parts(items, a.HK, a.row_wgs);
 }
 
 // What follows from the sizes alone.
 void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, float scale) {
-  a.parts = paged_parts_for(a.HK, cus);
   a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
   a.page_octets = static_cast<uint32_t>(page_size / 8);
   a.page_magic = addr::div_magic(a.page_octets);
-  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.HK, a.D, cus) ? kRowFormRows : INT32_MAX;
+  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
-  a.ragged_third = ragged_third_for(cus);
+  a.row_slots = addr::row_slots_per_head(a.HK, 2 * cus);
+  a.row_wgs = row_wgs_for(a.D, cus);
+  a.ragged_block = (cus + 7) & ~7;
+  a.row_blocks = 0;
+  if (a.row_limit != INT32_MAX) {                    // beside the chunk form: half the workgroups
+    a.row_wgs = cus;
+    a.row_blocks = static_cast<int>((row_most_parts(a) * a.HK + a.ragged_block - 1) / a.ragged_block);
+  }
   a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
   a.tq.tq = std::max(1, addr::chunk_tq(kChunkRows, a.G));
   a.tq.magic = addr::div_magic(a.tq.tq);
@@ -74,7 +87,7 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
 
 template <bool BF16, int DT>
 void launch_paged(const PagedArgs& a, hipStream_t st) {
-  const dim3 grid(a.parts, a.HK);
+  const dim3 grid(static_cast<unsigned>(row_most_parts(a) * a.HK));
   hipLaunchKernelGGL((paged_attention_kernel<BF16, DT>), grid, dim3(256), 0, st, a);
 }
 
@@ -91,62 +104,51 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
   const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D);
   const int64_t o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
-  const auto seq_at = [&](int s) { return seq_of_form<false>(a, s); };
-  std::vector<int64_t> start(a.B + 1, 0);
-  for (int s = 0; s < a.B; ++s) start[s + 1] = start[s] + addr::paged_seq_units(seq_at(s), a.G, a.window, kUnit);
-  const int64_t U = start[a.B];
-  const int most = a.row_limit == INT32_MAX ? a.parts : addr::ragged_row_parts(a.ragged_third, a.HK, a.parts);
-  const int parts = addr::paged_parts(U, most);
-  m.in("parts", 0, parts, a.parts);
-  if (a.row_limit != INT32_MAX) {                    // every ticket once
-    m.in("row parts", 0, static_cast<int64_t>(parts) * a.HK, a.ragged_third);
-    std::vector<char> pair(static_cast<size_t>(m.chunk_parts) * a.HK, 0);
-    for (int x = 0; x < 8; ++x) {
-      const addr::Tickets t = addr::tickets_of(x, static_cast<int>(pair.size()));
-      for (int i = 0; i < t.n; ++i) {
-        m.in("ticket", t.first + i, 1, static_cast<int64_t>(pair.size()));
-        if (!m.bad) ++pair[t.first + i];
-      }
-    }
-    for (char c : pair)
-      if (c != 1 && !m.bad) m.fail("a chunk part taken other than once", 0, 1, m.chunk_parts);
-  }
-  std::vector<char> slots(static_cast<size_t>(a.parts) * a.HK * 2, 0);
+  std::vector<char> slots(static_cast<size_t>(a.row_slots), 0);
   std::vector<char>& rows = m.rows;
-  const auto written = [&](const addr::PagedSeq& sq, int j, int h, int nrow) {
-    for (int q = 0; q < nrow; ++q) {
-      const int64_t rr = static_cast<int64_t>(j) * 16 + q;
-      const int64_t tok = sq.q0 + rr / a.G;
-      const int64_t head = h * a.G + rr % a.G;
-      m.in("output row", tok * a.H + head, 1, static_cast<int64_t>(a.T) * a.H);
-      if (m.bad) return;
-      if (rows[tok * a.H + head]++) m.fail("output row written twice", tok * a.H + head, 1, static_cast<int64_t>(a.T) * a.H);
-      for (int d = 0; d < a.D; d += 4) m.in("out", tok * a.o_ts + head * a.o_hs + d, 4, o_elems);
-    }
-  };
-  struct Join {
-    int part, h, s, j, first, nrow;
-  };
-  std::vector<Join> joins;
-  for (int part = 0; part < parts && !m.bad; ++part) {
-    const int64_t u0 = addr::paged_part_lo(U, parts, part), u1 = addr::paged_part_lo(U, parts, part + 1);
-    if (u0 >= u1) m.fail("a part without a unit", part, 1, parts);
-    int s = 0;
-    int64_t u = u0;
-    while (u < u1 && !m.bad) {
-      while (start[s + 1] <= u) ++s;
-      const addr::PagedSeq sq = seq_at(s);
-      const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
-      const int j = static_cast<int>((u - start[s]) / nu);
-      const int64_t item = start[s] + static_cast<int64_t>(j) * nu;
-      const int w0 = static_cast<int>(u - item), w1 = static_cast<int>(std::min<int64_t>(nu, u1 - item));
+  int64_t U = 0, items = 0;
+  for (int s = 0; s < a.B; ++s) {
+    const addr::PagedSeq sq = seq_of_form<false>(a, s);
+    U += addr::paged_seq_units(sq, a.G, a.window, kUnit);
+    items += addr::paged_tiles(sq, a.G);
+  }
+  const int most = addr::row_part_units(U, static_cast<int>(items), a.HK, a.row_wgs);
+  const uint32_t magic = addr::div_magic(most);
+  int64_t parts = 0, slot = 0;
+  for (int s = 0; s < a.B && !m.bad; ++s) {
+    const addr::PagedSeq sq = seq_of_form<false>(a, s);
+    const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
+    const int np = addr::row_parts(nu, most, magic);
+    const int64_t nrows = static_cast<int64_t>(sq.n) * a.G;
+    for (int j = 0; j < addr::paged_tiles(sq, a.G) && !m.bad; ++j) {
       const addr::PagedTile t = addr::paged_tile(sq, a.G, a.window, j);
-      const int64_t nrows = static_cast<int64_t>(sq.n) * a.G;
       const int nblk = (t.ve - t.first + F::kBlock - 1) / F::kBlock;
       if (nblk > nu * kPWaves) m.fail("blocks past the item's units", nblk, 0, nu * kPWaves);
-      const int b_end = std::min(w1 * kPWaves, nblk);
       const int nrow = static_cast<int>(std::min<int64_t>(16, nrows - static_cast<int64_t>(j) * 16));
-      for (int h = 0; h < a.HK; ++h) {
+      parts += np;
+      if (np > 1) {
+        m.in("partial results", slot, np, a.row_slots);
+        m.in("counters", (a.HK - 1) * static_cast<int64_t>(a.row_slots) + slot, 1, kHeadInts);
+        m.in("parts of an item", 0, np, addr::kMostParts);
+        slot += np;
+      }
+      int covered = 0;
+      for (int p = 0; p < np; ++p) {
+        int w0 = 0, w1 = nu;
+        if (np > 1) addr::chunk_part_range(nu, p, np, w0, w1);
+        if (w0 != covered) m.fail("a unit taken other than once", w0, 1, nu);
+        covered = w1;
+      }
+      if (covered != nu) m.fail("a unit taken other than once", covered, 1, nu);
+      for (int h = 0; h < a.HK && !m.bad; ++h) {
+        for (int q = 0; q < nrow; ++q) {
+          const int64_t rr = static_cast<int64_t>(j) * 16 + q;
+          const int64_t tok = sq.q0 + rr / a.G, head = h * a.G + rr % a.G;
+          m.in("output row", tok * a.H + head, 1, static_cast<int64_t>(a.T) * a.H);
+          if (m.bad) return;
+          if (rows[tok * a.H + head]++) m.fail("output row written twice", tok * a.H + head, 1, static_cast<int64_t>(a.T) * a.H);
+          m.in("out", tok * a.o_ts + head * a.o_hs, a.D, o_elems);
+        }
         for (int l = 0; l < 64; ++l) {
           const int lq = l & 15, lg = l >> 4;
           const int64_t r = static_cast<int64_t>(j) * 16 + lq;
@@ -159,7 +161,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
           }
           const int k_oct = BF16 ? 8 * (lq >> 2) : 8 * (lq >> 3), v_oct = BF16 ? 8 * lg : 8 * (lg >> 1);
           const int k_in = BF16 ? (lq & 3) : (lq & 7), v_in = BF16 ? 0 : 4 * (lg & 1);
-          for (int b = w0 * kPWaves; b < b_end + 2 * kPWaves && t.ve > 0 && b_end > w0 * kPWaves; ++b) {   // ids are read up to two rounds ahead
+          for (int b = 0; b < nblk + 2 * kPWaves && nblk > 0; ++b) {            // ids are read up to two rounds ahead
             const int tb = t.first + b * F::kBlock;
             uint32_t kp, kr, vp, vr;
             const int kt = addr::paged_octet(tb + k_oct, t.ve), vt = addr::paged_octet(tb + v_oct, t.ve);
@@ -185,35 +187,29 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
               }
           }
         }
-        if (w0 == 0 && w1 == nu) {
-          written(sq, j, h, nrow);
-        } else {
-          const int64_t slot = (static_cast<int64_t>(part) * a.HK + h) * 2 + (w0 == 0 ? 1 : 0);
-          m.in("workspace slot", slot, 1, static_cast<int64_t>(slots.size()));
-          if (m.bad) return;
-          if (slots[slot]++) m.fail("workspace slot written twice", slot, 1, static_cast<int64_t>(slots.size()));
-          if (w0 > 0 && w1 == nu) {
-            joins.push_back({part, h, s, j, addr::paged_part_of(U, parts, item), nrow});
-            if (addr::paged_part_of(U, parts, item + nu - 1) != part) m.fail("the part an item ends in", part, 0, parts);
-            m.in("counter", static_cast<int64_t>(part) * a.HK + h, 1, kHeadInts);
-          }
-        }
       }
-      u = item + w1;
     }
   }
-  for (const Join& jn : joins) {
-    for (int p = jn.first; p <= jn.part && !m.bad; ++p) {
-      const int64_t slot = (static_cast<int64_t>(p) * a.HK + jn.h) * 2 + (p == jn.first ? 1 : 0);
-      m.in("joined slot", slot, 1, static_cast<int64_t>(slots.size()));
-      if (m.bad) return;
-      if (slots[slot] != 1) m.fail("a joined slot that no part writes, or two joins read", slot, 1, static_cast<int64_t>(slots.size()));
-      slots[slot] = 2;
+  const int64_t grid = row_most_parts(a);
+  m.in("parts", 0, parts, grid);
+  if (a.row_limit == INT32_MAX) return;
+  // a ragged launch: every part of either form has one workgroup
+  std::vector<char> row(static_cast<size_t>(parts) * a.HK, 0), pair(static_cast<size_t>(m.chunk_parts) * a.HK, 0);
+  for (int64_t w = 0; w < ragged_grid(a); ++w) {
+    int i;
+    if (addr::ragged_role(static_cast<int>(w), a.ragged_block, a.row_blocks, i)) {
+      if (i < static_cast<int64_t>(row.size())) ++row[i];
+    } else {
+      const addr::Tickets t = addr::tickets_of(i & 7, static_cast<int>(pair.size()));
+      if ((i >> 3) >= t.n) continue;
+      m.in("ticket", t.first + (i >> 3), 1, static_cast<int64_t>(pair.size()));
+      if (!m.bad) ++pair[t.first + (i >> 3)];
     }
-    written(seq_at(jn.s), jn.j, jn.h, jn.nrow);
   }
-  for (char c : slots)
-    if (c == 1 && !m.bad) m.fail("a partial result that no join reads", 0, 1, 0);
+  for (char c : row)
+    if (c != 1 && !m.bad) m.fail("a row part taken other than once", 0, 1, parts);
+  for (char c : pair)
+    if (c != 1 && !m.bad) m.fail("a chunk part taken other than once", 0, 1, m.chunk_parts);
 }
 
 // The chunk form.
@@ -340,7 +336,7 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
                (long long)num_tokens, num_seqs);
   GS_CHECK_ARG(cu_seqlens != nullptr || num_tokens == num_seqs, "%s: num_tokens=%lld of num_seqs=%d without cu_seqlens", who,
                (long long)num_tokens, num_seqs);
-  GS_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536, "%s: heads=%d kv_heads=%d", who, heads, kv_heads);
+  GS_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536 && kv_heads <= 4096, "%s: heads=%d kv_heads=%d", who, heads, kv_heads);
   const bool bf16 = dtype == GS_DTYPE_BF16;
   const int ve = bf16 ? 8 : 4;
   GS_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % ve == 0, "%s: head_dim=%d must be a multiple of %d up to 256", who,
@@ -388,11 +384,12 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   a.chunk_ws = reinterpret_cast<float*>(a.chunk_list) + chunk_list_floats(kv_heads, cus);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
-    GS_CHECK_ARG(chunk_most_parts(a) * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
+    GS_CHECK_ARG(ragged_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
     launch_ragged(a, DT, st);
     GS_CHECK_LAUNCH(who);
     return GS_OK;
   }
+  GS_CHECK_ARG(row_most_parts(a) * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
   switch (DT) {
     case 64: bf16 ? launch_paged<true, 64>(a, st) : launch_paged<false, 64>(a, st); break;
     case 128: bf16 ? launch_paged<true, 128>(a, st) : launch_paged<false, 128>(a, st); break;

@@ -2,11 +2,13 @@
 // keys and values from the pages straight into registers.  Shared by the decode
 // kernel (gs_paged.hip) and the kernel for ragged batches (gs_chunk.hip).
 //
-// Every item -- a tile of 16 rows of a sequence, for one key/value head -- is a
-// run of units of 128 keys (fp32: 64); the batch's units in order are dealt to
-// `parts` workgroups in equal runs, so long and short sequences load them alike.
-// A workgroup whose run ends inside an item leaves a partial result; the last of
-// an item's workgroups to be done joins them, in the order of the keys.
+// An item is a tile of 16 rows of a sequence for one key/value head, a run of units
+// of 128 keys (fp32: 64).  A workgroup has one item, or one part of an item of many
+// units: few, long sequences are cut so that the GPU is filled once, many into parts
+// of at most twice a quarter of a workgroup's share, which level out.  A part leaves a
+// partial result; the last of an item's workgroups to be done joins them, in the order
+// of the keys.  (Equal runs of the batch's units, cut wherever they end, cost two
+// joins a workgroup and 114 us against XX for 256 sequences of 16 .. 2048 keys.)
 #pragma once
 
 #include "gs_paged.h"
@@ -78,19 +80,18 @@ struct RowShared {
   float o[kPWaves][16][DT + 4];
   float m[kPWaves][16], l[kPWaves][16];
   float red[256][5];
-  int64_t first;
-  int seq, q0, n, len;
   int last;
 };
 
-// The batch's schedule, kept in LDS so that a part is found without the registers
-// or the loads: thread t has the sequences from t * run on, run = ceil(B / 256).
+// The batch's schedule in LDS: thread t has the sequences from t * run on, run =
+// ceil(B / 256).
 struct Schedule {
-  int64_t row_at[257];               // row form: units before a thread's sequences; of the batch
   int q0[256], n[256], len[256];     // a thread's first sequence: its only one up to 256
   int64_t sum[kPWaves];
+  int items[kPWaves], slots[kPWaves];
+  int found[8];
 };
-// One of a form's sequences from the schedule.
+// The thread's first sequence as a form sees it.
 template <bool CHUNK>
 __device__ __forceinline__ addr::PagedSeq first_seq(const PagedArgs& a, const Schedule& sd) {
   const int t = threadIdx.x;
@@ -108,28 +109,114 @@ __device__ __forceinline__ void load_schedule(const PagedArgs& a, Schedule& sd) 
   sd.len[tid] = sq.len;
 }
 
+__device__ __forceinline__ int wave_scan(int v) {
+  const int l = lane_id();
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(v, d, 64);
+    if (l >= d) v += u;
+  }
+  return v;
+}
+
+// One part of the row form's work.
+struct RowItem {
+  int s, j, part, nparts, slot;      // slot: of the item's first partial result, or -1
+  int units;                         // of the item
+  addr::PagedSeq sq;
+};
+
+// The r-th part of the batch for one head, in order of sequences, tiles and parts; s <
+// 0: there is none.  Every thread of a workgroup of 256 calls it, after load_schedule.
 template <bool BF16, int DT>
-__device__ __forceinline__ void row_scan(const PagedArgs& a, Schedule& sd) {
+__device__ __forceinline__ RowItem find_row(const PagedArgs& a, Schedule& sd, int r) {
   constexpr int kUnit = PagedForm<BF16, DT>::kBlock * kPWaves;
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int run = (a.B + 255) >> 8;
   const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
-  int64_t mine = addr::paged_seq_units(first_seq<false>(a, sd), a.G, a.window, kUnit);
-  for (int s = s0 + 1; s < s1; ++s) mine += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
-  int64_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t up = __shfl_up(incl, d, 64);
-    if (l >= d) incl += up;
+  const addr::PagedSeq first = first_seq<false>(a, sd);
+  addr::PagedSeq sq = first;
+  int64_t U = 0;
+  int items = 0;
+  for (int s = s0; s < s1; ++s) {
+    if (s > s0) sq = seq_of_form<false>(a, s);
+    U += addr::paged_seq_units(sq, a.G, a.window, kUnit);
+    items += addr::paged_tiles(sq, a.G);
   }
-  if (l == 63) sd.sum[wave] = incl;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    U += __shfl_xor(U, d, 64);
+    items += __shfl_xor(items, d, 64);
+  }
+  if (l == 0) {
+    sd.sum[wave] = U;
+    sd.items[wave] = items;
+  }
+  if (tid == 0) sd.found[0] = -1;
   __syncthreads();
+  U = 0;
+  items = 0;
+#pragma unroll
+  for (int w = 0; w < kPWaves; ++w) {
+    U += sd.sum[w];
+    items += sd.items[w];
+  }
+  const int most = addr::row_part_units(U, items, a.HK, a.row_wgs);
+  const uint32_t magic = addr::div_magic(most);
+  int parts = 0, slots = 0;
+  sq = first;
+  for (int s = s0; s < s1; ++s) {
+    if (s > s0) sq = seq_of_form<false>(a, s);
+    const int nt = addr::paged_tiles(sq, a.G);
+    const int np = addr::row_parts(addr::paged_tile_units(sq, a.G, a.window, kUnit), most, magic);
+    parts += nt * np;
+    slots += np > 1 ? nt * np : 0;
+  }
+  int at = wave_scan(parts), sl = wave_scan(slots);
+  __syncthreads();
+  if (l == 63) {
+    sd.items[wave] = at;
+    sd.slots[wave] = sl;
+  }
+  __syncthreads();
+  at -= parts;
+  sl -= slots;
 #pragma unroll
   for (int w = 0; w < kPWaves; ++w)
-    if (w < wave) incl += sd.sum[w];
-  sd.row_at[tid] = incl - mine;
-  if (tid == 255) sd.row_at[256] = incl;
+    if (w < wave) {
+      at += sd.items[w];
+      sl += sd.slots[w];
+    }
+  if (r >= at && r < at + parts) {
+    sq = first;
+    for (int s = s0;; ++s) {
+      if (s > s0) sq = seq_of_form<false>(a, s);
+      const int nt = addr::paged_tiles(sq, a.G);
+      const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
+      const int np = addr::row_parts(nu, most, magic);
+      if (r < at + nt * np) {
+        const int x = r - at;
+        const int j = np > 1 ? x / np : x;
+        sd.found[0] = s;
+        sd.found[1] = j;
+        sd.found[2] = x - j * np;
+        sd.found[3] = np;
+        sd.found[4] = np > 1 ? sl + j * np : -1;
+        sd.found[5] = sq.q0;
+        sd.found[6] = sq.n;
+        sd.found[7] = sq.len;
+        break;
+      }
+      at += nt * np;
+      sl += np > 1 ? nt * np : 0;
+    }
+  }
   __syncthreads();
+  const int* f = sd.found;
+  const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
+  RowItem it{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), 0, {u(f[5]), u(f[6]), u(f[7])}};
+  it.units = addr::paged_tile_units(it.sq, a.G, a.window, kUnit);
+  return it;
 }
 
 // A row of the result from its sums.
@@ -188,20 +275,15 @@ __device__ __forceinline__ bool last_to_arrive(int* count, int of, int& shared) 
   return shared != 0;
 }
 
-// Joins an item's partial results, parts first .. last of head h: the maxima of 8
-// rows at a time through LDS, then each thread 4 columns of a row of every
-// groups-th part.
+// Joins an item's np partial results: the maxima of 8 rows at a time through LDS, then
+// each thread 4 columns of a row of every groups-th part.
 template <bool BF16, int DT>
-__device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSeq& sq, int j, int nrow, int h, int first,
-                                         int last, RowShared<DT>& sh) {
-  constexpr int kRows = 8;                           // kRows * np maxima fit into sh.o: np <= kMostParts
-  const int64_t slot_floats = addr::paged_partial_floats(DT);
+__device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSeq& sq, int j, int nrow, int h,
+                                         const float* first, int np, RowShared<DT>& sh) {
+  constexpr int kRows = 8;                           // kRows * np maxima fit into sh.o: np <= addr::kMostParts
   const int tid = threadIdx.x;
-  const int np = last - first + 1;
   float* sm = &sh.o[0][0][0];                        // [np][8]
-  const auto slot_of = [&](int p) {
-    return a.ws + ((static_cast<int64_t>(first + p) * a.HK + h) * 2 + (p == 0 ? 1 : 0)) * slot_floats;
-  };
+  const auto slot_of = [&](int p) { return first + p * addr::paged_partial_floats(DT); };
   for (int r0 = 0; r0 < nrow; r0 += kRows) {
     const int nr = min(kRows, nrow - r0);
     __syncthreads();
@@ -262,56 +344,18 @@ __device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSe
   }
 }
 
-// Part `part` of `parts` of the batch, for key/value head h.
+// One part of an item, for key/value head h.
 template <bool BF16, int DT>
-__device__ __forceinline__ void row_part(const PagedArgs& a, const Schedule& sd, int part, int parts, int h, RowShared<DT>& sh) {
+__device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, int h, RowShared<DT>& sh) {
   using F = PagedForm<BF16, DT>;
-  constexpr int kUnit = F::kBlock * kPWaves;
   constexpr int kOC = F::kVN * F::kVW;               // O^T tiles of 16 columns
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 15, lg = l >> 4;
-  const int64_t U = sd.row_at[256];
-  const int64_t u0 = addr::paged_part_lo(U, parts, part), u1 = addr::paged_part_lo(U, parts, part + 1);
-  __syncthreads();
-  if (sd.row_at[tid] <= u0 && u0 < sd.row_at[tid + 1]) {
-    // the sequence that unit u0 is of
-    const int run = (a.B + 255) >> 8;
-    int s = tid * run;
-    int64_t at = sd.row_at[tid];
-    addr::PagedSeq sq = first_seq<false>(a, sd);
-    for (;;) {
-      const int64_t n = addr::paged_seq_units(sq, a.G, a.window, kUnit);
-      if (u0 < at + n) break;
-      at += n;
-      sq = seq_of_form<false>(a, ++s);
-    }
-    sh.seq = s;
-    sh.first = at;
-    sh.q0 = sq.q0;
-    sh.n = sq.n;
-    sh.len = sq.len;
-  }
-  __syncthreads();
-  const auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  int s = uni(sh.seq);
-  int64_t base = sh.first;                           // unit the sequence starts at
-  addr::PagedSeq sq{uni(sh.q0), uni(sh.n), uni(sh.len)};
-  int64_t u = u0;
-  while (u < u1) {
-    const int64_t su = addr::paged_seq_units(sq, a.G, a.window, kUnit);
-    if (base + su <= u) {
-      base += su;
-      ++s;
-      sq = seq_of_form<false>(a, s);
-      continue;
-    }
-    const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
-    int j = 0;
-    if (sq.n * static_cast<int64_t>(a.G) > 16) j = static_cast<int>((u - base) / nu);
-    const int64_t item = base + static_cast<int64_t>(j) * nu;       // the item's first unit
-    const int w0 = static_cast<int>(u - item);
-    const int w1 = static_cast<int>(min(static_cast<int64_t>(nu), u1 - item));
-    const addr::PagedTile tile = addr::paged_tile(sq, a.G, a.window, j);
+  const int s = it.s, j = it.j;
+  const addr::PagedSeq& sq = it.sq;
+  const addr::PagedTile tile = addr::paged_tile(sq, a.G, a.window, j);
+  int w0 = 0, w1 = it.units;
+  if (it.nparts > 1) addr::chunk_part_range(it.units, it.part, it.nparts, w0, w1);
 
   // ---- the lane's query row ---------------------------------------------
   const int64_t rows = static_cast<int64_t>(sq.n) * a.G;
@@ -325,10 +369,10 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const Schedule& sd,
   u32x4 qf[F::kSteps];
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st) {
-    const int d = (16 / F::kES) * (4 * st + lg);
-    const bool ok = live && d < a.D;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + (qe + (d < a.D ? d : 0)) * F::kES);
-    qf[st] = ok ? x : u32x4{0, 0, 0, 0};
+  const int d = (16 / F::kES) * (4 * st + lg);
+  const bool ok = live && d < a.D;
+  const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + (qe + (d < a.D ? d : 0)) * F::kES);
+  qf[st] = ok ? x : u32x4{0, 0, 0, 0};
   }
 
   float m = -INFINITY, lsum = 0.f;
@@ -346,196 +390,189 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const Schedule& sd,
   const int k_in = BF16 ? (lq & 3) : (lq & 7);                  // K row within them (+ 4 for tile 1)
   const int v_in = BF16 ? 0 : 4 * (lg & 1);
   struct Ids {
-    int k, v;
-    uint32_t k_row, v_row;
+  int k, v;
+  uint32_t k_row, v_row;
   };
   const auto ids_of = [&](int b) {
-    const int tb = tile.first + b * F::kBlock;
-    uint32_t kp, kr, vp, vr;
-    addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + k_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, kp, kr);
-    addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + v_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, vp, vr);
-    return Ids{trow[kp], trow[vp], kr * 8, vr * 8};
+  const int tb = tile.first + b * F::kBlock;
+  uint32_t kp, kr, vp, vr;
+  addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + k_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, kp, kr);
+  addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + v_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, vp, vr);
+  return Ids{trow[kp], trow[vp], kr * 8, vr * 8};
   };
   const auto load = [&](const Ids& id, PagedBlock<BF16, DT>& x) {
-    const int64_t kb = addr::paged_page(id.k, a.num_pages) * a.k_ps + h * a.k_hs + (id.k_row + k_in) * a.k_rs;
-    const int64_t vb = addr::paged_page(id.v, a.num_pages) * a.v_ps + h * a.v_hs + (id.v_row + v_in) * a.v_rs;
+  const int64_t kb = addr::paged_page(id.k, a.num_pages) * a.k_ps + h * a.k_hs + (id.k_row + k_in) * a.k_rs;
+  const int64_t vb = addr::paged_page(id.v, a.num_pages) * a.v_ps + h * a.v_hs + (id.v_row + v_in) * a.v_rs;
 #pragma unroll
-    for (int u2 = 0; u2 < F::kKT; ++u2)
+  for (int u2 = 0; u2 < F::kKT; ++u2)
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st) {
-        const int d = (16 / F::kES) * (4 * st + lg);
-        x.k[u2][st] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + (kb + 4 * u2 * a.k_rs + (d < a.D ? d : 0)) * F::kES);
-      }
+    for (int st = 0; st < F::kSteps; ++st) {
+      const int d = (16 / F::kES) * (4 * st + lg);
+      x.k[u2][st] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + (kb + 4 * u2 * a.k_rs + (d < a.D ? d : 0)) * F::kES);
+    }
 #pragma unroll
-    for (int t = 0; t < F::kKeys; ++t)
+  for (int t = 0; t < F::kKeys; ++t)
 #pragma unroll
-      for (int n = 0; n < F::kVN; ++n) {
-        const int d = n * 16 * F::kVW + F::kVW * lq;
-        x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kES>::T*>(
-            static_cast<const char*>(a.v) + (vb + t * a.v_rs + (d < a.D ? d : 0)) * F::kES);
-      }
+    for (int n = 0; n < F::kVN; ++n) {
+      const int d = n * 16 * F::kVW + F::kVW * lq;
+      x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kES>::T*>(
+          static_cast<const char*>(a.v) + (vb + t * a.v_rs + (d < a.D ? d : 0)) * F::kES);
+    }
   };
   const int hi_min = sq.len - sq.n + tile.i0 + 1;               // keys below it and from lo_max on: seen by every row
   const int lo_max = a.window > 0 ? sq.len - sq.n + tile.i1 + 1 - a.window : 0;
   const auto step = [&](int b, PagedBlock<BF16, DT>& x) {
-    const int tb = tile.first + b * F::kBlock;
-    f32x4 sacc[F::kKT];
+  const int tb = tile.first + b * F::kBlock;
+  f32x4 sacc[F::kKT];
 #pragma unroll
-    for (int u2 = 0; u2 < F::kKT; ++u2) sacc[u2] = f32x4{0, 0, 0, 0};
-    const bool pad = DT > a.D;
+  for (int u2 = 0; u2 < F::kKT; ++u2) sacc[u2] = f32x4{0, 0, 0, 0};
+  const bool pad = DT > a.D;
 #pragma unroll
-    for (int st = 0; st < F::kSteps; ++st)
+  for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
-      for (int u2 = 0; u2 < F::kKT; ++u2) {
-        u32x4 kx = x.k[u2][st];
-        if (pad && (16 / F::kES) * (4 * st + lg) >= a.D) kx = u32x4{0, 0, 0, 0};
-        if constexpr (BF16) {
-          sacc[u2] = mfma16_bf16(kx, qf[st], sacc[u2]);
-        } else {
+    for (int u2 = 0; u2 < F::kKT; ++u2) {
+      u32x4 kx = x.k[u2][st];
+      if (pad && (16 / F::kES) * (4 * st + lg) >= a.D) kx = u32x4{0, 0, 0, 0};
+      if constexpr (BF16) {
+        sacc[u2] = mfma16_bf16(kx, qf[st], sacc[u2]);
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sacc[u2] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[st][e]), sacc[u2]);
-        }
-      }
-    float sc[F::kKeys];
-#pragma unroll
-    for (int i = 0; i < F::kKeys; ++i) sc[i] = sacc[i >> 2][i & 3] * a.scale_log2;
-    const int t0 = tb + F::kKeys * lg;                           // the lane's first key
-    if (tb + F::kBlock > hi_min || tb < lo_max) {
-#pragma unroll
-      for (int i = 0; i < F::kKeys; ++i) {
-        const int t = t0 + i;
-        if (t >= hi || t < lo) sc[i] = -INFINITY;
-        // a key that no row of the tile sees may hold anything: 0 * NaN is not 0
-        if (t >= tile.ve || t < tile.vs) {
-#pragma unroll
-          for (int n = 0; n < F::kVN; ++n)
-#pragma unroll
-            for (int w = 0; w < F::kVW * F::kES / 4; ++w) x.v[i][n][w] = 0;
-        }
+        for (int e = 0; e < 4; ++e)
+          sacc[u2] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[st][e]), sacc[u2]);
       }
     }
-    float mx = sc[0];
+  float sc[F::kKeys];
 #pragma unroll
-    for (int i = 1; i < F::kKeys; ++i) mx = fmaxf(mx, sc[i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any(mx > m)) {
-      const float mn = fmaxf(m, mx);
-      const float f = m == mn ? 1.f : exp2f(m - mn);             // m = mn = -inf: nothing summed yet
-      m = mn;
-      lsum *= f;
-#pragma unroll
-      for (int c = 0; c < kOC; ++c) o[c] *= f;
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-    float p[F::kKeys];
+  for (int i = 0; i < F::kKeys; ++i) sc[i] = sacc[i >> 2][i & 3] * a.scale_log2;
+  const int t0 = tb + F::kKeys * lg;                           // the lane's first key
+  if (tb + F::kBlock > hi_min || tb < lo_max) {
 #pragma unroll
     for (int i = 0; i < F::kKeys; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
-      lsum += p[i];
+      const int t = t0 + i;
+      if (t >= hi || t < lo) sc[i] = -INFINITY;
+      // a key that no row of the tile sees may hold anything: 0 * NaN is not 0
+      if (t >= tile.ve || t < tile.vs) {
+#pragma unroll
+        for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+          for (int w = 0; w < F::kVW * F::kES / 4; ++w) x.v[i][n][w] = 0;
+      }
     }
-    if constexpr (BF16) {
-      // probabilities enter the product in bf16 (relative error 2^-8, as
-      // the values and the result have); their total stays in fp32
-      u32x4 pf;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        pf[i] = static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i])) | (static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i + 1])) << 16);
-#pragma unroll
-      for (int n = 0; n < F::kVN; ++n)
-#pragma unroll
-        for (int c = 0; c < F::kVW; ++c) {
-          u32x4 vf;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vf[i] = pair16(x.v[2 * i][n][c >> 1], x.v[2 * i + 1][n][c >> 1], c & 1);
-          o[n * F::kVW + c] = mfma16_bf16(vf, pf, o[n * F::kVW + c]);
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < F::kVN; ++n)
-#pragma unroll
-        for (int c = 0; c < F::kVW; ++c)
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[n * F::kVW + c] = mfma16_f32(__uint_as_float(x.v[t][n][c]), p[t], o[n * F::kVW + c]);
-    }
-  };
-  int b = w0 * kPWaves + wave;
-  if (b < b_end) {
-    PagedBlock<BF16, DT> cur, nxt;
-    Ids id = ids_of(b);
-    load(id, cur);
-    id = ids_of(b + kPWaves);
-    for (; b + kPWaves < b_end; b += kPWaves) {
-      const Ids id2 = ids_of(b + 2 * kPWaves);
-      load(id, nxt);
-      step(b, cur);
-      cur = nxt;
-      id = id2;
-    }
-    step(b, cur);
   }
-
-
-    // ---- the four waves' results, joined ------------------------------------------
-    lsum += __shfl_xor(lsum, 16, 64);
-    lsum += __shfl_xor(lsum, 32, 64);
-    if (lg == 0) {
-      sh.m[wave][lq] = m;
-      sh.l[wave][lq] = lsum;
-    }
+  float mx = sc[0];
+#pragma unroll
+  for (int i = 1; i < F::kKeys; ++i) mx = fmaxf(mx, sc[i]);
+  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  if (__any(mx > m)) {
+    const float mn = fmaxf(m, mx);
+    const float f = m == mn ? 1.f : exp2f(m - mn);             // m = mn = -inf: nothing summed yet
+    m = mn;
+    lsum *= f;
+#pragma unroll
+    for (int c = 0; c < kOC; ++c) o[c] *= f;
+  }
+  const float ms = m == -INFINITY ? 0.f : m;
+  float p[F::kKeys];
+#pragma unroll
+  for (int i = 0; i < F::kKeys; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
+    lsum += p[i];
+  }
+  if constexpr (BF16) {
+    // probabilities enter the product in bf16 (relative error 2^-8, as
+    // the values and the result have); their total stays in fp32
+    u32x4 pf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      pf[i] = static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i])) | (static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i + 1])) << 16);
 #pragma unroll
     for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        // O^T row 4 lg + v of tile (n, c): column 16 kVW n + kVW (4 lg + v) + c
-        const int d = n * 16 * F::kVW + F::kVW * (4 * lg + v);
+      for (int c = 0; c < F::kVW; ++c) {
+        u32x4 vf;
 #pragma unroll
-        for (int c = 0; c < F::kVW; c += 4)
-          *reinterpret_cast<f32x4*>(&sh.o[wave][lq][d + c]) =
-              f32x4{o[n * F::kVW + c][v], o[n * F::kVW + c + 1][v], o[n * F::kVW + c + 2][v], o[n * F::kVW + c + 3][v]};
+        for (int i = 0; i < 4; ++i) vf[i] = pair16(x.v[2 * i][n][c >> 1], x.v[2 * i + 1][n][c >> 1], c & 1);
+        o[n * F::kVW + c] = mfma16_bf16(vf, pf, o[n * F::kVW + c]);
       }
-    __syncthreads();
-    const bool whole = w0 == 0 && w1 == nu;
-    const int nrow = static_cast<int>(min(static_cast<int64_t>(16), rows - static_cast<int64_t>(j) * 16));
-    float* slot = nullptr;
-    if (!whole)
-      slot = a.ws + ((static_cast<int64_t>(part) * a.HK + h) * 2 + (w0 == 0 ? 1 : 0)) * addr::paged_partial_floats(DT);
-    for (int it = tid; it < nrow * (DT / 4); it += 256) {
-      const int q = it / (DT / 4), d = (it - q * (DT / 4)) * 4;
-      float M = sh.m[0][q];
+  } else {
 #pragma unroll
-      for (int w = 1; w < kPWaves; ++w) M = fmaxf(M, sh.m[w][q]);
-      const float ms = M == -INFINITY ? 0.f : M;
-      float L = 0.f;
-      f32x4 acc = {0, 0, 0, 0};
+    for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-      for (int w = 0; w < kPWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(sh.m[w][q] - ms);
-        L += f * sh.l[w][q];
-        acc += f * *reinterpret_cast<const f32x4*>(&sh.o[w][q][d]);
-      }
-      if (!whole) {
-        put_partial(slot + q * DT + d, acc);
-        if (d == 0) {
-          put_partial(slot + 16 * DT + q, M);
-          put_partial(slot + 16 * DT + 16 + q, L);
-        }
-      } else {
-        const int64_t rr = static_cast<int64_t>(j) * 16 + q;
-        const int qo = static_cast<int>(rr / a.G);
-        row_store<BF16>(a, sq.q0 + qo, h * a.G + static_cast<int>(rr - static_cast<int64_t>(qo) * a.G), d, acc, M, L);
-      }
-    }
-    if (!whole) {
-      const int first = addr::paged_part_of(U, parts, item), last = addr::paged_part_of(U, parts, item + nu - 1);
-      if (last_to_arrive(a.row_count + static_cast<int64_t>(last) * a.HK + h, last - first + 1, sh.last))
-        row_join<BF16, DT>(a, sq, j, nrow, h, first, last, sh);
-    }
-    __syncthreads();
-    u = item + w1;
+      for (int c = 0; c < F::kVW; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          o[n * F::kVW + c] = mfma16_f32(__uint_as_float(x.v[t][n][c]), p[t], o[n * F::kVW + c]);
   }
+  };
+  int b = w0 * kPWaves + wave;
+  if (b < b_end) {
+  PagedBlock<BF16, DT> cur, nxt;
+  Ids id = ids_of(b);
+  load(id, cur);
+  id = ids_of(b + kPWaves);
+  for (; b + kPWaves < b_end; b += kPWaves) {
+    const Ids id2 = ids_of(b + 2 * kPWaves);
+    load(id, nxt);
+    step(b, cur);
+    cur = nxt;
+    id = id2;
+  }
+  step(b, cur);
+  }
+
+
+  // ---- the four waves' results, joined --------------------------------------------
+  lsum += __shfl_xor(lsum, 16, 64);
+  lsum += __shfl_xor(lsum, 32, 64);
+  if (lg == 0) {
+    sh.m[wave][lq] = m;
+    sh.l[wave][lq] = lsum;
+  }
+#pragma unroll
+  for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      // O^T row 4 lg + v of tile (n, c): column 16 kVW n + kVW (4 lg + v) + c
+      const int d = n * 16 * F::kVW + F::kVW * (4 * lg + v);
+#pragma unroll
+      for (int c = 0; c < F::kVW; c += 4)
+        *reinterpret_cast<f32x4*>(&sh.o[wave][lq][d + c]) =
+            f32x4{o[n * F::kVW + c][v], o[n * F::kVW + c + 1][v], o[n * F::kVW + c + 2][v], o[n * F::kVW + c + 3][v]};
+    }
+  __syncthreads();
+  const int nrow = static_cast<int>(min(static_cast<int64_t>(16), rows - static_cast<int64_t>(j) * 16));
+  const int64_t slot0 = static_cast<int64_t>(h) * a.row_slots + it.slot;
+  float* first = a.ws + slot0 * addr::paged_partial_floats(DT);
+  float* slot = first + it.part * addr::paged_partial_floats(DT);
+  for (int x = tid; x < nrow * (DT / 4); x += 256) {
+    const int q = x / (DT / 4), d = (x - q * (DT / 4)) * 4;
+    float M = sh.m[0][q];
+#pragma unroll
+    for (int w = 1; w < kPWaves; ++w) M = fmaxf(M, sh.m[w][q]);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kPWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(sh.m[w][q] - ms);
+      L += f * sh.l[w][q];
+      acc += f * *reinterpret_cast<const f32x4*>(&sh.o[w][q][d]);
+    }
+    if (it.nparts > 1) {
+      put_partial(slot + q * DT + d, acc);
+      if (d == 0) {
+        put_partial(slot + 16 * DT + q, M);
+        put_partial(slot + 16 * DT + 16 + q, L);
+      }
+    } else {
+      const int64_t rr = static_cast<int64_t>(j) * 16 + q;
+      const int qo = static_cast<int>(rr / a.G);
+      row_store<BF16>(a, sq.q0 + qo, h * a.G + static_cast<int>(rr - static_cast<int64_t>(qo) * a.G), d, acc, M, L);
+    }
+  }
+  if (it.nparts > 1 && last_to_arrive(a.row_count + slot0, it.nparts, sh.last))
+    row_join<BF16, DT>(a, sq, j, nrow, h, first, it.nparts, sh);
 }
 
 }  // namespace

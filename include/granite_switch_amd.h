@@ -576,7 +576,7 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * GS_PAGED_HEAD_BYTES are ZEROED before the first call (counters: every call
  * leaves them zero, so calls of any sizes may share one), the rest needs no
  * initialisation.  Calls that may overlap in time must not share one. */
-#define GS_PAGED_HEAD_BYTES 8192
+#define GS_PAGED_HEAD_BYTES 65536
 int64_t gs_paged_attention_workspace_bytes(int32_t dtype, int32_t heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t ragged);
 int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,

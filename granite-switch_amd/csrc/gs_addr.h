@@ -326,18 +326,13 @@ GS_HD int paged_tile_units(const PagedSeq& s, int G, int window, int unit) {
 GS_HD int64_t paged_seq_units(const PagedSeq& s, int G, int window, int unit) {
   return s.n == 0 ? 0 : static_cast<int64_t>(paged_tiles(s, G)) * paged_tile_units(s, G, window, unit);
 }
-// Times the workgroups are filled by `items` items a head: up to four.
-GS_HD int row_rounds(int64_t items, int HK, int wgs) {
-  const int64_t r = items * HK / wgs;
-  return r >= 4 ? 4 : r < 1 ? 1 : static_cast<int>(r);
-}
-// Units of a part at most, for `items` items of U units in all a head, on `wgs`
-// workgroups: an equal share of them, or of up to four times as many where there are
-// that many items, and four units at least.
-GS_HD int row_part_units(int64_t U, int items, int HK, int wgs) {
-  const int64_t n = static_cast<int64_t>(wgs) * row_rounds(items, HK, wgs);
-  const int64_t u = (U * HK + n - 1) / n;
-  return u < 4 ? 4 : static_cast<int>(u);
+// Units of a part at most, for U units in all a head on `wgs` workgroups: an equal share
+// of them.  Four times as many parts, where there are that many items, took 10% more of a
+// batch of 256 contexts: each costs its start; parts of four units at least took 7% more
+// of a window's 16.
+GS_HD int row_part_units(int64_t U, int HK, int wgs) {
+  const int64_t u = (U * HK + wgs - 1) / wgs;
+  return u < 1 ? 1 : static_cast<int>(u);
 }
 constexpr int kMostParts = 512;      // of an item
 GS_HD int row_parts(int units, int most, uint32_t magic) {
@@ -346,12 +341,10 @@ GS_HD int row_parts(int units, int most, uint32_t magic) {
   return q < kMostParts ? static_cast<int>(q) : kMostParts;
 }
 // Partial results of a head at most: an item of u > part units has u / part + 1 < 2 u /
-// part of them, and U / part <= 4 wgs / HK.
-GS_HD int row_slots_per_head(int HK, int wgs) { return (8 * wgs + HK - 1) / HK + 1; }
+// part of them, and U / part <= wgs / HK.
+GS_HD int row_slots_per_head(int HK, int wgs) { return (2 * wgs + HK - 1) / HK + 1; }
 // Parts of a head at most, for that many items: each one, and U / part more.
-GS_HD int64_t row_most_parts(int64_t items, int HK, int wgs) {
-  return items + (static_cast<int64_t>(wgs) * row_rounds(items, HK, wgs) + HK - 1) / HK;
-}
+GS_HD int64_t row_most_parts(int64_t items, int HK, int wgs) { return items + (wgs + HK - 1) / HK; }
 // Workgroup w of a ragged launch: blocks of `block` (a multiple of 8) chunk parts and
 // row parts in turn while there are row_blocks of these, then chunk parts.  True: row
 // part i; false: chunk part i.

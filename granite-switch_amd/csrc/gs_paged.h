@@ -32,6 +32,7 @@ struct PagedArgs {
   int B, T, H, HK, G, D;
   int window;
   int row_wgs;                      // workgroups that the row form fills
+  int64_t row_parts;                // its parts for each head, at most
   int row_slots;                    // its partial results for each head
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
   int chunk_slots;                  // workgroups that the chunk form fills

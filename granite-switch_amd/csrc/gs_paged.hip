@@ -74,10 +74,9 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.row_wgs = row_wgs_for(a.D, cus);
   a.ragged_block = (cus + 7) & ~7;
   a.row_blocks = 0;
-  if (a.row_limit != INT32_MAX) {                    // beside the chunk form: half the workgroups
-    a.row_wgs = cus;
-    a.row_blocks = static_cast<int>((row_most_parts(a) * a.HK + a.ragged_block - 1) / a.ragged_block);
-  }
+  if (a.row_limit != INT32_MAX) a.row_wgs = cus;     // beside the chunk form: half the workgroups
+  a.row_parts = row_most_parts(a);
+  if (a.row_limit != INT32_MAX) a.row_blocks = static_cast<int>((a.row_parts * a.HK + a.ragged_block - 1) / a.ragged_block);
   a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
   a.tq.tq = std::max(1, addr::chunk_tq(kChunkRows, a.G));
   a.tq.magic = addr::div_magic(a.tq.tq);
@@ -87,7 +86,7 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
 
 template <bool BF16, int DT>
 void launch_paged(const PagedArgs& a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(row_most_parts(a) * a.HK));
+  const dim3 grid(static_cast<unsigned>(a.row_parts * a.HK));
   hipLaunchKernelGGL((paged_attention_kernel<BF16, DT>), grid, dim3(256), 0, st, a);
 }
 
@@ -106,13 +105,9 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   const int64_t o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
   std::vector<char> slots(static_cast<size_t>(a.row_slots), 0);
   std::vector<char>& rows = m.rows;
-  int64_t U = 0, items = 0;
-  for (int s = 0; s < a.B; ++s) {
-    const addr::PagedSeq sq = seq_of_form<false>(a, s);
-    U += addr::paged_seq_units(sq, a.G, a.window, kUnit);
-    items += addr::paged_tiles(sq, a.G);
-  }
-  const int most = addr::row_part_units(U, static_cast<int>(items), a.HK, a.row_wgs);
+  int64_t U = 0;
+  for (int s = 0; s < a.B; ++s) U += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
+  const int most = addr::row_part_units(U, a.HK, a.row_wgs);
   const uint32_t magic = addr::div_magic(most);
   int64_t parts = 0, slot = 0;
   for (int s = 0; s < a.B && !m.bad; ++s) {
@@ -190,7 +185,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
       }
     }
   }
-  const int64_t grid = row_most_parts(a);
+  const int64_t grid = a.row_parts;
   m.in("parts", 0, parts, grid);
   if (a.row_limit == INT32_MAX) return;
   // a ragged launch: every part of either form has one workgroup
@@ -389,7 +384,7 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
     GS_CHECK_LAUNCH(who);
     return GS_OK;
   }
-  GS_CHECK_ARG(row_most_parts(a) * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
+  GS_CHECK_ARG(a.row_parts * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
   switch (DT) {
     case 64: bf16 ? launch_paged<true, 64>(a, st) : launch_paged<false, 64>(a, st); break;
     case 128: bf16 ? launch_paged<true, 128>(a, st) : launch_paged<false, 128>(a, st); break;

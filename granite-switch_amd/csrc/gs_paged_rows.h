@@ -3,12 +3,12 @@
 // kernel (gs_paged.hip) and the kernel for ragged batches (gs_chunk.hip).
 //
 // An item is a tile of 16 rows of a sequence for one key/value head, a run of units
-// of 128 keys (fp32: 64).  A workgroup has one item, or one part of an item of many
-// units: few, long sequences are cut so that the GPU is filled once, many into parts
-// of at most twice a quarter of a workgroup's share, which level out.  A part leaves a
-// partial result; the last of an item's workgroups to be done joins them, in the order
-// of the keys.  (Equal runs of the batch's units, cut wherever they end, cost two
-// joins a workgroup and 114 us against XX for 256 sequences of 16 .. 2048 keys.)
+// of 128 keys (fp32: 64).  A workgroup has one item, or one part of an item of more
+// units than a workgroup's equal share.  A part leaves a partial result; the last of an
+// item's workgroups to be done joins them, in the order of the keys.  The longest parts
+// start first: 110 us against 117 for 256 sequences of 16 .. 2047 keys (4 key/value
+// heads of 128, bf16).  Equal runs of the batch's units, cut wherever they end, cost two
+// joins a workgroup and took 114.
 #pragma once
 
 #include "gs_paged.h"
@@ -88,7 +88,8 @@ struct RowShared {
 struct Schedule {
   int q0[256], n[256], len[256];     // a thread's first sequence: its only one up to 256
   int64_t sum[kPWaves];
-  int items[kPWaves], slots[kPWaves];
+  uint64_t lo[kPWaves], hi[kPWaves];
+  int slots[kPWaves];
   int found[8];
 };
 // The thread's first sequence as a form sees it.
@@ -109,16 +110,6 @@ __device__ __forceinline__ void load_schedule(const PagedArgs& a, Schedule& sd) 
   sd.len[tid] = sq.len;
 }
 
-__device__ __forceinline__ int wave_scan(int v) {
-  const int l = lane_id();
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d, 64);
-    if (l >= d) v += u;
-  }
-  return v;
-}
-
 // One part of the row form's work.
 struct RowItem {
   int s, j, part, nparts, slot;      // slot: of the item's first partial result, or -1
@@ -137,56 +128,79 @@ __device__ __forceinline__ RowItem find_row(const PagedArgs& a, Schedule& sd, in
   const addr::PagedSeq first = first_seq<false>(a, sd);
   addr::PagedSeq sq = first;
   int64_t U = 0;
-  int items = 0;
   for (int s = s0; s < s1; ++s) {
     if (s > s0) sq = seq_of_form<false>(a, s);
     U += addr::paged_seq_units(sq, a.G, a.window, kUnit);
-    items += addr::paged_tiles(sq, a.G);
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    U += __shfl_xor(U, d, 64);
-    items += __shfl_xor(items, d, 64);
-  }
-  if (l == 0) {
-    sd.sum[wave] = U;
-    sd.items[wave] = items;
-  }
+  for (int d = 32; d; d >>= 1) U += __shfl_xor(U, d, 64);
+  if (l == 0) sd.sum[wave] = U;
   if (tid == 0) sd.found[0] = -1;
   __syncthreads();
   U = 0;
-  items = 0;
 #pragma unroll
-  for (int w = 0; w < kPWaves; ++w) {
-    U += sd.sum[w];
-    items += sd.items[w];
-  }
-  const int most = addr::row_part_units(U, items, a.HK, a.row_wgs);
+  for (int w = 0; w < kPWaves; ++w) U += sd.sum[w];
+  const int most = addr::row_part_units(U, a.HK, a.row_wgs);
   const uint32_t magic = addr::div_magic(most);
-  int parts = 0, slots = 0;
+  int parts = 0, slots = 0, longest = 0;
   sq = first;
   for (int s = s0; s < s1; ++s) {
     if (s > s0) sq = seq_of_form<false>(a, s);
     const int nt = addr::paged_tiles(sq, a.G);
-    const int np = addr::row_parts(addr::paged_tile_units(sq, a.G, a.window, kUnit), most, magic);
+    const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
+    const int np = addr::row_parts(nu, most, magic);
     parts += nt * np;
     slots += np > 1 ? nt * np : 0;
+    longest = max(longest, np > 1 ? most : nu);
   }
-  int at = wave_scan(parts), sl = wave_scan(slots);
-  __syncthreads();
+  // Order: by length, in eight classes, the longest first; within one by sequence.
+  // Eight 16-bit counts in two words; too many parts for them, one class.
+  const bool classes = a.row_parts < 65536;
+  uint32_t cls, rest;
+  addr::div_by(static_cast<uint32_t>(8 * (most - longest)), static_cast<uint32_t>(most), magic, cls, rest);
+  cls = classes ? min(cls, 7u) : 0;
+  const uint64_t one = static_cast<uint64_t>(parts) << (classes ? 16 * (cls & 3) : 0);
+  uint64_t lo = cls < 4 ? one : 0, hi = cls < 4 ? 0 : one;
+  int sl = slots;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t u = __shfl_up(lo, d, 64), v = __shfl_up(hi, d, 64);
+    const int w = __shfl_up(sl, d, 64);
+    if (l >= d) {
+      lo += u;
+      hi += v;
+      sl += w;
+    }
+  }
   if (l == 63) {
-    sd.items[wave] = at;
+    sd.lo[wave] = lo;
+    sd.hi[wave] = hi;
     sd.slots[wave] = sl;
   }
   __syncthreads();
-  at -= parts;
+  uint64_t all_lo = 0, all_hi = 0;
   sl -= slots;
 #pragma unroll
-  for (int w = 0; w < kPWaves; ++w)
+  for (int w = 0; w < kPWaves; ++w) {
+    const uint64_t x = sd.lo[w], y = sd.hi[w];
+    all_lo += x;
+    all_hi += y;
     if (w < wave) {
-      at += sd.items[w];
+      lo += x;
+      hi += y;
       sl += sd.slots[w];
     }
+  }
+  int at;
+  if (classes) {
+    constexpr uint64_t kOnes = 0x0001000100010001;   // times it: sums of the fields up to each
+    const uint64_t to_lo = all_lo * kOnes, to_hi = all_hi * kOnes + (to_lo >> 48) * kOnes;
+    const int sh16 = 16 * (cls & 3);
+    const uint64_t to = cls < 4 ? to_lo : to_hi, all = cls < 4 ? all_lo : all_hi, own = cls < 4 ? lo : hi;
+    at = static_cast<int>(((to >> sh16) & 65535) - ((all >> sh16) & 65535) + ((own >> sh16) & 65535)) - parts;
+  } else {
+    at = static_cast<int>(lo) - parts;
+  }
   if (r >= at && r < at + parts) {
     sq = first;
     for (int s = s0;; ++s) {
@@ -357,170 +371,183 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
   int w0 = 0, w1 = it.units;
   if (it.nparts > 1) addr::chunk_part_range(it.units, it.part, it.nparts, w0, w1);
 
-  // ---- the lane's query row ---------------------------------------------
+  // ---- the lane's query row ---------------------------------------------------------
   const int64_t rows = static_cast<int64_t>(sq.n) * a.G;
   const int64_t r = static_cast<int64_t>(j) * 16 + lq;
   const bool live = r < rows;
-  const int qi = live ? static_cast<int>(r / a.G) : tile.i0;
-  const int qh = h * a.G + (live ? static_cast<int>(r - static_cast<int64_t>(qi) * a.G) : 0);
-  const int hi = live ? sq.len - sq.n + qi + 1 : 0;             // sees [lo, hi)
+  int qi = tile.i0, qh = h * a.G;
+  if (live) {
+    if (rows <= 16) {                                // the one tile: small numbers
+      uint32_t x, y;
+      addr::div_by(lq, a.G, a.g_magic, x, y);
+      qi = static_cast<int>(x);
+      qh += static_cast<int>(y);
+    } else {
+      qi = static_cast<int>(r / a.G);
+      qh += static_cast<int>(r - static_cast<int64_t>(qi) * a.G);
+    }
+  }
+  const int hi = live ? sq.len - sq.n + qi + 1 : 0;  // sees [lo, hi)
   const int lo = a.window > 0 ? hi - a.window : 0;
   const int64_t qe = static_cast<int64_t>(sq.q0 + qi) * a.q_ts + static_cast<int64_t>(qh) * a.q_hs;
+  constexpr int kVec = 16 / F::kES;
   u32x4 qf[F::kSteps];
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st) {
-  const int d = (16 / F::kES) * (4 * st + lg);
-  const bool ok = live && d < a.D;
-  const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + (qe + (d < a.D ? d : 0)) * F::kES);
-  qf[st] = ok ? x : u32x4{0, 0, 0, 0};
+    const int d = kVec * (4 * st + lg);
+    const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + (qe + (d < a.D ? d : 0)) * F::kES);
+    qf[st] = live && d < a.D ? x : u32x4{0, 0, 0, 0};
   }
-
   float m = -INFINITY, lsum = 0.f;
   f32x4 o[kOC];
 #pragma unroll
   for (int c = 0; c < kOC; ++c) o[c] = f32x4{0, 0, 0, 0};
 
-  // ---- its keys -----------------------------------------------------------
+  // ---- its keys ---------------------------------------------------------------------
   const int nblk = (tile.ve - tile.first + F::kBlock - 1) / F::kBlock;
   const int b_end = min(w1 * kPWaves, nblk);
   const int32_t* trow = a.table + static_cast<int64_t>(s) * a.ld_table;
   // first keys of the 8 that the lane's K rows and its V rows are of
   const int k_oct = BF16 ? 8 * (lq >> 2) : 8 * (lq >> 3);
   const int v_oct = BF16 ? 8 * lg : 8 * (lg >> 1);
-  const int k_in = BF16 ? (lq & 3) : (lq & 7);                  // K row within them (+ 4 for tile 1)
+  const int k_in = BF16 ? (lq & 3) : (lq & 7);       // K row within them (+ 4 for tile 1)
   const int v_in = BF16 ? 0 : 4 * (lg & 1);
+  const char* k_head = static_cast<const char*>(a.k) + static_cast<int64_t>(h) * a.k_hs * F::kES;
+  const char* v_head = static_cast<const char*>(a.v) + static_cast<int64_t>(h) * a.v_hs * F::kES;
   struct Ids {
-  int k, v;
-  uint32_t k_row, v_row;
+    int k, v;
+    uint32_t k_row, v_row;
   };
   const auto ids_of = [&](int b) {
-  const int tb = tile.first + b * F::kBlock;
-  uint32_t kp, kr, vp, vr;
-  addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + k_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, kp, kr);
-  addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + v_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, vp, vr);
-  return Ids{trow[kp], trow[vp], kr * 8, vr * 8};
+    const int tb = tile.first + b * F::kBlock;
+    uint32_t kp, kr, vp, vr;
+    addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + k_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, kp, kr);
+    addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + v_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, vp, vr);
+    return Ids{trow[kp], trow[vp], kr * 8 + k_in, vr * 8 + v_in};
   };
   const auto load = [&](const Ids& id, PagedBlock<BF16, DT>& x) {
-  const int64_t kb = addr::paged_page(id.k, a.num_pages) * a.k_ps + h * a.k_hs + (id.k_row + k_in) * a.k_rs;
-  const int64_t vb = addr::paged_page(id.v, a.num_pages) * a.v_ps + h * a.v_hs + (id.v_row + v_in) * a.v_rs;
+    const char* kp = k_head + (addr::paged_page(id.k, a.num_pages) * a.k_ps + id.k_row * a.k_rs) * F::kES;
+    const char* vp = v_head + (addr::paged_page(id.v, a.num_pages) * a.v_ps + id.v_row * a.v_rs) * F::kES;
 #pragma unroll
-  for (int u2 = 0; u2 < F::kKT; ++u2)
+    for (int t = 0; t < F::kKT; ++t)
 #pragma unroll
-    for (int st = 0; st < F::kSteps; ++st) {
-      const int d = (16 / F::kES) * (4 * st + lg);
-      x.k[u2][st] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + (kb + 4 * u2 * a.k_rs + (d < a.D ? d : 0)) * F::kES);
-    }
+      for (int st = 0; st < F::kSteps; ++st) {
+        const int d = kVec * (4 * st + lg);
+        x.k[t][st] = *reinterpret_cast<const u32x4*>(kp + (4 * t * a.k_rs + (d < a.D ? d : 0)) * F::kES);
+      }
 #pragma unroll
-  for (int t = 0; t < F::kKeys; ++t)
+    for (int t = 0; t < F::kKeys; ++t)
 #pragma unroll
-    for (int n = 0; n < F::kVN; ++n) {
-      const int d = n * 16 * F::kVW + F::kVW * lq;
-      x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kES>::T*>(
-          static_cast<const char*>(a.v) + (vb + t * a.v_rs + (d < a.D ? d : 0)) * F::kES);
-    }
+      for (int n = 0; n < F::kVN; ++n) {
+        const int d = n * 16 * F::kVW + F::kVW * lq;
+        x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kES>::T*>(vp + (t * a.v_rs + (d < a.D ? d : 0)) * F::kES);
+      }
   };
-  const int hi_min = sq.len - sq.n + tile.i0 + 1;               // keys below it and from lo_max on: seen by every row
+  const int hi_min = sq.len - sq.n + tile.i0 + 1;    // keys below it and from lo_max on: seen by every row
   const int lo_max = a.window > 0 ? sq.len - sq.n + tile.i1 + 1 - a.window : 0;
-  const auto step = [&](int b, PagedBlock<BF16, DT>& x) {
-  const int tb = tile.first + b * F::kBlock;
-  f32x4 sacc[F::kKT];
-#pragma unroll
-  for (int u2 = 0; u2 < F::kKT; ++u2) sacc[u2] = f32x4{0, 0, 0, 0};
   const bool pad = DT > a.D;
+
+  const auto step = [&](int b, PagedBlock<BF16, DT>& x) {
+    const int tb = tile.first + b * F::kBlock;
+    f32x4 sacc[F::kKT];
 #pragma unroll
-  for (int st = 0; st < F::kSteps; ++st)
+    for (int t = 0; t < F::kKT; ++t) sacc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int u2 = 0; u2 < F::kKT; ++u2) {
-      u32x4 kx = x.k[u2][st];
-      if (pad && (16 / F::kES) * (4 * st + lg) >= a.D) kx = u32x4{0, 0, 0, 0};
-      if constexpr (BF16) {
-        sacc[u2] = mfma16_bf16(kx, qf[st], sacc[u2]);
-      } else {
+    for (int st = 0; st < F::kSteps; ++st)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          sacc[u2] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[st][e]), sacc[u2]);
+      for (int t = 0; t < F::kKT; ++t) {
+        u32x4 kx = x.k[t][st];
+        if (pad && kVec * (4 * st + lg) >= a.D) kx = u32x4{0, 0, 0, 0};
+        if constexpr (BF16) {
+          sacc[t] = mfma16_bf16(kx, qf[st], sacc[t]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sacc[t] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[st][e]), sacc[t]);
+        }
+      }
+    float sc[F::kKeys];
+#pragma unroll
+    for (int i = 0; i < F::kKeys; ++i) sc[i] = sacc[i >> 2][i & 3] * a.scale_log2;
+    if (tb + F::kBlock > hi_min || tb < lo_max) {
+      const int t0 = tb + F::kKeys * lg;           // the lane's first key
+#pragma unroll
+      for (int i = 0; i < F::kKeys; ++i) {
+        const int t = t0 + i;
+        if (t >= hi || t < lo) sc[i] = -INFINITY;
+        // a key that no row of the tile sees may hold anything: 0 * NaN is not 0
+        if (t >= tile.ve || t < tile.vs) {
+#pragma unroll
+          for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+            for (int w = 0; w < F::kVW * F::kES / 4; ++w) x.v[i][n][w] = 0;
+        }
       }
     }
-  float sc[F::kKeys];
+    float mx = sc[0];
 #pragma unroll
-  for (int i = 0; i < F::kKeys; ++i) sc[i] = sacc[i >> 2][i & 3] * a.scale_log2;
-  const int t0 = tb + F::kKeys * lg;                           // the lane's first key
-  if (tb + F::kBlock > hi_min || tb < lo_max) {
+    for (int i = 1; i < F::kKeys; ++i) mx = fmaxf(mx, sc[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    // the reference point follows the maximum once it has grown by 2^8: the sums
+    // stay far from their limits, and o is rarely scaled
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);   // m = mn = -inf: nothing summed yet
+      m = mn;
+      lsum *= f;
+#pragma unroll
+      for (int c = 0; c < kOC; ++c) o[c] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    float p[F::kKeys];
 #pragma unroll
     for (int i = 0; i < F::kKeys; ++i) {
-      const int t = t0 + i;
-      if (t >= hi || t < lo) sc[i] = -INFINITY;
-      // a key that no row of the tile sees may hold anything: 0 * NaN is not 0
-      if (t >= tile.ve || t < tile.vs) {
-#pragma unroll
-        for (int n = 0; n < F::kVN; ++n)
-#pragma unroll
-          for (int w = 0; w < F::kVW * F::kES / 4; ++w) x.v[i][n][w] = 0;
-      }
+      p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
+      lsum += p[i];
     }
-  }
-  float mx = sc[0];
+    if constexpr (BF16) {
+      // probabilities enter the product in bf16 (relative error 2^-8, as the
+      // values and the result have); their total stays in fp32
+      u32x4 pf;
 #pragma unroll
-  for (int i = 1; i < F::kKeys; ++i) mx = fmaxf(mx, sc[i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  if (__any(mx > m)) {
-    const float mn = fmaxf(m, mx);
-    const float f = m == mn ? 1.f : exp2f(m - mn);             // m = mn = -inf: nothing summed yet
-    m = mn;
-    lsum *= f;
+      for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
 #pragma unroll
-    for (int c = 0; c < kOC; ++c) o[c] *= f;
-  }
-  const float ms = m == -INFINITY ? 0.f : m;
-  float p[F::kKeys];
+      for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-  for (int i = 0; i < F::kKeys; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
-    lsum += p[i];
-  }
-  if constexpr (BF16) {
-    // probabilities enter the product in bf16 (relative error 2^-8, as
-    // the values and the result have); their total stays in fp32
-    u32x4 pf;
+        for (int c = 0; c < F::kVW; ++c) {
+          u32x4 vf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      pf[i] = static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i])) | (static_cast<uint32_t>(f32_to_bf16_bits(p[2 * i + 1])) << 16);
+          for (int i = 0; i < 4; ++i) vf[i] = pair16(x.v[2 * i][n][c >> 1], x.v[2 * i + 1][n][c >> 1], c & 1);
+          o[n * F::kVW + c] = mfma16_bf16(vf, pf, o[n * F::kVW + c]);
+        }
+    } else {
 #pragma unroll
-    for (int n = 0; n < F::kVN; ++n)
+      for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-      for (int c = 0; c < F::kVW; ++c) {
-        u32x4 vf;
+        for (int c = 0; c < F::kVW; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vf[i] = pair16(x.v[2 * i][n][c >> 1], x.v[2 * i + 1][n][c >> 1], c & 1);
-        o[n * F::kVW + c] = mfma16_bf16(vf, pf, o[n * F::kVW + c]);
-      }
-  } else {
-#pragma unroll
-    for (int n = 0; n < F::kVN; ++n)
-#pragma unroll
-      for (int c = 0; c < F::kVW; ++c)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          o[n * F::kVW + c] = mfma16_f32(__uint_as_float(x.v[t][n][c]), p[t], o[n * F::kVW + c]);
-  }
+          for (int t = 0; t < 4; ++t)
+            o[n * F::kVW + c] = mfma16_f32(__uint_as_float(x.v[t][n][c]), p[t], o[n * F::kVW + c]);
+    }
   };
+  // A block's loads are issued before the one ahead of it is used (one buffer, its keys
+  // and its values refilled in turn, and three workgroups a CU: 141 us against 124 for
+  // 256 sequences of 16 .. 2047 keys then), and page ids one block before them.
   int b = w0 * kPWaves + wave;
   if (b < b_end) {
-  PagedBlock<BF16, DT> cur, nxt;
-  Ids id = ids_of(b);
-  load(id, cur);
-  id = ids_of(b + kPWaves);
-  for (; b + kPWaves < b_end; b += kPWaves) {
-    const Ids id2 = ids_of(b + 2 * kPWaves);
-    load(id, nxt);
+    PagedBlock<BF16, DT> cur, nxt;
+    Ids id = ids_of(b);
+    load(id, cur);
+    id = ids_of(b + kPWaves);
+    for (; b + kPWaves < b_end; b += kPWaves) {
+      const Ids id2 = ids_of(b + 2 * kPWaves);
+      load(id, nxt);
+      step(b, cur);
+      cur = nxt;
+      id = id2;
+    }
     step(b, cur);
-    cur = nxt;
-    id = id2;
   }
-  step(b, cur);
-  }
-
 
   // ---- the four waves' results, joined --------------------------------------------
   lsum += __shfl_xor(lsum, 16, 64);

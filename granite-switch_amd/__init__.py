@@ -11,6 +11,7 @@ driven from Python on PyTorch-ROCm:
   hf_layers    HF-form ``SwitchedLoRALinear`` / ``MergedSwitchedLoRALinear``
   paged        paged key/value cache: rotated append, attention over it
   norms        the residual add between blocks with the norms around it
+  decoder      a decoder over the paged cache, put together from the above
   probe_routing  drop-in for ``granite_switch.probe_routing`` (probe-slot split)
   workloads    seeded synthetic benchmark shapes
 

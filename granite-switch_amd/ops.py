@@ -8,7 +8,8 @@ registers the same op names with the same argument lists, ``mutates_args`` and
 fake implementations, so callers such as ``SwitchedLoRALinear._run_expand``
 (src/granite_switch/vllm/core/lora.py:659-686) and ``WCrossShunt.forward``
 (src/granite_switch/vllm/decoder/shadow_residual/wcross_shunt.py:198-242) run
-unchanged on MI355X, plus three new ops for the y-given switched-LoRA path.
+unchanged on MI355X, plus three new ops for the y-given switched-LoRA path and
+four for the paged cache and the norms around the residual add.
 
 Only one provider of the ``granite_switch`` ops can be loaded in a process.
 """
@@ -17,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from . import kernels, switched
+from . import kernels, norms, paged, switched
 
 _NS = "granite_switch"
 
@@ -153,6 +154,62 @@ if not _registered("switched_lora_expand_add"):
     @switched_lora_expand_add.register_fake
     def _(y, z, seg_offsets, perm, b_pack, b_off, ranks, slice_bounds, max_rank):
         return None
+
+
+# ---------------------------------------------------------------------------
+# The paged cache and the residual stream
+# ---------------------------------------------------------------------------
+if not _registered("cache_slots"):
+
+    @torch.library.custom_op(f"{_NS}::cache_slots", mutates_args=())
+    def cache_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int, num_pages: int,
+                    cu_seqlens: torch.Tensor | None, num_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+        return paged.cache_slots(page_table, kv_lens, page_size, num_pages, cu_seqlens, num_tokens)
+
+    @cache_slots.register_fake
+    def _(page_table, kv_lens, page_size, num_pages, cu_seqlens, num_tokens):
+        return (torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device),
+                torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device))
+
+
+if not _registered("append_kv"):
+
+    @torch.library.custom_op(f"{_NS}::append_kv", mutates_args=("k_cache", "v_cache"))
+    def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
+                  interleaved: bool) -> torch.Tensor:
+        return paged.append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved=interleaved)
+
+    @append_kv.register_fake
+    def _(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved):
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+if not _registered("paged_attention"):
+
+    @torch.library.custom_op(f"{_NS}::paged_attention", mutates_args=())
+    def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                        kv_lens: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float | None, window: int,
+                        max_q: int | None) -> torch.Tensor:
+        return paged.paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, max_q=max_q)
+
+    @paged_attention.register_fake
+    def _(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, max_q):
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+if not _registered("residual_norm"):
+
+    @torch.library.custom_op(f"{_NS}::residual_norm", mutates_args=())
+    def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, scale: float,
+                      gate: torch.Tensor | None, post_weight: torch.Tensor | None,
+                      gate_act: str | None) -> tuple[torch.Tensor, torch.Tensor]:
+        return norms.residual_norm(x, residual, weight, eps, scale, gate, post_weight, gate_act)
+
+    @residual_norm.register_fake
+    def _(x, residual, weight, eps, scale, gate, post_weight, gate_act):
+        return (torch.empty(x.shape, dtype=x.dtype, device=x.device),
+                torch.empty(residual.shape, dtype=residual.dtype, device=residual.device))
 
 
 def op(name: str):

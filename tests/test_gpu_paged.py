@@ -217,6 +217,38 @@ def test_rows_that_see_nothing(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("batch,most,window", [(2, 20000, 0), (40, 6000, 0), (256, 2000, 0), (300, 900, 0), (40, 6000, 700)])
+def test_decode_uneven(dev, dtype, batch, most, window):
+    """Lengths from none to many times the mean: parts of all sizes, some items cut, some whole."""
+    _say(f"decode uneven {dtype} {batch} up to {most} window {window}")
+    rng = np.random.default_rng(batch)
+    lens = (most * rng.random(batch) ** 4).astype(int)
+    lens[0] = most
+    b = Batch(dev, [1] * batch, [x - 1 for x in lens.tolist()], 4, 2, 64, 16, dtype, seed=batch, decode=True)
+    lse = torch.empty(batch, 4, device=dev)
+    out = b.run(lse=lse, window=window)
+    torch.cuda.synchronize()
+    b.check(out, lse=lse, window=window)
+
+
+@pytest.mark.parametrize("heads,kv,dim,batch,most,window", [(8, 2, 128, 24, 7000, 0), (8, 2, 64, 24, 7000, 600),
+                                                            (4, 4, 128, 330, 700, 0), (16, 1, 96, 12, 3000, 0)])
+def test_ragged_uneven(dev, heads, kv, dim, batch, most, window):
+    """Decode rows, short and long chunks in one batch, over caches of all lengths: both forms, tiles cut and whole."""
+    _say(f"ragged uneven {heads}/{kv} x {dim} {batch} up to {most} window {window}")
+    rng = np.random.default_rng(heads + batch)
+    n = rng.choice([0, 1, 1, 2, 3, 4, 5, 17, 64, 129], size=batch).tolist()
+    cached = (most * rng.random(batch) ** 4).astype(int)
+    cached[-1] = most
+    n[-1] = 40
+    b = Batch(dev, n, cached.tolist(), heads, kv, dim, 16, BF16, seed=batch)
+    lse = torch.empty(sum(n), heads, device=dev)
+    out = b.run(window=window, lse=lse)
+    torch.cuda.synchronize()
+    b.check(out, window=window, lse=lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_large_pool(dev, dtype):
     """Element offsets past 2^32: the pool's last page is used."""
     dim, kv, page = 128, 2, 16

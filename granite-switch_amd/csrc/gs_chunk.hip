@@ -461,13 +461,14 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
   }
   float* p = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot + it.part) *
                               addr::chunk_partial_floats(kChunkRows, DT);
-  if (live) {
+  if (wave_live) {                                   // in the order of the registers: whole lines
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
 #pragma unroll
       for (int v = 0; v < 16; v += 4)
-        *reinterpret_cast<f32x4*>(p + r * DT + 32 * d + mfma32_row(v, l)) = f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
-    if (hl == 0) {
+        *reinterpret_cast<f32x4*>(p + ((((wave * kDT + d) * 4 + (v >> 2)) * 64 + l) << 2)) =
+            f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+    if (hl == 0 && live) {
       p[kChunkRows * DT + r] = m;
       p[kChunkRows * (DT + 1) + r] = lsum;
     }
@@ -476,23 +477,23 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
 }
 
 // The split tiles' parts, joined in the order of their keys: workgroups take (tile,
-// 16 rows, head) in turn, a thread 4 columns of a row, 8 parts' loads in flight.  (A
-// workgroup that joined its tile at the end of the launch above would read all its
-// parts alone: 14 parts of 128 rows took it 50 us.)
-constexpr int kJoinRows = 16;
+// an eighth of it, head) in turn, a thread 4 columns of a row, 8 parts' loads in
+// flight.  (A workgroup that joined its tile at the end of the launch above would read
+// all its parts alone: 14 parts of 128 rows took it 50 us.)
 template <int DT>
 __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
   constexpr int kBatch = 8;
-  constexpr int kGroups = kChunkRows / kJoinRows;
+  constexpr int kGroups = 8, kDT = DT / 32;
   const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
   const int total = a.chunk_list[0].x * kGroups * a.HK;
   for (int w = blockIdx.x; w < total; w += gridDim.x) {
     const int h = w % a.HK, g = (w / a.HK) % kGroups;
     const int4 e = a.chunk_list[1 + w / (a.HK * kGroups)];
     const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + e.w) * size;
-    for (int x = threadIdx.x; x < kJoinRows * (DT / 4); x += 256) {
-      const int jr = g * kJoinRows + x / (DT / 4), d = (x % (DT / 4)) * 4;
-      if (jr >= e.y) break;
+    for (int y = threadIdx.x; y < 128 * kDT; y += 256) {
+      const int x = g * 128 * kDT + y, l = x & 63;   // the x-th four floats: chunk_part's order
+      const int jr = x / (256 * kDT) * 32 + (l & 31), d = (x / 256 % kDT) * 32 + ((x >> 6) & 3) * 8 + (l >> 5) * 4;
+      if (jr >= e.y) continue;
       float M = -INFINITY, L = 0.f;
       f32x4 acc = {0, 0, 0, 0};
       for (int p0 = 0; p0 < e.z; p0 += kBatch) {
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const float* p = first + min(p0 + k, e.z - 1) * size;
-          px[k] = *reinterpret_cast<const f32x4*>(p + jr * DT + d);
+          px[k] = *reinterpret_cast<const f32x4*>(p + 4 * x);
           pm[k] = p[kChunkRows * DT + jr];
           pl[k] = p[kChunkRows * (DT + 1) + jr];
         }

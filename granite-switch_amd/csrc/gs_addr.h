@@ -415,18 +415,6 @@ GS_HD void chunk_part_range(int nkt, int p, int n, int& k0, int& k1) {
   k0 = static_cast<int>(static_cast<int64_t>(nkt) * p / n);
   k1 = static_cast<int>(static_cast<int64_t>(nkt) * (p + 1) / n);
 }
-// XCD x's tickets: a contiguous eighth of the (head, part) pairs.
-struct Tickets {
-  int first, n;
-};
-GS_HD Tickets tickets_of(int x, int pairs) {
-  Tickets t;
-  const int per = (pairs + 7) >> 3;
-  t.first = x * per;
-  const int left = pairs - t.first;
-  t.n = left < 0 ? 0 : imin(left, per);
-  return t;
-}
 constexpr int cmax(int a, int b) { return a > b ? a : b; }
 // Partial results a head can have: U2 / part_tiles < 2 slots / HK of them at most,
 // as a split tile has part_tiles key tiles or more for each of its parts.

@@ -57,139 +57,80 @@ struct ChunkItem {
   int order;                         // of the tile among the split ones
   addr::PagedSeq sq;
 };
-struct ChunkShared {
-  int at[256], split_at[256], tile_at[256];   // parts, partial results and split tiles before a thread's sequences
-  int4 count[256];                   // and of them; the key tiles of its longest part
-  int64_t work[kCWaves];
-  int found[9];
-};
-
-// How many key tiles a part of a split tile has.
-struct ChunkSplit {
-  int tiles;
+// The chunk form's parts (a tile of a sequence, or one of those it is split into) for
+// one head: the sequences with the longest parts first, in eight classes, a
+// sequence's tiles and parts from the last.
+struct ChunkOrder {
+  Batch4 q;
+  int tiles;                         // key tiles that a part of a split tile has
   uint32_t magic;
-};
-struct ChunkCount {
-  int nt, np, items, split, tiles;   // tiles, parts of each; parts, partial results and split tiles
-  int longest;                       // key tiles of its longest part
-};
-__device__ __forceinline__ ChunkCount chunk_count(const PagedArgs& a, const ChunkSplit& c, const addr::PagedSeq& sq) {
-  ChunkCount k;
-  k.nt = addr::chunk_tiles(sq, a.tq);
-  k.np = addr::chunk_parts(sq, a.tq, a.window, c.tiles, c.magic);
-  k.items = k.nt * k.np;
-  k.split = k.np > 1 ? k.items : 0;
-  k.tiles = k.np > 1 ? k.nt : 0;
-  k.longest = 0;
-  if (k.nt > 0) {
-    k.longest = addr::chunk_key_tiles(addr::chunk_tile(sq, a.tq.tq, a.window, k.nt - 1));
-    if (k.np > 1) k.longest = min(k.longest, 2 * c.tiles);
-  }
-  return k;
-}
-// The batch's parts (a tile of a sequence, or one of those it is split into) for
-// one head: the sequences with the longest parts first (past 256 sequences, runs of
-// them), their tiles and parts in order from the last; n is their number.
-__device__ __forceinline__ ChunkSplit chunk_scan(const PagedArgs& a, const Schedule& sd, ChunkShared& sh, int& n) {
-  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
-  const int run = (a.B + 255) >> 8;
-  const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
-  const addr::PagedSeq first = first_seq<true>(a, sd);
-  int64_t work = addr::chunk_work2(first, a.tq, a.window);
-  for (int s = s0 + 1; s < s1; ++s) work += addr::chunk_work2(seq_of_form<true>(a, s), a.tq, a.window);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
-  if (l == 0) sh.work[wave] = work;
-  __syncthreads();
-  work = 0;
-#pragma unroll
-  for (int w = 0; w < kCWaves; ++w) work += sh.work[w];
-  ChunkSplit c;
-  c.tiles = addr::chunk_part_tiles(work, a.chunk_share, kChunkLeast);
-  c.magic = addr::div_magic(c.tiles);
-  int4 mine = make_int4(0, 0, 0, 0);
-  addr::PagedSeq sq = first;
-  for (int s = s0; s < s1; ++s) {
-    if (s > s0) sq = seq_of_form<true>(a, s);
-    const ChunkCount k = chunk_count(a, c, sq);
-    mine.x += k.items;
-    mine.y += k.split;
-    mine.z += k.tiles;
-    mine.w = max(mine.w, k.longest);
-  }
-  sh.count[tid] = mine;
-  __syncthreads();
-  // Where each run's parts begin: per lanes of a wave compare one run with every
-  // per-th of the others.
-  const int used = min(a.B, 256);                    // runs
-  int lg = 0;
-  while (lg < 6 && (used << (lg + 1)) <= 256) ++lg;
-  const int per = 1 << lg, me = tid >> lg, sub = tid & (per - 1);
-  const int w = sh.count[me].w;
-  int at = 0, sl = 0, tl = 0, all = 0, all_tiles = 0;
-#pragma unroll 4
-  for (int t = sub; t < used; t += per) {
-    const int4 o = sh.count[t];
-    const bool before = o.w > w || (o.w == w && t < me);
-    at += before ? o.x : 0;
-    sl += before ? o.y : 0;
-    tl += before ? o.z : 0;
-    all += o.x;
-    all_tiles += o.z;
-  }
-  for (int d = 1; d < per; d <<= 1) {
-    at += __shfl_xor(at, d, 64);
-    sl += __shfl_xor(sl, d, 64);
-    tl += __shfl_xor(tl, d, 64);
-    all += __shfl_xor(all, d, 64);
-    all_tiles += __shfl_xor(all_tiles, d, 64);
-  }
-  if (sub == 0) {
-    sh.at[me] = at;
-    sh.split_at[me] = sl;
-    sh.tile_at[me] = tl;
-  }
-  __syncthreads();
-  n = __builtin_amdgcn_readfirstlane(all);
-  // for the join, with the entries that the tiles' first parts write
-  if (tid == 0 && blockIdx.x == 0) a.chunk_list[0].x = all_tiles;
-  return c;
-}
+  int longest;                       // key tiles of the longest part
+  ClassOrder order;
+  uint64_t split;                    // before the lane's: partial results, split tiles << 32
+  int total;
 
-// Part r (0 <= r < n) of the batch.  Every thread of the workgroup calls it.
-__device__ __forceinline__ ChunkItem find_chunk(const PagedArgs& a, const ChunkSplit& c, int r, const Schedule& sd, ChunkShared& sh) {
-  const int tid = threadIdx.x;
-  if (tid < a.B && r >= sh.at[tid] && r < sh.at[tid] + sh.count[tid].x) {
-    const int run = (a.B + 255) >> 8;
-    int at = sh.at[tid], sl = sh.split_at[tid], tl = sh.tile_at[tid], s = tid * run;
-    addr::PagedSeq sq = first_seq<true>(a, sd);
-    for (;;) {
-      const ChunkCount k = chunk_count(a, c, sq);
-      if (r < at + k.items) {
-        const int x = at + k.items - 1 - r;          // a sequence's last tiles, the longest, first
-        const int j = k.np > 1 ? x / k.np : x;
-        sh.found[0] = s;
-        sh.found[1] = j;
-        sh.found[2] = x - j * k.np;
-        sh.found[3] = k.np;
-        sh.found[4] = k.np > 1 ? sl + j * k.np : -1;
-        sh.found[5] = sq.q0;
-        sh.found[6] = sq.n;
-        sh.found[7] = sq.len;
-        sh.found[8] = tl + j;
-        break;
-      }
-      at += k.items;
-      sl += k.split;
-      tl += k.tiles;
-      sq = seq_of_form<true>(a, ++s);
-    }
+  struct Count {
+    int nt, np, longest;             // tiles, parts of each, key tiles of the longest part
+  };
+  __device__ __forceinline__ Count count(const PagedArgs& a, const addr::PagedSeq& sq) const {
+    Count c;
+    c.nt = addr::chunk_tiles(sq, a.tq);
+    c.longest = addr::chunk_key_tiles(addr::chunk_tile(sq, a.tq.tq, a.window, c.nt - 1));
+    c.np = addr::chunk_parts(sq, a.tq, a.window, tiles, magic);
+    if (c.np > 1) c.longest = min(c.longest, 2 * tiles);
+    return c;
   }
-  __syncthreads();
-  const int* f = sh.found;
-  const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
-  return ChunkItem{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), u(f[8]), {u(f[5]), u(f[6]), u(f[7])}};
-}
+  __device__ __forceinline__ int class_of(int x) const {   // x <= longest, only the order matters
+    return min(7, static_cast<int>(8.f * static_cast<float>(longest - x) * __builtin_amdgcn_rcpf(static_cast<float>(longest) + 1.f)));
+  }
+  __device__ __forceinline__ void plan(const PagedArgs& a) {
+    load_batch(a, q, 0);
+    uint64_t work = 0;
+    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) { work += addr::chunk_work2(sq, a.tq, a.window); });
+    tiles = addr::chunk_part_tiles(static_cast<int64_t>(of_lane(lane_sums(work), 63)), a.chunk_share, kChunkLeast);
+    magic = addr::div_magic(tiles);
+    int most = 0;
+    split = 0;
+    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      most = max(most, c.longest);
+      if (c.np > 1) split += static_cast<uint64_t>(c.nt) << 32 | static_cast<uint32_t>(c.nt * c.np);
+    });
+    longest = lanes_most(most);
+    order = ClassOrder{0, 0, a.chunk_parts >= 65536};
+    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      order.add(class_of(c.longest), c.nt * c.np);
+    });
+    total = order.place();
+    const uint64_t to = lane_sums(split);
+    // for the join, with the entries that the tiles' first parts write
+    if (threadIdx.x == 0 && blockIdx.x == 0) a.chunk_list[0].x = static_cast<int>(of_lane(to, 63) >> 32);
+    split = to - split;
+  }
+  // The r-th part (0 <= r < total).
+  __device__ __forceinline__ ChunkItem part(const PagedArgs& a, int r) {
+    ChunkItem it{-1, 0, 0, 1, 0, 0, {0, 0, 0}};
+    uint64_t sp = split;
+    each_seq<true>(a, q, [&](int s, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      const int x = r - order.next(class_of(c.longest), c.nt * c.np);
+      if (x >= 0 && x < c.nt * c.np) {
+        it.s = s;
+        it.j = c.nt * c.np - 1 - x;                  // a sequence's last tiles, the longest, first
+        it.nparts = c.np;
+        it.slot = static_cast<int>(static_cast<uint32_t>(sp));
+        it.order = static_cast<int>(sp >> 32);
+        it.sq = sq;
+      }
+      if (c.np > 1) sp += static_cast<uint64_t>(c.nt) << 32 | static_cast<uint32_t>(c.nt * c.np);
+    });
+    const int from = __builtin_ctzll(__ballot(it.s >= 0));
+    const auto u = [&](int x) { return __builtin_amdgcn_readlane(x, from); };   // uniform, and known to be
+    const int np = u(it.nparts), x = u(it.j), j = np > 1 ? x / np : x;
+    return ChunkItem{u(it.s), j, x - j * np, np, np > 1 ? u(it.slot) + j * np : -1, u(it.order) + j, {u(it.sq.q0), u(it.sq.n), u(it.sq.len)}};
+  }
+};
 
 // The maximum, or the sum, over a lane and the one 32 lanes away.
 __device__ __forceinline__ float max_halves(float x) {
@@ -532,25 +473,19 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
 template <int DT>
 __global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_kernel(PagedArgs) {
   __shared__ __attribute__((aligned(1024))) char lds[addr::cmax(kCStages * 2 * kCKeys * DT * 2, static_cast<int>(sizeof(RowShared<DT>)))];
-  __shared__ ChunkShared sh;
-  __shared__ Schedule sd;
-  load_schedule(fresh_args(), sd);
   int i;
   if (addr::ragged_role(blockIdx.x, fresh_args().ragged_block, fresh_args().row_blocks, i)) {
     const PagedArgs& a = fresh_args();
-    const int h = i % a.HK;
-    const RowItem it = find_row<true, DT>(a, sd, i / a.HK);
-    if (it.s >= 0) row_part<true, DT>(fresh_args(), it, h, *reinterpret_cast<RowShared<DT>*>(lds));
+    const int r = i / a.HK, h = i - r * a.HK;
+    RowOrder<true, DT> order;
+    order.plan(a);
+    if (r < order.total) row_part<true, DT>(fresh_args(), order.part(a, r), h, *reinterpret_cast<RowShared<DT>*>(lds));
   } else {
     const PagedArgs& a = fresh_args();
-    int n = 0;
-    const ChunkSplit cs = chunk_scan(a, sd, sh, n);
-    const addr::Tickets t = addr::tickets_of(i & 7, n * a.HK);
-    if ((i >> 3) >= t.n) return;
-    const int c = t.first + (i >> 3);
-    const int h = c / n;
-    const ChunkItem it = find_chunk(a, cs, c - h * n, sd, sh);
-    chunk_part<DT>(fresh_args(), it, h, lds);
+    ChunkOrder order;
+    order.plan(a);
+    const int r = i / a.HK, h = i - r * a.HK;        // 8 heads: a head's parts on one XCD
+    if (r < order.total) chunk_part<DT>(fresh_args(), order.part(a, r), h, lds);
   }
 }
 
@@ -576,7 +511,7 @@ int64_t chunk_most_parts(const PagedArgs& a) {
 
 int64_t ragged_grid(const PagedArgs& a) {
   return static_cast<int64_t>(a.row_blocks) * a.ragged_block +
-         std::max<int64_t>(static_cast<int64_t>(a.row_blocks) * a.ragged_block, (chunk_most_parts(a) * a.HK + 7) & ~int64_t(7));
+         std::max<int64_t>(static_cast<int64_t>(a.row_blocks) * a.ragged_block, (a.chunk_parts * a.HK + 7) & ~int64_t(7));
 }
 
 void launch_ragged(const PagedArgs& a, int DT, hipStream_t st) {

@@ -35,6 +35,7 @@ struct PagedArgs {
   int64_t row_parts;                // its parts for each head, at most
   int row_slots;                    // its partial results for each head
   int row_limit;                    // sequences of at most so many rows take the row form, others the chunk form
+  int64_t chunk_parts;              // chunk form: parts for each head, at most
   int chunk_slots;                  // workgroups that the chunk form fills
   int ragged_block, row_blocks;     // a ragged launch's order (addr::ragged_role)
   double chunk_share;               // HK / (2 chunk_slots)

@@ -17,15 +17,29 @@
 namespace gs {
 namespace {
 
-// Grid: parts x key/value heads, the heads of a part side by side.
+// Workgroups i of n of each key/value head take its parts i, 2 n - 1 - i, 2 n + i, ...:
+// the parts get shorter, so whoever has a longer one has a shorter one next.  One
+// start for several parts: 223 sequences of 4 .. 429 keys with 16 heads 60 us against 71
+// with a workgroup for each.
 template <bool BF16, int DT>
-__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs) {
   __shared__ RowShared<DT> sh;
-  __shared__ Schedule sd;
-  load_schedule(a, sd);
-  const int r = blockIdx.x / a.HK;
-  const RowItem it = find_row<BF16, DT>(a, sd, r);
-  if (it.s >= 0) row_part<BF16, DT>(a, it, blockIdx.x - r * a.HK, sh);
+  __shared__ RowOrder<BF16, DT> kept[64];            // a lane's, between parts
+  int total;
+  {
+    RowOrder<BF16, DT> order;
+    order.plan(fresh_args());
+    total = order.total;
+    if (threadIdx.x < 64) kept[threadIdx.x] = order;
+  }
+  const int HK = fresh_args().HK;
+  const int i = blockIdx.x / HK, h = blockIdx.x - i * HK, n = gridDim.x / HK;
+  for (int k = 0; k * n < total; ++k) {
+    __syncthreads();                                 // kept is there; every wave is past the part before
+    const int r = k * n + ((k & 1) != 0 ? n - 1 - i : i);
+    if (r >= total) continue;
+    row_part<BF16, DT>(fresh_args(), RowOrder<BF16, DT>(kept[lane_id()]).part(fresh_args(), r), h, sh);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -80,13 +94,17 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.chunk_share = static_cast<double>(a.HK) / (2.0 * a.chunk_slots);
   a.tq.tq = std::max(1, addr::chunk_tq(kChunkRows, a.G));
   a.tq.magic = addr::div_magic(a.tq.tq);
+  a.chunk_parts = a.row_limit != INT32_MAX ? chunk_most_parts(a) : 0;
   a.g_magic = addr::div_magic(a.G);
   a.scale_log2 = scale * 1.44269504088896340736f;
 }
 
 template <bool BF16, int DT>
 void launch_paged(const PagedArgs& a, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.row_parts * a.HK));
+  // Rows of a ragged batch: a sequence's tiles see more keys one after the other, a
+  // workgroup for each part evens that out (6 chunks of 151 .. 1001 rows, fp32: 133 us, 160 else).
+  const int64_t n = a.cu != nullptr ? a.row_parts : std::min<int64_t>(a.row_parts, std::max(1, a.row_wgs / a.HK));
+  const dim3 grid(static_cast<unsigned>(n * a.HK));
   hipLaunchKernelGGL((paged_attention_kernel<BF16, DT>), grid, dim3(256), 0, st, a);
 }
 
@@ -195,10 +213,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
     if (addr::ragged_role(static_cast<int>(w), a.ragged_block, a.row_blocks, i)) {
       if (i < static_cast<int64_t>(row.size())) ++row[i];
     } else {
-      const addr::Tickets t = addr::tickets_of(i & 7, static_cast<int>(pair.size()));
-      if ((i >> 3) >= t.n) continue;
-      m.in("ticket", t.first + (i >> 3), 1, static_cast<int64_t>(pair.size()));
-      if (!m.bad) ++pair[t.first + (i >> 3)];
+      if (i < static_cast<int64_t>(pair.size())) ++pair[i];
     }
   }
   for (char c : row)
@@ -289,7 +304,7 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
   m.in("list of split tiles", 4, 4 * split, chunk_list_floats(a.HK, a.chunk_slots / 2));
   m.in("partial results", 0, slots, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
   m.in("split tiles", 0, 2 * split, addr::chunk_slots_per_head(a.HK, a.chunk_slots));
-  m.in("parts", 0, n, chunk_most_parts(a));
+  m.in("parts", 0, n, a.chunk_parts);
   m.chunk_parts = n;
 }
 

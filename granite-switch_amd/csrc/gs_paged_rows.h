@@ -6,7 +6,7 @@
 // of 128 keys (fp32: 64).  A workgroup has one item, or one part of an item of more
 // units than a workgroup's equal share.  A part leaves a partial result; the last of an
 // item's workgroups to be done joins them, in the order of the keys.  The longest parts
-// start first: 110 us against 117 for 256 sequences of 16 .. 2047 keys (4 key/value
+// start first: 112 us against 118 for 256 sequences of 16 .. 2047 keys (4 key/value
 // heads of 128, bf16).  Equal runs of the batch's units, cut wherever they end, cost two
 // joins a workgroup and took 114.
 #pragma once
@@ -83,32 +83,107 @@ struct RowShared {
   int last;
 };
 
-// The batch's schedule in LDS: thread t has the sequences from t * run on, run =
-// ceil(B / 256).
-struct Schedule {
-  int q0[256], n[256], len[256];     // a thread's first sequence: its only one up to 256
-  int64_t sum[kPWaves];
-  uint64_t lo[kPWaves], hi[kPWaves];
-  int slots[kPWaves];
-  int found[8];
-};
-// The thread's first sequence as a form sees it.
-template <bool CHUNK>
-__device__ __forceinline__ addr::PagedSeq first_seq(const PagedArgs& a, const Schedule& sd) {
-  const int t = threadIdx.x;
-  return only_form<CHUNK>(a, addr::PagedSeq{sd.q0[t], sd.n[t], sd.len[t]});
+// ---------------------------------------------------------------------------
+// Which part is whose: every wave works the batch's schedule out for itself, a lane
+// per sequence, without LDS or a barrier (through them it took 4 us of a workgroup's
+// start).
+// ---------------------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_from(uint64_t x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(x)), CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(x >> 32)), CTRL, ROWS, 0xf, false);
+  return static_cast<uint32_t>(lo) | (static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32);
+}
+// Sums over the lanes up to each: within rows of 16 from 1, 2, 4 and 8 lanes before,
+// then from the last lanes of the rows before.
+__device__ __forceinline__ uint64_t lane_sums(uint64_t x) {
+  x += dpp_from<0x111, 0xf>(x);
+  x += dpp_from<0x112, 0xf>(x);
+  x += dpp_from<0x114, 0xf>(x);
+  x += dpp_from<0x118, 0xf>(x);
+  x += dpp_from<0x142, 0xa>(x);
+  x += dpp_from<0x143, 0xc>(x);
+  return x;
+}
+// The largest of the lanes' values, none below zero.
+__device__ __forceinline__ int lanes_most(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int l) {
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), l);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), l);
+  return lo | (static_cast<uint64_t>(hi) << 32);
 }
 
-// Each thread's own entries: no barrier between writing and reading them.
-__device__ __forceinline__ void load_schedule(const PagedArgs& a, Schedule& sd) {
-  const int tid = threadIdx.x;
-  const int run = (a.B + 255) >> 8;
-  addr::PagedSeq sq{0, 0, 0};
-  if (tid * run < a.B) sq = any_seq(a, tid * run);
-  sd.q0[tid] = sq.q0;
-  sd.n[tid] = sq.n;
-  sd.len[tid] = sq.len;
+// The batch's sequences, 256 at a time: lane l has s = base + 64 i + l.
+struct Batch4 {
+  int base;
+  addr::PagedSeq sq[4];
+};
+__device__ __forceinline__ void load_batch(const PagedArgs& a, Batch4& q, int base) {
+  q.base = base;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int s = base + 64 * i + lane_id();
+    q.sq[i] = addr::PagedSeq{0, 0, 0};
+    if (s < a.B) q.sq[i] = any_seq(a, s);
+  }
 }
+// f(s, sequence) for each of the lane's sequences that a form has rows of, in order.
+template <bool CHUNK, class F>
+__device__ __forceinline__ void each_seq(const PagedArgs& a, Batch4& q, const F& f) {
+  for (int base = 0; base < a.B; base += 256) {
+    if (base != q.base) load_batch(a, q, base);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (base + 64 * i >= a.B) break;
+      const addr::PagedSeq sq = only_form<CHUNK>(a, q.sq[i]);
+      if (sq.n > 0) f(base + 64 * i + lane_id(), sq);
+    }
+  }
+}
+
+// Places of the parts in the order of their classes (0 first), within a class by lane:
+// eight 16-bit counts in two words, or one class where there are more parts.
+struct ClassOrder {
+  uint64_t lo, hi;                   // counts of the lane's parts; then their places
+  bool one;
+  __device__ __forceinline__ void add(int cls, int parts) {
+    const uint64_t x = static_cast<uint64_t>(parts) << (one ? 0 : 16 * (cls & 3));
+    if (one || cls < 4) {
+      lo += x;
+    } else {
+      hi += x;
+    }
+  }
+  // counts to places; the number of parts
+  __device__ __forceinline__ int place() {
+    const uint64_t lo_to = lane_sums(lo), hi_to = lane_sums(hi);
+    const uint64_t lo_all = of_lane(lo_to, 63), hi_all = of_lane(hi_to, 63);
+    if (one) {
+      lo = lo_to - lo;
+      return static_cast<int>(lo_all);
+    }
+    constexpr uint64_t kOnes = 0x0001000100010001;   // times it: the fields up to each, added
+    const uint64_t lo_cls = lo_all * kOnes, hi_cls = hi_all * kOnes + (lo_cls >> 48) * kOnes;
+    lo = lo_cls - lo_all + lo_to - lo;
+    hi = hi_cls - hi_all + hi_to - hi;
+    return static_cast<int>(hi_cls >> 48);
+  }
+  // the place of the lane's next parts of a class
+  __device__ __forceinline__ int next(int cls, int parts) {
+    const int sh = 16 * (cls & 3);
+    const int at = one ? static_cast<int>(lo) : static_cast<int>(((cls < 4 ? lo : hi) >> sh) & 65535);
+    add(cls, parts);
+    return at;
+  }
+};
 
 // One part of the row form's work.
 struct RowItem {
@@ -117,121 +192,71 @@ struct RowItem {
   addr::PagedSeq sq;
 };
 
-// The r-th part of the batch for one head, in order of sequences, tiles and parts; s <
-// 0: there is none.  Every thread of a workgroup of 256 calls it, after load_schedule.
+// The row form's parts for one head, in eight classes of length, the longest first;
+// within one by lane.
 template <bool BF16, int DT>
-__device__ __forceinline__ RowItem find_row(const PagedArgs& a, Schedule& sd, int r) {
-  constexpr int kUnit = PagedForm<BF16, DT>::kBlock * kPWaves;
-  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
-  const int run = (a.B + 255) >> 8;
-  const int s0 = min(tid * run, a.B), s1 = min(s0 + run, a.B);
-  const addr::PagedSeq first = first_seq<false>(a, sd);
-  addr::PagedSeq sq = first;
-  int64_t U = 0;
-  for (int s = s0; s < s1; ++s) {
-    if (s > s0) sq = seq_of_form<false>(a, s);
-    U += addr::paged_seq_units(sq, a.G, a.window, kUnit);
+struct RowOrder {
+  static constexpr int kUnit = PagedForm<BF16, DT>::kBlock * kPWaves;
+  Batch4 q;
+  int most;                          // units of a part
+  uint32_t magic;
+  ClassOrder order;
+  int slots;                         // partial results before the lane's
+  int total;
+
+  struct Count {
+    int nt, nu, np, cls;
+  };
+  __device__ __forceinline__ Count count(const PagedArgs& a, const addr::PagedSeq& sq) const {
+    Count c;
+    c.nt = addr::paged_tiles(sq, a.G);
+    c.nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
+    c.np = addr::row_parts(c.nu, most, magic);
+    uint32_t x, rest;
+    addr::div_by(static_cast<uint32_t>(8 * (most - (c.np > 1 ? most : c.nu))), static_cast<uint32_t>(most), magic, x, rest);
+    c.cls = min(static_cast<int>(x), 7);
+    return c;
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) U += __shfl_xor(U, d, 64);
-  if (l == 0) sd.sum[wave] = U;
-  if (tid == 0) sd.found[0] = -1;
-  __syncthreads();
-  U = 0;
-#pragma unroll
-  for (int w = 0; w < kPWaves; ++w) U += sd.sum[w];
-  const int most = addr::row_part_units(U, a.HK, a.row_wgs);
-  const uint32_t magic = addr::div_magic(most);
-  int parts = 0, slots = 0, longest = 0;
-  sq = first;
-  for (int s = s0; s < s1; ++s) {
-    if (s > s0) sq = seq_of_form<false>(a, s);
-    const int nt = addr::paged_tiles(sq, a.G);
-    const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
-    const int np = addr::row_parts(nu, most, magic);
-    parts += nt * np;
-    slots += np > 1 ? nt * np : 0;
-    longest = max(longest, np > 1 ? most : nu);
+  __device__ __forceinline__ void plan(const PagedArgs& a) {
+    load_batch(a, q, 0);
+    uint64_t U = 0;
+    each_seq<false>(a, q, [&](int, const addr::PagedSeq& sq) { U += addr::paged_seq_units(sq, a.G, a.window, kUnit); });
+    most = addr::row_part_units(static_cast<int64_t>(of_lane(lane_sums(U), 63)), a.HK, a.row_wgs);
+    magic = addr::div_magic(most);
+    order = ClassOrder{0, 0, a.row_parts >= 65536};
+    uint64_t sl = 0;
+    each_seq<false>(a, q, [&](int, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      order.add(c.cls, c.nt * c.np);
+      sl += c.np > 1 ? c.nt * c.np : 0;
+    });
+    slots = static_cast<int>(lane_sums(sl) - sl);
+    total = order.place();
   }
-  // Order: by length, in eight classes, the longest first; within one by sequence.
-  // Eight 16-bit counts in two words; too many parts for them, one class.
-  const bool classes = a.row_parts < 65536;
-  uint32_t cls, rest;
-  addr::div_by(static_cast<uint32_t>(8 * (most - longest)), static_cast<uint32_t>(most), magic, cls, rest);
-  cls = classes ? min(cls, 7u) : 0;
-  const uint64_t one = static_cast<uint64_t>(parts) << (classes ? 16 * (cls & 3) : 0);
-  uint64_t lo = cls < 4 ? one : 0, hi = cls < 4 ? 0 : one;
-  int sl = slots;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t u = __shfl_up(lo, d, 64), v = __shfl_up(hi, d, 64);
-    const int w = __shfl_up(sl, d, 64);
-    if (l >= d) {
-      lo += u;
-      hi += v;
-      sl += w;
-    }
-  }
-  if (l == 63) {
-    sd.lo[wave] = lo;
-    sd.hi[wave] = hi;
-    sd.slots[wave] = sl;
-  }
-  __syncthreads();
-  uint64_t all_lo = 0, all_hi = 0;
-  sl -= slots;
-#pragma unroll
-  for (int w = 0; w < kPWaves; ++w) {
-    const uint64_t x = sd.lo[w], y = sd.hi[w];
-    all_lo += x;
-    all_hi += y;
-    if (w < wave) {
-      lo += x;
-      hi += y;
-      sl += sd.slots[w];
-    }
-  }
-  int at;
-  if (classes) {
-    constexpr uint64_t kOnes = 0x0001000100010001;   // times it: sums of the fields up to each
-    const uint64_t to_lo = all_lo * kOnes, to_hi = all_hi * kOnes + (to_lo >> 48) * kOnes;
-    const int sh16 = 16 * (cls & 3);
-    const uint64_t to = cls < 4 ? to_lo : to_hi, all = cls < 4 ? all_lo : all_hi, own = cls < 4 ? lo : hi;
-    at = static_cast<int>(((to >> sh16) & 65535) - ((all >> sh16) & 65535) + ((own >> sh16) & 65535)) - parts;
-  } else {
-    at = static_cast<int>(lo) - parts;
-  }
-  if (r >= at && r < at + parts) {
-    sq = first;
-    for (int s = s0;; ++s) {
-      if (s > s0) sq = seq_of_form<false>(a, s);
-      const int nt = addr::paged_tiles(sq, a.G);
-      const int nu = addr::paged_tile_units(sq, a.G, a.window, kUnit);
-      const int np = addr::row_parts(nu, most, magic);
-      if (r < at + nt * np) {
-        const int x = r - at;
-        const int j = np > 1 ? x / np : x;
-        sd.found[0] = s;
-        sd.found[1] = j;
-        sd.found[2] = x - j * np;
-        sd.found[3] = np;
-        sd.found[4] = np > 1 ? sl + j * np : -1;
-        sd.found[5] = sq.q0;
-        sd.found[6] = sq.n;
-        sd.found[7] = sq.len;
-        break;
+  // The r-th part (0 <= r < total).
+  __device__ __forceinline__ RowItem part(const PagedArgs& a, int r) {
+    ClassOrder o = order;
+    int sl = slots, at = 0;
+    RowItem it{-1, 0, 0, 1, -1, 0, {0, 0, 0}};
+    each_seq<false>(a, q, [&](int s, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      const int x = r - o.next(c.cls, c.nt * c.np);
+      if (x >= 0 && x < c.nt * c.np) {
+        it.s = s;
+        at = c.nt * c.np - 1 - x;                    // a sequence's last tiles, the longest, first
+        it.nparts = c.np;
+        it.slot = sl;
+        it.units = c.nu;
+        it.sq = sq;
       }
-      at += nt * np;
-      sl += np > 1 ? nt * np : 0;
-    }
+      sl += c.np > 1 ? c.nt * c.np : 0;
+    });
+    const int from = __builtin_ctzll(__ballot(it.s >= 0));
+    const auto u = [&](int x) { return __builtin_amdgcn_readlane(x, from); };   // uniform, and known to be
+    const int np = u(it.nparts), x = u(at), j = np > 1 ? x / np : x;
+    return RowItem{u(it.s), j, x - j * np, np, np > 1 ? u(it.slot) + j * np : -1, u(it.units), {u(it.sq.q0), u(it.sq.n), u(it.sq.len)}};
   }
-  __syncthreads();
-  const int* f = sd.found;
-  const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
-  RowItem it{u(f[0]), u(f[1]), u(f[2]), u(f[3]), u(f[4]), 0, {u(f[5]), u(f[6]), u(f[7])}};
-  it.units = addr::paged_tile_units(it.sq, a.G, a.window, kUnit);
-  return it;
-}
+};
 
 // A row of the result from its sums.
 template <bool BF16>

@@ -396,19 +396,26 @@ GS_HD int64_t chunk_work2(const PagedSeq& s, const ChunkTq& q, int window) {
   if (nt == 0) return 0;
   return static_cast<int64_t>(nt) * (chunk_key_tiles(chunk_tile(s, q.tq, window, 0)) + chunk_key_tiles(chunk_tile(s, q.tq, window, nt - 1)) + 1);
 }
-// Key tiles of a part for a batch of doubled work U2 a head: an equal share of
-// `slots` workgroups, and some at least.  share = HK / (2 slots).
+// Key tiles of a part for a batch of doubled work U2 a head: an equal share c of `slots`
+// workgroups, or 3.2 + 0.8 c where that is more: each part costs 0.05 us for its partial
+// result, so little work is not cut as far as it could be.  (8 chunks of 32 rows over
+// 2048 keys: 28.9 us, 30.8 with shares of four tiles.)  share = HK / (2 slots).
 GS_HD int chunk_part_tiles(int64_t U2, double share, int least) {
   const double c = static_cast<double>(U2) * share;
-  return c < least ? least : static_cast<int>(c) + 1;
+  const double w = 3.2 + 0.8 * c;
+  const double m = c > w ? c : w;
+  return m < least ? least : static_cast<int>(m) + 1;
 }
-// Parts of each of a sequence's tiles: those whose last tile has two parts' key tiles or more are split.
+// Parts of each of a sequence's tiles, by its last tile's key tiles; two short ones do not
+// pay (10 key tiles: 24.5 us whole, 30.8 in two parts each; 24: 41 and 49).
+constexpr int kChunkWhole = 28;
 GS_HD int chunk_parts(const PagedSeq& s, const ChunkTq& q, int window, int part_tiles, uint32_t part_magic) {
   const int nt = chunk_tiles(s, q);
   if (nt == 0) return 0;
+  const int nkt = chunk_key_tiles(chunk_tile(s, q.tq, window, nt - 1));
   uint32_t p, r;
-  div_by(static_cast<uint32_t>(chunk_key_tiles(chunk_tile(s, q.tq, window, nt - 1))), static_cast<uint32_t>(part_tiles), part_magic, p, r);
-  return p < 1 ? 1 : static_cast<int>(p);
+  div_by(static_cast<uint32_t>(nkt), static_cast<uint32_t>(part_tiles), part_magic, p, r);
+  return p < 2 || (p == 2 && nkt < kChunkWhole) ? 1 : static_cast<int>(p);
 }
 // Key tiles [k0, k1) of part p of n of a tile of nkt.
 GS_HD void chunk_part_range(int nkt, int p, int n, int& k0, int& k1) {

@@ -6,7 +6,9 @@
 //
 // gs_append_kv: the QKV projection's rows in, the rotated query rows out, the
 // rotated keys and the values into their slots -- one read and one write of
-// every element, 2 to 3 operations on it: the memory rate bounds it.
+// every element, 2 to 3 operations on it: the memory rate bounds it.  8192 tokens of 32
+// query and 8 key/value heads of 128, bf16: 43.4 us, 4.6 TB/s; 256 tokens 4.9 us, of
+// which the launch is most.
 #include <algorithm>
 
 #include "gs_paged.h"
@@ -196,11 +198,13 @@ __global__ __launch_bounds__(256) void cache_slots_kernel(const int32_t* table, 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Few tokens: every head of a token at once; many: each thread four heads or more.
+// Few tokens: every head of a token at once; many: each thread four heads or more, its
+// cosines and sines loaded once for them.  bf16, 32 + 8 + 8 heads of 128: 256 tokens 4.9
+// and 6.2 us, 512 5.6 and 6.6, 2048 12.6 and 11.7, 8192 45.7 and 43.5.
 void plan_append(AppendArgs& a, int cus) {
   const int n = a.H + 2 * a.HK;
   const int most = 256 / a.units;                        // units <= 256
-  a.groups = std::max(1, std::min(a.T <= cus ? n : (n + 3) / 4, most));
+  a.groups = std::max(1, std::min(a.T <= 2 * cus ? n : (n + 3) / 4, most));
   a.tokens = 256 / (a.units * a.groups);
 }
 

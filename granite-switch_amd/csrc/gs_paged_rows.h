@@ -3,12 +3,15 @@
 // kernel (gs_paged.hip) and the kernel for ragged batches (gs_chunk.hip).
 //
 // An item is a tile of 16 rows of a sequence for one key/value head, a run of units
-// of 128 keys (fp32: 64).  A workgroup has one item, or one part of an item of more
-// units than a workgroup's equal share.  A part leaves a partial result; the last of an
-// item's workgroups to be done joins them, in the order of the keys.  The longest parts
-// start first: 112 us against 118 for 256 sequences of 16 .. 2047 keys (4 key/value
-// heads of 128, bf16).  Equal runs of the batch's units, cut wherever they end, cost two
-// joins a workgroup and took 114.
+// of 128 keys (fp32: 64).  An item of more units than a workgroup's equal share is cut
+// into parts.  A part leaves a partial result; the last of an item's workgroups to be
+// done joins them, in the order of the keys.
+//
+// The memory rate bounds it: 2 G operations a byte of the cache (G query heads to a
+// key/value head).  256 sequences of 16 .. 2047 keys, 8 key/value heads of 128, bf16:
+// 109 us, 4.8 TB/s; one of 131071 keys: 104 us, 5.1 TB/s.  The longest parts
+// start first: 112 us against 118 for the 256 sequences.  Equal runs of the batch's
+// units, cut wherever they end, cost two joins a workgroup and took 114.
 #pragma once
 
 #include "gs_paged.h"

@@ -506,7 +506,7 @@ int64_t chunk_workspace_bytes(int HK, int DT, int cus) {
 
 // Tiles of a head at most: each sequence may end with a partial one.
 static int64_t chunk_most_tiles(const PagedArgs& a) {
-  return a.T / a.tq.tq + std::min(a.B, a.T);
+  return a.T / a.tq.tq + std::min(a.B, a.T / (a.row_limit / a.G + 1));   // a tile more for each sequence of more rows than row_limit
 }
 
 // Parts at most: tiles, and the split tiles' parts.

@@ -20,25 +20,38 @@ namespace {
 // Workgroups i of n of each key/value head take its parts i, 2 n - 1 - i, 2 n + i, ...:
 // the parts get shorter, so whoever has a longer one has a shorter one next.  One
 // start for several parts: 223 sequences of 4 .. 429 keys with 16 heads 60 us against 71
-// with a workgroup for each.
+// with a workgroup for each, 1024 of 16 .. 400 with 8 heads 164 against 229.  The first
+// wave lists up to 32 of a workgroup's parts in one pass over the batch.
+constexpr int kRowList = 32;
 template <bool BF16, int DT>
 __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs) {
   __shared__ RowShared<DT> sh;
-  __shared__ RowOrder<BF16, DT> kept[64];            // a lane's, between parts
-  int total;
-  {
-    RowOrder<BF16, DT> order;
-    order.plan(fresh_args());
-    total = order.total;
-    if (threadIdx.x < 64) kept[threadIdx.x] = order;
-  }
+  __shared__ RowOrder<BF16, DT> kept[64];            // a lane's, between lists
+  __shared__ RowEntry list[kRowList];
+  __shared__ int parts;
   const int HK = fresh_args().HK;
   const int i = blockIdx.x / HK, h = blockIdx.x - i * HK, n = gridDim.x / HK;
-  for (int k = 0; k * n < total; ++k) {
-    __syncthreads();                                 // kept is there; every wave is past the part before
-    const int r = k * n + ((k & 1) != 0 ? n - 1 - i : i);
-    if (r >= total) continue;
-    row_part<BF16, DT>(fresh_args(), RowOrder<BF16, DT>(kept[lane_id()]).part(fresh_args(), r), h, sh);
+  for (int k0 = 0;; k0 += kRowList) {
+    if (threadIdx.x < 64) {
+      const PagedArgs& a = fresh_args();
+      RowOrder<BF16, DT> order;
+      if (k0 == 0) {
+        order.plan(a);
+        kept[threadIdx.x] = order;
+        if (threadIdx.x == 0) parts = order.total;
+      } else {
+        order = kept[threadIdx.x];
+      }
+      order.list_parts(a, i, n, k0, k0 + kRowList, list);
+    }
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(parts);
+    for (int k = k0; k < k0 + kRowList && k * n < total; ++k) {
+      if (k * n + ((k & 1) != 0 ? n - 1 - i : i) >= total) continue;
+      row_part<BF16, DT>(fresh_args(), row_item(list[k - k0]), h, sh);
+      __syncthreads();                               // every wave is past what the part left in sh, and its entry
+    }
+    if ((k0 + kRowList) * n >= total) break;
   }
 }
 

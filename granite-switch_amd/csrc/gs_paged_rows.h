@@ -195,6 +195,17 @@ struct RowItem {
   addr::PagedSeq sq;
 };
 
+// A part as list_parts leaves it: its place among its sequence's from the last, and that
+// sequence's parts to a tile, first partial result and units to a tile.
+struct RowEntry {
+  int s, x, np, slot, units, q0, n, len;
+};
+__device__ __forceinline__ RowItem row_item(const RowEntry& e) {
+  const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };   // uniform, and known to be
+  const int np = u(e.np), x = u(e.x), j = np > 1 ? x / np : x;
+  return RowItem{u(e.s), j, x - j * np, np, np > 1 ? u(e.slot) + j * np : -1, u(e.units), {u(e.q0), u(e.n), u(e.len)}};
+}
+
 // The row form's parts for one head, in eight classes of length, the longest first;
 // within one by lane.
 template <bool BF16, int DT>
@@ -235,6 +246,25 @@ struct RowOrder {
     });
     slots = static_cast<int>(lane_sums(sl) - sl);
     total = order.place();
+  }
+  // Parts k n + i (k even) or k n + n - 1 - i (k odd) for k in [k0, k1), into list[k - k0],
+  // in one pass over the batch.
+  __device__ __forceinline__ void list_parts(const PagedArgs& a, int i, int n, int k0, int k1, RowEntry* list) const {
+    ClassOrder o = order;
+    int sl = slots;
+    Batch4 seqs = q;
+    const uint32_t n_magic = addr::div_magic(n);
+    each_seq<false>(a, seqs, [&](int s, const addr::PagedSeq& sq) {
+      const Count c = count(a, sq);
+      const int m = c.nt * c.np, at = o.next(c.cls, m);
+      uint32_t k, rest;
+      addr::div_by(static_cast<uint32_t>(at), static_cast<uint32_t>(n), n_magic, k, rest);
+      for (int kk = max(static_cast<int>(k), k0); kk < k1 && kk * n < at + m; ++kk) {
+        const int x = kk * n + ((kk & 1) != 0 ? n - 1 - i : i) - at;
+        if (x >= 0 && x < m) list[kk - k0] = RowEntry{s, m - 1 - x, c.np, sl, c.nu, sq.q0, sq.n, sq.len};   // the last tiles first
+      }
+      sl += c.np > 1 ? m : 0;
+    });
   }
   // The r-th part (0 <= r < total).
   __device__ __forceinline__ RowItem part(const PagedArgs& a, int r) {

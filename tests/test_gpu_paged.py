@@ -231,6 +231,22 @@ def test_decode_uneven(dev, dtype, batch, most, window):
     b.check(out, lse=lse, window=window)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_decode_many_short(dev, dtype):
+    """70000 sequences of one token or none: more parts than 16-bit counts hold, lists of parts filled again and again."""
+    _say(f"decode 70000 x 1 {dtype}")
+    B, kv, dim, page = 70000, 1, 16, 8
+    g = torch.Generator(device=dev).manual_seed(12)
+    k, v = (torch.randn(B, kv, page, dim, generator=g, device=dev).to(dtype) for _ in range(2))
+    q = torch.randn(B, 2, dim, generator=g, device=dev).to(dtype)
+    table = torch.randperm(B, generator=g, device=dev).to(torch.int32)[:, None].contiguous()
+    lens = torch.randint(0, 2, (B,), generator=g, device=dev).to(torch.int32)
+    out = paged.paged_attention(q, k, v, table, lens)
+    torch.cuda.synchronize()
+    want = v[table[:, 0].long(), 0, 0] * lens[:, None].to(dtype)      # a softmax over one key is 1
+    assert torch.equal(out, want[:, None].expand_as(out))
+
+
 @pytest.mark.parametrize("heads,kv,dim,batch,most,window", [(8, 2, 128, 24, 7000, 0), (8, 2, 64, 24, 7000, 600),
                                                             (4, 4, 128, 330, 700, 0), (16, 1, 96, 12, 3000, 0)])
 def test_ragged_uneven(dev, heads, kv, dim, batch, most, window):

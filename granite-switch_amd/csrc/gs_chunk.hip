@@ -1,6 +1,6 @@
-// Attention of a ragged bf16 batch over a paged cache (head widths up to 128): one
-// launch in which sequences of many rows take the chunk form here and those of few
-// (a decode row among prompts) the row form (gs_paged_rows.h).
+// Attention of a ragged bf16 batch over a paged cache (head widths up to 128, a scale
+// above zero): one launch in which sequences of many rows take the chunk form here and
+// those of few (a decode row among prompts) the row form (gs_paged_rows.h).
 //
 // Two workgroups share a compute unit: parts of the row form, which stream the cache,
 // and of the chunk form, which multiply, are launched in turn.

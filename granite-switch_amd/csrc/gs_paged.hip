@@ -95,7 +95,9 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
   a.page_octets = static_cast<uint32_t>(page_size / 8);
   a.page_magic = addr::div_magic(a.page_octets);
-  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) ? kRowFormRows : INT32_MAX;
+  // The chunk form hides keys and takes the maximum before it scales, which is right for a
+  // scale above zero only; the row form scales first.
+  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) && scale > 0.f ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
   a.row_slots = addr::row_slots_per_head(a.HK, 2 * cus);
   a.row_wgs = row_wgs_for(a.D, cus);

@@ -1,6 +1,7 @@
 // What the kernels over a paged cache share (gs_paged.hip, gs_chunk.hip).
 #pragma once
 
+#include <algorithm>
 #include <vector>
 
 #include "gs_addr.h"
@@ -89,6 +90,7 @@ inline bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 &&
 // ---------------------------------------------------------------------------
 struct PagedModel {
   int64_t bad = 0, checked = 0, chunk_parts = 0;
+  int window = 0;                                   // as the caller gave it
   std::vector<char> rows;                           // output rows written
   char msg[256] = "";
   void fail(const char* what, int64_t at, int64_t n, int64_t cap) {
@@ -99,6 +101,18 @@ struct PagedModel {
     if (at < 0 || at + n > cap) fail(what, at, n, cap);
   }
 };
+// What the rows of a tile see, from the definition in 64 bits, against what the kernels take
+// it for: every key that a row sees is among the tile's, none from before or past those.
+inline void model_seen(PagedModel& m, const addr::PagedSeq& sq, const addr::PagedTile& t) {
+  int64_t vs = INT64_MAX, ve = 0;
+  for (int qi = t.i0; qi <= t.i1; ++qi) {
+    const int64_t hi = static_cast<int64_t>(sq.len) - sq.n + qi + 1, lo = std::max<int64_t>(0, m.window > 0 ? hi - m.window : 0);
+    if (hi <= lo) continue;
+    vs = std::min(vs, lo);
+    ve = hi;
+  }
+  if (ve == 0 ? t.ve != t.vs : t.vs != vs || t.ve != ve) m.fail("keys that a tile's rows see", t.vs, t.ve - t.vs, ve);
+}
 inline int64_t extent3(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t cols) {
   return (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + cols;
 }

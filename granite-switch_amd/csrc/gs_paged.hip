@@ -90,9 +90,18 @@ int64_t row_most_parts(const PagedArgs& a) {
   return addr::row_most_parts(items, a.HK, a.row_wgs);
 }
 
+// The longest sequence that a page table addresses.
+int64_t paged_reach(int max_pages, int page_size) {
+  return std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
+}
+// The window that the kernels get: none where no sequence is longer.  They subtract it from
+// positions, which are negative for rows without one: num_tokens + window fits 32 bits.
+int paged_window(int window, int64_t reach) { return window < reach ? window : 0; }
+
 // What follows from the sizes alone.
 void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, float scale) {
-  a.max_len = std::min<int64_t>(static_cast<int64_t>(max_pages) * page_size, (int64_t(1) << 31) - (1 << 16));
+  a.max_len = paged_reach(max_pages, page_size);
+  a.window = paged_window(a.window, a.max_len);
   a.page_octets = static_cast<uint32_t>(page_size / 8);
   a.page_magic = addr::div_magic(a.page_octets);
   // The chunk form hides keys and takes the maximum before it scales, which is right for a
@@ -150,6 +159,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
     const int64_t nrows = static_cast<int64_t>(sq.n) * a.G;
     for (int j = 0; j < addr::paged_tiles(sq, a.G) && !m.bad; ++j) {
       const addr::PagedTile t = addr::paged_tile(sq, a.G, a.window, j);
+      model_seen(m, sq, t);
       const int nblk = (t.ve - t.first + F::kBlock - 1) / F::kBlock;
       if (nblk > nu * kPWaves) m.fail("blocks past the item's units", nblk, 0, nu * kPWaves);
       const int nrow = static_cast<int>(std::min<int64_t>(16, nrows - static_cast<int64_t>(j) * 16));
@@ -288,6 +298,7 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
     for (int j = 0; j < nt && !m.bad; ++j) {
       const addr::PagedTile t = addr::chunk_tile(sq, tq.tq, a.window, j);
       const int nkt = addr::chunk_key_tiles(t);
+      model_seen(m, sq, t);
       const int nrow = (t.i1 - t.i0 + 1) * a.G;
       if (nrow < 1 || nrow > kChunkRows) m.fail("rows of a tile", 0, nrow, kChunkRows);
       for (int h = 0; h < a.HK && !m.bad; ++h) {
@@ -370,6 +381,8 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   GS_CHECK_ARG(num_pages > 0 && num_pages < (int64_t(1) << 31) && max_pages >= 0 && ld_table >= max_pages,
                "%s: num_pages=%lld max_pages=%d ld_table=%lld", who, (long long)num_pages, max_pages, (long long)ld_table);
   GS_CHECK_ARG(window >= 0 && max_q >= 0, "%s: window=%d max_q=%d", who, window, max_q);
+  GS_CHECK_ARG(num_tokens + paged_window(window, paged_reach(max_pages, page_size)) < (int64_t(1) << 31),
+               "%s: num_tokens=%lld with window=%d past 32 bits", who, (long long)num_tokens, window);
   if (num_tokens == 0 || num_seqs == 0) return GS_OK;
   // the stride of a dimension of one is never used, and may be anything
   if (num_tokens == 1) q_ts = o_ts = 0;
@@ -449,6 +462,7 @@ int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int6
   a.window = window;
   plan_paged(a, bf16, cus, max_pages, page_size, 1.f);
   PagedModel m;
+  m.window = window;
   m.rows.assign(static_cast<size_t>(a.T) * a.H, 0);
   if (a.row_limit != INT32_MAX) paged_width(head_dim) == 64 ? model_chunk<64>(m, a) : model_chunk<128>(m, a);
   switch (paged_width(head_dim)) {

@@ -567,6 +567,8 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * too).  Rows of tokens that are in no sequence are not written.
  * Limits: head_dim a multiple of 8 (fp32: 4) up to 256, page_size a multiple
  * of 8; q, caches and out 16-byte aligned, strides multiples of 16 bytes.
+ * A window no sequence is longer than is none; num_tokens and a narrower one
+ * sum to less than 2^31.
  * kv_lens past the page table's reach are cut to it; page ids outside the
  * pool are read as page 0.  max_q: the most rows of a sequence where the caller
  * knows it (0: unknown); a smaller value than the batch has is an error of the

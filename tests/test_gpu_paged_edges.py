@@ -32,3 +32,15 @@ def test_ragged_scales(dev, scale, name, n, cached, heads, kv, dim, window):
     out = b.run(scale=scale, window=window, lse=lse)
     torch.cuda.synchronize()
     b.check(out, scale=scale, window=window, lse=lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30])
+def test_wide_windows(dev, dtype, window):
+    """A window wider than any cache is none, for rows without a position too."""
+    _say(f"window {window} {dtype}")
+    b = Batch(dev, [40, 3, 20, 1], [-25, -3, 5, 200], 8, 2, 64, dtype=dtype, seed=9)
+    out = b.run(window=window)
+    torch.cuda.synchronize()
+    b.check(out)
+    assert torch.equal(out, b.run())

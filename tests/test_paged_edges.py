@@ -1,0 +1,29 @@
+"""CPU tests of the paged cache's entry points where a call's arguments, not its sizes, are unusual."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from granite_switch_amd import _lib
+from test_paged_calls import ATTENTION, P, _refused
+from test_paged_model import BF16, FP32, _check_attention
+
+NO_WINDOW = 2 ** 31 - 1                                    # as wide as 32 bits hold
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("window", [NO_WINDOW, NO_WINDOW - 1, NO_WINDOW - 40, 2 ** 31 - 2 ** 16, 2 ** 30])
+@pytest.mark.parametrize("n,cached,heads,kv", [([40, 3, 20], [-25, -3, 5], 8, 2), ([200, 1], [-120, 300], 3, 3),
+                                               ([7, 1], [-3, 20], 48, 1)])
+def test_wide_windows(dtype, window, n, cached, heads, kv):
+    """Rows without a position have negative ones: their distance to a wide window's start passes 32 bits."""
+    cu = np.concatenate([[0], np.cumsum(n)])
+    _check_attention(dtype, np.asarray(n) + np.asarray(cached), cu, heads, kv, 64, 16, window, "heads", cus=16)
+
+
+def test_rows_and_window_past_32_bits():
+    """A table that reaches past a window of nearly 2^31 tokens: only as many rows as leave the sum in 32 bits."""
+    change = dict(cu=P, num_tokens=1 << 17, window=(1 << 31) - (1 << 17), max_pages=1 << 27, ld_table=1 << 27)
+    e = _refused("gs_paged_attention", ATTENTION, change)
+    assert e.status == _lib.GS_ERR_INVALID and "past 32 bits" in str(e)

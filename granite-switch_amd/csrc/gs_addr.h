@@ -297,6 +297,11 @@ GS_HD PagedSeq paged_seq(int lo, int hi, int len, int T, int64_t max_len) {
   s.len = len < 0 ? 0 : static_cast<int>(lmin(len, max_len));
   return s;
 }
+// The rows of no sequence are [0, first) and [last, T).
+GS_HD void paged_outside(int cu_first, int cu_last, int T, int& first, int& last) {
+  first = cu_first < 0 ? 0 : imin(cu_first, T);
+  last = cu_last < first ? first : imin(cu_last, T);
+}
 // Tile j of 16 (query, head) rows of a sequence, row r = query * G + head: the
 // queries i0 .. i1 it holds and the tokens [vs, ve) that some row of it sees
 // (none: ve = vs); first = vs rounded down to a multiple of 8.

@@ -472,6 +472,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
       row_store<true>(a, e.x + static_cast<int>(jq), h * a.G + static_cast<int>(jh), d, acc, M, L);
     }
   }
+  zero_outside<true>(a);
 }
 
 // Grid: addr::ragged_role.

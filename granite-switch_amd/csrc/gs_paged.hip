@@ -53,6 +53,7 @@ __global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel
     }
     if ((k0 + kRowList) * n >= total) break;
   }
+  zero_outside<BF16>(fresh_args());
 }
 
 // ---------------------------------------------------------------------------
@@ -334,7 +335,19 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
   m.chunk_parts = n;
 }
 
+// Every row of a sequence is written; the others are left to zero_outside.
 void model_rows(PagedModel& m, const PagedArgs& a) {
+  if (a.cu != nullptr) {
+    int first, last;
+    addr::paged_outside(a.cu[0], a.cu[a.B], a.T, first, last);
+    for (int t = 0; t < a.T; ++t)
+      for (int h = 0; h < a.H && (t < first || t >= last); ++h) {
+        if (m.rows[static_cast<int64_t>(t) * a.H + h]++) m.fail("output row of no sequence written by a part", t, 1, a.T);
+        m.in("out", t * a.o_ts + h * a.o_hs, a.D, extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D));
+      }
+    for (char c : m.rows)
+      if (c != 1 && !m.bad) m.fail("output row written other than once", 0, c, 1);
+  }
   for (int s = 0; s < a.B && !m.bad; ++s) {
     const addr::PagedSeq sq = a.cu != nullptr ? addr::paged_seq(a.cu[s], a.cu[s + 1], 0, a.T, 0) : addr::PagedSeq{s, 1, 0};
     for (int i = 0; i < sq.n; ++i)
@@ -383,14 +396,14 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   GS_CHECK_ARG(window >= 0 && max_q >= 0, "%s: window=%d max_q=%d", who, window, max_q);
   GS_CHECK_ARG(num_tokens + paged_window(window, paged_reach(max_pages, page_size)) < (int64_t(1) << 31),
                "%s: num_tokens=%lld with window=%d past 32 bits", who, (long long)num_tokens, window);
-  if (num_tokens == 0 || num_seqs == 0) return GS_OK;
+  if (num_tokens == 0) return GS_OK;
   // the stride of a dimension of one is never used, and may be anything
   if (num_tokens == 1) q_ts = o_ts = 0;
   if (heads == 1) q_hs = o_hs = 0;
   if (kv_heads == 1) k_hs = v_hs = 0;
   if (num_pages == 1) k_ps = v_ps = 0;
-  GS_CHECK_ARG(q != nullptr && k_cache != nullptr && v_cache != nullptr && out != nullptr && kv_lens != nullptr &&
-                   (page_table != nullptr || max_pages == 0), "%s: null tensor", who);
+  GS_CHECK_ARG(q != nullptr && k_cache != nullptr && v_cache != nullptr && out != nullptr &&
+                   (num_seqs == 0 || (kv_lens != nullptr && (page_table != nullptr || max_pages == 0))), "%s: null tensor", who);
   GS_CHECK_ARG(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && strides_ok(q_ts, q_hs, ve) &&
                    strides_ok(k_ps, k_hs, ve) && strides_ok(v_ps, v_hs, ve) && strides_ok(k_rs, v_rs, ve) &&
                    strides_ok(o_ts, o_hs, ve),
@@ -446,10 +459,10 @@ int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int6
                                  int64_t* checked) {
   const char* who = "gs_check_paged_addresses";
   const bool bf16 = dtype == GS_DTYPE_BF16;
-  GS_CHECK_ARG((bf16 || dtype == GS_DTYPE_FP32) && num_tokens > 0 && num_seqs > 0 && num_tokens < (int64_t(1) << 31) &&
+  GS_CHECK_ARG((bf16 || dtype == GS_DTYPE_FP32) && num_tokens > 0 && num_seqs >= 0 && num_tokens < (int64_t(1) << 31) &&
                    heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim <= 256 &&
                    head_dim % (bf16 ? 8 : 4) == 0 && page_size > 0 && page_size % 8 == 0 && num_pages > 0 &&
-                   max_pages >= 0 && ld_table >= max_pages && kv_lens != nullptr && window >= 0 && cus > 0 &&
+                   max_pages >= 0 && ld_table >= max_pages && (num_seqs == 0 || kv_lens != nullptr) && window >= 0 && cus > 0 &&
                    (cu_seqlens != nullptr || num_tokens == num_seqs), "%s: sizes", who);
   PagedArgs a{};
   a.q_ts = q_ts; a.q_hs = q_hs; a.o_ts = o_ts; a.o_hs = o_hs;

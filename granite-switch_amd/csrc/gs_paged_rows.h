@@ -306,6 +306,25 @@ __device__ __forceinline__ void row_store(const PagedArgs& a, int64_t tok, int h
     a.lse[tok * a.H + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
+// Rows of a ragged batch that are in no sequence get zeros, 16 bytes a thread, dealt out
+// over a launch's workgroups.
+template <bool BF16>
+__device__ __forceinline__ void zero_outside(const PagedArgs& a) {
+  if (a.cu == nullptr) return;
+  int first, last;
+  addr::paged_outside(a.cu[0], a.cu[a.B], a.T, first, last);
+  constexpr int kVec = BF16 ? 8 : 4;
+  const int pieces = a.D / kVec;
+  const int64_t row = static_cast<int64_t>(a.H) * pieces, n = (first + static_cast<int64_t>(a.T - last)) * row;
+  for (int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; x < n; x += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t i = x / row, t = i < first ? i : i - first + last;
+    const int in = static_cast<int>(x - i * row), head = in / pieces, d = (in - head * pieces) * kVec;
+    const int64_t e = t * a.o_ts + static_cast<int64_t>(head) * a.o_hs + d;
+    *reinterpret_cast<u32x4*>(static_cast<char*>(a.out) + e * (BF16 ? 2 : 4)) = u32x4{0, 0, 0, 0};
+    if (a.lse != nullptr && d == 0) a.lse[t * a.H + head] = -INFINITY;
+  }
+}
+
 // Partial results are written and read by workgroups of different XCDs, whose L2s
 // do not see each other's lines: agent-scope accesses, which go through to memory
 // (writing an L2 back at a release instead took 30 us of a decode call's 114).

@@ -299,7 +299,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     workspace  uint8, ``workspace_bytes`` long, zeroed before its first call and used
                by nothing else (one per stream is kept when None)
 
-    A row that sees nothing (an empty sequence) gives zeros.
+    A row that sees nothing (an empty sequence), or that is in no sequence (past
+    cu_seqlens[B], where a step is padded to a fixed number of rows), gives zeros.
     """
     dev = q.device
     key = (q.shape, q.stride(), q.dtype, dev, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
@@ -316,7 +317,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     code, T, B, H, HK, D, q_st, k_st, v_st, pages, page, table, o_st, most, need, default_scale = plan
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if T == 0 or B == 0:
+    if T == 0:
         return out
     stream = _lib.stream_ptr(dev)
     if workspace is None:
@@ -360,7 +361,7 @@ def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window
     if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
         raise ValueError(f"{who}: workspace must be a contiguous uint8 tensor")
     with torch.cuda.device(dev):
-        need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None) if T and B else 0
+        need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None) if T else 0
     return (_DTYPES[dtype], T, B, H, HK, D, q.stride()[:2], k_cache.stride()[:3], v_cache.stride()[:3], k_cache.shape[0],
             k_cache.shape[2], (_table_ld(page_table), page_table.shape[1]),
             (H * D, D) if out is None else out.stride()[:2], 1 if cu_seqlens is None else int(max_q or 0), need,

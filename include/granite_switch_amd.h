@@ -564,7 +564,8 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * that sees nothing (an empty sequence, p < 0) gets zeros.  lse [num_tokens,
  * heads] fp32 or NULL: the natural logarithm of the softmax's total, -inf for
  * such a row.  Cache rows that no row of a call sees may hold anything (NaN
- * too).  Rows of tokens that are in no sequence are not written.
+ * too).  Rows before cu_seqlens[0] and from cu_seqlens[num_seqs] on are in no
+ * sequence and get the same zeros and -inf.
  * Limits: head_dim a multiple of 8 (fp32: 4) up to 256, page_size a multiple
  * of 8; q, caches and out 16-byte aligned, strides multiples of 16 bytes.
  * A window no sequence is longer than is none; num_tokens and a narrower one

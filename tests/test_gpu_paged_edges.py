@@ -44,3 +44,33 @@ def test_wide_windows(dev, dtype, window):
     torch.cuda.synchronize()
     b.check(out)
     assert torch.equal(out, b.run())
+
+
+@pytest.mark.parametrize("dtype,dim,max_q", [(BF16, 64, 0), (BF16, 128, 40), (BF16, 256, 0), (FP32, 80, 0), (BF16, 64, 2)])
+@pytest.mark.parametrize("before,after", [(0, 3), (2, 0), (1, 700)])
+def test_rows_of_no_sequence(dev, dtype, dim, max_q, before, after):
+    """A step padded to a fixed number of rows: those of no sequence give zeros, whatever out held."""
+    _say(f"rows of no sequence {dtype} x {dim}: {before}, {after}")
+    n = [2, 1, 1] if max_q == 2 else [5, 1, 40]
+    b = Batch(dev, n, [10, 20, 30], 8, 2, dim, dtype=dtype, seed=dim)
+    T = b.q.shape[0]
+    pad = lambda m: torch.randn(m, 8, dim, device=dev).to(dtype)
+    q = torch.cat([pad(before), b.q, pad(after)])
+    wide = torch.full((q.shape[0], 10, dim), math.nan, dtype=dtype, device=dev)
+    out, lse = wide[:, 1:9], torch.full((q.shape[0], 8), math.nan, device=dev)
+    paged.paged_attention(q, b.k, b.v, b.table, b.lens, b.cu + before, out=out, lse=lse, max_q=max_q or None)
+    torch.cuda.synchronize()
+    b.check(out[before:before + T], lse=lse[before:before + T])
+    edge = [*range(before), *range(before + T, q.shape[0])]
+    assert bool((out[edge] == 0).all()) and bool((lse[edge] == -math.inf).all())
+    assert bool(wide[:, 0].isnan().all()) and bool(wide[:, 9].isnan().all()), "columns outside out were written"
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 256), (FP32, 64)])
+def test_no_sequences(dev, dtype, dim):
+    _say(f"no sequences {dtype} x {dim}")
+    b = Batch(dev, [5], [10], 8, 2, dim, dtype=dtype)
+    out, lse = torch.full_like(b.q, math.nan), torch.full((5, 8), math.nan, device=dev)
+    got = paged.paged_attention(b.q, b.k, b.v, b.table[:0], b.lens[:0], b.cu[:1], out=out, lse=lse)
+    torch.cuda.synchronize()
+    assert got is out and bool((out == 0).all()) and bool((lse == -math.inf).all())

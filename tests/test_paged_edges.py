@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -27,3 +29,20 @@ def test_rows_and_window_past_32_bits():
     change = dict(cu=P, num_tokens=1 << 17, window=(1 << 31) - (1 << 17), max_pages=1 << 27, ld_table=1 << 27)
     e = _refused("gs_paged_attention", ATTENTION, change)
     assert e.status == _lib.GS_ERR_INVALID and "past 32 bits" in str(e)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (BF16, 128), (BF16, 256), (FP32, 64)])
+@pytest.mark.parametrize("cu,rows", [([0, 3, 40], 45), ([0, 0], 7), ([5, 25, 26], 26), ([2, 4], 300), ([0], 9), ([3], 9),
+                                     ([0, 4, 9], 9)])
+def test_rows_of_no_sequence(dtype, dim, cu, rows):
+    """Rows before the first sequence and past the last are written too, every row once."""
+    B, heads, kv, page, pages = len(cu) - 1, 6, 2, 16, 8
+    lens = np.asarray([cu[s + 1] - cu[s] + 7 for s in range(B)], np.int32)
+    table = np.tile(np.arange(4, dtype=np.int32), (max(B, 1), 1))
+    cu = np.asarray(cu, np.int32)
+    msg, checked = ctypes.create_string_buffer(256), ctypes.c_int64()
+    st = (kv * page * dim, page * dim, dim)
+    bad = _lib.load().gs_check_paged_addresses(dtype, heads * dim, dim, *st, *st, pages, page, table.ctypes.data, 4, 4,
+                                               lens.ctypes.data, cu.ctypes.data, B, rows, heads, kv, dim, 0, heads * dim,
+                                               dim, 16, msg, 256, ctypes.byref(checked))
+    assert bad == 0, (bad, msg.value.decode() or _lib.last_error())

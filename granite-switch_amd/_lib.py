@@ -104,6 +104,7 @@ SIGNATURES = {
                            + [c_i64, c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_i32, c_i32,
                               c_i32, c_i32, ctypes.c_float, c_i32, c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64,
                               c_void_p]),
+    "gs_capture_id": (c_i32, [c_void_p, c_void_p]),
     "gs_check_paged_addresses": (c_i64, [c_i32] + [c_i64] * 9 + [c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p,
                                          c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32,
                                          ctypes.c_char_p, c_i64, c_void_p]),
@@ -175,6 +176,13 @@ def stream_ptr(device: torch.device | None = None) -> int:
     if device is not None and device.index is not None and _raw_stream is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def capture_id(stream: int) -> int:
+    """The id of the graph capture that ``stream`` is part of; 0: none."""
+    found = c_i64()
+    call("gs_capture_id", stream, ctypes.byref(found))
+    return found.value
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

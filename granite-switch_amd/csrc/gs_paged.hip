@@ -450,6 +450,19 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   return GS_OK;
 }
 
+int gs_capture_id(void* stream, int64_t* id) {
+  GS_CHECK_ARG(id != nullptr, "gs_capture_id: id is null");
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long found = 0;
+  const hipError_t e = hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &found);
+  if (e != hipSuccess) {
+    set_error("gs_capture_id: %s", hipGetErrorString(e));
+    return GS_ERR_HIP;
+  }
+  *id = status == hipStreamCaptureStatusActive ? static_cast<int64_t>(found) : 0;
+  return GS_OK;
+}
+
 int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int64_t k_ps, int64_t k_hs, int64_t k_rs,
                                  int64_t v_ps, int64_t v_hs, int64_t v_rs, int64_t num_pages, int32_t page_size,
                                  const int32_t* page_table, int64_t ld_table, int32_t max_pages,

@@ -246,22 +246,25 @@ def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out) ->
 # Attention
 # ---------------------------------------------------------------------------
 # One workspace for each stream: calls on one stream follow each other, calls on
-# different streams may overlap.  Its counters start at zero and every call leaves
-# them so.  A replaced buffer is kept (``_retired``): a captured graph may still
-# hold its address.
+# different streams may overlap.  A captured graph may be replayed on any stream,
+# beside its capture stream's calls and other graphs: its calls get one of the
+# graph's own, from its pool, for each of the capture's streams.  The counters
+# start at zero (in a graph: on every replay) and every call leaves them so.
 _workspaces: dict = {}
-_retired: list = []
+_captured: dict = {}       # by stream: the last capture on it and that capture's buffer
 
 
 def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
     key = (device.index, stream)
+    if torch.cuda.is_current_stream_capturing():
+        capture = _lib.capture_id(stream)
+        last, buf = _captured.get(key, (0, None))
+        if last != capture or capture == 0 or buf.numel() < need:
+            buf = torch.zeros(need, dtype=torch.uint8, device=device)
+            _captured[key] = (capture, buf)
+        return buf
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < need:
-        if torch.cuda.is_current_stream_capturing():
-            # a buffer of the graph's own: it lives as long as the graph's pool does
-            return torch.zeros(need, dtype=torch.uint8, device=device)
-        if buf is not None:
-            _retired.append(buf)
         buf = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
     return buf
 

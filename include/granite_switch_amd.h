@@ -591,6 +591,11 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int
                        float scale, int32_t window, void* out, int64_t o_token_stride, int64_t o_head_stride,
                        float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The id of the graph capture that `stream` is part of, 0 where it is in none:
+ * calls of one capture on one stream may share a workspace, a graph shares its
+ * with nothing else. */
+int gs_capture_id(void* stream, int64_t* id);
+
 /* Test support (no counterpart in the reference; makes no HIP call).  The
  * accesses of gs_paged_attention (every part, wave, lane and block, with `cus`
  * compute units), or of gs_append_kv, replayed on the host for host copies of

@@ -74,3 +74,60 @@ def test_no_sequences(dev, dtype, dim):
     got = paged.paged_attention(b.q, b.k, b.v, b.table[:0], b.lens[:0], b.cu[:1], out=out, lse=lse)
     torch.cuda.synchronize()
     assert got is out and bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_graphs_beside_eager_calls(dev, ragged):
+    """Two graphs captured on a stream that has a workspace, replayed on two others while it works: the same bits."""
+    _say(f"graphs beside eager calls, ragged {ragged}")
+    n = [1, 40, 3, 130, 1] if ragged else [1] * 40
+    bs = [Batch(dev, n, [2100 + 613 * i % 3000 for i in range(len(n))], 8, 2, 128, seed=s, decode=not ragged) for s in (1, 2, 3)]
+    want = [b.run() for b in bs]
+    torch.cuda.synchronize()
+    for b, w in zip(bs, want):
+        b.check(w)
+    home, others, graphs, outs = torch.cuda.Stream(), [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+    with torch.cuda.stream(home):
+        bs[2].run()
+    torch.cuda.synchronize()
+    for b in bs[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=home):
+            b.run()
+            outs.append(b.run())                           # two calls of one capture
+        graphs.append(g)
+    for _ in range(4):
+        for o in outs:
+            o.fill_(math.nan)
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(3):
+            for g, s in zip(graphs, others):
+                with torch.cuda.stream(s):
+                    g.replay()
+            with torch.cuda.stream(home):
+                eager.append(bs[2].run())
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), "a graph's result differs"
+        assert all(torch.equal(e, want[2]) for e in eager), "an eager result differs"
+
+
+def test_capture_ids(dev):
+    """Each capture has an id of its own, the same on every stream that it forks to; none outside of one."""
+    from granite_switch_amd import _lib
+
+    s, fork, x, ids = torch.cuda.Stream(), torch.cuda.Stream(), torch.zeros(8, device=dev), []
+    torch.cuda.synchronize()
+    assert _lib.capture_id(s.cuda_stream) == 0
+    for _ in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            x.add_(1)
+            ids.append(_lib.capture_id(s.cuda_stream))
+            fork.wait_stream(s)
+            with torch.cuda.stream(fork):
+                x.add_(1)
+                assert _lib.capture_id(fork.cuda_stream) == ids[-1]
+            s.wait_stream(fork)
+        assert _lib.capture_id(s.cuda_stream) == 0 and _lib.capture_id(fork.cuda_stream) == 0
+    assert len(set(ids)) == 3 and 0 not in ids

@@ -6,8 +6,9 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
-from granite_switch_amd import _lib
+from granite_switch_amd import _lib, paged
 from test_paged_calls import ATTENTION, P, _refused
 from test_paged_model import BF16, FP32, _check_attention
 
@@ -46,3 +47,29 @@ def test_rows_of_no_sequence(dtype, dim, cu, rows):
                                                lens.ctypes.data, cu.ctypes.data, B, rows, heads, kv, dim, 0, heads * dim,
                                                dim, 16, msg, 256, ctypes.byref(checked))
     assert bad == 0, (bad, msg.value.decode() or _lib.last_error())
+
+
+def test_captured_calls_share_no_workspace(monkeypatch):
+    """A graph may be replayed on any stream: what it uses is neither a stream's own buffer nor another graph's."""
+    capture = {"id": 0}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture["id"] != 0)
+    monkeypatch.setattr(_lib, "capture_id", lambda stream: capture["id"], raising=False)
+    for name in ("_workspaces", "_captured"):
+        monkeypatch.setattr(paged, name, {}, raising=False)
+    get = lambda stream, need=1 << 17: paged._workspace(torch.device("cpu"), stream, need)
+    eager = get(5)
+    assert get(5, 100) is eager and get(6) is not eager
+    capture["id"] = 1
+    first = get(5)
+    assert first is not eager and first.numel() >= 1 << 17
+    assert get(5, 100) is first, "the calls of one capture follow each other on its stream"
+    assert get(6) is not first, "another stream of the capture may run beside it"
+    larger = get(5, 1 << 18)
+    assert larger.numel() >= 1 << 18 and get(5) is larger
+    capture["id"] = 2
+    second = get(5)
+    assert second is not eager and second is not first and second is not larger
+    capture["id"] = 0
+    assert get(5) is eager
+    for buf in (eager, first, larger, second):
+        assert not buf[: 65536].any(), "counters start at zero"

@@ -31,6 +31,7 @@ GS_MAX_SLICES = 8
 GS_MAX_RANK = 512
 GS_RANK_CLASS_SPLIT = 64
 GS_NOALLOC_SCRATCH_BYTES = 64 << 20
+GS_PAGED_HEAD_BYTES = 65536
 GS_GATE_NONE = 0
 GS_GATE_SIGMOID = 1
 GS_GATE_TANH = 2

@@ -254,18 +254,24 @@ _workspaces: dict = {}
 _captured: dict = {}       # by stream: the last capture on it and that capture's buffer
 
 
+def _new_workspace(device: torch.device, need: int) -> torch.Tensor:
+    buf = torch.empty(need, dtype=torch.uint8, device=device)
+    buf[:_lib.GS_PAGED_HEAD_BYTES].zero_()     # the rest, up to tens of MB, is written before it is read
+    return buf
+
+
 def _workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
     key = (device.index, stream)
     if torch.cuda.is_current_stream_capturing():
         capture = _lib.capture_id(stream)
         last, buf = _captured.get(key, (0, None))
         if last != capture or capture == 0 or buf.numel() < need:
-            buf = torch.zeros(need, dtype=torch.uint8, device=device)
+            buf = _new_workspace(device, need)
             _captured[key] = (capture, buf)
         return buf
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < need:
-        buf = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+        buf = _workspaces[key] = _new_workspace(device, need)
     return buf
 
 
@@ -299,8 +305,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     window     > 0: a row sees the last ``window`` tokens up to its own
     lse        [T, heads] float32: receives the log of each softmax's total
     max_q      the most query rows of a sequence where the caller knows it
-    workspace  uint8, ``workspace_bytes`` long, zeroed before its first call and used
-               by nothing else (one per stream is kept when None)
+    workspace  uint8, ``workspace_bytes`` long, its first 64 KB zeroed before its first
+               call, and used by nothing else (one per stream is kept when None)
 
     A row that sees nothing (an empty sequence), or that is in no sequence (past
     cu_seqlens[B], where a step is padded to a fixed number of rows), gives zeros.

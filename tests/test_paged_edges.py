@@ -73,3 +73,16 @@ def test_captured_calls_share_no_workspace(monkeypatch):
     assert get(5) is eager
     for buf in (eager, first, larger, second):
         assert not buf[: 65536].any(), "counters start at zero"
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_only_the_counters_are_cleared(monkeypatch, captured):
+    """A workspace is up to tens of megabytes, its counters 64 KB: a graph clears them on every replay."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: captured)
+    monkeypatch.setattr(_lib, "capture_id", lambda stream: 3)
+    monkeypatch.setattr(paged, "_workspaces", {})
+    monkeypatch.setattr(paged, "_captured", {})
+    monkeypatch.setattr(torch, "empty", lambda n, **kw: torch.full((n,), 255, **kw))
+    buf = paged._workspace(torch.device("cpu"), 5, 1 << 20)
+    head = _lib.GS_PAGED_HEAD_BYTES
+    assert buf.numel() == 1 << 20 and not buf[:head].any() and bool((buf[head:] == 255).all())

@@ -124,11 +124,15 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.scale_log2 = scale * 1.44269504088896340736f;
 }
 
+// Workgroups of the row form for each head.  Rows of a ragged batch: a sequence's tiles
+// see more keys one after the other, a workgroup for each part evens that out (6 chunks of
+// 151 .. 1001 rows, fp32: 133 us, 160 else).
+int64_t row_grid(const PagedArgs& a) {
+  return a.cu != nullptr ? a.row_parts : std::min<int64_t>(a.row_parts, std::max(1, a.row_wgs / a.HK));
+}
+
 template <bool BF16, int DT>
-void launch_paged(const PagedArgs& a, hipStream_t st) {
-  // Rows of a ragged batch: a sequence's tiles see more keys one after the other, a
-  // workgroup for each part evens that out (6 chunks of 151 .. 1001 rows, fp32: 133 us, 160 else).
-  const int64_t n = a.cu != nullptr ? a.row_parts : std::min<int64_t>(a.row_parts, std::max(1, a.row_wgs / a.HK));
+void launch_paged(const PagedArgs& a, int64_t n, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(n * a.HK));
   hipLaunchKernelGGL((paged_attention_kernel<BF16, DT>), grid, dim3(256), 0, st, a);
 }
@@ -434,17 +438,22 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
   a.chunk_list = reinterpret_cast<int4*>(a.ws + row_partial_floats(kv_heads, head_dim, cus));
   a.chunk_ws = reinterpret_cast<float*>(a.chunk_list) + chunk_list_floats(kv_heads, cus);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t n = row_grid(a);
   if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
     GS_CHECK_ARG(ragged_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
     launch_ragged(a, DT, st);
     GS_CHECK_LAUNCH(who);
     return GS_OK;
   }
-  GS_CHECK_ARG(a.row_parts * a.HK < (int64_t(1) << 31), "%s: too many tiles", who);
+  // max_q says that no sequence is the chunk form's: workgroups for such a batch, which take
+  // whatever parts the lengths turn out to make
+  a.row_limit = INT32_MAX;
+  a.row_parts = row_most_parts(a);
+  GS_CHECK_ARG(n * a.HK < (int64_t(1) << 31) && a.row_parts < (int64_t(1) << 31), "%s: too many tiles", who);
   switch (DT) {
-    case 64: bf16 ? launch_paged<true, 64>(a, st) : launch_paged<false, 64>(a, st); break;
-    case 128: bf16 ? launch_paged<true, 128>(a, st) : launch_paged<false, 128>(a, st); break;
-    default: bf16 ? launch_paged<true, 256>(a, st) : launch_paged<false, 256>(a, st); break;
+    case 64: bf16 ? launch_paged<true, 64>(a, n, st) : launch_paged<false, 64>(a, n, st); break;
+    case 128: bf16 ? launch_paged<true, 128>(a, n, st) : launch_paged<false, 128>(a, n, st); break;
+    default: bf16 ? launch_paged<true, 256>(a, n, st) : launch_paged<false, 256>(a, n, st); break;
   }
   GS_CHECK_LAUNCH(who);
   return GS_OK;

@@ -304,7 +304,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scale      of the scores (1 / sqrt(D) when None)
     window     > 0: a row sees the last ``window`` tokens up to its own
     lse        [T, heads] float32: receives the log of each softmax's total
-    max_q      the most query rows of a sequence where the caller knows it
+    max_q      the most query rows of a sequence where the caller knows it: a choice of
+               kernels only, one that is too small costs time
     workspace  uint8, ``workspace_bytes`` long, its first 64 KB zeroed before its first
                call, and used by nothing else (one per stream is kept when None)
 

@@ -572,8 +572,8 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * sum to less than 2^31.
  * kv_lens past the page table's reach are cut to it; page ids outside the
  * pool are read as page 0.  max_q: the most rows of a sequence where the caller
- * knows it (0: unknown); a smaller value than the batch has is an error of the
- * caller's that leaves those rows unwritten.
+ * knows it (0: unknown), a choice of kernels only: a smaller value than the batch
+ * has is slower, not wrong.
  * workspace: gs_paged_attention_workspace_bytes (ragged: for calls with
  * cu_seqlens) whatever the batch, 16-byte aligned; its first
  * GS_PAGED_HEAD_BYTES are ZEROED before the first call (counters: every call

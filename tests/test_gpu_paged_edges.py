@@ -131,3 +131,15 @@ def test_capture_ids(dev):
             s.wait_stream(fork)
         assert _lib.capture_id(s.cuda_stream) == 0 and _lib.capture_id(fork.cuda_stream) == 0
     assert len(set(ids)) == 3 and 0 not in ids
+
+
+@pytest.mark.parametrize("n,max_q", [([1, 1, 0, 2, 1, 4], 4), ([1, 1, 0, 2, 1, 4], 2), ([5, 1, 40, 130], 1), ([5, 1, 40, 130], 3)])
+@pytest.mark.parametrize("heads,kv,dim,window", [(8, 2, 128, 0), (4, 4, 64, 90), (6, 3, 80, 0)])
+def test_few_rows_by_hint(dev, n, max_q, heads, kv, dim, window):
+    """max_q keeps a batch of short rows off the chunk form; one that is too small costs time, no rows."""
+    _say(f"rows {n}, max_q {max_q}, {heads}/{kv} x {dim} window {window}")
+    b = Batch(dev, n, [700, 3, 50, 0, 64, 2100][: len(n)], heads, kv, dim, seed=dim)
+    out, lse = torch.full_like(b.q, math.nan), torch.full((sum(n), heads), math.nan, device=dev)
+    b.run(window=window, max_q=max_q, out=out, lse=lse)
+    torch.cuda.synchronize()
+    b.check(out, window=window, lse=lse)

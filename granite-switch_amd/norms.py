@@ -91,6 +91,8 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
     if residual.dim() == 0:
         raise ValueError("residual_norm: residual must have a hidden dimension")
     hidden = residual.shape[-1]
+    if hidden >= 2 ** 31:
+        raise ValueError(f"residual_norm: hidden={hidden} (up to 2^31 - 1)")
     if weight.dtype in _DTYPES and x is None and out is not None:
         dtype = out.dtype
     else:

@@ -27,6 +27,7 @@ import torch
 
 from . import _lib
 
+_INT32 = 2 ** 31 - 1        # what the library's 32-bit arguments hold; ctypes cuts larger values silently
 _DTYPES = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_FP32}
 
 
@@ -80,8 +81,8 @@ def _caches(who: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_he
                              f"both caches alike, got {c.dtype} {tuple(c.shape)}")
         if c.stride(3) != 1 and head_dim > 1:
             raise ValueError(f"{who}: {name}'s head dimension must be contiguous (strides {c.stride()})")
-    if k_cache.shape[0] == 0 or k_cache.shape[2] == 0:
-        raise ValueError(f"{who}: the caches hold no rows ({tuple(k_cache.shape)})")
+    if k_cache.shape[0] == 0 or not 0 < k_cache.shape[2] <= _INT32:
+        raise ValueError(f"{who}: pages of {k_cache.shape[2]} rows, {k_cache.shape[0]} of them (1 .. 2^31 - 1 rows)")
 
 
 def _on_gpu(who: str, device: torch.device, *ts) -> None:
@@ -152,6 +153,8 @@ def cache_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int,
         num_tokens = B
     elif num_tokens != B:
         raise ValueError(f"cache_slots: num_tokens={num_tokens} of {B} sequences without cu_seqlens")
+    if not 0 < page_size <= _INT32:
+        raise ValueError(f"cache_slots: page_size={page_size}")
     slots = torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device)
     positions = torch.empty(num_tokens, dtype=torch.int64, device=kv_lens.device)
     _lib.call("gs_cache_slots", page_table.data_ptr(), _table_ld(page_table), page_table.shape[1], int(num_pages),
@@ -324,7 +327,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if plan is None:
         plan = _keep(_attention_plans, key, _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window,
                                                             out, lse, max_q, workspace))
-    code, T, B, H, HK, D, q_st, k_st, v_st, pages, page, table, o_st, most, need, default_scale = plan
+    code, T, B, H, HK, D, q_st, k_st, v_st, pages, page, table, o_st, window, most, need, default_scale = plan
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if T == 0:
@@ -374,7 +377,8 @@ def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window
         need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None) if T else 0
     return (_DTYPES[dtype], T, B, H, HK, D, q.stride()[:2], k_cache.stride()[:3], v_cache.stride()[:3], k_cache.shape[0],
             k_cache.shape[2], (_table_ld(page_table), page_table.shape[1]),
-            (H * D, D) if out is None else out.stride()[:2], 1 if cu_seqlens is None else int(max_q or 0), need,
+            (H * D, D) if out is None else out.stride()[:2], min(window, _INT32),      # no sequence is longer
+            1 if cu_seqlens is None else min(int(max_q or 0), _INT32), need,
             1.0 / math.sqrt(D))
 
 

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from granite_switch_amd import paged
+from granite_switch_amd import norms, paged
 from test_gpu_paged import BF16, FP32, Batch, _say
 
 pytestmark = pytest.mark.gpu
@@ -143,3 +143,26 @@ def test_few_rows_by_hint(dev, n, max_q, heads, kv, dim, window):
     b.run(window=window, max_q=max_q, out=out, lse=lse)
     torch.cuda.synchronize()
     b.check(out, window=window, lse=lse)
+
+
+def test_sizes_past_32_bits(dev):
+    """What the library takes as 32 bits is not cut to them: a wider window is none, other sizes are refused."""
+    _say("sizes past 32 bits")
+    b = Batch(dev, [5, 1, 40], [10, 20, 30], 8, 2, 64)
+    want = b.run()
+    assert not torch.equal(b.run(window=5), want)
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 70):
+        assert torch.equal(b.run(window=window), want), window
+    assert torch.equal(b.run(max_q=2 ** 32 + 1), want)
+    for kw in (dict(page_size=2 ** 32 + 16), dict(page_size=-(2 ** 32) + 16)):
+        with pytest.raises(ValueError, match="page_size"):
+            paged.cache_slots(b.table, b.lens, num_pages=b.k.shape[0], cu_seqlens=b.cu, num_tokens=46, **kw)
+    rows = torch.empty(1, 1, 1, 64, dtype=BF16, device=dev).expand(1, 1, 2 ** 32 + 16, 64)
+    one, slots = torch.empty(1, 1, 64, dtype=BF16, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match="rows"):
+        paged.append_kv_(None, one, one, rows, rows, slots)
+    with pytest.raises(ValueError, match="rows"):
+        paged.paged_attention(one, rows, rows, b.table[:1], b.lens[:1])
+    row = torch.empty(2 ** 32 + 8, dtype=BF16, device=dev)
+    with pytest.raises(ValueError, match="hidden"):
+        norms.residual_norm(row[None], row[None], row)

@@ -13,6 +13,8 @@ host synchronisation; no gradients are computed.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -70,7 +72,7 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
             dev = x.device
             y = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out
             r = torch.empty(x.shape, dtype=residual.dtype, device=dev) if residual_out is None else residual_out
-            if rows:
+            if rows and hidden:
                 _lib.call("gs_residual_norm", code, x.data_ptr(), ldx, residual.data_ptr(), ldr, r_code,
                           None if gate is None else gate.data_ptr(), *g_st, act,
                           None if post_weight is None else post_weight.data_ptr(), weight.data_ptr(), w_code, eps, scale,
@@ -108,22 +110,22 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
             raise ValueError(f"residual_norm: {name} must be a contiguous [{hidden}] tensor of {dtype} or float32, both "
                              f"weights alike, got {w.dtype} {tuple(w.shape)}")
     shape = residual.shape
+    rows = math.prod(shape[:-1])
     for t in (x, weight, gate, post_weight, out, residual_out):
         if t is not None and t.device != residual.device:
             raise ValueError("residual_norm: tensors must live on one GPU")
 
     def flat(t):
-        return t if t.dim() == 2 else t.reshape(-1, hidden)
+        return t if t.dim() == 2 else t.reshape(rows, hidden)
 
     def flat_out(name, t, dt):
         if t is None:
             return None
         if t.shape != shape or t.dtype != dt:
             raise ValueError(f"residual_norm: {name} is {t.dtype} {tuple(t.shape)}, expected {dt} {tuple(shape)}")
-        return t if t.dim() == 2 else t.view(-1, hidden)      # raises where a copy would be needed
+        return t if t.dim() == 2 else t.view(rows, hidden)      # raises where a copy would be needed
 
     r2 = flat(residual)
-    rows = r2.shape[0]
     _rows("residual", r2, r2.shape, residual.dtype)
     x2 = None if x is None else _rows("x", flat(x), r2.shape, dtype)
     y2 = flat_out("out", out, dtype)

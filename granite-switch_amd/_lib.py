@@ -186,5 +186,11 @@ def capture_id(stream: int) -> int:
     return found.value
 
 
+def no_gradients(who: str) -> RuntimeError:
+    """For a call whose inputs autograd tracks: their gradients would be lost silently."""
+    return RuntimeError(f"{who} computes no gradients: call it under torch.no_grad() / torch.inference_mode(), or with "
+                        "tensors that do not require grad")
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()

@@ -8,7 +8,8 @@
 
 with rms(t) = t * rsqrt(mean(t^2) + eps).  Sums and r' are held in fp32; y is
 taken from r' before r' is rounded.  Launched on torch's current stream without
-host synchronisation; no gradients are computed.
+host synchronisation.  No gradients are computed: inputs that autograd tracks are
+refused where gradients are enabled.
 """
 
 from __future__ import annotations
@@ -58,6 +59,10 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
     out, residual_out: results (allocated when None); ``residual_out=residual``
               updates the stream in place, ``out=x`` reuses x
     """
+    if torch.is_grad_enabled() and (residual.requires_grad or weight.requires_grad
+                                    or (x is not None and x.requires_grad) or (gate is not None and gate.requires_grad)
+                                    or (post_weight is not None and post_weight.requires_grad)):
+        raise _lib.no_gradients("residual_norm")
     if x is not None and x.dim() == 2 and residual.dim() == 2:
         key = (x.shape, x.stride(), x.dtype, x.device, residual.shape, residual.stride(), residual.dtype, residual.device,
                weight.shape, weight.stride(), weight.dtype, weight.device,

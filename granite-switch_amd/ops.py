@@ -178,7 +178,8 @@ if not _registered("append_kv"):
     def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   slots: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
                   interleaved: bool) -> torch.Tensor:
-        return paged.append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved=interleaved)
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return paged.append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved=interleaved)
 
     @append_kv.register_fake
     def _(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved):
@@ -191,7 +192,8 @@ if not _registered("paged_attention"):
     def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
                         kv_lens: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float | None, window: int,
                         max_q: int | None) -> torch.Tensor:
-        return paged.paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, max_q=max_q)
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return paged.paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, max_q=max_q)
 
     @paged_attention.register_fake
     def _(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, max_q):
@@ -204,7 +206,8 @@ if not _registered("residual_norm"):
     def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, scale: float,
                       gate: torch.Tensor | None, post_weight: torch.Tensor | None,
                       gate_act: str | None) -> tuple[torch.Tensor, torch.Tensor]:
-        return norms.residual_norm(x, residual, weight, eps, scale, gate, post_weight, gate_act)
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return norms.residual_norm(x, residual, weight, eps, scale, gate, post_weight, gate_act)
 
     @residual_norm.register_fake
     def _(x, residual, weight, eps, scale, gate, post_weight, gate_act):

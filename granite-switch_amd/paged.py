@@ -16,7 +16,8 @@ base model's cached prefix this way: its few invocation tokens are a chunk of
 queries (``cu_seqlens``) over a long cache.
 
 Everything is launched on torch's current stream without host synchronisation;
-bfloat16 or float32; no gradients are computed.
+bfloat16 or float32.  No gradients are computed: inputs that autograd tracks are
+refused where gradients are enabled.
 """
 
 from __future__ import annotations
@@ -178,6 +179,10 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
     q_out     receives q (allocated when None; q itself: in place).  q None: only
               k and v are handled, and None is returned.
     """
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                    or (q is not None and q.requires_grad)
+                                    or (cos_sin is not None and cos_sin.requires_grad)):
+        raise _lib.no_gradients("append_kv_")
     dev = k.device
     key = (None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype, dev, v.shape,
            v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape,
@@ -315,6 +320,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     A row that sees nothing (an empty sequence), or that is in no sequence (past
     cu_seqlens[B], where a step is padded to a fixed number of rows), gives zeros.
     """
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise _lib.no_gradients("paged_attention")
     dev = q.device
     key = (q.shape, q.stride(), q.dtype, dev, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, page_table.shape, page_table.stride(),

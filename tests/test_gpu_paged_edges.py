@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from granite_switch_amd import norms, paged
+from granite_switch_amd import norms, ops, paged
 from test_gpu_paged import BF16, FP32, Batch, _say
 
 pytestmark = pytest.mark.gpu
@@ -166,3 +166,22 @@ def test_sizes_past_32_bits(dev):
     row = torch.empty(2 ** 32 + 8, dtype=BF16, device=dev)
     with pytest.raises(ValueError, match="hidden"):
         norms.residual_norm(row[None], row[None], row)
+
+
+def test_registered_ops_and_autograd(dev):
+    """The registered ops take tracked inputs as any op without a formula does: forward works, backward says so."""
+    _say("registered ops, tracked inputs")
+    b = Batch(dev, [5, 1, 40], [10, 20, 30], 8, 2, 64)
+    want = b.run()
+    q = b.q.clone().requires_grad_()
+    got = ops.op("paged_attention")(q, b.k, b.v, b.table, b.lens, b.cu, None, 0, None)
+    assert torch.equal(got, want)
+    x, w = torch.randn(4, 64, device=dev, requires_grad=True), torch.ones(64, device=dev)
+    y, r = ops.op("residual_norm")(x, torch.zeros(4, 64, device=dev), w, 1e-5, 1.0, None, None, None)
+    assert torch.equal(r, x)
+    k = torch.randn(3, 2, 64, device=dev).to(BF16).requires_grad_()
+    slots = torch.arange(3, device=dev)
+    ops.op("append_kv")(b.q[:3], k, k, b.k, b.v, slots, None, None, False)
+    assert torch.equal(b.k[0, :, :3].transpose(0, 1), k)
+    with pytest.raises(RuntimeError):
+        got.sum().backward()

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from granite_switch_amd import _lib, paged
+from granite_switch_amd import _lib, norms, paged
 from test_paged_calls import ATTENTION, P, _refused
 from test_paged_model import BF16, FP32, _check_attention
 
@@ -86,3 +86,29 @@ def test_only_the_counters_are_cleared(monkeypatch, captured):
     buf = paged._workspace(torch.device("cpu"), 5, 1 << 20)
     head = _lib.GS_PAGED_HEAD_BYTES
     assert buf.numel() == 1 << 20 and not buf[:head].any() and bool((buf[head:] == 255).all())
+
+
+def _tracked():
+    """Calls of the entry points, each with one input that autograd tracks; every tensor is on the CPU, which comes later."""
+    t = lambda *s: torch.zeros(*s)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    slots = torch.zeros(2, dtype=torch.int64)
+    attention = dict(q=t(2, 8, 64), k_cache=t(4, 2, 16, 64), v_cache=t(4, 2, 16, 64), page_table=torch.zeros(2, 1, dtype=torch.int32),
+                     kv_lens=i32(1, 1))
+    append = dict(q=t(2, 8, 64), k=t(2, 2, 64), v=t(2, 2, 64), k_cache=t(4, 2, 16, 64), v_cache=t(4, 2, 16, 64), slots=slots,
+                  positions=slots, cos_sin=t(4, 64))
+    norm = dict(x=t(2, 64), residual=t(2, 64), weight=t(64), gate=t(2, 64), post_weight=t(64))
+    for f, base, names in ((paged.paged_attention, attention, ("q", "k_cache", "v_cache")),
+                           (paged.append_kv_, append, ("q", "k", "v", "k_cache", "v_cache", "cos_sin")),
+                           (norms.residual_norm, norm, ("x", "residual", "weight", "gate", "post_weight"))):
+        for name in names:
+            yield pytest.param(f, {**base, name: base[name].clone().requires_grad_()}, id=f"{f.__name__}-{name}")
+
+
+@pytest.mark.parametrize("f,kw", _tracked())
+def test_tracked_inputs_are_refused(f, kw):
+    """Nothing here computes gradients: a call that autograd would have to follow says so."""
+    with pytest.raises(RuntimeError, match="no gradients"):
+        f(**kw)
+    with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):
+        f(**kw)

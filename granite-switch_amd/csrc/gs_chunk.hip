@@ -348,7 +348,8 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
         p[i] = __builtin_amdgcn_exp2f(fmaf(sc[g >> 1][8 * (g & 1) + i], a.scale_log2, -ms));
         lsum += p[i];
       }
-      // bf16 probabilities (relative error 2^-8, as the values and the result have); the total stays in fp32
+      // bf16 probabilities, as in the row form, with the same error; two bf16 numbers for each
+      // would be half as many products again, and products bound this form.  The total stays in fp32.
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
     }

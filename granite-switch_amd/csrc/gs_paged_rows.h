@@ -583,8 +583,12 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
       lsum += p[i];
     }
     if constexpr (BF16) {
-      // probabilities enter the product in bf16 (relative error 2^-8, as the
-      // values and the result have); their total stays in fp32
+      // Probabilities enter the product in bf16, their total stays in fp32.  Each is off by
+      // up to 2^-8 of itself, as the values and the result are; with values of both signs a
+      // result's error against 64 bits grows to at most sqrt(2) of what its own rounding
+      // leaves: 1.9e-3 for 256 sequences of 16 .. 2047 keys and 2.2e-3 for one of 131071.  As
+      // the sum of two bf16 numbers each they give 1.7e-3 and take 110.7 and 106.7 us, where
+      // this takes 109.0 and 104.8.
       u32x4 pf;
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);

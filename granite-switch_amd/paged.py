@@ -311,6 +311,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                cu_seqlens[s + 1], its last tokens; None: one row per sequence
     scale      of the scores (1 / sqrt(D) when None)
     window     > 0: a row sees the last ``window`` tokens up to its own
+    out        receives the result (allocated when None; q itself: in place)
     lse        [T, heads] float32: receives the log of each softmax's total
     max_q      the most query rows of a sequence where the caller knows it: a choice of
                kernels only, one that is too small costs time
@@ -319,6 +320,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     A row that sees nothing (an empty sequence), or that is in no sequence (past
     cu_seqlens[B], where a step is padded to a fixed number of rows), gives zeros.
+    Keys and values that no row of the call sees may hold anything; a value that is
+    not finite may also reach rows of its sequence that come before it.
     """
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise _lib.no_gradients("paged_attention")

@@ -533,7 +533,8 @@ int64_t gs_check_gemm_addresses(int64_t M, int64_t N, int64_t K, int64_t lda, in
  * for the pairs (j, j + R/2), or (2j, 2j + 1) with interleaved != 0; columns
  * from R on are copied (R = 0: no rotation, positions and cos_sin NULL).
  * Computed in fp32, rounded once.  q [num_tokens, heads, head_dim], k and v
- * [num_tokens, kv_heads, head_dim] with token and head strides; q_out may be q.
+ * [num_tokens, kv_heads, head_dim] with token and head strides; q_out may be
+ * q, with q's strides, and overlaps nothing else.
  * heads = 0: q and q_out are not used.  A slot outside [0, num_pages *
  * page_size) stores nothing (padding rows: -1); two tokens of a call must not
  * have the same slot.  Positions outside the table take its first or last row.
@@ -564,8 +565,11 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * that sees nothing (an empty sequence, p < 0) gets zeros.  lse [num_tokens,
  * heads] fp32 or NULL: the natural logarithm of the softmax's total, -inf for
  * such a row.  Cache rows that no row of a call sees may hold anything (NaN
- * too).  Rows before cu_seqlens[0] and from cu_seqlens[num_seqs] on are in no
- * sequence and get the same zeros and -inf.
+ * too); a value that is not finite, in a row that some row of the call sees,
+ * may also reach rows of its sequence that do not (0 times it is NaN).  Rows
+ * before cu_seqlens[0] and from cu_seqlens[num_seqs] on are in no sequence and
+ * get the same zeros and -inf.  out may be q, with q's strides, and overlaps
+ * nothing else.
  * Limits: head_dim a multiple of 8 (fp32: 4) up to 256, page_size a multiple
  * of 8; q, caches and out 16-byte aligned, strides multiples of 16 bytes.
  * A window no sequence is longer than is none; num_tokens and a narrower one

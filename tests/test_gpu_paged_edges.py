@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from granite_switch_amd import norms, ops, paged
+from granite_switch_amd import _lib, norms, ops, paged
 from test_gpu_paged import BF16, FP32, Batch, _say
 
 pytestmark = pytest.mark.gpu
@@ -114,8 +114,6 @@ def test_graphs_beside_eager_calls(dev, ragged):
 
 def test_capture_ids(dev):
     """Each capture has an id of its own, the same on every stream that it forks to; none outside of one."""
-    from granite_switch_amd import _lib
-
     s, fork, x, ids = torch.cuda.Stream(), torch.cuda.Stream(), torch.zeros(8, device=dev), []
     torch.cuda.synchronize()
     assert _lib.capture_id(s.cuda_stream) == 0
@@ -185,3 +183,36 @@ def test_registered_ops_and_autograd(dev):
     assert torch.equal(b.k[0, :, :3].transpose(0, 1), k)
     with pytest.raises(RuntimeError):
         got.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_own_workspace(dev, dtype):
+    """One workspace for calls of all kinds, one after the other: each leaves its counters at zero."""
+    _say(f"own workspace {dtype}")
+    n = [1, 40, 3, 130, 1]
+    cached = [2100, 900, 5000, 3000, 0]
+    ragged = Batch(dev, n, cached, 8, 2, 128, dtype=dtype, seed=1)
+    decode = Batch(dev, [1] * 5, cached, 8, 2, 128, dtype=dtype, seed=2, decode=True)
+    need = paged.workspace_bytes(dtype, 8, 2, 128, ragged=True)
+    assert need >= paged.workspace_bytes(dtype, 8, 2, 128)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=dev)
+    ws[:_lib.GS_PAGED_HEAD_BYTES] = 0
+    for b in (ragged, decode, ragged, decode):
+        out = b.run(workspace=ws)
+        torch.cuda.synchronize()
+        assert not ws[:_lib.GS_PAGED_HEAD_BYTES].any()
+        b.check(out)
+        assert torch.equal(out, b.run())
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim", [(BF16, 8, 2, 128), (BF16, 6, 2, 80), (BF16, 16, 2, 256), (FP32, 6, 2, 64)])
+def test_out_in_place(dev, dtype, heads, kv, dim):
+    """The result may take the queries' place."""
+    _say(f"out is q {dtype} {heads}/{kv} x {dim}")
+    for decode in (False, True):
+        n = [1] * 4 if decode else [1, 40, 3, 130]
+        b = Batch(dev, n, [4100, 900, 5000, 3000], heads, kv, dim, dtype=dtype, seed=3, decode=decode)
+        want, q = b.run(), b.q.clone()
+        got = paged.paged_attention(q, b.k, b.v, b.table, b.lens, b.cu, out=q)
+        torch.cuda.synchronize()
+        assert got is q and torch.equal(q, want)

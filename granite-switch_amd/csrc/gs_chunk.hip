@@ -19,10 +19,11 @@
 // 16 scores of 32 keys are, packed in order, the operand that O^T = V^T P^T takes
 // (its keys permuted alike: V^T is read transposed from LDS, 4 keys at a time).
 //
-// Its products bound it: 4 D operations a score.  8192 rows of 16 prompts (32 query, 8
-// key/value heads of 128): 104 us, 630 TFLOP/s of the products that the mask leaves,
-// 1078 in the loop, where a large library product reaches 1392.  A step of 48 decode
-// rows and 16 chunks of 256 over up to 3839 keys: 90 us.
+// 4 D operations a score, and on the vector units its exponential, maximum, total and
+// packing: these take 54% of the SIMDs' cycles and the products 30% (prompts), with two waves a
+// SIMD to overlap them.  8192 rows of 16 prompts (32 query, 8 key/value heads of 128):
+// 105 us, 620 TFLOP/s of the products that the mask leaves, where a large library product
+// reaches 1586.  A step of 48 decode rows and 16 chunks of 256 over up to 3839 keys: 90 us.
 #include <algorithm>
 
 #include "gs_paged_rows.h"
@@ -348,8 +349,8 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
         p[i] = __builtin_amdgcn_exp2f(fmaf(sc[g >> 1][8 * (g & 1) + i], a.scale_log2, -ms));
         lsum += p[i];
       }
-      // bf16 probabilities, as in the row form, with the same error; two bf16 numbers for each
-      // would be half as many products again, and products bound this form.  The total stays in fp32.
+      // bf16 probabilities with the error they have in the row form; two bf16 numbers for each
+      // are half as many products again, where instructions bound.  The total stays in fp32.
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
     }

@@ -9,7 +9,7 @@
 // One pass: a row's values stay in registers between the two sums, so x, r and
 // the gate are read once and r' and y written once -- 8 bytes an element in
 // bf16 against 2 to 3 operations a byte: the memory rate bounds it.  4144 rows of
-// 4096, bf16: 23.5 us, 5.8 TB/s.  Sums and r' are held in fp32; y is taken from the r'
+// 4096, bf16: 23.4 us, 5.8 TB/s.  Sums and r' are held in fp32; y is taken from the r'
 // before its rounding.
 #include <hip/hip_runtime.h>
 

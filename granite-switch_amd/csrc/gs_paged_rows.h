@@ -9,9 +9,9 @@
 //
 // The memory rate bounds it: 2 G operations a byte of the cache (G query heads to a
 // key/value head).  256 sequences of 16 .. 2047 keys, 8 key/value heads of 128, bf16:
-// 109 us, 4.8 TB/s; one of 131071 keys: 105 us, 5.1 TB/s.  The longest parts
-// start first: 112 us against 118 for the 256 sequences.  Equal runs of the batch's
-// units, cut wherever they end, cost two joins a workgroup and took 114.
+// 109 us, 4.8 TB/s; one of 131071 keys: 105 us, 5.1 TB/s; a bare read reaches 6.8.  The
+// longest parts start first: 112 us against 118 for the 256 sequences.  Equal runs of the
+// batch's units, cut wherever they end, cost two joins a workgroup and took 114.
 #pragma once
 
 #include "gs_paged.h"

@@ -62,8 +62,8 @@ class SwitchedDecoderLayer(nn.Module):
         if not gate_up.fuse_swiglu:
             raise ValueError("SwitchedDecoderLayer: gate_up needs fuse_swiglu")
         self.qkv, self.o_proj, self.gate_up, self.down = qkv, o_proj, gate_up, down
-        self.register_buffer("input_norm", input_norm)
-        self.register_buffer("mlp_norm", mlp_norm)
+        self.register_buffer("input_norm", input_norm.detach())
+        self.register_buffer("mlp_norm", mlp_norm.detach())
         self.heads, self.kv_heads, self.head_dim, self.eps = heads, kv_heads, head_dim, eps
         self.residual_multiplier, self.attention_multiplier, self.window = residual_multiplier, attention_multiplier, window
 
@@ -92,7 +92,7 @@ class SwitchedDecoder(nn.Module):
     def __init__(self, layers: list, final_norm: torch.Tensor, num_adapters: int):
         super().__init__()
         self.layers = nn.ModuleList(layers)
-        self.register_buffer("final_norm", final_norm)
+        self.register_buffer("final_norm", final_norm.detach())
         self.num_adapters = num_adapters
         self.ctx = LoRAContext()
         self.meta = FusedLoRAKernelMeta(final_norm.device)

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from granite_switch_amd import _lib, norms, paged
+from granite_switch_amd import _lib, decoder, norms, paged, vllm_layers
 from test_paged_calls import ATTENTION, P, _refused
 from test_paged_model import BF16, FP32, _check_attention
 
@@ -112,3 +112,15 @@ def test_tracked_inputs_are_refused(f, kw):
         f(**kw)
     with torch.no_grad(), pytest.raises(ValueError, match="on the GPU"):
         f(**kw)
+
+
+def test_decoder_keeps_norm_weights_out_of_autograd():
+    """A model's norm weights are parameters: the decoder, which computes no gradients, takes their values."""
+    lin = lambda n_in, slices, **kw: vllm_layers.SwitchedLoRALinear(
+        torch.nn.Linear(n_in, sum(slices), bias=False), 1, 8, num_slices=len(slices), output_slices=slices, **kw)
+    w = [torch.nn.Parameter(torch.ones(64)) for _ in range(3)]
+    layer = decoder.SwitchedDecoderLayer(lin(64, (128, 64, 64)), lin(128, (64,)), lin(64, (128, 128), fuse_swiglu=True),
+                                         lin(128, (64,)), w[0], w[1], heads=2, kv_heads=1, head_dim=64)
+    dec = decoder.SwitchedDecoder([layer], w[2], 1)
+    for got, given in ((layer.input_norm, w[0]), (layer.mlp_norm, w[1]), (dec.final_norm, w[2])):
+        assert not got.requires_grad and got.data_ptr() == given.data_ptr()

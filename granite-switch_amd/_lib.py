@@ -26,6 +26,7 @@ GS_ERR_HIP = 2
 GS_ERR_WORKSPACE = 3
 GS_DTYPE_BF16 = 0
 GS_DTYPE_FP32 = 1
+GS_DTYPE_E4M3 = 2
 GS_MAX_ADAPTERS = 256
 GS_MAX_SLICES = 8
 GS_MAX_RANK = 512
@@ -98,6 +99,12 @@ SIGNATURES = {
     "gs_append_kv": (c_i32, [c_i32] + [c_void_p, c_i64, c_i64] * 3 + [c_i64, c_i32, c_i32, c_i32, c_void_p, c_void_p,
                              c_i64, c_i32, c_i32, c_void_p] + [c_void_p, c_i64, c_i64, c_i64] * 2
                      + [c_i64, c_i32, c_void_p, c_i64, c_i64, c_void_p]),
+    "gs_append_kv_normed": (c_i32, [c_i32] + [c_void_p, c_i64, c_i64] * 3 + [c_i64, c_i32, c_i32, c_i32, c_void_p, c_void_p,
+                                    c_i32, ctypes.c_float, c_void_p, c_void_p, c_i64, c_i32, c_i32, c_void_p, c_i32]
+                            + [c_void_p, c_i64, c_i64, c_i64] * 2 + [c_void_p, c_i64, c_i64] * 2
+                            + [c_i64, c_i32, c_void_p, c_i64, c_i64, c_void_p]),
+    "gs_read_kv": (c_i32, [c_i32, c_i32] + [c_void_p, c_i64, c_i64, c_i64] * 2 + [c_void_p, c_i64, c_i64] * 2
+                   + [c_i64, c_i32, c_i32, c_i32, c_void_p, c_i64] + [c_void_p, c_i64, c_i64] * 2 + [c_void_p]),
     "gs_cache_slots": (c_i32, [c_void_p, c_i64, c_i32, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_void_p,
                                c_void_p, c_void_p]),
     "gs_paged_attention_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32, c_i32]),
@@ -105,6 +112,11 @@ SIGNATURES = {
                            + [c_i64, c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_i32, c_i32,
                               c_i32, c_i32, ctypes.c_float, c_i32, c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64,
                               c_void_p]),
+    "gs_paged_attention_e4m3": (c_i32, [c_i32, c_void_p, c_i64, c_i64] + [c_void_p, c_i64, c_i64, c_i64] * 2
+                                + [c_void_p, c_i64, c_i64] * 2
+                                + [c_i64, c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p, c_i32, c_i64, c_i32, c_i32,
+                                   c_i32, c_i32, ctypes.c_float, c_i32, c_void_p, c_i64, c_i64, c_void_p, c_void_p, c_i64,
+                                   c_void_p]),
     "gs_capture_id": (c_i32, [c_void_p, c_void_p]),
     "gs_check_paged_addresses": (c_i64, [c_i32] + [c_i64] * 9 + [c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p,
                                          c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32,
@@ -112,6 +124,11 @@ SIGNATURES = {
     "gs_check_append_addresses": (c_i64, [c_i32, c_i32] + [c_i64] * 5 + [c_i32, c_i32, c_i32, c_void_p, c_i64, c_i32,
                                           c_i32, c_void_p] + [c_i64] * 4 + [c_i32, c_i32, ctypes.c_char_p, c_i64,
                                           c_void_p]),
+    "gs_check_paged_e4m3_addresses": (c_i64, [c_i32] + [c_i64] * 11 + [c_i32, c_void_p, c_i64, c_i32, c_void_p, c_void_p,
+                                              c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_i32,
+                                              ctypes.c_char_p, c_i64, c_void_p]),
+    "gs_check_rows_addresses": (c_i64, [c_i32, c_i32, c_i32] + [c_i64] * 5 + [c_i32, c_i32, c_i32, c_void_p, c_i64, c_i32,
+                                        c_i32, c_void_p] + [c_i64] * 6 + [c_i32, c_i32, ctypes.c_char_p, c_i64, c_void_p]),
     "gs_residual_norm": (c_i32, [c_i32, c_void_p, c_i64, c_void_p, c_i64, c_i32, c_void_p, c_i64, c_i64, c_i32,
                                  c_void_p, c_void_p, c_i32, ctypes.c_float, ctypes.c_float, c_i64, c_i32, c_void_p,
                                  c_i64, c_void_p, c_i64, c_void_p]),

@@ -284,6 +284,12 @@ GS_HD int append_pair(int u, int VE) { return VE * u; }
 // The table row of a position (those outside the table: its first or last).
 GS_HD int64_t append_pos(int64_t pos, int64_t max_pos) { return pos < 0 ? 0 : lmin(pos, max_pos - 1); }
 GS_HD bool append_stored(int64_t slot, int64_t num_slots) { return slot >= 0 && slot < num_slots; }
+// The scale's byte e + 127 of a quantised row whose largest finite magnitude has these
+// bits: the least e >= -126 with m <= 448 2^e = 1.75 2^(8 + e).
+GS_HD int e8m0_of(uint32_t bits) {
+  const int code = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return code < 1 ? 1 : code;
+}
 // A sequence of a batch: its first query row and number of query rows within
 // the T rows given, and its cached tokens within what its table row addresses.
 struct PagedSeq {

@@ -43,6 +43,9 @@ struct PagedArgs {
   addr::ChunkTq tq;                 // queries of a chunk tile
   uint32_t g_magic;                 // div_magic(G)
   float scale_log2;
+  const uint8_t* ks;                // scales of a quantised cache, page and head strides
+  const uint8_t* vs;
+  int64_t ks_ps, ks_hs, vs_ps, vs_hs;
 };
 
 __device__ __host__ __forceinline__ addr::PagedSeq any_seq(const PagedArgs& a, int s) {
@@ -80,6 +83,8 @@ int64_t chunk_workspace_bytes(int HK, int DT, int cus);
 int64_t chunk_most_parts(const PagedArgs& a);
 int64_t ragged_grid(const PagedArgs& a);
 void launch_ragged(const PagedArgs& a, int DT, hipStream_t st);
+// The row form over a quantised cache (gs_paged_e4m3.hip), on that many workgroups.
+void launch_rows_e4m3(const PagedArgs& a, bool bf16, int DT, int64_t workgroups, hipStream_t st);
 
 // Strides that keep rows on 16-byte boundaries.
 inline bool strides_ok(int64_t a, int64_t b, int n) { return a >= 0 && b >= 0 && a % n == 0 && b % n == 0; }

@@ -17,45 +17,6 @@
 namespace gs {
 namespace {
 
-// Workgroups i of n of each key/value head take its parts i, 2 n - 1 - i, 2 n + i, ...:
-// the parts get shorter, so whoever has a longer one has a shorter one next.  One
-// start for several parts: 223 sequences of 4 .. 429 keys with 16 heads 60 us against 71
-// with a workgroup for each, 1024 of 16 .. 400 with 8 heads 164 against 229.  The first
-// wave lists up to 32 of a workgroup's parts in one pass over the batch.
-constexpr int kRowList = 32;
-template <bool BF16, int DT>
-__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs) {
-  __shared__ RowShared<DT> sh;
-  __shared__ RowOrder<BF16, DT> kept[64];            // a lane's, between lists
-  __shared__ RowEntry list[kRowList];
-  __shared__ int parts;
-  const int HK = fresh_args().HK;
-  const int i = blockIdx.x / HK, h = blockIdx.x - i * HK, n = gridDim.x / HK;
-  for (int k0 = 0;; k0 += kRowList) {
-    if (threadIdx.x < 64) {
-      const PagedArgs& a = fresh_args();
-      RowOrder<BF16, DT> order;
-      if (k0 == 0) {
-        order.plan(a);
-        kept[threadIdx.x] = order;
-        if (threadIdx.x == 0) parts = order.total;
-      } else {
-        order = kept[threadIdx.x];
-      }
-      order.list_parts(a, i, n, k0, k0 + kRowList, list);
-    }
-    __syncthreads();
-    const int total = __builtin_amdgcn_readfirstlane(parts);
-    for (int k = k0; k < k0 + kRowList && k * n < total; ++k) {
-      if (k * n + ((k & 1) != 0 ? n - 1 - i : i) >= total) continue;
-      row_part<BF16, DT>(fresh_args(), row_item(list[k - k0]), h, sh);
-      __syncthreads();                               // every wave is past what the part left in sh, and its entry
-    }
-    if ((k0 + kRowList) * n >= total) break;
-  }
-  zero_outside<BF16>(fresh_args());
-}
-
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -76,6 +37,7 @@ int64_t row_partial_floats(int HK, int D, int cus) {
 // Whether ragged calls of these sizes have a chunk form, and the rows up to
 // which a sequence stays with the row form.
 bool chunk_form(bool bf16, int G, int D) { return bf16 && D <= 128 && G <= kChunkRows; }
+bool has_chunk_form(const PagedArgs& a, bool bf16) { return a.ks == nullptr && chunk_form(bf16, a.G, a.D); }
 constexpr int kRowFormRows = 16;
 
 int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus) {
@@ -107,7 +69,7 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.page_magic = addr::div_magic(a.page_octets);
   // The chunk form hides keys and takes the maximum before it scales, which is right for a
   // scale above zero only; the row form scales first.
-  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) && scale > 0.f ? kRowFormRows : INT32_MAX;
+  a.row_limit = a.cu != nullptr && has_chunk_form(a, bf16) && scale > 0.f ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
   a.row_slots = addr::row_slots_per_head(a.HK, 2 * cus);
   a.row_wgs = row_wgs_for(a.D, cus);
@@ -139,17 +101,19 @@ void launch_paged(const PagedArgs& a, int64_t n, hipStream_t st) {
 
 
 // The attention kernels for one width and element type.
-template <bool BF16, int DT>
+template <bool BF16, int DT, bool E4M3>
 void model_attention(PagedModel& m, const PagedArgs& a) {
-  using F = PagedForm<BF16, DT>;
+  using F = PagedForm<BF16, DT, E4M3>;
   constexpr int kUnit = F::kBlock * kPWaves;
-  constexpr int kVec = 16 / F::kES;
+  constexpr int kVec = 16 / F::kES, kKVec = 16 / F::kCS;
   const int max_pages = static_cast<int>(a.max_len / (8 * a.page_octets));
   const int64_t page_rows = 8 * a.page_octets;
   const int64_t k_elems = extent3(a.num_pages, a.k_ps, a.HK, a.k_hs, page_rows, a.k_rs, a.D);
   const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
   const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D);
   const int64_t o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
+  const int64_t ks_elems = extent3(a.num_pages, a.ks_ps, a.HK, a.ks_hs, page_rows, 1, 1);
+  const int64_t vs_elems = extent3(a.num_pages, a.vs_ps, a.HK, a.vs_hs, page_rows, 1, 1);
   std::vector<char> slots(static_cast<size_t>(a.row_slots), 0);
   std::vector<char>& rows = m.rows;
   int64_t U = 0;
@@ -199,7 +163,7 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
           const int qi = live ? static_cast<int>(r / a.G) : t.i0;
           const int64_t qh = h * a.G + (live ? r - static_cast<int64_t>(qi) * a.G : 0);
           for (int st = 0; st < F::kSteps; ++st) {
-            const int d = kVec * (4 * st + lg);
+            const int d = row_q_col<BF16, DT, E4M3>(st, lg);
             m.in("q", (sq.q0 + qi) * a.q_ts + qh * a.q_hs + (d < a.D ? d : 0), kVec, q_elems);
           }
           const int k_oct = BF16 ? 8 * (lq >> 2) : 8 * (lq >> 3), v_oct = BF16 ? 8 * lg : 8 * (lg >> 1);
@@ -214,14 +178,20 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
             m.in("page table row", kp, 1, max_pages);
             m.in("page table row", vp, 1, max_pages);
             if (m.bad) return;
-            const int64_t kb = addr::paged_page(a.table[s * a.ld_table + kp], a.num_pages) * a.k_ps + h * a.k_hs + (kr * 8 + k_in) * a.k_rs;
-            const int64_t vb = addr::paged_page(a.table[s * a.ld_table + vp], a.num_pages) * a.v_ps + h * a.v_hs + (vr * 8 + v_in) * a.v_rs;
+            const int64_t k_page = addr::paged_page(a.table[s * a.ld_table + kp], a.num_pages);
+            const int64_t v_page = addr::paged_page(a.table[s * a.ld_table + vp], a.num_pages);
+            const int64_t kb = k_page * a.k_ps + h * a.k_hs + (kr * 8 + k_in) * a.k_rs;
+            const int64_t vb = v_page * a.v_ps + h * a.v_hs + (vr * 8 + v_in) * a.v_rs;
+            if (E4M3) {
+              m.in("k scales", k_page * a.ks_ps + h * a.ks_hs + kr * 8, 8, ks_elems);
+              m.in("v scales", v_page * a.vs_ps + h * a.vs_hs + vr * 8, 8, vs_elems);
+            }
             m.in("page row", kr * 8 + k_in + 4 * (F::kKT - 1), 1, page_rows);
             m.in("page row", vr * 8 + v_in + F::kKeys - 1, 1, page_rows);
             for (int u2 = 0; u2 < F::kKT; ++u2)
-              for (int st = 0; st < F::kSteps; ++st) {
-                const int d = kVec * (4 * st + lg);
-                m.in("k cache", kb + 4 * u2 * a.k_rs + (d < a.D ? d : 0), kVec, k_elems);
+              for (int p = 0; p < F::kKP; ++p) {
+                const int d = row_k_col<BF16, DT, E4M3>(p, lg);
+                m.in("k cache", kb + 4 * u2 * a.k_rs + (d < a.D ? d : 0), kKVec, k_elems);
               }
             for (int tt = 0; tt < F::kKeys; ++tt)
               for (int n = 0; n < F::kVN; ++n) {
@@ -360,6 +330,155 @@ void model_rows(PagedModel& m, const PagedArgs& a) {
   }
 }
 
+// Scales of a quantised cache (k NULL: it is not).
+struct Scales {
+  const uint8_t* k;
+  int64_t k_ps, k_hs;
+  const uint8_t* v;
+  int64_t v_ps, v_hs;
+};
+
+int paged_attention(const char* who, bool e4m3, Scales sc, int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs, const void* k_cache, int64_t k_ps,
+                    int64_t k_hs, int64_t k_rs, const void* v_cache, int64_t v_ps, int64_t v_hs, int64_t v_rs,
+                    int64_t num_pages, int32_t page_size, const int32_t* page_table, int64_t ld_table,
+                    int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                    int64_t num_tokens, int32_t max_q, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                    float scale, int32_t window, void* out, int64_t o_ts, int64_t o_hs, float* lse,
+                    void* workspace, int64_t workspace_bytes, void* stream) {
+  GS_CHECK_ARG(dtype == GS_DTYPE_BF16 || dtype == GS_DTYPE_FP32, "%s: dtype=%d", who, dtype);
+  GS_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t(1) << 31) && num_seqs >= 0, "%s: num_tokens=%lld num_seqs=%d", who,
+               (long long)num_tokens, num_seqs);
+  GS_CHECK_ARG(cu_seqlens != nullptr || num_tokens == num_seqs, "%s: num_tokens=%lld of num_seqs=%d without cu_seqlens", who,
+               (long long)num_tokens, num_seqs);
+  GS_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536 && kv_heads <= 4096, "%s: heads=%d kv_heads=%d", who, heads, kv_heads);
+  const bool bf16 = dtype == GS_DTYPE_BF16;
+  const int ve = bf16 ? 8 : 4;
+  const int de = e4m3 ? 16 : ve;                     // elements of 16 bytes of a cache row
+  GS_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % de == 0, "%s: head_dim=%d must be a multiple of %d up to 256", who,
+               head_dim, de);
+  GS_CHECK_ARG(page_size > 0 && page_size % 8 == 0, "%s: page_size=%d must be a multiple of 8", who, page_size);
+  GS_CHECK_ARG(num_pages > 0 && num_pages < (int64_t(1) << 31) && max_pages >= 0 && ld_table >= max_pages,
+               "%s: num_pages=%lld max_pages=%d ld_table=%lld", who, (long long)num_pages, max_pages, (long long)ld_table);
+  GS_CHECK_ARG(window >= 0 && max_q >= 0, "%s: window=%d max_q=%d", who, window, max_q);
+  GS_CHECK_ARG(num_tokens + paged_window(window, paged_reach(max_pages, page_size)) < (int64_t(1) << 31),
+               "%s: num_tokens=%lld with window=%d past 32 bits", who, (long long)num_tokens, window);
+  if (num_tokens == 0) return GS_OK;
+  // the stride of a dimension of one is never used, and may be anything
+  if (num_tokens == 1) q_ts = o_ts = 0;
+  if (heads == 1) q_hs = o_hs = 0;
+  if (kv_heads == 1) k_hs = v_hs = sc.k_hs = sc.v_hs = 0;
+  if (num_pages == 1) k_ps = v_ps = sc.k_ps = sc.v_ps = 0;
+  GS_CHECK_ARG(q != nullptr && k_cache != nullptr && v_cache != nullptr && out != nullptr &&
+                   (num_seqs == 0 || (kv_lens != nullptr && (page_table != nullptr || max_pages == 0))) &&
+                   (!e4m3 || (sc.k != nullptr && sc.v != nullptr)), "%s: null tensor", who);
+  GS_CHECK_ARG(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && strides_ok(q_ts, q_hs, ve) &&
+                   strides_ok(k_ps, k_hs, de) && strides_ok(v_ps, v_hs, de) && strides_ok(k_rs, v_rs, de) &&
+                   strides_ok(o_ts, o_hs, ve),
+               "%s: q, the caches and out must be 16-byte aligned with strides that are multiples of 16 bytes", who);
+  GS_CHECK_ARG(!e4m3 || (reinterpret_cast<uintptr_t>(sc.k) % 8 == 0 && reinterpret_cast<uintptr_t>(sc.v) % 8 == 0 &&
+                         strides_ok(sc.k_ps, sc.k_hs, 8) && strides_ok(sc.v_ps, sc.v_hs, 8)),
+               "%s: the scales must be 8-byte aligned with strides that are multiples of 8", who);
+  const int cus = device_cus();
+  const int64_t need = attention_ws_bytes(bf16, cu_seqlens != nullptr, heads / kv_heads, kv_heads, head_dim, cus);
+  if (workspace == nullptr || workspace_bytes < need) {
+    set_error("%s: workspace of %lld bytes needed (got %lld)", who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+    return GS_ERR_WORKSPACE;
+  }
+  GS_CHECK_ARG(aligned16(workspace), "%s: workspace must be 16-byte aligned", who);
+  PagedArgs a{};
+  a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
+  a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
+  a.k = k_cache; a.k_ps = k_ps; a.k_hs = k_hs; a.k_rs = k_rs;
+  a.v = v_cache; a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
+  a.table = page_table; a.ld_table = ld_table;
+  a.lens = kv_lens; a.cu = cu_seqlens; a.lse = lse;
+  a.num_pages = static_cast<int>(num_pages);
+  a.B = num_seqs; a.T = static_cast<int>(num_tokens);
+  a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
+  a.window = window;
+  a.ks = sc.k; a.ks_ps = sc.k_ps; a.ks_hs = sc.k_hs;
+  a.vs = sc.v; a.vs_ps = sc.v_ps; a.vs_hs = sc.v_hs;
+  plan_paged(a, bf16, cus, max_pages, page_size, scale);
+  const int DT = paged_width(head_dim);
+  int* head = static_cast<int*>(workspace);
+  a.row_count = head;
+  a.ws = reinterpret_cast<float*>(head + kHeadInts);
+  a.chunk_list = reinterpret_cast<int4*>(a.ws + row_partial_floats(kv_heads, head_dim, cus));
+  a.chunk_ws = reinterpret_cast<float*>(a.chunk_list) + chunk_list_floats(kv_heads, cus);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t n = row_grid(a);
+  if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
+    GS_CHECK_ARG(ragged_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
+    launch_ragged(a, DT, st);
+    GS_CHECK_LAUNCH(who);
+    return GS_OK;
+  }
+  // max_q says that no sequence is the chunk form's: workgroups for such a batch, which take
+  // whatever parts the lengths turn out to make
+  a.row_limit = INT32_MAX;
+  a.row_parts = row_most_parts(a);
+  GS_CHECK_ARG(n * a.HK < (int64_t(1) << 31) && a.row_parts < (int64_t(1) << 31), "%s: too many tiles", who);
+  if (e4m3) {
+    launch_rows_e4m3(a, bf16, DT, n * a.HK, st);
+    GS_CHECK_LAUNCH(who);
+    return GS_OK;
+  }
+  switch (DT) {
+    case 64: bf16 ? launch_paged<true, 64>(a, n, st) : launch_paged<false, 64>(a, n, st); break;
+    case 128: bf16 ? launch_paged<true, 128>(a, n, st) : launch_paged<false, 128>(a, n, st); break;
+    default: bf16 ? launch_paged<true, 256>(a, n, st) : launch_paged<false, 256>(a, n, st); break;
+  }
+  GS_CHECK_LAUNCH(who);
+  return GS_OK;
+}
+
+template <int DT>
+void model_width(PagedModel& m, const PagedArgs& a, bool bf16, bool e4m3) {
+  if (bf16) e4m3 ? model_attention<true, DT, true>(m, a) : model_attention<true, DT, false>(m, a);
+  else e4m3 ? model_attention<false, DT, true>(m, a) : model_attention<false, DT, false>(m, a);
+}
+
+int64_t check_addresses(const char* who, bool e4m3, int64_t s_ps, int64_t s_hs, int32_t dtype, int64_t q_ts, int64_t q_hs, int64_t k_ps, int64_t k_hs, int64_t k_rs,
+                        int64_t v_ps, int64_t v_hs, int64_t v_rs, int64_t num_pages, int32_t page_size,
+                        const int32_t* page_table, int64_t ld_table, int32_t max_pages,
+                        const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                        int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t window,
+                        int64_t o_ts, int64_t o_hs, int32_t cus, char* msg, int64_t msg_len,
+                        int64_t* checked) {
+  const bool bf16 = dtype == GS_DTYPE_BF16;
+  GS_CHECK_ARG((bf16 || dtype == GS_DTYPE_FP32) && num_tokens > 0 && num_seqs >= 0 && num_tokens < (int64_t(1) << 31) &&
+                   heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim <= 256 &&
+                   head_dim % (e4m3 ? 16 : bf16 ? 8 : 4) == 0 && page_size > 0 && page_size % 8 == 0 && num_pages > 0 &&
+                   max_pages >= 0 && ld_table >= max_pages && (num_seqs == 0 || kv_lens != nullptr) && window >= 0 && cus > 0 &&
+                   (cu_seqlens != nullptr || num_tokens == num_seqs), "%s: sizes", who);
+  PagedArgs a{};
+  a.q_ts = q_ts; a.q_hs = q_hs; a.o_ts = o_ts; a.o_hs = o_hs;
+  a.k_ps = k_ps; a.k_hs = k_hs; a.k_rs = k_rs;
+  a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
+  a.table = page_table; a.ld_table = ld_table; a.lens = kv_lens; a.cu = cu_seqlens;
+  a.num_pages = static_cast<int>(num_pages);
+  a.B = num_seqs; a.T = static_cast<int>(num_tokens);
+  a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
+  a.window = window;
+  static const uint8_t held = 0;
+  if (e4m3) a.ks = a.vs = &held;                     // only whether there are scales
+  a.ks_ps = a.vs_ps = s_ps; a.ks_hs = a.vs_hs = s_hs;
+  plan_paged(a, bf16, cus, max_pages, page_size, 1.f);
+  PagedModel m;
+  m.window = window;
+  m.rows.assign(static_cast<size_t>(a.T) * a.H, 0);
+  if (a.row_limit != INT32_MAX) paged_width(head_dim) == 64 ? model_chunk<64>(m, a) : model_chunk<128>(m, a);
+  switch (paged_width(head_dim)) {
+    case 64: model_width<64>(m, a, bf16, e4m3); break;
+    case 128: model_width<128>(m, a, bf16, e4m3); break;
+    default: model_width<256>(m, a, bf16, e4m3); break;
+  }
+  model_rows(m, a);
+  if (checked) *checked = m.checked;
+  if (msg && msg_len > 0) snprintf(msg, static_cast<size_t>(msg_len), "%s", m.msg);
+  return m.bad;
+}
+
 }  // namespace
 }  // namespace gs
 
@@ -383,80 +502,26 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs,
                        int64_t num_tokens, int32_t max_q, int32_t heads, int32_t kv_heads, int32_t head_dim,
                        float scale, int32_t window, void* out, int64_t o_ts, int64_t o_hs, float* lse,
                        void* workspace, int64_t workspace_bytes, void* stream) {
-  const char* who = "gs_paged_attention";
-  GS_CHECK_ARG(dtype == GS_DTYPE_BF16 || dtype == GS_DTYPE_FP32, "%s: dtype=%d", who, dtype);
-  GS_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t(1) << 31) && num_seqs >= 0, "%s: num_tokens=%lld num_seqs=%d", who,
-               (long long)num_tokens, num_seqs);
-  GS_CHECK_ARG(cu_seqlens != nullptr || num_tokens == num_seqs, "%s: num_tokens=%lld of num_seqs=%d without cu_seqlens", who,
-               (long long)num_tokens, num_seqs);
-  GS_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536 && kv_heads <= 4096, "%s: heads=%d kv_heads=%d", who, heads, kv_heads);
-  const bool bf16 = dtype == GS_DTYPE_BF16;
-  const int ve = bf16 ? 8 : 4;
-  GS_CHECK_ARG(head_dim > 0 && head_dim <= 256 && head_dim % ve == 0, "%s: head_dim=%d must be a multiple of %d up to 256", who,
-               head_dim, ve);
-  GS_CHECK_ARG(page_size > 0 && page_size % 8 == 0, "%s: page_size=%d must be a multiple of 8", who, page_size);
-  GS_CHECK_ARG(num_pages > 0 && num_pages < (int64_t(1) << 31) && max_pages >= 0 && ld_table >= max_pages,
-               "%s: num_pages=%lld max_pages=%d ld_table=%lld", who, (long long)num_pages, max_pages, (long long)ld_table);
-  GS_CHECK_ARG(window >= 0 && max_q >= 0, "%s: window=%d max_q=%d", who, window, max_q);
-  GS_CHECK_ARG(num_tokens + paged_window(window, paged_reach(max_pages, page_size)) < (int64_t(1) << 31),
-               "%s: num_tokens=%lld with window=%d past 32 bits", who, (long long)num_tokens, window);
-  if (num_tokens == 0) return GS_OK;
-  // the stride of a dimension of one is never used, and may be anything
-  if (num_tokens == 1) q_ts = o_ts = 0;
-  if (heads == 1) q_hs = o_hs = 0;
-  if (kv_heads == 1) k_hs = v_hs = 0;
-  if (num_pages == 1) k_ps = v_ps = 0;
-  GS_CHECK_ARG(q != nullptr && k_cache != nullptr && v_cache != nullptr && out != nullptr &&
-                   (num_seqs == 0 || (kv_lens != nullptr && (page_table != nullptr || max_pages == 0))), "%s: null tensor", who);
-  GS_CHECK_ARG(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && strides_ok(q_ts, q_hs, ve) &&
-                   strides_ok(k_ps, k_hs, ve) && strides_ok(v_ps, v_hs, ve) && strides_ok(k_rs, v_rs, ve) &&
-                   strides_ok(o_ts, o_hs, ve),
-               "%s: q, the caches and out must be 16-byte aligned with strides that are multiples of %d elements", who, ve);
-  const int cus = device_cus();
-  const int64_t need = attention_ws_bytes(bf16, cu_seqlens != nullptr, heads / kv_heads, kv_heads, head_dim, cus);
-  if (workspace == nullptr || workspace_bytes < need) {
-    set_error("%s: workspace of %lld bytes needed (got %lld)", who, (long long)need, (long long)(workspace ? workspace_bytes : 0));
-    return GS_ERR_WORKSPACE;
-  }
-  GS_CHECK_ARG(aligned16(workspace), "%s: workspace must be 16-byte aligned", who);
-  PagedArgs a{};
-  a.q = q; a.q_ts = q_ts; a.q_hs = q_hs;
-  a.out = out; a.o_ts = o_ts; a.o_hs = o_hs;
-  a.k = k_cache; a.k_ps = k_ps; a.k_hs = k_hs; a.k_rs = k_rs;
-  a.v = v_cache; a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
-  a.table = page_table; a.ld_table = ld_table;
-  a.lens = kv_lens; a.cu = cu_seqlens; a.lse = lse;
-  a.num_pages = static_cast<int>(num_pages);
-  a.B = num_seqs; a.T = static_cast<int>(num_tokens);
-  a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
-  a.window = window;
-  plan_paged(a, bf16, cus, max_pages, page_size, scale);
-  const int DT = paged_width(head_dim);
-  int* head = static_cast<int*>(workspace);
-  a.row_count = head;
-  a.ws = reinterpret_cast<float*>(head + kHeadInts);
-  a.chunk_list = reinterpret_cast<int4*>(a.ws + row_partial_floats(kv_heads, head_dim, cus));
-  a.chunk_ws = reinterpret_cast<float*>(a.chunk_list) + chunk_list_floats(kv_heads, cus);
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t n = row_grid(a);
-  if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
-    GS_CHECK_ARG(ragged_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
-    launch_ragged(a, DT, st);
-    GS_CHECK_LAUNCH(who);
-    return GS_OK;
-  }
-  // max_q says that no sequence is the chunk form's: workgroups for such a batch, which take
-  // whatever parts the lengths turn out to make
-  a.row_limit = INT32_MAX;
-  a.row_parts = row_most_parts(a);
-  GS_CHECK_ARG(n * a.HK < (int64_t(1) << 31) && a.row_parts < (int64_t(1) << 31), "%s: too many tiles", who);
-  switch (DT) {
-    case 64: bf16 ? launch_paged<true, 64>(a, n, st) : launch_paged<false, 64>(a, n, st); break;
-    case 128: bf16 ? launch_paged<true, 128>(a, n, st) : launch_paged<false, 128>(a, n, st); break;
-    default: bf16 ? launch_paged<true, 256>(a, n, st) : launch_paged<false, 256>(a, n, st); break;
-  }
-  GS_CHECK_LAUNCH(who);
-  return GS_OK;
+  return paged_attention("gs_paged_attention", false, Scales{}, dtype, q, q_ts, q_hs, k_cache, k_ps, k_hs, k_rs,
+                         v_cache, v_ps, v_hs, v_rs, num_pages, page_size, page_table, ld_table, max_pages, kv_lens,
+                         cu_seqlens, num_seqs, num_tokens, max_q, heads, kv_heads, head_dim, scale, window, out, o_ts,
+                         o_hs, lse, workspace, workspace_bytes, stream);
+}
+
+int gs_paged_attention_e4m3(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs, const void* k_cache, int64_t k_ps,
+                            int64_t k_hs, int64_t k_rs, const void* v_cache, int64_t v_ps, int64_t v_hs, int64_t v_rs,
+                            const uint8_t* k_scales, int64_t ks_ps, int64_t ks_hs, const uint8_t* v_scales, int64_t vs_ps,
+                            int64_t vs_hs,
+                            int64_t num_pages, int32_t page_size, const int32_t* page_table, int64_t ld_table,
+                            int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                            int64_t num_tokens, int32_t max_q, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                            float scale, int32_t window, void* out, int64_t o_ts, int64_t o_hs, float* lse,
+                            void* workspace, int64_t workspace_bytes, void* stream) {
+  return paged_attention("gs_paged_attention_e4m3", true, Scales{k_scales, ks_ps, ks_hs, v_scales, vs_ps, vs_hs},
+                         dtype, q, q_ts, q_hs, k_cache, k_ps, k_hs, k_rs, v_cache, v_ps, v_hs, v_rs, num_pages,
+                         page_size, page_table, ld_table, max_pages, kv_lens, cu_seqlens, num_seqs, num_tokens, max_q,
+                         heads, kv_heads, head_dim, scale, window, out, o_ts, o_hs, lse, workspace, workspace_bytes,
+                         stream);
 }
 
 int gs_capture_id(void* stream, int64_t* id) {
@@ -479,36 +544,22 @@ int64_t gs_check_paged_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int6
                                  int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t window,
                                  int64_t o_ts, int64_t o_hs, int32_t cus, char* msg, int64_t msg_len,
                                  int64_t* checked) {
-  const char* who = "gs_check_paged_addresses";
-  const bool bf16 = dtype == GS_DTYPE_BF16;
-  GS_CHECK_ARG((bf16 || dtype == GS_DTYPE_FP32) && num_tokens > 0 && num_seqs >= 0 && num_tokens < (int64_t(1) << 31) &&
-                   heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim <= 256 &&
-                   head_dim % (bf16 ? 8 : 4) == 0 && page_size > 0 && page_size % 8 == 0 && num_pages > 0 &&
-                   max_pages >= 0 && ld_table >= max_pages && (num_seqs == 0 || kv_lens != nullptr) && window >= 0 && cus > 0 &&
-                   (cu_seqlens != nullptr || num_tokens == num_seqs), "%s: sizes", who);
-  PagedArgs a{};
-  a.q_ts = q_ts; a.q_hs = q_hs; a.o_ts = o_ts; a.o_hs = o_hs;
-  a.k_ps = k_ps; a.k_hs = k_hs; a.k_rs = k_rs;
-  a.v_ps = v_ps; a.v_hs = v_hs; a.v_rs = v_rs;
-  a.table = page_table; a.ld_table = ld_table; a.lens = kv_lens; a.cu = cu_seqlens;
-  a.num_pages = static_cast<int>(num_pages);
-  a.B = num_seqs; a.T = static_cast<int>(num_tokens);
-  a.H = heads; a.HK = kv_heads; a.G = heads / kv_heads; a.D = head_dim;
-  a.window = window;
-  plan_paged(a, bf16, cus, max_pages, page_size, 1.f);
-  PagedModel m;
-  m.window = window;
-  m.rows.assign(static_cast<size_t>(a.T) * a.H, 0);
-  if (a.row_limit != INT32_MAX) paged_width(head_dim) == 64 ? model_chunk<64>(m, a) : model_chunk<128>(m, a);
-  switch (paged_width(head_dim)) {
-    case 64: bf16 ? model_attention<true, 64>(m, a) : model_attention<false, 64>(m, a); break;
-    case 128: bf16 ? model_attention<true, 128>(m, a) : model_attention<false, 128>(m, a); break;
-    default: bf16 ? model_attention<true, 256>(m, a) : model_attention<false, 256>(m, a); break;
-  }
-  model_rows(m, a);
-  if (checked) *checked = m.checked;
-  if (msg && msg_len > 0) snprintf(msg, static_cast<size_t>(msg_len), "%s", m.msg);
-  return m.bad;
+  return check_addresses("gs_check_paged_addresses", false, 0, 0, dtype, q_ts, q_hs, k_ps, k_hs, k_rs, v_ps, v_hs,
+                         v_rs, num_pages, page_size, page_table, ld_table, max_pages, kv_lens, cu_seqlens, num_seqs,
+                         num_tokens, heads, kv_heads, head_dim, window, o_ts, o_hs, cus, msg, msg_len, checked);
+}
+
+int64_t gs_check_paged_e4m3_addresses(int32_t dtype, int64_t q_ts, int64_t q_hs, int64_t k_ps, int64_t k_hs, int64_t k_rs,
+                                      int64_t v_ps, int64_t v_hs, int64_t v_rs, int64_t s_ps, int64_t s_hs, int64_t num_pages, int32_t page_size,
+                                      const int32_t* page_table, int64_t ld_table, int32_t max_pages,
+                                      const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                                      int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t window,
+                                      int64_t o_ts, int64_t o_hs, int32_t cus, char* msg, int64_t msg_len,
+                                      int64_t* checked) {
+  return check_addresses("gs_check_paged_e4m3_addresses", true, s_ps, s_hs, dtype, q_ts, q_hs, k_ps, k_hs, k_rs, v_ps,
+                         v_hs, v_rs, num_pages, page_size, page_table, ld_table, max_pages, kv_lens, cu_seqlens,
+                         num_seqs, num_tokens, heads, kv_heads, head_dim, window, o_ts, o_hs, cus, msg, msg_len,
+                         checked);
 }
 
 }  // extern "C"

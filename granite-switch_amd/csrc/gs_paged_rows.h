@@ -14,6 +14,8 @@
 // batch's units, cut wherever they end, cost two joins a workgroup and took 114.
 #pragma once
 
+#include <type_traits>
+
 #include "gs_paged.h"
 
 namespace gs {
@@ -21,29 +23,46 @@ namespace {
 
 // What the two element types differ in.  Both use 16 x 16 products: S^T = K Q^T
 // with the keys as rows, so a lane has one query row's scores of consecutive
-// keys, which is the operand that O^T = V^T P^T takes them as.
-template <bool BF16, int DT>
+// keys, which is the operand that O^T = V^T P^T takes them as.  A quantised cache's
+// rows (E4M3) become bf16 or fp32 operands in registers: a lane's 16 bytes of a key are
+// 16 columns, so its query columns are the same ones.
+template <bool BF16, int DT, bool E4M3 = false>
 struct PagedForm;
-template <int DT>
-struct PagedForm<true, DT> {
+template <int DT, bool E4M3>
+struct PagedForm<true, DT, E4M3> {
   static constexpr int kBlock = 32;                 // keys of a wave's block
-  static constexpr int kSteps = DT / 32;            // K pieces of 16 bytes per key row and lane
+  static constexpr int kSteps = DT / 32;            // query pieces of 16 bytes per row and lane
+  static constexpr int kKP = E4M3 ? DT / 64 : kSteps;   // K pieces of 16 bytes per key row and lane
   static constexpr int kKT = 2;                     // 16-key tiles of S^T in a block
-  static constexpr int kVW = DT >= 128 ? 8 : 4;     // columns of a V vector
+  static constexpr int kVW = E4M3 && DT == 256 ? 16 : DT >= 128 ? 8 : 4;   // columns of a V vector
   static constexpr int kVN = DT / (16 * kVW);       // V vectors of a lane and key
   static constexpr int kKeys = 8;                   // keys of a lane: 8 g .. 8 g + 7
   static constexpr int kES = 2;
+  static constexpr int kCS = E4M3 ? 1 : 2;          // bytes of a cache's element
 };
-template <int DT>
-struct PagedForm<false, DT> {
+template <int DT, bool E4M3>
+struct PagedForm<false, DT, E4M3> {
   static constexpr int kBlock = 16;
   static constexpr int kSteps = DT / 16;
+  static constexpr int kKP = E4M3 ? DT / 64 : kSteps;
   static constexpr int kKT = 1;
-  static constexpr int kVW = 4;
-  static constexpr int kVN = DT / 64;
+  static constexpr int kVW = E4M3 && DT >= 128 ? 8 : 4;
+  static constexpr int kVN = DT / (16 * kVW);
   static constexpr int kKeys = 4;                   // keys 4 g .. 4 g + 3
   static constexpr int kES = 4;
+  static constexpr int kCS = E4M3 ? 1 : 4;
 };
+// First column of query piece st of lane group lg, and of its K piece kp.
+template <bool BF16, int DT, bool E4M3>
+__device__ __host__ __forceinline__ int row_q_col(int st, int lg) {
+  constexpr int kVec = BF16 ? 8 : 4;
+  constexpr int kPer = E4M3 ? 16 / kVec : 1;        // query pieces of a K piece
+  return kVec * (kPer * (4 * (st / kPer) + lg) + st % kPer);
+}
+template <bool BF16, int DT, bool E4M3>
+__device__ __host__ __forceinline__ int row_k_col(int kp, int lg) {
+  return (E4M3 ? 16 : BF16 ? 8 : 4) * (4 * kp + lg);
+}
 
 __device__ __forceinline__ f32x4 mfma16_bf16(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -67,13 +86,25 @@ template <>
 struct VVec<8> {
   typedef u32x2 T;
 };
+template <>
+struct VVec<4> {
+  typedef uint32_t T __attribute__((ext_vector_type(1)));
+};
+
+// The power of two of byte `at` of a word of scales; 0 for code 0.
+__device__ __forceinline__ float scale_of(uint32_t w, int at) { return __uint_as_float(((w >> (8 * at)) & 255u) << 23); }
 
 // One 32-key (16-key, fp32) block's keys and values in a wave's registers.
-template <bool BF16, int DT>
+struct NoScales {};
+struct BlockScales {
+  u32x2 k, v;                                       // of the 8 keys of the lane's K rows; of its V rows
+};
+template <bool BF16, int DT, bool E4M3 = false>
 struct PagedBlock {
-  using F = PagedForm<BF16, DT>;
-  u32x4 k[F::kKT][F::kSteps];
-  typename VVec<F::kVW * F::kES>::T v[F::kKeys][F::kVN];
+  using F = PagedForm<BF16, DT, E4M3>;
+  u32x4 k[F::kKT][F::kKP];
+  typename VVec<F::kVW * F::kCS>::T v[F::kKeys][F::kVN];
+  std::conditional_t<E4M3, BlockScales, NoScales> s;
 };
 
 constexpr int kPWaves = 4;
@@ -436,9 +467,9 @@ __device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSe
 }
 
 // One part of an item, for key/value head h.
-template <bool BF16, int DT>
+template <bool BF16, int DT, bool E4M3 = false>
 __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, int h, RowShared<DT>& sh) {
-  using F = PagedForm<BF16, DT>;
+  using F = PagedForm<BF16, DT, E4M3>;
   constexpr int kOC = F::kVN * F::kVW;               // O^T tiles of 16 columns
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 15, lg = l >> 4;
@@ -467,11 +498,10 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
   const int hi = live ? sq.len - sq.n + qi + 1 : 0;  // sees [lo, hi)
   const int lo = a.window > 0 ? hi - a.window : 0;
   const int64_t qe = static_cast<int64_t>(sq.q0 + qi) * a.q_ts + static_cast<int64_t>(qh) * a.q_hs;
-  constexpr int kVec = 16 / F::kES;
   u32x4 qf[F::kSteps];
 #pragma unroll
   for (int st = 0; st < F::kSteps; ++st) {
-    const int d = kVec * (4 * st + lg);
+    const int d = row_q_col<BF16, DT, E4M3>(st, lg);
     const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.q) + (qe + (d < a.D ? d : 0)) * F::kES);
     qf[st] = live && d < a.D ? x : u32x4{0, 0, 0, 0};
   }
@@ -489,8 +519,8 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
   const int v_oct = BF16 ? 8 * lg : 8 * (lg >> 1);
   const int k_in = BF16 ? (lq & 3) : (lq & 7);       // K row within them (+ 4 for tile 1)
   const int v_in = BF16 ? 0 : 4 * (lg & 1);
-  const char* k_head = static_cast<const char*>(a.k) + static_cast<int64_t>(h) * a.k_hs * F::kES;
-  const char* v_head = static_cast<const char*>(a.v) + static_cast<int64_t>(h) * a.v_hs * F::kES;
+  const char* k_head = static_cast<const char*>(a.k) + static_cast<int64_t>(h) * a.k_hs * F::kCS;
+  const char* v_head = static_cast<const char*>(a.v) + static_cast<int64_t>(h) * a.v_hs * F::kCS;
   struct Ids {
     int k, v;
     uint32_t k_row, v_row;
@@ -502,44 +532,71 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
     addr::div_by(static_cast<uint32_t>(addr::paged_octet(tb + v_oct, tile.ve)) >> 3, a.page_octets, a.page_magic, vp, vr);
     return Ids{trow[kp], trow[vp], kr * 8 + k_in, vr * 8 + v_in};
   };
-  const auto load = [&](const Ids& id, PagedBlock<BF16, DT>& x) {
-    const char* kp = k_head + (addr::paged_page(id.k, a.num_pages) * a.k_ps + id.k_row * a.k_rs) * F::kES;
-    const char* vp = v_head + (addr::paged_page(id.v, a.num_pages) * a.v_ps + id.v_row * a.v_rs) * F::kES;
+  const auto load = [&](const Ids& id, PagedBlock<BF16, DT, E4M3>& x) {
+    const int64_t k_page = addr::paged_page(id.k, a.num_pages), v_page = addr::paged_page(id.v, a.num_pages);
+    const char* kp = k_head + (k_page * a.k_ps + id.k_row * a.k_rs) * F::kCS;
+    const char* vp = v_head + (v_page * a.v_ps + id.v_row * a.v_rs) * F::kCS;
+    if constexpr (E4M3) {
+      x.s.k = *reinterpret_cast<const u32x2*>(a.ks + k_page * a.ks_ps + h * a.ks_hs + (id.k_row & ~7u));
+      x.s.v = *reinterpret_cast<const u32x2*>(a.vs + v_page * a.vs_ps + h * a.vs_hs + (id.v_row & ~7u));
+    }
 #pragma unroll
     for (int t = 0; t < F::kKT; ++t)
 #pragma unroll
-      for (int st = 0; st < F::kSteps; ++st) {
-        const int d = kVec * (4 * st + lg);
-        x.k[t][st] = *reinterpret_cast<const u32x4*>(kp + (4 * t * a.k_rs + (d < a.D ? d : 0)) * F::kES);
+      for (int p = 0; p < F::kKP; ++p) {
+        const int d = row_k_col<BF16, DT, E4M3>(p, lg);
+        x.k[t][p] = *reinterpret_cast<const u32x4*>(kp + (4 * t * a.k_rs + (d < a.D ? d : 0)) * F::kCS);
       }
 #pragma unroll
     for (int t = 0; t < F::kKeys; ++t)
 #pragma unroll
       for (int n = 0; n < F::kVN; ++n) {
         const int d = n * 16 * F::kVW + F::kVW * lq;
-        x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kES>::T*>(vp + (t * a.v_rs + (d < a.D ? d : 0)) * F::kES);
+        x.v[t][n] = *reinterpret_cast<const typename VVec<F::kVW * F::kCS>::T*>(vp + (t * a.v_rs + (d < a.D ? d : 0)) * F::kCS);
       }
   };
   const int hi_min = sq.len - sq.n + tile.i0 + 1;    // keys below it and from lo_max on: seen by every row
   const int lo_max = a.window > 0 ? sq.len - sq.n + tile.i1 + 1 - a.window : 0;
   const bool pad = DT > a.D;
 
-  const auto step = [&](int b, PagedBlock<BF16, DT>& x) {
+  const auto step = [&](int b, PagedBlock<BF16, DT, E4M3>& x) {
     const int tb = tile.first + b * F::kBlock;
     f32x4 sacc[F::kKT];
 #pragma unroll
     for (int t = 0; t < F::kKT; ++t) sacc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int st = 0; st < F::kSteps; ++st)
+    for (int p = 0; p < F::kKP; ++p)
 #pragma unroll
       for (int t = 0; t < F::kKT; ++t) {
-        u32x4 kx = x.k[t][st];
-        if (pad && kVec * (4 * st + lg) >= a.D) kx = u32x4{0, 0, 0, 0};
-        if constexpr (BF16) {
-          sacc[t] = mfma16_bf16(kx, qf[st], sacc[t]);
-        } else {
+        u32x4 kx = x.k[t][p];
+        if (pad && row_k_col<BF16, DT, E4M3>(p, lg) >= a.D) kx = u32x4{0, 0, 0, 0};
+        if constexpr (!E4M3 && BF16) {
+          sacc[t] = mfma16_bf16(kx, qf[p], sacc[t]);
+        } else if constexpr (!E4M3) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sacc[t] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[st][e]), sacc[t]);
+          for (int e = 0; e < 4; ++e) sacc[t] = mfma16_f32(__uint_as_float(kx[e]), __uint_as_float(qf[p][e]), sacc[t]);
+        } else if constexpr (BF16) {                 // y 2^e is exact in bf16
+          const float f = scale_of(x.s.k[t], k_in);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            u32x4 ky;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              ky[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kx[2 * e + w], f, false));
+              ky[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kx[2 * e + w], f, true));
+            }
+            sacc[t] = mfma16_bf16(ky, qf[2 * p + e], sacc[t]);
+          }
+        } else {
+          const float f = scale_of(k_in < 4 ? x.s.k[0] : x.s.k[1], k_in & 3);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(kx[e], f, false);
+            const f32x2_t up = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(kx[e], f, true);
+            const float ky[4] = {lo[0], lo[1], up[0], up[1]};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sacc[t] = mfma16_f32(ky[w], __uint_as_float(qf[4 * p + e][w]), sacc[t]);
+          }
         }
       }
     float sc[F::kKeys];
@@ -556,7 +613,12 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
 #pragma unroll
           for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-            for (int w = 0; w < F::kVW * F::kES / 4; ++w) x.v[i][n][w] = 0;
+            for (int w = 0; w < F::kVW * F::kCS / 4; ++w) x.v[i][n][w] = 0;
+          if constexpr (E4M3) {                      // nor is 0 * inf: its scale is zero, too
+            const int at = (BF16 ? i : v_in + i);
+            x.s.v[0] = at < 4 ? x.s.v[0] & ~(255u << (8 * (at & 3))) : x.s.v[0];
+            x.s.v[1] = at < 4 ? x.s.v[1] : x.s.v[1] & ~(255u << (8 * (at & 3)));
+          }
         }
       }
     }
@@ -581,8 +643,34 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
     for (int i = 0; i < F::kKeys; ++i) {
       p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
       lsum += p[i];
+      if constexpr (E4M3) p[i] *= scale_of(BF16 ? x.s.v[i >> 2] : v_in == 0 ? x.s.v[0] : x.s.v[1], i & 3);
     }
-    if constexpr (BF16) {
+    if constexpr (BF16 && E4M3) {
+      // The values' scales are the probabilities', which then are rounded as below: a column's
+      // bytes of two keys are brought together before they become bf16.
+      u32x4 pf;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+#pragma unroll
+      for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+        for (int w = 0; w < F::kVW / 4; ++w)
+#pragma unroll
+          for (int up = 0; up < 2; ++up) {
+            u32x4 vf[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t y = __builtin_amdgcn_perm(x.v[2 * i + 1][n][w], x.v[2 * i][n][w], up ? 0x07030602u : 0x05010400u);
+              vf[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, false));
+              vf[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, true));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = n * F::kVW + 4 * w + 2 * up + e;
+              o[c] = mfma16_bf16(vf[e], pf, o[c]);
+            }
+          }
+    } else if constexpr (BF16) {
       // Probabilities enter the product in bf16, their total stays in fp32.  Each is off by
       // up to 2^-8 of itself, as the values and the result are; with values of both signs a
       // result's error against 64 bits grows to at most sqrt(2) of what its own rounding
@@ -601,6 +689,19 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
           for (int i = 0; i < 4; ++i) vf[i] = pair16(x.v[2 * i][n][c >> 1], x.v[2 * i + 1][n][c >> 1], c & 1);
           o[n * F::kVW + c] = mfma16_bf16(vf, pf, o[n * F::kVW + c]);
         }
+    } else if constexpr (E4M3) {
+#pragma unroll
+      for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+        for (int w = 0; w < F::kVW / 4; ++w)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const f32x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.v[t][n][w], 1.f, false);
+            const f32x2_t up = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(x.v[t][n][w], 1.f, true);
+            const float y[4] = {lo[0], lo[1], up[0], up[1]};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n * F::kVW + 4 * w + e] = mfma16_f32(y[e], p[t], o[n * F::kVW + 4 * w + e]);
+          }
     } else {
 #pragma unroll
       for (int n = 0; n < F::kVN; ++n)
@@ -616,7 +717,7 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
   // 256 sequences of 16 .. 2047 keys then), and page ids one block before them.
   int b = w0 * kPWaves + wave;
   if (b < b_end) {
-    PagedBlock<BF16, DT> cur, nxt;
+    PagedBlock<BF16, DT, E4M3> cur, nxt;
     Ids id = ids_of(b);
     load(id, cur);
     id = ids_of(b + kPWaves);
@@ -681,6 +782,45 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
   }
   if (it.nparts > 1 && last_to_arrive(a.row_count + slot0, it.nparts, sh.last))
     row_join<BF16, DT>(a, sq, j, nrow, h, first, it.nparts, sh);
+}
+
+// Workgroups i of n of each key/value head take its parts i, 2 n - 1 - i, 2 n + i, ...:
+// the parts get shorter, so whoever has a longer one has a shorter one next.  One
+// start for several parts: 223 sequences of 4 .. 429 keys with 16 heads 60 us against 71
+// with a workgroup for each, 1024 of 16 .. 400 with 8 heads 164 against 229.  The first
+// wave lists up to 32 of a workgroup's parts in one pass over the batch.
+constexpr int kRowList = 32;
+template <bool BF16, int DT, bool E4M3 = false>
+__global__ __launch_bounds__(256, DT == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs) {
+  __shared__ RowShared<DT> sh;
+  __shared__ RowOrder<BF16, DT> kept[64];            // a lane's, between lists
+  __shared__ RowEntry list[kRowList];
+  __shared__ int parts;
+  const int HK = fresh_args().HK;
+  const int i = blockIdx.x / HK, h = blockIdx.x - i * HK, n = gridDim.x / HK;
+  for (int k0 = 0;; k0 += kRowList) {
+    if (threadIdx.x < 64) {
+      const PagedArgs& a = fresh_args();
+      RowOrder<BF16, DT> order;
+      if (k0 == 0) {
+        order.plan(a);
+        kept[threadIdx.x] = order;
+        if (threadIdx.x == 0) parts = order.total;
+      } else {
+        order = kept[threadIdx.x];
+      }
+      order.list_parts(a, i, n, k0, k0 + kRowList, list);
+    }
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(parts);
+    for (int k = k0; k < k0 + kRowList && k * n < total; ++k) {
+      if (k * n + ((k & 1) != 0 ? n - 1 - i : i) >= total) continue;
+      row_part<BF16, DT, E4M3>(fresh_args(), row_item(list[k - k0]), h, sh);
+      __syncthreads();                               // every wave is past what the part left in sh, and its entry
+    }
+    if ((k0 + kRowList) * n >= total) break;
+  }
+  zero_outside<BF16>(fresh_args());
 }
 
 }  // namespace

@@ -5,7 +5,7 @@ invocation tokens of an adapter that switches on mid-sequence, in one batch):
 
     y, r = residual_norm(x, r, input_norm, scale=m)      the block before, the residual stream, the norm
     q, k, v = qkv(y)                                     switched projection, slices of its output
-    q = append_kv_(q, k, v, cache, slots, positions)     rotated; keys and values stored
+    q = append_kv_(q, k, v, cache, slots, positions)     normed, rotated; keys and values stored
     o = paged_attention(q, cache, page_table, kv_lens)   this step's tokens included
     y, r = residual_norm(o_proj(o), r, mlp_norm, scale=m)
     x = down(swiglu(gate_up(y)))                         switched projections
@@ -48,12 +48,15 @@ class SwitchedDecoderLayer(nn.Module):
 
     ``qkv`` has three slices (heads * head_dim, kv_heads * head_dim twice),
     ``gate_up`` two with ``fuse_swiglu``; ``window`` > 0 is a sliding window.
+    ``q_norm`` and ``k_norm`` [head_dim] norm each head before its rotation.  The
+    cache is a pair of tensors or of ``paged.QuantizedCache``.
     """
 
     def __init__(self, qkv: SwitchedLoRALinear, o_proj: SwitchedLoRALinear, gate_up: SwitchedLoRALinear,
                  down: SwitchedLoRALinear, input_norm: torch.Tensor, mlp_norm: torch.Tensor, heads: int, kv_heads: int,
                  head_dim: int, eps: float = 1e-5, residual_multiplier: float = 1.0,
-                 attention_multiplier: float | None = None, window: int = 0):
+                 attention_multiplier: float | None = None, window: int = 0, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None):
         super().__init__()
         widths = (heads * head_dim, kv_heads * head_dim, kv_heads * head_dim)
         if qkv.output_slices != widths:
@@ -64,6 +67,10 @@ class SwitchedDecoderLayer(nn.Module):
         self.qkv, self.o_proj, self.gate_up, self.down = qkv, o_proj, gate_up, down
         self.register_buffer("input_norm", input_norm.detach())
         self.register_buffer("mlp_norm", mlp_norm.detach())
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None and tuple(w.shape) != (head_dim,):
+                raise ValueError(f"SwitchedDecoderLayer: {name} is {tuple(w.shape)}, heads of {head_dim}")
+            self.register_buffer(name, None if w is None else w.detach())
         self.heads, self.kv_heads, self.head_dim, self.eps = heads, kv_heads, head_dim, eps
         self.residual_multiplier, self.attention_multiplier, self.window = residual_multiplier, attention_multiplier, window
 
@@ -71,14 +78,15 @@ class SwitchedDecoderLayer(nn.Module):
         return [self.qkv, self.o_proj, self.gate_up, self.down]
 
     def forward(self, x: torch.Tensor | None, residual: torch.Tensor, step: PagedStep,
-                cache: tuple[torch.Tensor, torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+                cache: tuple) -> tuple[torch.Tensor, torch.Tensor]:
         """``(x, residual)`` [T, hidden]: the block before and the stream (x None: the first layer), and after."""
         T, D = residual.shape[0], self.head_dim
         y, residual = norms.residual_norm(x, residual, self.input_norm, self.eps, self.residual_multiplier)
         qkv = self.qkv(y)[0]
         nq, nk = self.heads * D, self.kv_heads * D
         q, k, v = (qkv[:, a:b].unflatten(1, (-1, D)) for a, b in ((0, nq), (nq, nq + nk), (nq + nk, nq + 2 * nk)))
-        q = paged.append_kv_(q, k, v, *cache, step.slots, step.positions, step.cos_sin)
+        q = paged.append_kv_(q, k, v, *cache, step.slots, step.positions, step.cos_sin, q_norm=self.q_norm,
+                             k_norm=self.k_norm, eps=self.eps)
         o = paged.paged_attention(q, *cache, step.page_table, step.kv_lens, step.cu_seqlens, self.attention_multiplier,
                                   self.window, max_q=step.max_q)
         y, residual = norms.residual_norm(self.o_proj(o.view(T, nq))[0], residual, self.mlp_norm, self.eps,

@@ -9,7 +9,7 @@ fake implementations, so callers such as ``SwitchedLoRALinear._run_expand``
 (src/granite_switch/vllm/core/lora.py:659-686) and ``WCrossShunt.forward``
 (src/granite_switch/vllm/decoder/shadow_residual/wcross_shunt.py:198-242) run
 unchanged on MI355X, plus three new ops for the y-given switched-LoRA path and
-four for the paged cache and the norms around the residual add.
+seven for the paged cache and the norms around the residual add.
 
 Only one provider of the ``granite_switch`` ops can be loaded in a process.
 """
@@ -183,6 +183,57 @@ if not _registered("append_kv"):
 
     @append_kv.register_fake
     def _(q, k, v, k_cache, v_cache, slots, positions, cos_sin, interleaved):
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def _cache(values: torch.Tensor, scales: torch.Tensor | None):
+    return values if scales is None else paged.QuantizedCache(values, scales)
+
+
+if not _registered("append_kv_normed"):
+
+    @torch.library.custom_op(f"{_NS}::append_kv_normed", mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
+    def append_kv_normed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, slots: torch.Tensor,
+                         positions: torch.Tensor | None, cos_sin: torch.Tensor | None, interleaved: bool,
+                         q_norm: torch.Tensor | None, k_norm: torch.Tensor | None, eps: float) -> torch.Tensor:
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return paged.append_kv_(q, k, v, _cache(k_cache, k_scales), _cache(v_cache, v_scales), slots, positions, cos_sin,
+                                    interleaved=interleaved, q_norm=q_norm, k_norm=k_norm, eps=eps)
+
+    @append_kv_normed.register_fake
+    def _(q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, cos_sin, interleaved, q_norm, k_norm, eps):
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+if not _registered("read_kv"):
+
+    @torch.library.custom_op(f"{_NS}::read_kv", mutates_args=())
+    def read_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor | None, v_scales: torch.Tensor | None,
+                slots: torch.Tensor, dtype: torch.dtype | None) -> tuple[torch.Tensor, torch.Tensor]:
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return paged.read_kv(_cache(k_cache, k_scales), _cache(v_cache, v_scales), slots, dtype)
+
+    @read_kv.register_fake
+    def _(k_cache, v_cache, k_scales, v_scales, slots, dtype):
+        dtype = dtype or (k_cache.dtype if k_scales is None else torch.bfloat16)
+        shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
+        return torch.empty(shape, dtype=dtype, device=slots.device), torch.empty(shape, dtype=dtype, device=slots.device)
+
+
+if not _registered("paged_attention_e4m3"):
+
+    @torch.library.custom_op(f"{_NS}::paged_attention_e4m3", mutates_args=())
+    def paged_attention_e4m3(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                             v_scales: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                             cu_seqlens: torch.Tensor | None, scale: float | None, window: int,
+                             max_q: int | None) -> torch.Tensor:
+        with torch.no_grad():          # autograd is the op's: a backward through it raises
+            return paged.paged_attention(q, _cache(k_cache, k_scales), _cache(v_cache, v_scales), page_table, kv_lens,
+                                         cu_seqlens, scale, window, max_q=max_q)
+
+    @paged_attention_e4m3.register_fake
+    def _(q, k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, cu_seqlens, scale, window, max_q):
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 

@@ -15,6 +15,10 @@ among them.  An aLoRA adapter that switches on mid-sequence attends over the
 base model's cached prefix this way: its few invocation tokens are a chunk of
 queries (``cu_seqlens``) over a long cache.
 
+A cache may be quantised (``allocate_quantized_cache``, ``QuantizedCache``): e4m3
+values and a power of two for each row, half the bytes of bfloat16.  The calls are
+the same; ``read_kv`` gives rows back.
+
 Everything is launched on torch's current stream without host synchronisation;
 bfloat16 or float32.  No gradients are computed: inputs that autograd tracks are
 refused where gradients are enabled.
@@ -23,6 +27,7 @@ refused where gradients are enabled.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -42,6 +47,31 @@ def allocate_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int,
     """
     shape = (num_pages, kv_heads, page_size, head_dim)
     return torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+
+
+class QuantizedCache(NamedTuple):
+    """A key or a value cache of 8-bit rows: a row of ``values`` times its power of two in ``scales``.
+
+    values [num_pages, kv_heads, page_size, head_dim] float8_e4m3fn
+    scales [num_pages, kv_heads, page_size] float8_e8m0fnu, a head's scales of a page side by side
+
+    ``append_kv_`` takes the smallest power of two (2^-126 at least) that keeps a row's
+    largest magnitude within 448, the largest e4m3 value, and rounds to nearest, ties to
+    even: a value is off by at most 2^-4 of itself, or 2^-10 of its scale where that is
+    more.  What is not finite becomes NaN, and the row's other values are kept.
+    """
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+
+def allocate_quantized_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int,
+                             device="cuda") -> tuple[QuantizedCache, QuantizedCache]:
+    """A key and a value cache of e4m3 rows, laid out as ``allocate_cache`` has them; not initialised."""
+    one = lambda: QuantizedCache(  # noqa: E731
+        torch.empty((num_pages, kv_heads, page_size, head_dim), dtype=torch.float8_e4m3fn, device=device),
+        torch.empty((num_pages, kv_heads, page_size), dtype=torch.float8_e8m0fnu, device=device))
+    return one(), one()
 
 
 def rope_table(max_pos: int, rot_dim: int, theta: float = 10000.0, device="cuda",
@@ -86,6 +116,24 @@ def _caches(who: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_he
         raise ValueError(f"{who}: pages of {k_cache.shape[2]} rows, {k_cache.shape[0]} of them (1 .. 2^31 - 1 rows)")
 
 
+def _scales(who: str, k_scales: torch.Tensor, v_scales: torch.Tensor, values: torch.Tensor):
+    for name, t in (("k_cache", k_scales), ("v_cache", v_scales)):
+        if t.dtype != torch.float8_e8m0fnu or t.shape != values.shape[:3]:
+            raise ValueError(f"{who}: {name}'s scales must be a float8_e8m0fnu tensor {tuple(values.shape[:3])}, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+        if t.stride(2) != 1 and t.shape[2] > 1:
+            raise ValueError(f"{who}: {name}'s scales of a page must lie side by side (strides {t.stride()})")
+
+
+def _parts(who: str, k_cache, v_cache):
+    """``(k values, v values, k scales, v scales)``; no scales for a cache that is not quantised."""
+    if isinstance(k_cache, QuantizedCache) != isinstance(v_cache, QuantizedCache):
+        raise ValueError(f"{who}: one cache is quantised, the other is not")
+    if isinstance(k_cache, QuantizedCache):
+        return k_cache.values, v_cache.values, k_cache.scales, v_cache.scales
+    return k_cache, v_cache, None, None
+
+
 def _on_gpu(who: str, device: torch.device, *ts) -> None:
     if device.type != "cuda":
         raise ValueError(f"{who}: tensors must live on the GPU")
@@ -117,8 +165,19 @@ def _table_ld(page_table: torch.Tensor) -> int:
 # tensors (never by their addresses): a serving loop's calls repeat a few, and the
 # checks take longer than a small call's kernel (9 of 15 us).
 _append_plans: dict = {}
+_rows_plans: dict = {}
+_read_plans: dict = {}
 _attention_plans: dict = {}
 _PLAN_CAP = 4096
+
+
+def _layout(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _elsewhere(dev: torch.device) -> bool:
+    """Whether ``dev`` is a GPU that is not the current one: a launch goes to the current one's queues."""
+    return dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device()
 
 
 def _keep(plans: dict, key, plan):
@@ -164,13 +223,15 @@ def cache_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int,
     return slots, positions
 
 
-def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache, v_cache,
                slots: torch.Tensor, positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
-               q_out: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+               q_out: torch.Tensor | None = None, interleaved: bool = False, q_norm: torch.Tensor | None = None,
+               k_norm: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor | None:
     """Rotate q and k by their positions, store k and v into the cache; returns the rotated q.
 
     q [T, heads, D], k and v [T, kv_heads, D]: views with contiguous head rows,
     such as slices of the QKV projection's output
+    k_cache, v_cache: tensors of their type, or both ``QuantizedCache``
     slots     [T] int64: page * page_size + row; one outside the pool (-1) stores
               nothing (padding rows).  No two tokens may share a slot.
     positions [T] int64 and cos_sin [max_pos, R] fp32 (``rope_table``): the first R
@@ -178,7 +239,14 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
               with ``interleaved``, the others copied.  cos_sin None: no rotation.
     q_out     receives q (allocated when None; q itself: in place).  q None: only
               k and v are handled, and None is returned.
+    q_norm, k_norm [D], of q's type or float32: each head of q (k) is normed before its
+              rotation, x / sqrt(mean(x^2) + eps) * weight, in the same pass
     """
+    if _elsewhere(k.device):
+        with torch.cuda.device(k.device):
+            return append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm, eps)
+    if q_norm is not None or k_norm is not None or isinstance(k_cache, QuantizedCache) or isinstance(v_cache, QuantizedCache):
+        return _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm, eps)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
                                     or (q is not None and q.requires_grad)
                                     or (cos_sin is not None and cos_sin.requires_grad)):
@@ -205,7 +273,54 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
     return q_out
 
 
-def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out) -> tuple:
+def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm,
+                 eps) -> torch.Tensor | None:
+    """``append_kv_`` with norms of the heads, or into a quantised cache."""
+    k_cache, v_cache, k_scales, v_scales = _parts("append_kv_", k_cache, v_cache)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k, v, k_cache, v_cache, cos_sin, q_norm, k_norm)):
+        raise _lib.no_gradients("append_kv_")
+    key = tuple(map(_layout, (q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, cos_sin, q_out, q_norm, k_norm)))
+    plan = _rows_plans.get(key)
+    if plan is None:
+        plan = _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales, v_scales)
+        plan = _keep(_rows_plans, key, plan + _norms_plan(q, k, q_norm, k_norm)
+                     + ((_lib.GS_DTYPE_E4M3, k_scales.stride()[:2], v_scales.stride()[:2]) if k_scales is not None
+                        else (plan[0], (0, 0), (0, 0))))
+    (code, T, H, HK, D, R, q_st, k_st, v_st, kc_st, vc_st, o_st, max_pos, pages, page, norm_code, cache_code, ks_st,
+     vs_st) = plan
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=k.device)
+    if T == 0:
+        return q_out
+    ptr = _lib.ptr
+    _lib.call("gs_append_kv_normed", code, ptr(q), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, T, H, HK, D,
+              ptr(q_norm), ptr(k_norm), norm_code, eps, positions.data_ptr() if R else None, cos_sin.data_ptr() if R else None,
+              max_pos, R, 1 if interleaved else 0, slots.data_ptr(), cache_code, k_cache.data_ptr(), *kc_st,
+              v_cache.data_ptr(), *vc_st, ptr(k_scales), *ks_st, ptr(v_scales), *vs_st, pages, page,
+              None if q is None else q_out.data_ptr(), *o_st, _lib.stream_ptr(k.device))
+    return q_out
+
+
+def _norms_plan(q, k, q_norm, k_norm) -> tuple:
+    who, dtype = "append_kv_", k.dtype
+    _on_gpu(who, k.device, q_norm, k_norm)
+    if q_norm is not None and q is None:
+        raise ValueError(f"{who}: q_norm without q")
+    found = None
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is None:
+            continue
+        if tuple(w.shape) != (k.shape[2],) or not w.is_contiguous() or w.dtype not in (dtype, torch.float32):
+            raise ValueError(f"{who}: {name} must be a contiguous tensor [{k.shape[2]}] of {dtype} or float32, got {w.dtype} "
+                             f"{tuple(w.shape)}")
+        if found is not None and w.dtype != found:
+            raise ValueError(f"{who}: q_norm is {found}, k_norm {w.dtype}")
+        found = w.dtype
+    return (_DTYPES[found or dtype],)
+
+
+def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales=None, v_scales=None) -> tuple:
     """The checks of an ``append_kv_`` call, and its arguments that are not addresses."""
     who = "append_kv_"
     dtype = k.dtype
@@ -214,12 +329,14 @@ def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out) ->
     if k.dim() != 3:
         raise ValueError(f"{who}: k must be [tokens, kv_heads, head_dim], got {tuple(k.shape)}")
     T, HK, D = k.shape
-    _on_gpu(who, k.device, q, v, k_cache, v_cache, slots, positions, cos_sin, q_out)
+    _on_gpu(who, k.device, q, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales, v_scales)
     _heads3(who, "k", k, T, dtype)
     _heads3(who, "v", v, T, dtype)
     if v.shape != k.shape:
         raise ValueError(f"{who}: v is {tuple(v.shape)}, k {tuple(k.shape)}")
-    _caches(who, k_cache, v_cache, dtype, HK, D)
+    _caches(who, k_cache, v_cache, dtype if k_scales is None else torch.float8_e4m3fn, HK, D)
+    if k_scales is not None:
+        _scales(who, k_scales, v_scales, k_cache)
     _ints(who, "slots", slots, torch.int64, (T,))
     R = 0
     if cos_sin is not None:
@@ -248,6 +365,72 @@ def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out) ->
     return (_DTYPES[dtype], T, H, HK, D, R, (0, 0) if q is None else q.stride()[:2], k.stride()[:2], v.stride()[:2],
             k_cache.stride()[:3], v_cache.stride()[:3], o_st, cos_sin.shape[0] if R else 0, k_cache.shape[0],
             k_cache.shape[2])
+
+
+# ---------------------------------------------------------------------------
+# Read
+# ---------------------------------------------------------------------------
+def read_kv(k_cache, v_cache, slots: torch.Tensor, dtype: torch.dtype | None = None, k_out: torch.Tensor | None = None,
+            v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of the cache by their slots: ``(k, v)`` [T, kv_heads, D], as ``append_kv_`` takes them.
+
+    k_cache, v_cache: tensors, or both ``QuantizedCache``
+    slots  [T] int64 (``cache_slots`` with a sequence's whole length gives all its rows);
+           one outside the pool gives zeros, and one may come more than once
+    dtype  of the result: bfloat16 (the default) or float32 for a quantised cache, whose
+           values are exact in both from 2^-126 on; the cache's own otherwise
+    k_out, v_out receive the result (allocated when None): views with contiguous head rows
+    """
+    who = "read_kv"
+    if _elsewhere(slots.device):
+        with torch.cuda.device(slots.device):
+            return read_kv(k_cache, v_cache, slots, dtype, k_out, v_out)
+    k_cache, v_cache, k_scales, v_scales = _parts(who, k_cache, v_cache)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (k_cache, v_cache, k_out, v_out)):
+        raise _lib.no_gradients(who)
+    key = (dtype, *map(_layout, (k_cache, v_cache, k_scales, v_scales, slots, k_out, v_out)))
+    plan = _read_plans.get(key)
+    if plan is None:
+        plan = _keep(_read_plans, key, _read_plan(k_cache, v_cache, k_scales, v_scales, slots, dtype, k_out, v_out))
+    dtype, code, cache_code, kc_st, vc_st, ks_st, vs_st, pages, page, HK, D, T, ko_st, vo_st = plan
+    if k_out is None:
+        k_out = torch.empty((T, HK, D), dtype=dtype, device=slots.device)
+    if v_out is None:
+        v_out = torch.empty((T, HK, D), dtype=dtype, device=slots.device)
+    if T:
+        _lib.call("gs_read_kv", code, cache_code, k_cache.data_ptr(), *kc_st, v_cache.data_ptr(), *vc_st, _lib.ptr(k_scales),
+                  *ks_st, _lib.ptr(v_scales), *vs_st, pages, page, HK, D, slots.data_ptr(), T, k_out.data_ptr(), *ko_st,
+                  v_out.data_ptr(), *vo_st, _lib.stream_ptr(slots.device))
+    return k_out, v_out
+
+
+def _read_plan(k_cache, v_cache, k_scales, v_scales, slots, dtype, k_out, v_out) -> tuple:
+    """The checks of a ``read_kv`` call, and its arguments that are not addresses."""
+    who = "read_kv"
+    quant = k_scales is not None
+    if dtype is None:
+        dtype = torch.bfloat16 if quant else k_cache.dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"{who}: unsupported dtype {dtype}; expected bfloat16 or float32")
+    if k_cache.dim() != 4 or slots.dim() != 1:
+        raise ValueError(f"{who}: a cache is [pages, kv_heads, page_size, head_dim] and slots [tokens], got "
+                         f"{tuple(k_cache.shape)} and {tuple(slots.shape)}")
+    _on_gpu(who, slots.device, k_cache, v_cache, k_scales, v_scales, k_out, v_out)
+    pages, HK, page, D = k_cache.shape
+    T = slots.shape[0]
+    _caches(who, k_cache, v_cache, torch.float8_e4m3fn if quant else dtype, HK, D)
+    if quant:
+        _scales(who, k_scales, v_scales, k_cache)
+    _ints(who, "slots", slots, torch.int64, (T,))
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is not None:
+            _heads3(who, name, t, T, dtype)
+            if tuple(t.shape) != (T, HK, D):
+                raise ValueError(f"{who}: {name} is {tuple(t.shape)}, expected {(T, HK, D)}")
+    return (dtype, _DTYPES[dtype], _lib.GS_DTYPE_E4M3 if quant else _DTYPES[dtype], k_cache.stride()[:3],
+            v_cache.stride()[:3], k_scales.stride()[:2] if quant else (0, 0), v_scales.stride()[:2] if quant else (0, 0),
+            pages, page, HK, D, T, (HK * D, D) if k_out is None else k_out.stride()[:2],
+            (HK * D, D) if v_out is None else v_out.stride()[:2])
 
 
 # ---------------------------------------------------------------------------
@@ -298,13 +481,14 @@ def workspace_bytes(dtype: torch.dtype, heads: int, kv_heads: int, head_dim: int
     return n
 
 
-def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+def paged_attention(q: torch.Tensor, k_cache, v_cache, page_table: torch.Tensor,
                     kv_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None, scale: float | None = None,
                     window: int = 0, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
                     max_q: int | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the batch's query rows over the paged cache; returns ``out`` [T, heads, D].
 
     q          [T, heads, D]; heads a multiple of the cache's kv_heads
+    k_cache, v_cache: tensors of q's type, or both ``QuantizedCache`` (D a multiple of 16)
     page_table [B, max_pages] int32, kv_lens [B] int32: the sequences' pages and
                lengths, the call's own tokens (already appended) counted
     cu_seqlens [B + 1] int32: sequence s has query rows cu_seqlens[s] ..
@@ -323,21 +507,28 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Keys and values that no row of the call sees may hold anything; a value that is
     not finite may also reach rows of its sequence that come before it.
     """
+    dev = q.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, out, lse, max_q,
+                                   workspace)
+    k_cache, v_cache, k_scales, v_scales = _parts("paged_attention", k_cache, v_cache)
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise _lib.no_gradients("paged_attention")
-    dev = q.device
     key = (q.shape, q.stride(), q.dtype, dev, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, page_table.shape, page_table.stride(),
            page_table.dtype, page_table.device, kv_lens.shape, kv_lens.stride(), kv_lens.dtype, kv_lens.device,
            None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device),
            window, max_q, None if out is None else (out.shape, out.stride(), out.dtype, out.device),
            None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
-           None if workspace is None else (workspace.shape, workspace.stride(), workspace.dtype, workspace.device))
+           None if workspace is None else (workspace.shape, workspace.stride(), workspace.dtype, workspace.device),
+           None if k_scales is None else (k_scales.shape, k_scales.stride(), k_scales.dtype, k_scales.device, v_scales.shape,
+                                          v_scales.stride(), v_scales.dtype, v_scales.device))
     plan = _attention_plans.get(key)
     if plan is None:
         plan = _keep(_attention_plans, key, _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window,
-                                                            out, lse, max_q, workspace))
-    code, T, B, H, HK, D, q_st, k_st, v_st, pages, page, table, o_st, window, most, need, default_scale = plan
+                                                            out, lse, max_q, workspace, k_scales, v_scales))
+    code, T, B, H, HK, D, q_st, k_st, v_st, s_st, pages, page, table, o_st, window, most, need, default_scale = plan
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     if T == 0:
@@ -345,14 +536,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     stream = _lib.stream_ptr(dev)
     if workspace is None:
         workspace = _workspace(dev, stream, need)
-    _lib.call("gs_paged_attention", code, q.data_ptr(), *q_st, k_cache.data_ptr(), *k_st, v_cache.data_ptr(), *v_st, pages,
-              page, page_table.data_ptr(), *table, kv_lens.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-              B, T, most, H, HK, D, default_scale if scale is None else scale, window, out.data_ptr(), *o_st,
+    scales = () if k_scales is None else (k_scales.data_ptr(), *s_st[:2], v_scales.data_ptr(), *s_st[2:])
+    _lib.call("gs_paged_attention_e4m3" if scales else "gs_paged_attention", code, q.data_ptr(), *q_st, k_cache.data_ptr(),
+              *k_st, v_cache.data_ptr(), *v_st, *scales, pages, page, page_table.data_ptr(), *table, kv_lens.data_ptr(),
+              None if cu_seqlens is None else cu_seqlens.data_ptr(), B, T, most, H, HK, D,
+              default_scale if scale is None else scale, window, out.data_ptr(), *o_st,
               None if lse is None else lse.data_ptr(), workspace.data_ptr(), workspace.numel(), stream)
     return out
 
 
-def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window, out, lse, max_q, workspace) -> tuple:
+def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window, out, lse, max_q, workspace, k_scales,
+                    v_scales) -> tuple:
     """The checks of a ``paged_attention`` call, and its arguments that are not addresses."""
     who = "paged_attention"
     dtype = q.dtype
@@ -361,8 +555,10 @@ def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window
     _heads3(who, "q", q, None, dtype)
     T, H, D = q.shape
     dev = q.device
-    _on_gpu(who, dev, k_cache, v_cache, page_table, kv_lens, cu_seqlens, out, lse, workspace)
-    _caches(who, k_cache, v_cache, dtype, None, D)
+    _on_gpu(who, dev, k_cache, v_cache, page_table, kv_lens, cu_seqlens, out, lse, workspace, k_scales, v_scales)
+    _caches(who, k_cache, v_cache, dtype if k_scales is None else torch.float8_e4m3fn, None, D)
+    if k_scales is not None:
+        _scales(who, k_scales, v_scales, k_cache)
     HK = k_cache.shape[1]
     B = kv_lens.shape[0]
     if HK == 0 or H % HK or H == 0:
@@ -385,11 +581,13 @@ def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window
         raise ValueError(f"{who}: workspace must be a contiguous uint8 tensor")
     with torch.cuda.device(dev):
         need = workspace_bytes(dtype, H, HK, D, cu_seqlens is not None) if T else 0
-    return (_DTYPES[dtype], T, B, H, HK, D, q.stride()[:2], k_cache.stride()[:3], v_cache.stride()[:3], k_cache.shape[0],
-            k_cache.shape[2], (_table_ld(page_table), page_table.shape[1]),
+    return (_DTYPES[dtype], T, B, H, HK, D, q.stride()[:2], k_cache.stride()[:3], v_cache.stride()[:3],
+            None if k_scales is None else k_scales.stride()[:2] + v_scales.stride()[:2], k_cache.shape[0], k_cache.shape[2],
+            (_table_ld(page_table), page_table.shape[1]),
             (H * D, D) if out is None else out.stride()[:2], min(window, _INT32),      # no sequence is longer
             1 if cu_seqlens is None else min(int(max_q or 0), _INT32), need,
             1.0 / math.sqrt(D))
 
 
-__all__ = ["allocate_cache", "append_kv_", "cache_slots", "paged_attention", "rope_table", "workspace_bytes"]
+__all__ = ["QuantizedCache", "allocate_cache", "allocate_quantized_cache", "append_kv_", "cache_slots", "paged_attention",
+           "read_kv", "rope_table", "workspace_bytes"]

@@ -63,6 +63,7 @@ extern "C" {
 
 #define GS_DTYPE_BF16 0
 #define GS_DTYPE_FP32 1
+#define GS_DTYPE_E4M3 2      /* a quantised cache's elements (cache_dtype arguments) */
 
 #define GS_MAX_ADAPTERS 256  /* global adapter ids handled by the segment builder */
 #define GS_MAX_SLICES 8      /* output slices per projection (QKV = 3, gate_up = 2) */
@@ -549,6 +550,43 @@ int gs_append_kv(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q
                  int64_t vc_head_stride, int64_t vc_row_stride, int64_t num_pages, int32_t page_size, void* q_out,
                  int64_t qo_token_stride, int64_t qo_head_stride, void* stream);
 
+/* A quantised cache (cache_dtype GS_DTYPE_E4M3) keeps a row -- a head's key or
+ * value of one token -- as e4m3 values y, one byte each (sign, 4 bits of
+ * exponent, 3 of mantissa, no infinities), and a scale 2^e, x = y 2^e, whose
+ * byte is e + 127.  Storing takes the least e >= -126 with |x| <= 448 2^e for
+ * the row's finite x, and rounds x 2^-e to nearest, ties to even; what is not
+ * finite becomes NaN.  The scales are [num_pages, kv_heads, page_size] bytes
+ * with page and head strides, a head's scales of a page side by side.
+ *
+ * gs_append_kv_normed: gs_append_kv with the norms of queries and keys for each
+ * head before the rotation, x rsqrt(mean(x^2) + eps) w over the head's columns
+ * (q_norm, k_norm [head_dim] of norm_dtype -- dtype or fp32 -- or NULL: none),
+ * and with a cache of dtype or quantised (scales: NULL unless it is).  In fp32
+ * throughout, rounded once.  The rest as gs_append_kv. */
+int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                        const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                        const int64_t* positions, const float* cos_sin, int64_t max_pos, int32_t rot_dim,
+                        int32_t interleaved, const int64_t* slots, int32_t cache_dtype, void* k_cache,
+                        int64_t kc_page_stride, int64_t kc_head_stride, int64_t kc_row_stride, void* v_cache,
+                        int64_t vc_page_stride, int64_t vc_head_stride, int64_t vc_row_stride, uint8_t* k_scales,
+                        int64_t ks_page_stride, int64_t ks_head_stride, uint8_t* v_scales, int64_t vs_page_stride,
+                        int64_t vs_head_stride, int64_t num_pages, int32_t page_size, void* q_out,
+                        int64_t qo_token_stride, int64_t qo_head_stride, void* stream);
+
+/* Rows of a cache by their slots: k_out and v_out [num_tokens, kv_heads,
+ * head_dim] of dtype, with token and head strides; a slot outside the pool
+ * gives zeros.  A quantised row's x = y 2^e is exact in either dtype from 2^-126
+ * on, a cache that is not quantised has dtype.  A slot may come more than once. */
+int gs_read_kv(int32_t dtype, int32_t cache_dtype, const void* k_cache, int64_t kc_page_stride, int64_t kc_head_stride,
+               int64_t kc_row_stride, const void* v_cache, int64_t vc_page_stride, int64_t vc_head_stride,
+               int64_t vc_row_stride, const uint8_t* k_scales, int64_t ks_page_stride, int64_t ks_head_stride,
+               const uint8_t* v_scales, int64_t vs_page_stride, int64_t vs_head_stride, int64_t num_pages,
+               int32_t page_size, int32_t kv_heads, int32_t head_dim, const int64_t* slots, int64_t num_tokens,
+               void* k_out, int64_t ko_token_stride, int64_t ko_head_stride, void* v_out, int64_t vo_token_stride,
+               int64_t vo_head_stride, void* stream);
+
 /* The slot and the position of each of a batch's tokens (once per step, for
  * every layer): token t, row i of sequence s with n rows, is the sequence's
  * token p = kv_lens[s] - n + i.  slots[t] = -1 where p < 0, past the page
@@ -595,6 +633,25 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int
                        float scale, int32_t window, void* out, int64_t o_token_stride, int64_t o_head_stride,
                        float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* gs_paged_attention over a quantised cache: k and v rows are y 2^e of the
+ * cache's e4m3 values and scales, taken as they stand.  A scale byte of 0 counts as
+ * zero for values; one of 255 (NaN), or a value that is NaN, is as a value that is not
+ * finite above.
+ * head_dim a multiple of 16 up to 256; caches 16-byte aligned with strides that
+ * are multiples of 16, scales 8-byte aligned with strides that are multiples of
+ * 8.  dtype is that of q and out; the workspace is gs_paged_attention's, and
+ * may be shared with its calls. */
+int gs_paged_attention_e4m3(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                            const void* k_cache, int64_t k_page_stride, int64_t k_head_stride, int64_t k_row_stride,
+                            const void* v_cache, int64_t v_page_stride, int64_t v_head_stride, int64_t v_row_stride,
+                            const uint8_t* k_scales, int64_t ks_page_stride, int64_t ks_head_stride,
+                            const uint8_t* v_scales, int64_t vs_page_stride, int64_t vs_head_stride,
+                            int64_t num_pages, int32_t page_size, const int32_t* page_table, int64_t ld_table,
+                            int32_t max_pages, const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                            int64_t num_tokens, int32_t max_q, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                            float scale, int32_t window, void* out, int64_t o_token_stride, int64_t o_head_stride,
+                            float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* The id of the graph capture that `stream` is part of, 0 where it is in none:
  * calls of one capture on one stream may share a workspace, a graph shares its
  * with nothing else. */
@@ -622,6 +679,26 @@ int64_t gs_check_append_addresses(int32_t dtype, int32_t vec, int64_t q_token_st
                                   int32_t rot_dim, int32_t interleaved, const int64_t* slots, int64_t cache_page_stride,
                                   int64_t cache_head_stride, int64_t cache_row_stride, int64_t num_pages,
                                   int32_t page_size, int32_t cus, char* msg, int64_t msg_len, int64_t* checked);
+
+/* The same of gs_paged_attention_e4m3 (scales' strides shared by keys and
+ * values), and of gs_append_kv_normed with gs_read_kv of the same slots. */
+int64_t gs_check_paged_e4m3_addresses(int32_t dtype, int64_t q_token_stride, int64_t q_head_stride, int64_t k_page_stride,
+                                      int64_t k_head_stride, int64_t k_row_stride, int64_t v_page_stride,
+                                      int64_t v_head_stride, int64_t v_row_stride, int64_t s_page_stride,
+                                      int64_t s_head_stride, int64_t num_pages, int32_t page_size,
+                                      const int32_t* page_table, int64_t ld_table, int32_t max_pages,
+                                      const int32_t* kv_lens, const int32_t* cu_seqlens, int32_t num_seqs,
+                                      int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                      int32_t window, int64_t o_token_stride, int64_t o_head_stride, int32_t cus,
+                                      char* msg, int64_t msg_len, int64_t* checked);
+int64_t gs_check_rows_addresses(int32_t dtype, int32_t quantised, int32_t vec, int64_t q_token_stride,
+                                int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                const int64_t* positions, int64_t max_pos, int32_t rot_dim, int32_t interleaved,
+                                const int64_t* slots, int64_t cache_page_stride, int64_t cache_head_stride,
+                                int64_t cache_row_stride, int64_t s_page_stride, int64_t s_head_stride,
+                                int64_t num_pages, int32_t page_size, int32_t cus, char* msg, int64_t msg_len,
+                                int64_t* checked);
 
 /* ------------------------------------------------------------------------
  * The residual add between two blocks with the norms around it, one pass:

@@ -19,7 +19,8 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_NAME = "libgranite_switch_amd.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ("gs_meta.hip", "gs_lora.hip", "gs_small.hip", "gs_xext.hip", "gs_gemm.hip", "gs_append.hip",
-           "gs_append_rows.hip", "gs_paged.hip", "gs_paged_e4m3.hip", "gs_chunk.hip", "gs_norm.hip")
+           "gs_append_rows.hip", "gs_paged.hip", "gs_paged_e4m3.hip", "gs_chunk.hip",
+           "gs_chunk_e4m3.hip", "gs_norm.hip")
 ARCH = os.environ.get("GS_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

@@ -26,127 +26,10 @@
 // reaches 1586.  A step of 48 decode rows and 16 chunks of 256 over up to 3839 keys: 90 us.
 #include <algorithm>
 
-#include "gs_paged_rows.h"
+#include "gs_chunk.h"
 
 namespace gs {
 namespace {
-
-constexpr int kCWaves = 4;
-constexpr int kCKeys = 64;
-constexpr int kCStages = 2;
-
-// V rows that no query of a tile sees are zero in LDS: the cache may hold
-// anything there, and 0 * NaN is not 0.
-__device__ const u32x4 g_zero16 = {0, 0, 0, 0};
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-// 4 x 16 elements, transposed: lane i of 16 gives the address of 4 elements of
-// row i / 4 and gets column i of the 4 rows.
-__device__ __forceinline__ uint64_t read_tr(const char* p) {
-  return __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p)));
-}
-
-// As dma16, with the wait state that M0 needs.
-__device__ __forceinline__ void dma16_row(const char* src, uint32_t lds_dst) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_dst) : "memory", "m0");
-}
-// As above from a uniform base and the lane's byte offset.
-__device__ __forceinline__ void dma16_off(const char* base, uint32_t off, uint32_t lds_dst) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_dst) : "memory", "m0");
-}
-constexpr int wait_vm_lds0(int n) { return (n & 15) | (7 << 4) | ((n >> 4) << 14); }
-
-struct ChunkItem {
-  int s, j, part, nparts, slot;      // slot: of the tile's first partial result, or -1
-  int order;                         // of the tile among the split ones
-  addr::PagedSeq sq;
-};
-// The chunk form's parts (a tile of a sequence, or one of those it is split into) for
-// one head: the sequences with the longest parts first, in eight classes, a
-// sequence's tiles and parts from the last.
-struct ChunkOrder {
-  Batch4 q;
-  int tiles;                         // key tiles that a part of a split tile has
-  uint32_t magic;
-  int longest;                       // key tiles of the longest part
-  ClassOrder order;
-  uint64_t split;                    // before the lane's: partial results, split tiles << 32
-  int total;
-
-  struct Count {
-    int nt, np, longest;             // tiles, parts of each, key tiles of the longest part
-  };
-  __device__ __forceinline__ Count count(const PagedArgs& a, const addr::PagedSeq& sq) const {
-    Count c;
-    c.nt = addr::chunk_tiles(sq, a.tq);
-    c.longest = addr::chunk_key_tiles(addr::chunk_tile(sq, a.tq.tq, a.window, c.nt - 1));
-    c.np = addr::chunk_parts(sq, a.tq, a.window, tiles, magic);
-    if (c.np > 1) c.longest = min(c.longest, 2 * tiles);
-    return c;
-  }
-  __device__ __forceinline__ int class_of(int x) const {   // x <= longest, only the order matters
-    return min(7, static_cast<int>(8.f * static_cast<float>(longest - x) * __builtin_amdgcn_rcpf(static_cast<float>(longest) + 1.f)));
-  }
-  __device__ __forceinline__ void plan(const PagedArgs& a) {
-    load_batch(a, q, 0);
-    uint64_t work = 0;
-    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) { work += addr::chunk_work2(sq, a.tq, a.window); });
-    tiles = addr::chunk_part_tiles(static_cast<int64_t>(of_lane(lane_sums(work), 63)), a.chunk_share, kChunkLeast);
-    magic = addr::div_magic(tiles);
-    int most = 0;
-    split = 0;
-    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) {
-      const Count c = count(a, sq);
-      most = max(most, c.longest);
-      if (c.np > 1) split += static_cast<uint64_t>(c.nt) << 32 | static_cast<uint32_t>(c.nt * c.np);
-    });
-    longest = lanes_most(most);
-    order = ClassOrder{0, 0, a.chunk_parts >= 65536};
-    each_seq<true>(a, q, [&](int, const addr::PagedSeq& sq) {
-      const Count c = count(a, sq);
-      order.add(class_of(c.longest), c.nt * c.np);
-    });
-    total = order.place();
-    const uint64_t to = lane_sums(split);
-    // for the join, with the entries that the tiles' first parts write
-    if (threadIdx.x == 0 && blockIdx.x == 0) a.chunk_list[0].x = static_cast<int>(of_lane(to, 63) >> 32);
-    split = to - split;
-  }
-  // The r-th part (0 <= r < total).
-  __device__ __forceinline__ ChunkItem part(const PagedArgs& a, int r) {
-    ChunkItem it{-1, 0, 0, 1, 0, 0, {0, 0, 0}};
-    uint64_t sp = split;
-    each_seq<true>(a, q, [&](int s, const addr::PagedSeq& sq) {
-      const Count c = count(a, sq);
-      const int x = r - order.next(class_of(c.longest), c.nt * c.np);
-      if (x >= 0 && x < c.nt * c.np) {
-        it.s = s;
-        it.j = c.nt * c.np - 1 - x;                  // a sequence's last tiles, the longest, first
-        it.nparts = c.np;
-        it.slot = static_cast<int>(static_cast<uint32_t>(sp));
-        it.order = static_cast<int>(sp >> 32);
-        it.sq = sq;
-      }
-      if (c.np > 1) sp += static_cast<uint64_t>(c.nt) << 32 | static_cast<uint32_t>(c.nt * c.np);
-    });
-    const int from = __builtin_ctzll(__ballot(it.s >= 0));
-    const auto u = [&](int x) { return __builtin_amdgcn_readlane(x, from); };   // uniform, and known to be
-    const int np = u(it.nparts), x = u(it.j), j = np > 1 ? x / np : x;
-    return ChunkItem{u(it.s), j, x - j * np, np, np > 1 ? u(it.slot) + j * np : -1, u(it.order) + j, {u(it.sq.q0), u(it.sq.n), u(it.sq.len)}};
-  }
-};
-
-// The maximum, or the sum, over a lane and the one 32 lanes away.
-__device__ __forceinline__ float max_halves(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 // One part: 128 rows of a sequence and head h over its key tiles.
 template <int DT>
@@ -157,45 +40,14 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
   constexpr int kRowsPer = 1024 / kRowB;            // rows a wave transfer moves
   constexpr int kMoves = 8 / kRowsPer;              // transfers for 8 keys (as many for the values); a wave moves 16 keys
   constexpr int kSteps = DT / 16;
-  constexpr int kDT = DT / 32;                      // O^T tiles of 32 columns
 
   const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   const int lq = l & 31, hl = l >> 5;
   const int s = it.s;
-  const addr::PagedSeq& sq = it.sq;
-  const addr::PagedTile tile = addr::chunk_tile(sq, a.tq.tq, a.window, it.j);
-  const int nkt = addr::chunk_key_tiles(tile);
-  int kt0 = 0, kt1 = nkt;
-  if (it.nparts > 1) addr::chunk_part_range(nkt, it.part, it.nparts, kt0, kt1);
-
-  // ---- the lane's query row ---------------------------------------------------
-  const int nrow = (tile.i1 - tile.i0 + 1) * a.G;
-  const int r = wave * 32 + lq;
-  const bool live = r < nrow;
-  uint32_t r_q, r_h;
-  addr::div_by(live ? r : 0, a.G, a.g_magic, r_q, r_h);
-  const int qi = tile.i0 + static_cast<int>(r_q);
-  const int qh = h * a.G + static_cast<int>(r_h);
-  const int hi = live ? sq.len - sq.n + qi + 1 : 0;                // sees [lo, hi)
-  const int lo = a.window > 0 ? hi - a.window : 0;
-  const int64_t tok = sq.q0 + qi;
+  const ChunkRow w = chunk_row(a, it, h);
+  const addr::PagedTile& tile = w.tile;
   u32x4 qf[kSteps];
-  {
-    const char* qp = static_cast<const char*>(a.q) + (tok * a.q_ts + static_cast<int64_t>(qh) * a.q_hs) * 2;
-#pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-      const int d = 16 * st + 8 * hl;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(qp + (d < a.D ? d : 0) * 2);
-      qf[st] = live && d < a.D ? x : u32x4{0, 0, 0, 0};
-    }
-  }
-  // what the wave's rows see between them: [any_lo, any_hi); all of them: [all_lo, all_hi)
-  const int w0 = wave * 32, w1 = min(w0 + 31, nrow - 1);
-  const bool wave_live = w0 < nrow;
-  const int base_pos = sq.len - sq.n + tile.i0 + 1;
-  const int all_hi = __builtin_amdgcn_readfirstlane(base_pos + w0 / a.G);
-  const int any_hi = __builtin_amdgcn_readfirstlane(wave_live ? base_pos + w1 / a.G : 0);
-  const int any_lo = a.window > 0 ? all_hi - a.window : 0, all_lo = a.window > 0 ? any_hi - a.window : 0;
+  chunk_queries<DT>(a, w, qf);
 
   // ---- transfers ------------------------------------------------------------------
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)(lds)));
@@ -236,7 +88,7 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
 #pragma unroll
     for (int x = 0; x < kMoves; ++x) k_pos[oc][x] = k_off[x] + addr::chunk_k_pos(DT, 8 * oc + x * kRowsPer + t_row, t_pos) * 16;
   const auto issue = [&](int kt, int stage) {
-    const int i32 = (kt - kt0) & 31;
+    const int i32 = (kt - w.kt0) & 31;
     if (i32 == 0) load_ids(kt);
 #pragma unroll
     for (int oc = 0; oc < 2; ++oc) {
@@ -264,23 +116,16 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
     }
   };
 
-  f32x16 o[kDT];
-#pragma unroll
-  for (int d = 0; d < kDT; ++d)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
-  float m = -INFINITY, lsum = 0.f;
+  ChunkSums<DT> sum;
+  sum.clear();
 
-  // LDS addresses of the lane's operand rows: the permutations are exclusive ors, so
-  // a K step or a column tile is one more on the address of the first.
-  const uint32_t k_at = lq * kRowB + addr::chunk_k_pos(DT, lq, hl) * 16;
-  const int v_row = 4 * hl + ((l & 15) >> 2);
-  const uint32_t v_at = kTileB + v_row * kRowB + addr::chunk_v_pos(DT, v_row, 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) * 16 + (l & 1) * 8;
+  // LDS address of the lane's operand rows of K, as chunk_v_at.
+  const uint32_t k_at = lq * kRowB + addr::chunk_k_pos(DT, lq, hl) * 16, v_at = kTileB + chunk_v_at<DT>();
 
   // Tile kt, in `stage`; `next` tells whether tile kt + 1 is moved to the other one.
   const auto compute = [&](int kt, int stage, bool next) {
     const int tb = tile.first + kt * kCKeys;
-    const bool active = wave_live && tb < any_hi && tb + kCKeys > any_lo;
+    const bool active = w.wave_live && tb < w.any_hi && tb + kCKeys > w.any_lo;
     // every read of K on its way before the first product, the transfers' addresses made meanwhile
     u32x4 kf[kSteps][2];
     if (active) {
@@ -301,200 +146,30 @@ __device__ __forceinline__ void chunk_part(const PagedArgs& a, const ChunkItem& 
     for (int st = 0; st < kSteps; ++st)
 #pragma unroll
       for (int u = 0; u < 2; ++u) sc[u] = mfma32_bf16(kf[st][u], qf[st], sc[u]);
-    // the first half of V under the softmax
-    uint64_t vf[kDT][4][2];
-    const auto read_v = [&](int d) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) vf[d][g][x] = read_tr(lds + ((v_at + stage * kStageB) ^ (d * 64)) + (g * 16 + 8 * x) * kRowB);
-    };
-#pragma unroll
-    for (int d = 0; d < kDT / 2; ++d) read_v(d);
-    __builtin_amdgcn_sched_barrier(0);
-    if (tb + kCKeys > all_hi || tb < all_lo) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int t = tb + 32 * u + mfma32_row(v, l);
-          if (t >= hi || t < lo) sc[u][v] = -INFINITY;
-        }
-    }
-    float mx = sc[0][0];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, sc[u][v]);
-    mx = max_halves(mx) * a.scale_log2;
-    // the reference point follows the maximum once it has grown by 2^8: the sums
-    // stay far from their limits, and o is rarely scaled
-    if (__any(mx > m + 8.f)) {
-      const float mn = fmaxf(m, mx);
-      const float f = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      lsum *= f;
-#pragma unroll
-      for (int d = 0; d < kDT; ++d)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[d][v] *= f;
-    }
-    const float ms = m == -INFINITY ? 0.f : m;
-    u32x4 pf[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(sc[g >> 1][8 * (g & 1) + i], a.scale_log2, -ms));
-        lsum += p[i];
-      }
-      // bf16 probabilities with the error they have in the row form; two bf16 numbers for each
-      // are half as many products again, where instructions bound.  The total stays in fp32.
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-    }
-#pragma unroll
-    for (int d = kDT / 2; d < kDT; ++d) read_v(d);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int d = 0; d < kDT; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const u32x4 x = {static_cast<uint32_t>(vf[d][g][0]), static_cast<uint32_t>(vf[d][g][0] >> 32),
-                         static_cast<uint32_t>(vf[d][g][1]), static_cast<uint32_t>(vf[d][g][1] >> 32)};
-        o[d] = mfma32_bf16(x, pf[g], o[d]);
-      }
+    chunk_values<DT>(a, w, tb, sc, lds, v_at + stage * kStageB, sum);
   };
 
   // ---- the walk over the keys ---------------------------------------------------
-  const int n = kt1 - kt0;
+  const int n = w.kt1 - w.kt0;
   if (n > 0) {
-    issue(kt0, 0);
+    issue(w.kt0, 0);
     int stage = 0;
     for (int i = 0; i < n; ++i) {
       mem_fence_compiler();
       __builtin_amdgcn_s_waitcnt(wait_vm_lds0(0));                 // own transfers landed, own reads done
       __builtin_amdgcn_s_barrier();
       mem_fence_compiler();
-      compute(kt0 + i, stage, i + 1 < n);
+      compute(w.kt0 + i, stage, i + 1 < n);
       stage ^= 1;
     }
   }
-
-  // ---- results --------------------------------------------------------------------
-  lsum = sum_halves(lsum);
-  if (it.slot < 0) {
-    const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + tok * a.o_ts + static_cast<int64_t>(qh) * a.o_hs;
-    // A lane has columns 8 k + 4 hl .. + 3 of its row for every k: swapped between the
-    // two halves of the wave, 8 consecutive ones of every other k.
-#pragma unroll
-    for (int d = 0; d < kDT; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; v += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = lsum == 0.f ? 0.f : o[d][v + 2 * i] * inv, y = lsum == 0.f ? 0.f : o[d][v + 2 * i + 1] * inv;
-          w[i] = pack_bf16x2(x, y);
-        }
-        const auto p0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-        const auto p1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-        const int col = 32 * d + 2 * v + 8 * hl;
-        if (live && col < a.D) *reinterpret_cast<u32x4*>(out + col) = u32x4{p0[0], p1[0], p0[1], p1[1]};
-      }
-    if (a.lse != nullptr && hl == 0 && live) a.lse[tok * a.H + qh] = lsum == 0.f ? -INFINITY : (m + log2f(lsum)) * 0.6931471805599453f;
-    return;
-  }
-  float* p = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + it.slot + it.part) *
-                              addr::chunk_partial_floats(kChunkRows, DT);
-  if (wave_live) {                                   // in the order of the registers: whole lines
-#pragma unroll
-    for (int d = 0; d < kDT; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; v += 4)
-        *reinterpret_cast<f32x4*>(p + ((((wave * kDT + d) * 4 + (v >> 2)) * 64 + l) << 2)) =
-            f32x4{o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
-    if (hl == 0 && live) {
-      p[kChunkRows * DT + r] = m;
-      p[kChunkRows * (DT + 1) + r] = lsum;
-    }
-  }
-  if (it.part == 0 && h == 0 && tid == 0) a.chunk_list[1 + it.order] = make_int4(sq.q0 + tile.i0, nrow, it.nparts, it.slot);
+  chunk_results<DT>(a, it, h, w, sum);
 }
 
-// The split tiles' parts, joined in the order of their keys: workgroups take (tile,
-// an eighth of it, head) in turn, a thread 4 columns of a row, 8 parts' loads in
-// flight.  (A workgroup that joined its tile at the end of the launch above would read
-// all its parts alone: 14 parts of 128 rows took it 50 us.)
-template <int DT>
-__global__ __launch_bounds__(256) void chunk_join_kernel(PagedArgs a) {
-  constexpr int kBatch = 8;
-  constexpr int kGroups = 8, kDT = DT / 32;
-  const int64_t size = addr::chunk_partial_floats(kChunkRows, DT);
-  const int total = a.chunk_list[0].x * kGroups * a.HK;
-  for (int w = blockIdx.x; w < total; w += gridDim.x) {
-    const int h = w % a.HK, g = (w / a.HK) % kGroups;
-    const int4 e = a.chunk_list[1 + w / (a.HK * kGroups)];
-    const float* first = a.chunk_ws + (static_cast<int64_t>(h) * addr::chunk_slots_per_head(a.HK, a.chunk_slots) + e.w) * size;
-    for (int y = threadIdx.x; y < 128 * kDT; y += 256) {
-      const int x = g * 128 * kDT + y, l = x & 63;   // the x-th four floats: chunk_part's order
-      const int jr = x / (256 * kDT) * 32 + (l & 31), d = (x / 256 % kDT) * 32 + ((x >> 6) & 3) * 8 + (l >> 5) * 4;
-      if (jr >= e.y) continue;
-      float M = -INFINITY, L = 0.f;
-      f32x4 acc = {0, 0, 0, 0};
-      for (int p0 = 0; p0 < e.z; p0 += kBatch) {
-        f32x4 px[kBatch];
-        float pm[kBatch], pl[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const float* p = first + min(p0 + k, e.z - 1) * size;
-          px[k] = *reinterpret_cast<const f32x4*>(p + 4 * x);
-          pm[k] = p[kChunkRows * DT + jr];
-          pl[k] = p[kChunkRows * (DT + 1) + jr];
-        }
-        float Mn = M;
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) Mn = fmaxf(Mn, pm[k]);
-        const float ms = Mn == -INFINITY ? 0.f : Mn;
-        const float f0 = __builtin_amdgcn_exp2f(M - ms);           // M = -inf: nothing summed yet
-        L *= f0;
-        acc *= f0;
-        M = Mn;
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const float f = p0 + k < e.z ? __builtin_amdgcn_exp2f(pm[k] - ms) : 0.f;
-          L += f * pl[k];
-          acc += f * px[k];
-        }
-      }
-      uint32_t jq, jh;
-      addr::div_by(jr, a.G, a.g_magic, jq, jh);
-      row_store<true>(a, e.x + static_cast<int>(jq), h * a.G + static_cast<int>(jh), d, acc, M, L);
-    }
-  }
-  zero_outside<true>(a);
-}
-
-// Grid: addr::ragged_role.
 template <int DT>
 __global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_kernel(PagedArgs) {
   __shared__ __attribute__((aligned(1024))) char lds[addr::cmax(kCStages * 2 * kCKeys * DT * 2, static_cast<int>(sizeof(RowShared<DT>)))];
-  int i;
-  if (addr::ragged_role(blockIdx.x, fresh_args().ragged_block, fresh_args().row_blocks, i)) {
-    const PagedArgs& a = fresh_args();
-    const int r = i / a.HK, h = i - r * a.HK;
-    RowOrder<true, DT> order;
-    order.plan(a);
-    if (r < order.total) row_part<true, DT>(fresh_args(), order.part(a, r), h, *reinterpret_cast<RowShared<DT>*>(lds));
-  } else {
-    const PagedArgs& a = fresh_args();
-    ChunkOrder order;
-    order.plan(a);
-    const int r = i / a.HK, h = i - r * a.HK;        // 8 heads: a head's parts on one XCD
-    if (r < order.total) chunk_part<DT>(fresh_args(), order.part(a, r), h, lds);
-  }
+  ragged_work<DT, false>(lds, [&](const PagedArgs& a, const ChunkItem& it, int h) { chunk_part<DT>(a, it, h, lds); });
 }
 
 }  // namespace

@@ -83,6 +83,7 @@ int64_t chunk_workspace_bytes(int HK, int DT, int cus);
 int64_t chunk_most_parts(const PagedArgs& a);
 int64_t ragged_grid(const PagedArgs& a);
 void launch_ragged(const PagedArgs& a, int DT, hipStream_t st);
+void launch_ragged_e4m3(const PagedArgs& a, int DT, hipStream_t st);   // over a quantised cache (gs_chunk_e4m3.hip)
 // The row form over a quantised cache (gs_paged_e4m3.hip), on that many workgroups.
 void launch_rows_e4m3(const PagedArgs& a, bool bf16, int DT, int64_t workgroups, hipStream_t st);
 

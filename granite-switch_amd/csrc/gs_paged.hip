@@ -37,7 +37,6 @@ int64_t row_partial_floats(int HK, int D, int cus) {
 // Whether ragged calls of these sizes have a chunk form, and the rows up to
 // which a sequence stays with the row form.
 bool chunk_form(bool bf16, int G, int D) { return bf16 && D <= 128 && G <= kChunkRows; }
-bool has_chunk_form(const PagedArgs& a, bool bf16) { return a.ks == nullptr && chunk_form(bf16, a.G, a.D); }
 constexpr int kRowFormRows = 16;
 
 int64_t attention_ws_bytes(bool bf16, bool ragged, int G, int HK, int D, int cus) {
@@ -69,7 +68,7 @@ void plan_paged(PagedArgs& a, bool bf16, int cus, int max_pages, int page_size, 
   a.page_magic = addr::div_magic(a.page_octets);
   // The chunk form hides keys and takes the maximum before it scales, which is right for a
   // scale above zero only; the row form scales first.
-  a.row_limit = a.cu != nullptr && has_chunk_form(a, bf16) && scale > 0.f ? kRowFormRows : INT32_MAX;
+  a.row_limit = a.cu != nullptr && chunk_form(bf16, a.G, a.D) && scale > 0.f ? kRowFormRows : INT32_MAX;
   a.chunk_slots = chunk_slots_for(cus);
   a.row_slots = addr::row_slots_per_head(a.HK, 2 * cus);
   a.row_wgs = row_wgs_for(a.D, cus);
@@ -222,20 +221,34 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
     if (c != 1 && !m.bad) m.fail("a chunk part taken other than once", 0, 1, m.chunk_parts);
 }
 
-// The chunk form.
-template <int DT>
-void model_chunk(PagedModel& m, const PagedArgs& a) {
-  constexpr int kWaves = 4, kRowB = DT * 2, kTileB = 64 * kRowB, kRowsPer = 1024 / kRowB;
-  // what the transfers leave in LDS, and what the operand reads take from it
+// What the chunk form's transfers leave in LDS, and what the operand reads take from it.
+template <int DT, bool E4M3>
+void model_chunk_lds(PagedModel& m) {
+  constexpr int kWaves = 4, kRowB = DT * 2, kTileB = 64 * kRowB;
   std::vector<int> k_lds(kTileB / 16, -1), v_lds(kTileB / 16, -1);
+  const auto put = [&](std::vector<int>& lds, int at, int piece) {
+    m.in("stored (LDS)", at, 16, kTileB);
+    if (m.bad) return;
+    if (lds[at / 16] != -1) m.fail("a place stored twice", at, 16, kTileB);
+    lds[at / 16] = piece;
+  };
   for (int w = 0; w < kWaves; ++w)
-    for (int x = 0; x < 16 / kRowsPer; ++x)
-      for (int l = 0; l < 64; ++l) {
-        const int row = 16 * w + x * kRowsPer + l / (64 / kRowsPer), pos = l % (64 / kRowsPer);
-        const int at = ((16 * w + x * kRowsPer) * kRowB + l * 16) / 16;
-        k_lds[at] = row * 64 + addr::chunk_k_pos(DT, row, pos);
-        v_lds[at] = row * 64 + addr::chunk_v_pos(DT, row, pos);
+    for (int l = 0; l < 64; ++l) {
+      constexpr int kRowsPer = E4M3 ? 1024 / DT : 1024 / kRowB, kLanes = 64 / kRowsPer;
+      for (int x = 0; x < 16 / kRowsPer; ++x) {
+        const int in = x * kRowsPer + l / kLanes, pos = l % kLanes, row = 16 * w + in;
+        if (E4M3) {                                  // 16 columns of the cache, stored as two pieces
+          for (int e = 0; e < 2; ++e) {
+            put(k_lds, row * kRowB + addr::chunk_k_pos(DT, in, 2 * pos + e) * 16, row * 64 + 2 * pos + e);
+            put(v_lds, row * kRowB + addr::chunk_v_pos(DT, in, 2 * pos + e) * 16, row * 64 + 2 * pos + e);
+          }
+        } else {                                     // a transfer moves to consecutive places
+          const int at = (16 * w + x * kRowsPer) * kRowB + l * 16;
+          put(k_lds, at, row * 64 + addr::chunk_k_pos(DT, row, pos));
+          put(v_lds, at, row * 64 + addr::chunk_v_pos(DT, row, pos));
+        }
       }
+    }
   for (int l = 0; l < 64; ++l) {
     const int lq = l & 31, hl = l >> 5, v_row = 4 * hl + ((l & 15) >> 2);
     for (int u = 0; u < 2; ++u)
@@ -253,10 +266,18 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
           if (v_lds[at / 16] != (g * 16 + 8 * x + v_row) * 64 + piece) m.fail("V operand of another piece", at, 8, kTileB);
         }
   }
+}
+// The chunk form.
+void model_chunk(PagedModel& m, const PagedArgs& a, bool e4m3) {
+  const bool wide = paged_width(a.D) == 128;
+  if (e4m3) wide ? model_chunk_lds<128, true>(m) : model_chunk_lds<64, true>(m);
+  else wide ? model_chunk_lds<128, false>(m) : model_chunk_lds<64, false>(m);
   const int max_pages = static_cast<int>(a.max_len / (8 * a.page_octets));
   const int64_t page_rows = 8 * a.page_octets;
   const int64_t k_elems = extent3(a.num_pages, a.k_ps, a.HK, a.k_hs, page_rows, a.k_rs, a.D);
   const int64_t v_elems = extent3(a.num_pages, a.v_ps, a.HK, a.v_hs, page_rows, a.v_rs, a.D);
+  const int64_t ks_elems = extent3(a.num_pages, a.ks_ps, a.HK, a.ks_hs, page_rows, 1, 1);
+  const int64_t vs_elems = extent3(a.num_pages, a.vs_ps, a.HK, a.vs_hs, page_rows, 1, 1);
   const int64_t q_elems = extent3(a.T, a.q_ts, a.H, a.q_hs, 1, 0, a.D), o_elems = extent3(a.T, a.o_ts, a.H, a.o_hs, 1, 0, a.D);
   const addr::ChunkTq& tq = a.tq;
   int64_t U2 = 0, n = 0, slots = 0, split = 0;
@@ -297,6 +318,8 @@ void model_chunk(PagedModel& m, const PagedArgs& a) {
               m.in("page row", row * 8 + rr, 1, page_rows);
               m.in("k cache", page * a.k_ps + h * a.k_hs + (row * 8 + rr) * a.k_rs, a.D, k_elems);
               m.in("v cache", page * a.v_ps + h * a.v_hs + (row * 8 + rr) * a.v_rs, a.D, v_elems);
+              if (e4m3) m.in("k scales", page * a.ks_ps + h * a.ks_hs + row * 8 + rr, 1, ks_elems);
+              if (e4m3) m.in("v scales", page * a.vs_ps + h * a.vs_hs + row * 8 + rr, 1, vs_elems);
             }
           }
       }
@@ -409,7 +432,7 @@ int paged_attention(const char* who, bool e4m3, Scales sc, int32_t dtype, const 
   const int64_t n = row_grid(a);
   if (a.row_limit != INT32_MAX && (max_q == 0 || static_cast<int64_t>(max_q) * a.G > a.row_limit)) {
     GS_CHECK_ARG(ragged_grid(a) < (int64_t(1) << 31), "%s: too many tiles", who);
-    launch_ragged(a, DT, st);
+    e4m3 ? launch_ragged_e4m3(a, DT, st) : launch_ragged(a, DT, st);
     GS_CHECK_LAUNCH(who);
     return GS_OK;
   }
@@ -467,7 +490,7 @@ int64_t check_addresses(const char* who, bool e4m3, int64_t s_ps, int64_t s_hs, 
   PagedModel m;
   m.window = window;
   m.rows.assign(static_cast<size_t>(a.T) * a.H, 0);
-  if (a.row_limit != INT32_MAX) paged_width(head_dim) == 64 ? model_chunk<64>(m, a) : model_chunk<128>(m, a);
+  if (a.row_limit != INT32_MAX) model_chunk(m, a, e4m3);
   switch (paged_width(head_dim)) {
     case 64: model_width<64>(m, a, bf16, e4m3); break;
     case 128: model_width<128>(m, a, bf16, e4m3); break;

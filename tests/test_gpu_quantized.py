@@ -426,6 +426,33 @@ def test_small_and_large_rows(dev, dtype):
         b.check(b.run())
 
 
+@pytest.mark.parametrize("dim", [64, 128, 80])
+def test_queries_of_uneven_columns(dev, dim):
+    """Query and key rows whose columns differ by up to 2^30 and 2^12: sums of products of all sizes."""
+    _say(f"uneven columns, {dim}")
+    b = QBatch(dev, [70, 40], [30, 200], 8, 2, dim, seed=dim, spread=0.0)
+    g = torch.Generator(device=dev).manual_seed(2)
+    down = torch.randint(-30, 1, (b.q.shape[0], 1, dim), generator=g, device=dev)
+    down[:, :, 0] = 0
+    up = torch.randint(-3, 4, (b.q.shape[0], 8, 1), generator=g, device=dev)
+    b.q = (b.q.float() * torch.exp2((down + up).float())).to(BF16)
+    b.check(b.run())
+
+
+def test_queries_that_are_not_finite(dev):
+    """They reach their own rows only."""
+    _say("queries that are not finite")
+    b = QBatch(dev, [40, 50], [30, 0], 8, 2, 64, seed=5)
+    want = b.run()
+    for bad in (math.nan, math.inf, -math.inf):
+        b2 = b.q.clone()
+        b2[7, 3, 11] = b2[60, 1, 40] = bad
+        got = paged.paged_attention(b2, b.k, b.v, b.table, b.lens, b.cu)
+        odd = torch.zeros(got.shape[:2], dtype=torch.bool, device=dev)
+        odd[7, 3] = odd[60, 1] = True
+        assert bool(got[odd].isnan().any()) and torch.equal(got[~odd], want[~odd])
+
+
 def test_rows_of_no_sequence_and_out_in_place(dev):
     _say("padded step, out in place")
     b = QBatch(dev, [0, 33, 7], [5, 60, 300], 8, 2, 64, seed=2)

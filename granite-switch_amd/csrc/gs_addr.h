@@ -290,6 +290,17 @@ GS_HD int e8m0_of(uint32_t bits) {
   const int code = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return code < 1 ? 1 : code;
 }
+// `some` of `all` workgroups spread evenly: with share = spread_share(some, all), workgroup b
+// is the spread_before(b)-th of them if `is`, else the (b - spread_before(b))-th of the others.
+// all share = some 2^32 + d with d < all < 2^32, so there are exactly `some`.
+GS_HD uint32_t spread_share(int some, int all) {
+  return some == 0 ? 0 : some == all ? 0xffffffffu : static_cast<uint32_t>(((static_cast<uint64_t>(some) << 32) + all - 1) / all);
+}
+GS_HD int spread_before(int b, uint32_t share, int some) {
+  if (share == 0xffffffffu) return imin(b, some);
+  return static_cast<int>((static_cast<uint64_t>(b) * share) >> 32);
+}
+GS_HD bool spread_is(int b, uint32_t share, int some) { return spread_before(b + 1, share, some) > spread_before(b, share, some); }
 // A sequence of a batch: its first query row and number of query rows within
 // the T rows given, and its cached tokens within what its table row addresses.
 struct PagedSeq {

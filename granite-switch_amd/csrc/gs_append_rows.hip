@@ -24,24 +24,46 @@ namespace gs {
 namespace {
 
 struct RowsArgs {
-  AppendArgs a;
+  AppendArgs a;                                      // without units, groups and tokens
   const void* qw;                                    // norm weights [D] or NULL
   const void* kw;
   bool w_bf16;
-  float eps, inv_d;
+  float eps;
   uint8_t* ks;                                       // scales; a head's of a page side by side
   uint8_t* vs;
   int64_t ks_ps, ks_hs, vs_ps, vs_hs;
-  int lanes, lanes_log;                              // of a head
+  uint32_t page_magic;                               // div_magic(page_size) where slots fit 31 bits, or 0
+  int units, lanes_log;                              // column units and lanes of a head
+  int groups[3], tokens[3], blocks[3];               // queries, keys, values: heads at a time and tokens of a workgroup, workgroups
+  uint32_t k_share, v_share;                         // keys' share of the workgroups, values' of the others
 };
+enum Kind { kQueries, kKeys, kValues };
+// Workgroup b's kind, and which of that kind's it is: spread evenly, so that those that
+// compute more (keys) run beside those that move more.
+__device__ __host__ __forceinline__ Kind rows_kind(const RowsArgs& r, int b, int& block) {
+  block = addr::spread_before(b, r.k_share, r.blocks[kKeys]);
+  if (addr::spread_is(b, r.k_share, r.blocks[kKeys])) return kKeys;
+  b -= block;
+  block = addr::spread_before(b, r.v_share, r.blocks[kValues]);
+  if (addr::spread_is(b, r.v_share, r.blocks[kValues])) return kValues;
+  block = b - block;
+  return kQueries;
+}
 
 // Sums, and maxima, over the 2^n adjacent lanes of a head.
 template <int CTRL>
 __device__ __forceinline__ float dpp_other(float x) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, false));
 }
-template <class F>
-__device__ __forceinline__ float over_lanes(float x, int lanes, const F& f) {
+template <int CTRL>
+__device__ __forceinline__ double dpp_other(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xf, 0xf, false);
+  const uint32_t up = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, lo | (static_cast<uint64_t>(up) << 32));
+}
+template <class T, class F>
+__device__ __forceinline__ T over_lanes(T x, int lanes, const F& f) {
   if (lanes > 1) x = f(x, dpp_other<0xB1>(x));       // lanes 1, 2 apart
   if (lanes > 2) x = f(x, dpp_other<0x4E>(x));
   if (lanes > 4) x = f(x, dpp_other<0x141>(x));      // mirrored in 8, in 16: the other four, the other eight
@@ -94,27 +116,87 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* x, float inv
   }
 }
 
-// Thread mapping as append_kv_kernel's (gs_append.hip) with a head's units on a power of
-// two of lanes, NU to a lane: the vector forms have one, the scalar one a wave for a head.
-template <bool BF16, int VE, bool PAIRS, bool QUANT>
-__global__ __launch_bounds__(256) void append_rows_kernel(RowsArgs r) {
+// 1 / sqrt(x) from the instruction's 24 bits, twice refined.
+__device__ __forceinline__ double rsqrt64(double x) {
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y *= 1.5 - 0.5 * x * y * y;
+  return y;
+}
+// x in fp32, to the odd neighbour where it is none: another rounding, to fewer bits, is then
+// that of x itself.
+__device__ __forceinline__ float round_odd(double x) {
+  const float f = static_cast<float>(x);
+  const double back = static_cast<double>(f);
+  const uint32_t b = __float_as_uint(f);
+  const bool move = back != x && (b & 1u) == 0 && is_finite(f);
+  return __uint_as_float(move ? (fabs(x) > fabs(back) ? b + 1 : b - 1) : b);
+}
+
+// VE elements as they are in memory.
+template <bool BF16, int VE>
+struct RowVec {
+  u32x4 w;
+  __device__ __forceinline__ void load(const char* p) { w = ld16(p); }
+  __device__ __forceinline__ void none() { w = u32x4{0, 0, 0, 0}; }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (BF16) return __uint_as_float((i & 1) != 0 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    else return __uint_as_float(w[i]);
+  }
+};
+template <bool BF16>
+struct RowVec<BF16, 1> {
+  float w;
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (BF16) w = bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(p));
+    else w = *reinterpret_cast<const float*>(p);
+  }
+  __device__ __forceinline__ void none() { w = 0.f; }
+  __device__ __forceinline__ float at(int) const { return w; }
+};
+
+// The rows of one kind for a workgroup's tokens.  A thread takes a unit of columns as
+// append_kv_kernel (gs_append.hip) does -- two vectors of VE, partners of a rotation -- of
+// every groups-th head of its token; a head's units are on 2^n adjacent lanes, one to a
+// lane, or up to NU (element by element: a wave to a head).  Loads of kBatch heads are in
+// flight, one head's columns are unpacked.
+//
+// Keys that are normed or rotated on their way into a quantised cache take that in 64 bits:
+// in 32, one in 10^6 of them ends at the other e4m3 neighbour, 2^-3 away.  A thread has one
+// head of these at a time, or its 64-bit numbers leave too few registers for waves that hide
+// the loads.
+template <bool BF16, int VE, bool PAIRS, bool QUANT, int KIND>
+__device__ __forceinline__ void append_rows(const RowsArgs& r, int block) {
   constexpr int NU = VE == 1 ? 4 : 1;
-  constexpr int kBatch = VE == 1 ? 1 : 4;            // heads whose loads are in flight together
+  constexpr int kES = BF16 ? 2 : 4;
+  constexpr bool kE4m3 = QUANT && KIND != kQueries;
+  constexpr int kBatch = VE == 1 || (kE4m3 && KIND == kKeys) ? 1 : 4;
   const AppendArgs& a = r.a;
-  const int tid = threadIdx.x;
-  const int per_token = a.groups << r.lanes_log;
-  const int tok = tid / per_token;
-  if (tok >= a.tokens) return;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * a.tokens + tok;
-  if (t >= a.T) return;
-  const int in_tok = tid - tok * per_token;
-  const int grp = in_tok >> r.lanes_log, u0 = in_tok & (r.lanes - 1);
+  const int groups = r.groups[KIND], tokens = r.tokens[KIND], heads = KIND == kQueries ? a.H : a.HK;
+  const int tid = threadIdx.x, lanes = 1 << r.lanes_log;
+  const int g = tid >> r.lanes_log, u0 = tid & (lanes - 1);
+  const int tok = g / groups, grp = g - tok * groups;
+  const int64_t t = static_cast<int64_t>(block) * tokens + tok;
+  if (tok >= tokens || t >= a.T) return;
+  uint32_t page = 0, prow = 0;
+  if (KIND != kQueries) {
+    const int64_t slot = a.slots[t];
+    if (!addr::append_stored(slot, a.num_slots)) return;
+    if (r.page_magic != 0) {
+      addr::div_by(static_cast<uint32_t>(slot), a.page_size, r.page_magic, page, prow);
+    } else {
+      page = static_cast<uint32_t>(static_cast<uint64_t>(slot) / a.page_size);
+      prow = static_cast<uint32_t>(slot - static_cast<int64_t>(page) * a.page_size);
+    }
+  }
+  const void* norm = KIND == kQueries ? r.qw : KIND == kKeys ? r.kw : nullptr;
   addr::AppendCols c[NU];
-  float cs[NU][VE], sn[NU][VE], wq[NU][2][VE], wk[NU][2][VE];
+  float cs[NU][VE], sn[NU][VE], w[NU][2][VE];
 #pragma unroll
   for (int n = 0; n < NU; ++n) {
-    const int u = u0 + n * r.lanes;
-    c[n] = u < a.units ? addr::append_cols(u, VE, a.D, a.R, PAIRS) : addr::AppendCols{-1, -1, false};
+    const int u = u0 + n * lanes;
+    c[n] = u < r.units ? addr::append_cols(u, VE, a.D, a.R, PAIRS) : addr::AppendCols{-1, -1, false};
+    if (KIND == kValues) continue;
     if (c[n].rot) {
       const float* row = a.cos_sin + addr::append_pos(a.positions[t], a.max_pos) * a.R;
       const int j0 = addr::append_pair(u, VE);
@@ -124,102 +206,177 @@ __global__ __launch_bounds__(256) void append_rows_kernel(RowsArgs r) {
         sn[n][i] = row[a.R / 2 + j0 + i];
       }
     }
-    const auto weights = [&](const void* w, float (*to)[VE]) {
-      if (w == nullptr) return;
+    if (norm != nullptr) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int col = x == 0 ? c[n].c0 : c[n].c1;
+        const int col = max(x == 0 ? c[n].c0 : c[n].c1, 0);
+        if (BF16 && r.w_bf16) {
+          RowVec<true, VE> v;
+          v.load(static_cast<const char*>(norm) + col * 2);
 #pragma unroll
-        for (int i = 0; i < VE; ++i)
-          to[x][i] = col < 0 ? 0.f : r.w_bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(w)[col + i]) : static_cast<const float*>(w)[col + i];
+          for (int i = 0; i < VE; ++i) w[n][x][i] = v.at(i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VE; i += 4) {
+            RowVec<false, VE == 1 ? 1 : 4> v;
+            v.load(static_cast<const char*>(norm) + (col + i) * 4);
+#pragma unroll
+            for (int e = 0; e < (VE == 1 ? 1 : 4); ++e) w[n][x][i + e] = v.at(e);
+          }
+        }
       }
-    };
-    weights(r.qw, wq[n]);
-    weights(r.kw, wk[n]);
+    }
   }
-  const int64_t slot = a.slots[t];
-  const bool stored = addr::append_stored(slot, a.num_slots);
-  const uint32_t page = stored ? static_cast<uint32_t>(static_cast<uint64_t>(slot) / a.page_size) : 0u;
-  const uint32_t prow = stored ? static_cast<uint32_t>(slot - static_cast<int64_t>(page) * a.page_size) : 0u;
-  const int heads = a.H + 2 * a.HK;
-  for (int h0 = grp; h0 < heads; h0 += kBatch * a.groups) {
-    float x0[kBatch][NU][VE], x1[kBatch][NU][VE];
+  const char* src = static_cast<const char*>(KIND == kQueries ? a.q : KIND == kKeys ? a.k : a.v) +
+                    t * (KIND == kQueries ? a.q_ts : KIND == kKeys ? a.k_ts : a.v_ts) * kES;
+  const int64_t src_hs = (KIND == kQueries ? a.q_hs : KIND == kKeys ? a.k_hs : a.v_hs) * kES;
+  constexpr int kDS = kE4m3 ? 1 : kES;
+  char* dst = static_cast<char*>(KIND == kQueries ? a.q_out : KIND == kKeys ? a.kc : a.vc) +
+              (KIND == kQueries ? t * a.qo_ts : KIND == kKeys ? page * a.kc_ps + prow * a.kc_rs : page * a.vc_ps + prow * a.vc_rs) * kDS;
+  const int64_t dst_hs = (KIND == kQueries ? a.qo_hs : KIND == kKeys ? a.kc_hs : a.vc_hs) * kDS;
+  const auto lane_sum = [&](auto x) { return over_lanes(x, lanes, [](auto p, auto q) { return p + q; }); };
+  for (int h0 = grp; h0 < heads; h0 += kBatch * groups) {
+    RowVec<BF16, VE> x0[kBatch][NU], x1[kBatch][NU];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int h = h0 + b * a.groups;
+      const int h = h0 + b * groups;
       if (h >= heads) continue;
-      const bool isq = h < a.H, isk = !isq && h < a.H + a.HK;
-      const void* src = isq ? a.q : isk ? a.k : a.v;
-      const int64_t base = isq ? t * a.q_ts + h * a.q_hs
-                         : isk ? t * a.k_ts + (h - a.H) * a.k_hs : t * a.v_ts + (h - a.H - a.HK) * a.v_hs;
+      const char* p = src + h * src_hs;
 #pragma unroll
       for (int n = 0; n < NU; ++n) {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) x0[b][n][i] = x1[b][n][i] = 0.f;
-        if (c[n].c0 >= 0) append_load<BF16, VE>(src, base + c[n].c0, x0[b][n]);
-        if (c[n].c1 >= 0) append_load<BF16, VE>(src, base + c[n].c1, x1[b][n]);
+        if (c[n].c0 >= 0) x0[b][n].load(p + c[n].c0 * kES);
+        else x0[b][n].none();
+        if (c[n].c1 >= 0) x1[b][n].load(p + c[n].c1 * kES);
+        else x1[b][n].none();
       }
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int h = h0 + b * a.groups;
+      const int h = h0 + b * groups;
       if (h >= heads) continue;
-      const bool isq = h < a.H, isk = !isq && h < a.H + a.HK;
-      if (!isq && !stored) continue;
-      if ((isq && r.qw != nullptr) || (isk && r.kw != nullptr)) {
-        float ss = 0.f;
+      float f0[NU][VE], f1[NU][VE];
+      if (kE4m3 && KIND == kKeys && (norm != nullptr || a.R > 0)) {
+        double f = 1;
+        if (norm != nullptr) {
+          double ss = 0;
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+          for (int n = 0; n < NU; ++n)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) ss += x0[b][n][i] * x0[b][n][i] + x1[b][n][i] * x1[b][n][i];
-        ss = over_lanes(ss, r.lanes, [](float x, float y) { return x + y; });
-        const float f = rsqrtf(ss * r.inv_d + r.eps);
+            for (int i = 0; i < VE; ++i) {
+              const double p = x0[b][n].at(i), q = x1[b][n].at(i);
+              ss = fma(p, p, fma(q, q, ss));
+            }
+          f = rsqrt64(lane_sum(ss) / a.D + r.eps);
+        }
+        // a pair of partners at a time, and what does not depend on the head not kept in 64 bits
+        const auto pair = [&](float p32, float q32, float wp, float wq, float c32, float s32, bool rot, float& to_p, float& to_q) {
+          asm("" : "+v"(wp), "+v"(wq), "+v"(c32), "+v"(s32));
+          double p = p32, q = q32;
+          if (norm != nullptr) {
+            p *= f * wp;
+            q *= f * wq;
+          }
+          if (rot) {
+            const double cd = c32, sd = s32, p0 = p, q0 = q;
+            p = p0 * cd - q0 * sd;
+            q = q0 * cd + p0 * sd;
+          }
+          to_p = round_odd(p);
+          to_q = round_odd(q);
+        };
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+          if constexpr (!PAIRS || VE == 1) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i)
+              pair(x0[b][n].at(i), x1[b][n].at(i), w[n][0][i], w[n][1][i], cs[n][i], sn[n][i], c[n].rot, f0[n][i], f1[n][i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VE / 2; ++i) {
+              const int u = 2 * i, v = 2 * i + 1, k = VE / 2 + i;
+              pair(x0[b][n].at(u), x0[b][n].at(v), w[n][0][u], w[n][0][v], cs[n][i], sn[n][i], c[n].rot, f0[n][u], f0[n][v]);
+              pair(x1[b][n].at(u), x1[b][n].at(v), w[n][1][u], w[n][1][v], cs[n][k], sn[n][k], c[n].rot, f1[n][u], f1[n][v]);
+            }
+          }
+        }
+      } else {
 #pragma unroll
         for (int n = 0; n < NU; ++n)
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            x0[b][n][i] *= f * (isq ? wq : wk)[n][0][i];
-            x1[b][n][i] *= f * (isq ? wq : wk)[n][1][i];
+            f0[n][i] = x0[b][n].at(i);
+            f1[n][i] = x1[b][n].at(i);
           }
-      }
+        if (KIND != kValues && norm != nullptr) {
+          float ss = 0.f;
 #pragma unroll
-      for (int n = 0; n < NU; ++n)
-        if (c[n].rot && (isq || isk)) rotate<VE, PAIRS>(x0[b][n], x1[b][n], cs[n], sn[n]);
-      float inv = 1.f;
-      if (QUANT && !isq) {
+          for (int n = 0; n < NU; ++n)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) ss += f0[n][i] * f0[n][i] + f1[n][i] * f1[n][i];
+          const float f = rsqrtf(lane_sum(ss) * (1.f / a.D) + r.eps);
+#pragma unroll
+          for (int n = 0; n < NU; ++n)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+              f0[n][i] *= f * w[n][0][i];
+              f1[n][i] *= f * w[n][1][i];
+            }
+        }
+        if (KIND != kValues) {
+#pragma unroll
+          for (int n = 0; n < NU; ++n)
+            if (c[n].rot) rotate<VE, PAIRS>(f0[n], f1[n], cs[n], sn[n]);
+        }
+      }
+      char* p = dst + h * dst_hs;
+      if constexpr (kE4m3) {
         float m = 0.f;
 #pragma unroll
         for (int n = 0; n < NU; ++n)
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            m = is_finite(x0[b][n][i]) ? fmaxf(m, fabsf(x0[b][n][i])) : m;
-            m = is_finite(x1[b][n][i]) ? fmaxf(m, fabsf(x1[b][n][i])) : m;
+            m = is_finite(f0[n][i]) ? fmaxf(m, fabsf(f0[n][i])) : m;
+            m = is_finite(f1[n][i]) ? fmaxf(m, fabsf(f1[n][i])) : m;
           }
-        m = over_lanes(m, r.lanes, [](float x, float y) { return fmaxf(x, y); });
+        m = over_lanes(m, lanes, [](float x, float y) { return fmaxf(x, y); });
         const int code = addr::e8m0_of(__float_as_uint(m));
-        inv = __uint_as_float(static_cast<uint32_t>(254 - code) << 23);
+        const float inv = __uint_as_float(static_cast<uint32_t>(254 - code) << 23);
         if (u0 == 0) {
-          if (isk) r.ks[page * r.ks_ps + (h - a.H) * r.ks_hs + prow] = static_cast<uint8_t>(code);
-          else r.vs[page * r.vs_ps + (h - a.H - a.HK) * r.vs_hs + prow] = static_cast<uint8_t>(code);
+          uint8_t* s = KIND == kKeys ? r.ks + page * r.ks_ps + h * r.ks_hs : r.vs + page * r.vs_ps + h * r.vs_hs;
+          s[prow] = static_cast<uint8_t>(code);
         }
-      }
-      void* dst = isq ? a.q_out : isk ? a.kc : a.vc;
-      const int64_t base = isq ? t * a.qo_ts + h * a.qo_hs
-                         : isk ? page * a.kc_ps + (h - a.H) * a.kc_hs + prow * a.kc_rs
-                               : page * a.vc_ps + (h - a.H - a.HK) * a.vc_hs + prow * a.vc_rs;
 #pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        if (c[n].c0 < 0) continue;
-        if (QUANT && !isq) {
-          store_e4m3<VE>(static_cast<uint8_t*>(dst) + base + c[n].c0, x0[b][n], inv);
-          if (c[n].c1 >= 0) store_e4m3<VE>(static_cast<uint8_t*>(dst) + base + c[n].c1, x1[b][n], inv);
-        } else {
-          append_store<BF16, VE>(dst, base + c[n].c0, x0[b][n]);
-          if (c[n].c1 >= 0) append_store<BF16, VE>(dst, base + c[n].c1, x1[b][n]);
+        for (int n = 0; n < NU; ++n) {
+          if (c[n].c0 >= 0) store_e4m3<VE>(reinterpret_cast<uint8_t*>(p) + c[n].c0, f0[n], inv);
+          if (c[n].c1 >= 0) store_e4m3<VE>(reinterpret_cast<uint8_t*>(p) + c[n].c1, f1[n], inv);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+          if (c[n].c0 >= 0) append_store<BF16, VE>(p, c[n].c0, f0[n]);
+          if (c[n].c1 >= 0) append_store<BF16, VE>(p, c[n].c1, f1[n]);
         }
       }
     }
   }
+}
+
+// The kernel's only argument, to be loaded where it is used: the three kinds' fields together
+// would keep the scalar registers full throughout.
+__device__ __forceinline__ const RowsArgs& fresh_rows() {
+  typedef const __attribute__((address_space(4))) RowsArgs* Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const RowsArgs*)(p);
+}
+
+template <bool BF16, int VE, bool PAIRS, bool QUANT>
+__global__ __launch_bounds__(256, 4) void append_rows_kernel(RowsArgs) {
+  int block;
+  const Kind kind = rows_kind(fresh_rows(), blockIdx.x, block);
+  if (kind == kKeys) append_rows<BF16, VE, PAIRS, QUANT, kKeys>(fresh_rows(), block);
+  else if (kind == kValues) append_rows<BF16, VE, PAIRS, QUANT, kValues>(fresh_rows(), block);
+  else append_rows<BF16, VE, PAIRS, QUANT, kQueries>(fresh_rows(), block);
 }
 
 // ---------------------------------------------------------------------------
@@ -308,17 +465,23 @@ __global__ __launch_bounds__(256) void read_kv_kernel(ReadArgs r) {
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Heads and tokens of a workgroup as gs_append_kv's.
-void plan_rows(RowsArgs& r, int ve, int cus) {
-  AppendArgs& a = r.a;
-  a.units = addr::append_units(ve, a.D, a.R);
+// Few tokens: every head of a token at once; many: each thread four heads, its cosines,
+// sines and weights loaded once for them.
+void plan_rows(RowsArgs& r, int ve, bool quant, int cus) {
+  const AppendArgs& a = r.a;
+  r.units = addr::append_units(ve, a.D, a.R);
   r.lanes_log = 0;
-  while ((1 << r.lanes_log) < a.units && r.lanes_log < 6) ++r.lanes_log;
-  r.lanes = 1 << r.lanes_log;
-  const int n = a.H + 2 * a.HK;
+  while ((1 << r.lanes_log) < r.units && r.lanes_log < 6) ++r.lanes_log;
   const int most = 256 >> r.lanes_log;
-  a.groups = std::max(1, std::min(a.T <= 2 * cus ? n : (n + 3) / 4, most));
-  a.tokens = most / a.groups;
+  for (int kind = 0; kind < 3; ++kind) {
+    const int n = kind == kQueries ? a.H : a.HK;
+    r.groups[kind] = std::max(1, std::min(a.T <= 2 * cus || (quant && kind == kKeys) ? n : (n + 3) / 4, most));
+    r.tokens[kind] = most / r.groups[kind];
+    r.blocks[kind] = n == 0 ? 0 : (a.T + r.tokens[kind] - 1) / r.tokens[kind];
+  }
+  r.k_share = addr::spread_share(r.blocks[kKeys], r.blocks[kQueries] + r.blocks[kKeys] + r.blocks[kValues]);
+  r.v_share = addr::spread_share(r.blocks[kValues], r.blocks[kQueries] + r.blocks[kValues]);
+  r.page_magic = a.num_slots < (int64_t(1) << 31) ? addr::div_magic(a.page_size) : 0;
 }
 
 void plan_read(ReadArgs& r, int ve) {
@@ -345,53 +508,68 @@ void model_rows_append(PagedModel& m, const RowsArgs& r, bool quant, const int64
   const int64_t k_elems = extent3(a.T, a.k_ts, a.HK, a.k_hs, 1, 0, a.D);
   const int64_t c_elems = extent3(pages, a.kc_ps, a.HK, a.kc_hs, a.page_size, a.kc_rs, a.D);
   const int64_t s_elems = extent3(pages, r.ks_ps, a.HK, r.ks_hs, a.page_size, 1, 1);
-  const int heads = a.H + 2 * a.HK;
-  const int per_token = a.groups << r.lanes_log;
-  if (per_token * a.tokens > 256 || a.tokens < 1) m.fail("threads of a workgroup", 0, per_token * a.tokens, 256);
-  if (a.units > NU * r.lanes) m.fail("units of a head", 0, a.units, NU * r.lanes);
-  std::vector<int> seen(static_cast<size_t>(heads) * a.D), scales(heads);
-  for (int64_t blk = 0; blk * a.tokens < a.T && !m.bad; ++blk)
-    for (int tok = 0; tok < a.tokens && blk * a.tokens + tok < a.T; ++tok) {
-      const int64_t t = blk * a.tokens + tok;
-      std::fill(seen.begin(), seen.end(), 0);
-      std::fill(scales.begin(), scales.end(), 0);
-      const bool stored = addr::append_stored(slots[t], a.num_slots);
-      const int64_t page = stored ? slots[t] / a.page_size : 0, prow = stored ? slots[t] - page * a.page_size : 0;
-      for (int in_tok = 0; in_tok < per_token; ++in_tok)
+  if (r.units > NU << r.lanes_log) m.fail("units of a head", 0, r.units, NU << r.lanes_log);
+  std::vector<int> taken[3];
+  for (int kind = 0; kind < 3; ++kind) taken[kind].assign(r.blocks[kind], 0);
+  for (int b = 0; b < r.blocks[0] + r.blocks[1] + r.blocks[2]; ++b) {
+    int block;
+    const Kind kind = rows_kind(r, b, block);
+    m.in("workgroup", block, 1, r.blocks[kind]);
+    if (m.bad) return;
+    if (++taken[kind][block] != 1) m.fail("a workgroup's rows taken twice", block, 1, r.blocks[kind]);
+  }
+  for (int kind = 0; kind < 3; ++kind) {
+    const int groups = r.groups[kind], tokens = r.tokens[kind], heads = kind == kQueries ? a.H : a.HK, lanes = 1 << r.lanes_log;
+    if (groups * tokens * lanes > 256 || tokens < 1) m.fail("threads of a workgroup", 0, groups * tokens * lanes, 256);
+    std::vector<int> seen(static_cast<size_t>(a.T) * heads * a.D, 0), scales(static_cast<size_t>(a.T) * heads, 0);
+    for (int64_t block = 0; block < r.blocks[kind] && !m.bad; ++block)
+      for (int tid = 0; tid < 256 && !m.bad; ++tid) {
+        const int g = tid >> r.lanes_log, u0 = tid & (lanes - 1), tok = g / groups, grp = g - tok * groups;
+        const int64_t t = block * tokens + tok;
+        if (tok >= tokens || t >= a.T) continue;
+        const bool stored = addr::append_stored(slots[t], a.num_slots);
+        uint32_t page = 0, prow = 0;
+        if (stored) {
+          page = static_cast<uint32_t>(slots[t] / a.page_size);
+          prow = static_cast<uint32_t>(slots[t] - static_cast<int64_t>(page) * a.page_size);
+          uint32_t p2 = page, r2 = prow;
+          if (r.page_magic != 0) addr::div_by(static_cast<uint32_t>(slots[t]), a.page_size, r.page_magic, p2, r2);
+          if (p2 != page || r2 != prow) m.fail("division", slots[t], 0, a.page_size);
+        }
         for (int n = 0; n < NU; ++n) {
-          const int grp = in_tok >> r.lanes_log, u0 = in_tok & (r.lanes - 1), u = u0 + n * r.lanes;
-          if (u >= a.units) continue;
+          const int u = u0 + n * lanes;
+          if (u >= r.units) continue;
           const addr::AppendCols c = addr::append_cols(u, VE, a.D, a.R, PAIRS);
-          if (c.rot) {
+          if (c.rot && kind != kValues) {
             const int64_t row = addr::append_pos(positions[t], a.max_pos) * a.R;
             m.in("cosines", row + addr::append_pair(u, VE), VE, row + a.R / 2);
             m.in("cos_sin", row + a.R / 2 + addr::append_pair(u, VE), VE, a.max_pos * a.R);
           }
-          for (int h = grp; h < heads; h += a.groups) {
-            if (u0 == 0 && n == 0 && h >= a.H) {
-              ++scales[h];
-              if (quant && stored) m.in("scales", page * r.ks_ps + (h < a.H + a.HK ? h - a.H : h - a.H - a.HK) * r.ks_hs + prow, 1, s_elems);
+          for (int h = grp; h < heads; h += groups) {
+            if (u0 == 0 && n == 0 && kind != kQueries) {
+              ++scales[t * heads + h];
+              if (quant && stored) m.in("scales", page * r.ks_ps + h * r.ks_hs + prow, 1, s_elems);
             }
             for (int col : {c.c0, c.c1}) {
               if (col < 0) continue;
               m.in("norm weights", col, VE, a.D);
-              for (int i = 0; i < VE && col + i < a.D; ++i) ++seen[static_cast<size_t>(h) * a.D + col + i];
-              if (h < a.H) {
+              for (int i = 0; i < VE && col + i < a.D; ++i) ++seen[(t * heads + h) * a.D + col + i];
+              if (kind == kQueries) {
                 m.in("q", t * a.q_ts + h * a.q_hs + col, VE, q_elems);
                 m.in("q_out", t * a.qo_ts + h * a.qo_hs + col, VE, qo_elems);
               } else {
-                const int hk = h < a.H + a.HK ? h - a.H : h - a.H - a.HK;
-                m.in("k or v", t * a.k_ts + hk * a.k_hs + col, VE, k_elems);
-                if (stored) m.in("cache", page * a.kc_ps + hk * a.kc_hs + prow * a.kc_rs + col, VE, c_elems);
+                m.in("k or v", t * a.k_ts + h * a.k_hs + col, VE, k_elems);
+                if (stored) m.in("cache", page * a.kc_ps + h * a.kc_hs + prow * a.kc_rs + col, VE, c_elems);
               }
             }
           }
         }
-      for (int h = a.H; h < heads; ++h)
-        if (scales[h] != 1 && !m.bad) m.fail("a scale written other than once", h, scales[h], 1);
-      for (size_t i = 0; i < seen.size(); ++i)
-        if (seen[i] != 1 && !m.bad) m.fail("a column taken other than once", static_cast<int64_t>(i), 1, a.D);
-    }
+      }
+    for (int x : scales)
+      if (x != 1 && kind != kQueries && !m.bad) m.fail("a scale written other than once", 0, x, 1);
+    for (int x : seen)
+      if (x != 1 && !m.bad) m.fail("a column taken other than once", 0, x, 1);
+  }
 }
 
 void model_read(PagedModel& m, const ReadArgs& r, int ve, const int64_t* slots) {
@@ -466,7 +644,7 @@ int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs
   const int ve = bf16 ? 8 : 4;
   const auto fits = [&](const void* p, int64_t ts, int64_t hs) { return aligned16(p) && multiples(ve, {ts, hs}); };
   const int cache_align = quant ? ve : 16;           // bytes of a store
-  const bool vec = head_dim % ve == 0 && rot_dim % (2 * ve) == 0 && fits(k, k_ts, k_hs) && fits(v, v_ts, v_hs) &&
+  const bool vec = head_dim % ve == 0 && aligned16(q_norm) && aligned16(k_norm) && rot_dim % (2 * ve) == 0 && fits(k, k_ts, k_hs) && fits(v, v_ts, v_hs) &&
                    (heads == 0 || (fits(q, q_ts, q_hs) && fits(q_out, qo_ts, qo_hs))) && aligned_to(k_cache, cache_align) &&
                    aligned_to(v_cache, cache_align) && multiples(ve, {kc_ps, kc_hs, kc_rs, vc_ps, vc_hs, vc_rs});
   RowsArgs r{};
@@ -486,11 +664,12 @@ int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs
   r.kw = k_norm;
   r.w_bf16 = norm_dtype == GS_DTYPE_BF16;
   r.eps = eps;
-  r.inv_d = 1.0f / static_cast<float>(head_dim);
   r.ks = k_scales; r.ks_ps = ks_ps; r.ks_hs = ks_hs;
   r.vs = v_scales; r.vs_ps = vs_ps; r.vs_hs = vs_hs;
-  plan_rows(r, vec ? ve : 1, device_cus());
-  const dim3 grid(static_cast<unsigned>((num_tokens + a.tokens - 1) / a.tokens));
+  plan_rows(r, vec ? ve : 1, quant, device_cus());
+  const int64_t blocks = static_cast<int64_t>(r.blocks[0]) + r.blocks[1] + r.blocks[2];
+  GS_CHECK_ARG(blocks < (int64_t(1) << 31), "%s: num_tokens=%lld with %d + %d heads", who, (long long)num_tokens, heads, kv_heads);
+  const dim3 grid(static_cast<unsigned>(blocks));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, r); };
   const auto pick = [&](auto b, auto w) {
@@ -584,7 +763,7 @@ int64_t gs_check_rows_addresses(int32_t dtype, int32_t quant, int32_t vec, int64
   a.page_size = static_cast<uint32_t>(page_size);
   a.T = static_cast<int>(num_tokens);
   a.H = heads; a.HK = kv_heads; a.D = head_dim; a.R = rot_dim;
-  plan_rows(r, ve, cus);
+  plan_rows(r, ve, quant != 0, cus);
   PagedModel m;
   const bool pr = interleaved != 0;
   if (ve == 8) pr ? model_rows_append<8, true>(m, r, quant != 0, slots, positions) : model_rows_append<8, false>(m, r, quant != 0, slots, positions);

@@ -408,12 +408,6 @@ __device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSe
   const auto slot_of = [&](int p) { return first + p * addr::paged_partial_floats(DT); };
   for (int r0 = 0; r0 < nrow; r0 += kRows) {
     const int nr = min(kRows, nrow - r0);
-    __syncthreads();
-    for (int x = tid; x < np * kRows; x += 256) {
-      const int q = x & (kRows - 1);
-      sm[x] = q < nr ? get_partial(slot_of(x / kRows) + 16 * DT + r0 + q) : -INFINITY;
-    }
-    __syncthreads();
     const int items = nr * (DT / 4);                 // (row, 4 columns)
     const int groups = max(1, 256 / items);
     for (int base = 0; base < items; base += 256) {
@@ -423,25 +417,38 @@ __device__ __forceinline__ void row_join(const PagedArgs& a, const addr::PagedSe
       const int q = in ? x / (DT / 4) : 0, d = in ? (x - q * (DT / 4)) * 4 : 0;
       float M = -INFINITY, L = 0.f;
       f32x4 acc = {0, 0, 0, 0};
+      // 16 parts' loads in flight at a time; past the last they repeat it with weight 0
+      f32x4 px[16];
+      float lx[16];
+      const auto load = [&](int p0) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float* sl = slot_of(min(p0 + k * groups, np - 1));
+          px[k] = get_partial4(sl + (r0 + q) * DT + d);
+          lx[k] = get_partial(sl + 16 * DT + 16 + r0 + q);
+        }
+      };
+      if (in) load(g);
+      if (base == 0) {                               // the maxima meanwhile
+        __syncthreads();
+        for (int x = tid; x < np * kRows; x += 256) {
+          const int q = x & (kRows - 1);
+          sm[x] = q < nr ? get_partial(slot_of(x / kRows) + 16 * DT + r0 + q) : -INFINITY;
+        }
+        __syncthreads();
+      }
       if (in) {
+#pragma unroll 8
         for (int p = 0; p < np; ++p) M = fmaxf(M, sm[p * kRows + q]);
         const float ms = M == -INFINITY ? 0.f : M;
-        // 16 parts' loads in flight at a time; past the last they repeat it with weight 0
         for (int p0 = g; p0 < np; p0 += 16 * groups) {
-          f32x4 x[16];
-          float lx[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const float* sl = slot_of(min(p0 + k * groups, np - 1));
-            x[k] = get_partial4(sl + (r0 + q) * DT + d);
-            lx[k] = get_partial(sl + 16 * DT + 16 + r0 + q);
-          }
+          if (p0 != g) load(p0);
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             const int p = p0 + k * groups;
             const float f = p < np ? __builtin_amdgcn_exp2f(sm[min(p, np - 1) * kRows + q] - ms) : 0.f;
             L += f * lx[k];
-            acc += f * x[k];
+            acc += f * px[k];
           }
         }
       }

@@ -86,8 +86,12 @@ __device__ __forceinline__ void chunk_part_e4m3(const PagedArgs& a, const ChunkI
       };
       put(sel16(cols, k_raw[x]), cols ? __uint_as_float(k_scale[x] << 23) : 1.f, to + addr::chunk_k_pos(DT, row, 2 * t_pos) * 16,
           to + addr::chunk_k_pos(DT, row, 2 * t_pos + 1) * 16);
-      put(sel16(seen && cols, v_raw[x]), seen ? __uint_as_float(v_scale[x] << 23) : 1.f,
-          to + kTileB + addr::chunk_v_pos(DT, row, 2 * t_pos) * 16, to + kTileB + addr::chunk_v_pos(DT, row, 2 * t_pos + 1) * 16);
+      // odd rows store their second piece first: neighbours' rows are on different banks
+      const u32x4 vr = v_raw[x];
+      const bool odd = (row & 1) != 0;
+      put(sel16(seen && cols, odd ? u32x4{vr[2], vr[3], vr[0], vr[1]} : vr), seen ? __uint_as_float(v_scale[x] << 23) : 1.f,
+          to + kTileB + addr::chunk_v_pos(DT, row, 2 * t_pos + (row & 1)) * 16,
+          to + kTileB + addr::chunk_v_pos(DT, row, 2 * t_pos + 1 - (row & 1)) * 16);
     }
   };
 

@@ -185,6 +185,11 @@ def call(name: str, *args) -> int:
     return rc
 
 
+def prepared(name: str, args) -> list:
+    """A call's arguments as the binding has them: those that repeat are converted once (a third of a long call's time)."""
+    return [a if a is None or t is c_void_p else t(a) for a, t in zip(args, SIGNATURES[name][1], strict=True)]
+
+
 # the stream's handle without a Stream object around it (a launch asks once)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 

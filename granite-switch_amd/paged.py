@@ -277,32 +277,51 @@ def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, in
                  eps) -> torch.Tensor | None:
     """``append_kv_`` with norms of the heads, or into a quantised cache."""
     k_cache, v_cache, k_scales, v_scales = _parts("append_kv_", k_cache, v_cache)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, v, k_cache, v_cache, cos_sin, q_norm, k_norm)):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)
+                                    or k_cache.requires_grad or v_cache.requires_grad
+                                    or (cos_sin is not None and cos_sin.requires_grad)
+                                    or (q_norm is not None and q_norm.requires_grad)
+                                    or (k_norm is not None and k_norm.requires_grad)):
         raise _lib.no_gradients("append_kv_")
-    key = tuple(map(_layout, (q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, cos_sin, q_out, q_norm, k_norm)))
+    key = (interleaved, eps, *map(_layout, (q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, cos_sin, q_out,
+                                            q_norm, k_norm)))
     plan = _rows_plans.get(key)
     if plan is None:
-        plan = _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales, v_scales)
-        plan = _keep(_rows_plans, key, plan + _norms_plan(q, k, q_norm, k_norm)
-                     + ((_lib.GS_DTYPE_E4M3, k_scales.stride()[:2], v_scales.stride()[:2]) if k_scales is not None
-                        else (plan[0], (0, 0), (0, 0))))
-    (code, T, H, HK, D, R, q_st, k_st, v_st, kc_st, vc_st, o_st, max_pos, pages, page, norm_code, cache_code, ks_st,
-     vs_st) = plan
+        code, T, H, HK, D, R, q_st, k_st, v_st, kc_st, vc_st, o_st, max_pos, pages, page = _append_plan(
+            q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales, v_scales)
+        norm_code = _norms_code(q, k, q_norm, k_norm)
+        quant = k_scales is not None
+        args = _lib.prepared("gs_append_kv_normed", (
+            code, None, *q_st, None, *k_st, None, *v_st, T, H, HK, D, None, None, norm_code, eps, None, None, max_pos, R,
+            1 if interleaved else 0, None, _lib.GS_DTYPE_E4M3 if quant else code, None, *kc_st, None, *vc_st, None,
+            *(k_scales.stride()[:2] if quant else (0, 0)), None, *(v_scales.stride()[:2] if quant else (0, 0)), pages, page,
+            None, *o_st, None))
+        plan = _keep(_rows_plans, key, (T, R, args))
+    T, R, args = plan
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=k.device)
     if T == 0:
         return q_out
-    ptr = _lib.ptr
-    _lib.call("gs_append_kv_normed", code, ptr(q), *q_st, k.data_ptr(), *k_st, v.data_ptr(), *v_st, T, H, HK, D,
-              ptr(q_norm), ptr(k_norm), norm_code, eps, positions.data_ptr() if R else None, cos_sin.data_ptr() if R else None,
-              max_pos, R, 1 if interleaved else 0, slots.data_ptr(), cache_code, k_cache.data_ptr(), *kc_st,
-              v_cache.data_ptr(), *vc_st, ptr(k_scales), *ks_st, ptr(v_scales), *vs_st, pages, page,
-              None if q is None else q_out.data_ptr(), *o_st, _lib.stream_ptr(k.device))
+    args = args.copy()                                     # the addresses, where the library's arguments have them
+    if q is not None:
+        args[1], args[41] = q.data_ptr(), q_out.data_ptr()
+        if q_norm is not None:
+            args[14] = q_norm.data_ptr()
+    args[4], args[7] = k.data_ptr(), v.data_ptr()
+    if k_norm is not None:
+        args[15] = k_norm.data_ptr()
+    if R:
+        args[18], args[19] = positions.data_ptr(), cos_sin.data_ptr()
+    args[23], args[25], args[29] = slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if k_scales is not None:
+        args[33], args[36] = k_scales.data_ptr(), v_scales.data_ptr()
+    args[44] = _lib.stream_ptr(k.device)
+    _lib.call("gs_append_kv_normed", *args)
     return q_out
 
 
-def _norms_plan(q, k, q_norm, k_norm) -> tuple:
+def _norms_code(q, k, q_norm, k_norm) -> int:
+    """The checks of the norms' weights; their type."""
     who, dtype = "append_kv_", k.dtype
     _on_gpu(who, k.device, q_norm, k_norm)
     if q_norm is not None and q is None:
@@ -317,7 +336,7 @@ def _norms_plan(q, k, q_norm, k_norm) -> tuple:
         if found is not None and w.dtype != found:
             raise ValueError(f"{who}: q_norm is {found}, k_norm {w.dtype}")
         found = w.dtype
-    return (_DTYPES[found or dtype],)
+    return _DTYPES[found or dtype]
 
 
 def _append_plan(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, k_scales=None, v_scales=None) -> tuple:
@@ -386,21 +405,27 @@ def read_kv(k_cache, v_cache, slots: torch.Tensor, dtype: torch.dtype | None = N
         with torch.cuda.device(slots.device):
             return read_kv(k_cache, v_cache, slots, dtype, k_out, v_out)
     k_cache, v_cache, k_scales, v_scales = _parts(who, k_cache, v_cache)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (k_cache, v_cache, k_out, v_out)):
+    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad
+                                    or (k_out is not None and k_out.requires_grad)
+                                    or (v_out is not None and v_out.requires_grad)):
         raise _lib.no_gradients(who)
     key = (dtype, *map(_layout, (k_cache, v_cache, k_scales, v_scales, slots, k_out, v_out)))
     plan = _read_plans.get(key)
     if plan is None:
         plan = _keep(_read_plans, key, _read_plan(k_cache, v_cache, k_scales, v_scales, slots, dtype, k_out, v_out))
-    dtype, code, cache_code, kc_st, vc_st, ks_st, vs_st, pages, page, HK, D, T, ko_st, vo_st = plan
+    shape, dtype, args = plan
+    dev = slots.device
     if k_out is None:
-        k_out = torch.empty((T, HK, D), dtype=dtype, device=slots.device)
+        k_out = torch.empty(shape, dtype=dtype, device=dev)
     if v_out is None:
-        v_out = torch.empty((T, HK, D), dtype=dtype, device=slots.device)
-    if T:
-        _lib.call("gs_read_kv", code, cache_code, k_cache.data_ptr(), *kc_st, v_cache.data_ptr(), *vc_st, _lib.ptr(k_scales),
-                  *ks_st, _lib.ptr(v_scales), *vs_st, pages, page, HK, D, slots.data_ptr(), T, k_out.data_ptr(), *ko_st,
-                  v_out.data_ptr(), *vo_st, _lib.stream_ptr(slots.device))
+        v_out = torch.empty(shape, dtype=dtype, device=dev)
+    if shape[0]:
+        args = args.copy()                                 # the addresses, where the library's arguments have them
+        args[2], args[6] = k_cache.data_ptr(), v_cache.data_ptr()
+        if k_scales is not None:
+            args[10], args[13] = k_scales.data_ptr(), v_scales.data_ptr()
+        args[20], args[22], args[25], args[28] = slots.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _lib.stream_ptr(dev)
+        _lib.call("gs_read_kv", *args)
     return k_out, v_out
 
 
@@ -427,10 +452,12 @@ def _read_plan(k_cache, v_cache, k_scales, v_scales, slots, dtype, k_out, v_out)
             _heads3(who, name, t, T, dtype)
             if tuple(t.shape) != (T, HK, D):
                 raise ValueError(f"{who}: {name} is {tuple(t.shape)}, expected {(T, HK, D)}")
-    return (dtype, _DTYPES[dtype], _lib.GS_DTYPE_E4M3 if quant else _DTYPES[dtype], k_cache.stride()[:3],
-            v_cache.stride()[:3], k_scales.stride()[:2] if quant else (0, 0), v_scales.stride()[:2] if quant else (0, 0),
-            pages, page, HK, D, T, (HK * D, D) if k_out is None else k_out.stride()[:2],
-            (HK * D, D) if v_out is None else v_out.stride()[:2])
+    code = _DTYPES[dtype]
+    return (T, HK, D), dtype, _lib.prepared("gs_read_kv", (
+        code, _lib.GS_DTYPE_E4M3 if quant else code, None, *k_cache.stride()[:3], None, *v_cache.stride()[:3], None,
+        *(k_scales.stride()[:2] if quant else (0, 0)), None, *(v_scales.stride()[:2] if quant else (0, 0)), pages, page, HK,
+        D, None, T, None, *((HK * D, D) if k_out is None else k_out.stride()[:2]), None,
+        *((HK * D, D) if v_out is None else v_out.stride()[:2]), None))
 
 
 # ---------------------------------------------------------------------------

@@ -468,21 +468,26 @@ __global__ __launch_bounds__(256) void read_kv_kernel(ReadArgs r) {
 // ---------------------------------------------------------------------------
 // Few tokens: every head of a token at once; many: each thread four heads, its cosines,
 // sines and weights loaded once for them.
-void plan_rows(RowsArgs& r, int ve, bool quant, int cus) {
+// False: more workgroups than a launch has.
+bool plan_rows(RowsArgs& r, int ve, bool quant, int cus) {
   const AppendArgs& a = r.a;
   r.units = addr::append_units(ve, a.D, a.R);
   r.lanes_log = 0;
   while ((1 << r.lanes_log) < r.units && r.lanes_log < 6) ++r.lanes_log;
   const int most = 256 >> r.lanes_log;
+  int64_t all = 0;
   for (int kind = 0; kind < 3; ++kind) {
     const int n = kind == kQueries ? a.H : a.HK;
     r.groups[kind] = std::max(1, std::min(a.T <= 2 * cus || (quant && kind == kKeys) ? n : (n + 3) / 4, most));
     r.tokens[kind] = most / r.groups[kind];
-    r.blocks[kind] = n == 0 ? 0 : (a.T + r.tokens[kind] - 1) / r.tokens[kind];
+    r.blocks[kind] = n == 0 ? 0 : static_cast<int>((static_cast<int64_t>(a.T) + r.tokens[kind] - 1) / r.tokens[kind]);
+    all += r.blocks[kind];
   }
+  if (all >= (int64_t(1) << 31)) return false;
   r.k_share = addr::spread_share(r.blocks[kKeys], r.blocks[kQueries] + r.blocks[kKeys] + r.blocks[kValues]);
   r.v_share = addr::spread_share(r.blocks[kValues], r.blocks[kQueries] + r.blocks[kValues]);
   r.page_magic = a.num_slots < (int64_t(1) << 31) ? addr::div_magic(a.page_size) : 0;
+  return true;
 }
 
 void plan_read(ReadArgs& r, int ve) {
@@ -667,10 +672,9 @@ int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs
   r.eps = eps;
   r.ks = k_scales; r.ks_ps = ks_ps; r.ks_hs = ks_hs;
   r.vs = v_scales; r.vs_ps = vs_ps; r.vs_hs = vs_hs;
-  plan_rows(r, vec ? ve : 1, quant, device_cus());
-  const int64_t blocks = static_cast<int64_t>(r.blocks[0]) + r.blocks[1] + r.blocks[2];
-  GS_CHECK_ARG(blocks < (int64_t(1) << 31), "%s: num_tokens=%lld with %d + %d heads", who, (long long)num_tokens, heads, kv_heads);
-  const dim3 grid(static_cast<unsigned>(blocks));
+  GS_CHECK_ARG(plan_rows(r, vec ? ve : 1, quant, device_cus()), "%s: num_tokens=%lld with %d + %d heads of %d are too many", who,
+               (long long)num_tokens, heads, kv_heads, head_dim);
+  const dim3 grid(static_cast<unsigned>(r.blocks[0] + r.blocks[1] + r.blocks[2]));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, r); };
   const auto pick = [&](auto b, auto w) {
@@ -764,7 +768,7 @@ int64_t gs_check_rows_addresses(int32_t dtype, int32_t quant, int32_t vec, int64
   a.page_size = static_cast<uint32_t>(page_size);
   a.T = static_cast<int>(num_tokens);
   a.H = heads; a.HK = kv_heads; a.D = head_dim; a.R = rot_dim;
-  plan_rows(r, ve, quant != 0, cus);
+  GS_CHECK_ARG(plan_rows(r, ve, quant != 0, cus), "%s: too many rows", who);
   PagedModel m;
   const bool pr = interleaved != 0;
   if (ve == 8) pr ? model_rows_append<8, true>(m, r, quant != 0, slots, positions) : model_rows_append<8, false>(m, r, quant != 0, slots, positions);

@@ -47,22 +47,34 @@ __device__ __forceinline__ void chunk_part_e4m3(const PagedArgs& a, const ChunkI
     id_page = addr::paged_page(trow[pg], a.num_pages);
     id_row = static_cast<int>(row8 * 8);
   };
+  // a lane's places in the 8 rows of a page that it loads from
+  const int in8 = t_row & 7, col = t_pos * 16 < a.D ? t_pos * 16 : 0;
+  const int64_t k_lane = in8 * a.k_rs + col, v_lane = in8 * a.v_rs + col;
   u32x4 k_raw[kMoves], v_raw[kMoves];
   uint32_t k_scale[kMoves], v_scale[kMoves];
   const auto issue = [&](int kt) {
     const int i32 = (kt - w.kt0) & 31;
     if (i32 == 0) load_ids(kt);
-    const int64_t page0 = __builtin_amdgcn_readlane(id_page, 2 * i32), page1 = __builtin_amdgcn_readlane(id_page, 2 * i32 + 1);
-    const int row0 = __builtin_amdgcn_readlane(id_row, 2 * i32), row1 = __builtin_amdgcn_readlane(id_row, 2 * i32 + 1);
-    const int col = t_pos * 16 < a.D ? t_pos * 16 : 0;
+    const char* kb[2];
+    const char* vb[2];
+    const uint8_t* ksb[2];
+    const uint8_t* vsb[2];
+#pragma unroll
+    for (int oc = 0; oc < 2; ++oc) {                   // uniform: the first row of 8
+      const int64_t page = __builtin_amdgcn_readlane(id_page, 2 * i32 + oc);
+      const int row = __builtin_amdgcn_readlane(id_row, 2 * i32 + oc);
+      kb[oc] = k_head + page * a.k_ps + row * a.k_rs;
+      vb[oc] = v_head + page * a.v_ps + row * a.v_rs;
+      ksb[oc] = ks_head + page * a.ks_ps + row;
+      vsb[oc] = vs_head + page * a.vs_ps + row;
+    }
 #pragma unroll
     for (int x = 0; x < kMoves; ++x) {
-      const int row = x * kRowsPer + t_row, in = row & 7;
-      const int64_t page = row < 8 ? page0 : page1, at = (row < 8 ? row0 : row1) + in;
-      k_raw[x] = ld16(k_head + page * a.k_ps + at * a.k_rs + col);
-      v_raw[x] = ld16(v_head + page * a.v_ps + at * a.v_rs + col);
-      k_scale[x] = ks_head[page * a.ks_ps + at];
-      v_scale[x] = vs_head[page * a.vs_ps + at];
+      const bool second = kMoves == 2 ? x == 1 : t_row >= 8;
+      k_raw[x] = ld16((second ? kb[1] : kb[0]) + k_lane);
+      v_raw[x] = ld16((second ? vb[1] : vb[0]) + v_lane);
+      k_scale[x] = (second ? ksb[1] : ksb[0])[in8];
+      v_scale[x] = (second ? vsb[1] : vsb[0])[in8];
     }
   };
   // What `issue` loaded into LDS.  Values that no query of the tile sees are zero: the cache

@@ -518,6 +518,29 @@ def test_captured(dev):
             assert torch.equal(a, b), i
 
 
+def test_two_streams(dev):
+    """Append and attention on two streams at once: each as on its own."""
+    _say("two streams")
+    cases = [QBatch(dev, [70, 1, 40, 9], [3000, 2000, 0, 900], 8, 2, 64, seed=s) for s in (1, 2)]
+    want = [b.run() for b in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(6):
+        for i, (b, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                n = b.len[0]
+                slots, _ = paged.cache_slots(b.table[:1], b.lens[:1], b.page, b.k.values.shape[0],
+                                             torch.tensor([0, n], dtype=torch.int32, device=dev), n)
+                k, v = paged.read_kv(b.k, b.v, slots)
+                paged.append_kv_(None, k, v, b.k, b.v, slots)            # the same rows again: their values do not change
+                got[i].append(b.run())
+    torch.cuda.synchronize()
+    for x, y in zip(want, got):
+        for z in y:
+            assert torch.equal(x, z)
+
+
 def test_registered_ops(dev):
     _say("registered ops")
     g = torch.Generator(device=dev).manual_seed(9)

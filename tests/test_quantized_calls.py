@@ -51,6 +51,11 @@ def test_append_arguments(change):
     _refused("gs_append_kv_normed", APPEND, change)
 
 
+def test_more_rows_than_a_launch_has():
+    _refused("gs_append_kv_normed", APPEND, dict(num_tokens=2 ** 31 - 1, q_ts=4096, heads=32, head_dim=512, q_hs=512, k_hs=512,
+                                                 v_hs=512, o_hs=512))
+
+
 @pytest.mark.parametrize("change", [
     dict(dtype=7), dict(dtype=E4M3), dict(cache_dtype=FP32), dict(num_tokens=-1), dict(kv_heads=0), dict(head_dim=513),
     dict(page_size=0), dict(num_pages=0), dict(slots=None), dict(k_cache=None), dict(v_cache=None), dict(k_scales=None),

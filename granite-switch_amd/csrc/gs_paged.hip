@@ -117,7 +117,8 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   std::vector<char>& rows = m.rows;
   int64_t U = 0;
   for (int s = 0; s < a.B; ++s) U += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
-  const int most = addr::row_part_units(U, a.HK, a.row_wgs);
+  int most = addr::row_part_units(U, a.HK, a.row_wgs);
+  if (E4M3 && a.row_limit != INT32_MAX) most = std::max(most, addr::kRaggedRowUnits);
   const uint32_t magic = addr::div_magic(most);
   int64_t parts = 0, slot = 0;
   for (int s = 0; s < a.B && !m.bad; ++s) {

@@ -64,6 +64,11 @@ __device__ __forceinline__ double dpp_other(double x) {
 }
 template <class T, class F>
 __device__ __forceinline__ T over_lanes(T x, int lanes, const F& f) {
+  if (lanes == 8) {                                  // 128 bf16 columns, 64 fp32 ones
+    x = f(x, dpp_other<0xB1>(x));
+    x = f(x, dpp_other<0x4E>(x));
+    return f(x, dpp_other<0x141>(x));
+  }
   if (lanes > 1) x = f(x, dpp_other<0xB1>(x));       // lanes 1, 2 apart
   if (lanes > 2) x = f(x, dpp_other<0x4E>(x));
   if (lanes > 4) x = f(x, dpp_other<0x141>(x));      // mirrored in 8, in 16: the other four, the other eight
@@ -96,12 +101,12 @@ __device__ __forceinline__ void rotate(float* x0, float* x1, const float* cs, co
   }
 }
 
-// VE values as e4m3 in the low bytes; what is not finite becomes NaN.
+// VE values as e4m3 in the low bytes.
 template <int VE>
 __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* x, float inv) {
   float y[VE];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) y[i] = is_finite(x[i]) ? x[i] * inv : __uint_as_float(0x7fc00000u);
+  for (int i = 0; i < VE; ++i) y[i] = x[i] * inv;
   if constexpr (VE == 1) {
     *p = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[0], 0, false));
   } else {
@@ -235,13 +240,16 @@ __device__ __forceinline__ void append_rows(const RowsArgs& r, int block) {
               (KIND == kQueries ? t * a.qo_ts : KIND == kKeys ? page * a.kc_ps + prow * a.kc_rs : page * a.vc_ps + prow * a.vc_rs) * kDS;
   const int64_t dst_hs = (KIND == kQueries ? a.qo_hs : KIND == kKeys ? a.kc_hs : a.vc_hs) * kDS;
   const auto lane_sum = [&](auto x) { return over_lanes(x, lanes, [](auto p, auto q) { return p + q; }); };
-  for (int h0 = grp; h0 < heads; h0 += kBatch * groups) {
+  const int64_t src_step = groups * src_hs, dst_step = groups * dst_hs;
+  src += grp * src_hs;
+  dst += grp * dst_hs;
+  for (int h0 = grp; h0 < heads; h0 += kBatch * groups, src += kBatch * src_step, dst += kBatch * dst_step) {
     RowVec<BF16, VE> x0[kBatch][NU], x1[kBatch][NU];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int h = h0 + b * groups;
       if (h >= heads) continue;
-      const char* p = src + h * src_hs;
+      const char* p = src + b * src_step;
 #pragma unroll
       for (int n = 0; n < NU; ++n) {
         if (c[n].c0 >= 0) x0[b][n].load(p + c[n].c0 * kES);
@@ -328,17 +336,27 @@ __device__ __forceinline__ void append_rows(const RowsArgs& r, int block) {
             if (c[n].rot) rotate<VE, PAIRS>(f0[n], f1[n], cs[n], sn[n]);
         }
       }
-      char* p = dst + h * dst_hs;
+      char* p = dst + b * dst_step;
       if constexpr (kE4m3) {
-        float m = 0.f;
+        const auto largest = [&] {                   // NaN is never the larger one
+          float m = 0.f;
 #pragma unroll
-        for (int n = 0; n < NU; ++n)
+          for (int n = 0; n < NU; ++n)
 #pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            m = is_finite(f0[n][i]) ? fmaxf(m, fabsf(f0[n][i])) : m;
-            m = is_finite(f1[n][i]) ? fmaxf(m, fabsf(f1[n][i])) : m;
-          }
-        m = over_lanes(m, lanes, [](float x, float y) { return fmaxf(x, y); });
+            for (int i = 0; i < VE; ++i) m = fmaxf(fmaxf(m, fabsf(f0[n][i])), fabsf(f1[n][i]));
+          return over_lanes(m, lanes, [](float x, float y) { return fmaxf(x, y); });
+        };
+        float m = largest();
+        if (!is_finite(m)) {                         // infinities become NaN, which e4m3 has
+#pragma unroll
+          for (int n = 0; n < NU; ++n)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+              f0[n][i] = is_finite(f0[n][i]) ? f0[n][i] : __uint_as_float(0x7fc00000u);
+              f1[n][i] = is_finite(f1[n][i]) ? f1[n][i] : __uint_as_float(0x7fc00000u);
+            }
+          m = largest();
+        }
         const int code = addr::e8m0_of(__float_as_uint(m));
         const float inv = __uint_as_float(static_cast<uint32_t>(254 - code) << 23);
         if (u0 == 0) {

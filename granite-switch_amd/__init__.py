@@ -9,7 +9,7 @@ driven from Python on PyTorch-ROCm:
   meta         ``LoRAContext`` / ``FusedLoRAKernelMeta``
   vllm_layers  vLLM-form ``SwitchedLoRALinear`` (fused w_ext GEMM + expand)
   hf_layers    HF-form ``SwitchedLoRALinear`` / ``MergedSwitchedLoRALinear``
-  paged        paged key/value cache: rotated append, attention over it
+  paged        paged key/value cache, plain or quantised: rotated append, attention over it
   norms        the residual add between blocks with the norms around it
   decoder      a decoder over the paged cache, put together from the above
   probe_routing  drop-in for ``granite_switch.probe_routing`` (probe-slot split)

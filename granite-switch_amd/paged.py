@@ -101,6 +101,8 @@ def _heads3(who: str, name: str, t: torch.Tensor, tokens: int | None, dtype) -> 
                          f"head_dim], got {t.dtype} {tuple(t.shape)}")
     if t.stride(2) != 1 and t.shape[2] > 1:
         raise ValueError(f"{who}: {name}'s head dimension must be contiguous (strides {t.stride()})")
+    if max(t.shape[1:]) > _INT32:
+        raise ValueError(f"{who}: {name} has {t.shape[1]} heads of {t.shape[2]} (2^31 - 1 at most)")
     return t
 
 
@@ -112,8 +114,9 @@ def _caches(who: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, kv_he
                              f"both caches alike, got {c.dtype} {tuple(c.shape)}")
         if c.stride(3) != 1 and head_dim > 1:
             raise ValueError(f"{who}: {name}'s head dimension must be contiguous (strides {c.stride()})")
-    if k_cache.shape[0] == 0 or not 0 < k_cache.shape[2] <= _INT32:
-        raise ValueError(f"{who}: pages of {k_cache.shape[2]} rows, {k_cache.shape[0]} of them (1 .. 2^31 - 1 rows)")
+    if k_cache.shape[0] == 0 or not 0 < k_cache.shape[2] <= _INT32 or k_cache.shape[1] > _INT32:
+        raise ValueError(f"{who}: {k_cache.shape[0]} pages of {k_cache.shape[2]} rows and {k_cache.shape[1]} heads "
+                         "(1 .. 2^31 - 1)")
 
 
 def _scales(who: str, k_scales: torch.Tensor, v_scales: torch.Tensor, values: torch.Tensor):

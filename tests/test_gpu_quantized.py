@@ -390,6 +390,18 @@ def test_chunks(dev, dtype, heads, kv, dim, page, layout):
     b.check(b.run(window=1, max_q=1), window=1)           # a max_q that is too small costs time only
 
 
+def test_many_sequences(dev):
+    """More sequences than a wave's lanes hold at a time, and more parts than a list: decode rows, then a ragged step."""
+    _say("many sequences")
+    rng = np.random.default_rng(4)
+    b = QBatch(dev, [1] * 700, rng.integers(-1, 60, 700).tolist(), 4, 2, 64, seed=1, decode=True)
+    b.check(b.run())
+    n = rng.integers(0, 9, 300)
+    n[::50] = 40
+    b = QBatch(dev, n.tolist(), rng.integers(0, 90, 300).tolist(), 8, 2, 64, seed=2)
+    b.check(b.run())
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_long_contexts(dev, dtype):
     _say(f"long contexts {dtype}")

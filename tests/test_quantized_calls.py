@@ -132,6 +132,13 @@ def test_python_refusals(monkeypatch):
             append(q=None, q_norm=t(64))
         with pytest.raises(TypeError, match="unsupported dtype"):
             append(k=k.half())
+        far = 2 ** 32 + 2                                  # 2 in 32 bits
+        with pytest.raises(ValueError, match="heads of 64"):
+            append(q=t(1, 1, 64).expand(3, far, 64))
+        with pytest.raises(ValueError, match="heads of 64"):
+            append(k=t(1, 1, 64).expand(3, far, 64))
+        with pytest.raises(ValueError, match="pages of"):
+            paged.read_kv(t(4, 1, 16, 64).expand(4, far, 16, 64), t(4, 1, 16, 64).expand(4, far, 16, 64), slots)
         read = lambda kc=kc, vc=vc, slots=slots, **kw: paged.read_kv(kc, vc, slots, **kw)
         with pytest.raises(TypeError, match="unsupported dtype"):
             read(dtype=torch.float16)

@@ -174,10 +174,6 @@ _attention_plans: dict = {}
 _PLAN_CAP = 4096
 
 
-def _layout(t):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
 def _elsewhere(dev: torch.device) -> bool:
     """Whether ``dev`` is a GPU that is not the current one: a launch goes to the current one's queues."""
     return dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device()
@@ -286,8 +282,17 @@ def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, in
                                     or (q_norm is not None and q_norm.requires_grad)
                                     or (k_norm is not None and k_norm.requires_grad)):
         raise _lib.no_gradients("append_kv_")
-    key = (interleaved, eps, *map(_layout, (q, k, v, k_cache, v_cache, k_scales, v_scales, slots, positions, cos_sin, q_out,
-                                            q_norm, k_norm)))
+    key = (interleaved, eps, None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype,
+           k.device, v.shape, v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+           v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+           None if k_scales is None else (k_scales.shape, k_scales.stride(), k_scales.dtype, k_scales.device, v_scales.shape,
+                                          v_scales.stride(), v_scales.dtype, v_scales.device),
+           slots.shape, slots.stride(), slots.dtype, slots.device,
+           None if positions is None else (positions.shape, positions.stride(), positions.dtype, positions.device),
+           None if cos_sin is None else (cos_sin.shape, cos_sin.stride(), cos_sin.dtype, cos_sin.device),
+           None if q_out is None else (q_out.shape, q_out.stride(), q_out.dtype, q_out.device),
+           None if q_norm is None else (q_norm.shape, q_norm.stride(), q_norm.dtype, q_norm.device),
+           None if k_norm is None else (k_norm.shape, k_norm.stride(), k_norm.dtype, k_norm.device))
     plan = _rows_plans.get(key)
     if plan is None:
         code, T, H, HK, D, R, q_st, k_st, v_st, kc_st, vc_st, o_st, max_pos, pages, page = _append_plan(
@@ -302,7 +307,7 @@ def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, in
         plan = _keep(_rows_plans, key, (T, R, args))
     T, R, args = plan
     if q is not None and q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=k.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)     # half of torch.empty's time
     if T == 0:
         return q_out
     args = args.copy()                                     # the addresses, where the library's arguments have them
@@ -412,16 +417,22 @@ def read_kv(k_cache, v_cache, slots: torch.Tensor, dtype: torch.dtype | None = N
                                     or (k_out is not None and k_out.requires_grad)
                                     or (v_out is not None and v_out.requires_grad)):
         raise _lib.no_gradients(who)
-    key = (dtype, *map(_layout, (k_cache, v_cache, k_scales, v_scales, slots, k_out, v_out)))
+    key = (dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(),
+           v_cache.dtype, v_cache.device,
+           None if k_scales is None else (k_scales.shape, k_scales.stride(), k_scales.dtype, k_scales.device, v_scales.shape,
+                                          v_scales.stride(), v_scales.dtype, v_scales.device),
+           slots.shape, slots.stride(), slots.dtype, slots.device,
+           None if k_out is None else (k_out.shape, k_out.stride(), k_out.dtype, k_out.device),
+           None if v_out is None else (v_out.shape, v_out.stride(), v_out.dtype, v_out.device))
     plan = _read_plans.get(key)
     if plan is None:
         plan = _keep(_read_plans, key, _read_plan(k_cache, v_cache, k_scales, v_scales, slots, dtype, k_out, v_out))
     shape, dtype, args = plan
     dev = slots.device
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=dev)
+        k_out = slots.new_empty(shape, dtype=dtype)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=dev)
+        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
     if shape[0]:
         args = args.copy()                                 # the addresses, where the library's arguments have them
         args[2], args[6] = k_cache.data_ptr(), v_cache.data_ptr()
@@ -560,7 +571,7 @@ def paged_attention(q: torch.Tensor, k_cache, v_cache, page_table: torch.Tensor,
                                                             out, lse, max_q, workspace, k_scales, v_scales))
     code, T, B, H, HK, D, q_st, k_st, v_st, s_st, pages, page, table, o_st, window, most, need, default_scale = plan
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if T == 0:
         return out
     stream = _lib.stream_ptr(dev)

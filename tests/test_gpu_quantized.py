@@ -258,6 +258,42 @@ def test_append_in_place_and_strided(dev):
         assert torch.equal(kv[0], paged.read_kv(*one, slots)[0])
 
 
+def test_calls_without_rows(dev):
+    _say("calls without rows")
+    kc, vc = (make_cache(dev, 2, 2, 16, 64) for _ in range(2))
+    none = torch.empty(0, dtype=torch.int64, device=dev)
+    q, k = torch.empty(0, 8, 64, dtype=BF16, device=dev), torch.empty(0, 2, 64, dtype=BF16, device=dev)
+    w = torch.ones(64, dtype=BF16, device=dev)
+    for caches in ((kc, vc), (torch.zeros(2, 2, 16, 64, dtype=BF16, device=dev),) * 2):
+        out = paged.append_kv_(q, k, k, *caches, none, none, paged.rope_table(8, 64, device=dev), q_norm=w, k_norm=w)
+        assert out.shape == q.shape
+        assert all(x.shape == (0, 2, 64) and x.dtype == BF16 for x in paged.read_kv(*caches, none))
+    out = paged.paged_attention(q, kc, vc, torch.empty(0, 1, dtype=torch.int32, device=dev),
+                                torch.empty(0, dtype=torch.int32, device=dev))
+    assert out.shape == q.shape
+    assert bool((_bytes(kc.values) == 0x7F).all()) and bool((_bytes(kc.scales) == 0xFF).all())
+
+
+def test_results_are_contiguous_whatever_the_inputs(dev):
+    """Queries in another order of their dimensions: new results are [T, heads, D] in memory."""
+    _say("permuted inputs")
+    g = torch.Generator(device=dev).manual_seed(8)
+    T, H, HK, D = 33, 6, 3, 64
+    q = torch.randn(H, T, D, generator=g, device=dev).to(BF16).transpose(0, 1)
+    k, v = (torch.randn(HK, T, D, generator=g, device=dev).to(BF16).transpose(0, 1) for _ in range(2))
+    slots, pos, rope = torch.arange(T, device=dev), torch.arange(T, device=dev), paged.rope_table(64, D, device=dev)
+    w = torch.randn(D, generator=g, device=dev).to(BF16)
+    res = []
+    for args in ((q, k, v), (q.contiguous(), k.contiguous(), v.contiguous())):
+        caches = [make_cache(dev, 3, HK, 16, D) for _ in range(2)]
+        out = paged.append_kv_(*args, *caches, slots, pos, rope, q_norm=w, k_norm=w)
+        o = paged.paged_attention(args[0], *caches, torch.arange(3, dtype=torch.int32, device=dev)[None],
+                                  torch.tensor([T], dtype=torch.int32, device=dev), torch.tensor([0, T], dtype=torch.int32, device=dev))
+        assert out.is_contiguous() and o.is_contiguous()
+        res.append((out, o, *paged.read_kv(*caches, slots)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 # ---------------------------------------------------------------------------
 # Read
 # ---------------------------------------------------------------------------

@@ -124,11 +124,13 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* x, float inv
   }
 }
 
-// 1 / sqrt(x) from the instruction's 24 bits, twice refined.
+// 1 / sqrt(x) from the instruction's 24 bits, twice refined; 0 for an infinity, whose product
+// with its 0 is kept out of the refinement.
 __device__ __forceinline__ double rsqrt64(double x) {
   double y = __builtin_amdgcn_rsq(x);
+  const double h = 0.5 * fmin(x, 1.7976931348623157e308);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) y *= 1.5 - 0.5 * x * y * y;
+  for (int i = 0; i < 2; ++i) y *= 1.5 - h * y * y;
   return y;
 }
 // x in fp32, to the odd neighbour where it is none: another rounding, to fewer bits, is then

@@ -230,6 +230,36 @@ def test_append_extremes(dev, dtype, dim):
         assert torch.equal(got, y.float())
 
 
+@pytest.mark.parametrize("dim", [128, 33])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("quant", [True, False])
+def test_norms_of_rows_that_are_not_finite(dev, quant, dtype, dim):
+    """x / sqrt(mean(x^2) + eps): an infinity gives NaN beside zeros, a NaN gives NaN everywhere; other heads as without."""
+    _say(f"norms, not finite {dtype} quant={quant} {dim}")
+    g = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randn(9, 4, dim, generator=g, device=dev).to(dtype)
+    w = (1 + 0.3 * torch.randn(dim, generator=g, device=dev)).to(dtype)
+    slots = torch.arange(9, device=dev)
+
+    def run(x):
+        caches = make_cache(dev, 1, 4, 16, dim), make_cache(dev, 1, 4, 16, dim)
+        if not quant:
+            caches = [torch.zeros(1, 4, 16, dim, dtype=dtype, device=dev) for _ in range(2)]
+        q = paged.append_kv_(x, x, x, *caches, slots, q_norm=w, k_norm=w)
+        return q, paged.read_kv(*caches, slots, FP32 if quant else None)[0]
+
+    plain = run(x)
+    for bad in (math.inf, -math.inf, math.nan):
+        odd = x.clone()
+        odd[3, 1, 2] = bad
+        for got, want in zip(run(odd), plain):
+            want = want.clone()
+            want[3, 1] = math.nan if math.isnan(bad) else 0.0
+            want[3, 1, 2] = math.nan
+            assert torch.equal(got.isnan(), want.isnan())
+            assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
 def test_append_in_place_and_strided(dev):
     _say("append in place, scales with strides of their own")
     g = torch.Generator(device=dev).manual_seed(4)

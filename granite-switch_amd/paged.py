@@ -282,6 +282,7 @@ def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, in
                                     or (q_norm is not None and q_norm.requires_grad)
                                     or (k_norm is not None and k_norm.requires_grad)):
         raise _lib.no_gradients("append_kv_")
+    interleaved, eps = bool(interleaved), float(eps)       # a tensor's value now, not the tensor
     key = (interleaved, eps, None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype,
            k.device, v.shape, v.stride(), v.dtype, v.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,

@@ -260,6 +260,18 @@ def test_norms_of_rows_that_are_not_finite(dev, quant, dtype, dim):
             assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
+def test_eps_by_value(dev):
+    """An eps that is a tensor, or an int, counts as the number it holds at the call."""
+    x = torch.randn(5, 2, 64, generator=torch.Generator(device=dev).manual_seed(8), device=dev)
+    w, slots = torch.ones(64, device=dev), torch.full((5,), -1, device=dev)
+    caches = paged.allocate_cache(1, 2, 16, 64, FP32, dev)
+    run = lambda eps: paged.append_kv_(x, x, x, *caches, slots, q_norm=w, eps=eps)  # noqa: E731
+    eps = torch.tensor(1e-5)
+    assert torch.equal(run(eps), run(1e-5))
+    eps.fill_(2.0)
+    assert torch.equal(run(eps), run(2)) and not torch.equal(run(2.0), run(1e-5))
+
+
 def test_append_in_place_and_strided(dev):
     _say("append in place, scales with strides of their own")
     g = torch.Generator(device=dev).manual_seed(4)

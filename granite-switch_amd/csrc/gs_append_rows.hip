@@ -489,6 +489,8 @@ __global__ __launch_bounds__(256) void read_kv_kernel(ReadArgs r) {
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
+constexpr int64_t kMostBlocks = int64_t(1) << 24;    // of 256 threads: a launch has less than 2^32
+
 // Few tokens: every head of a token at once; many: each thread four heads, its cosines,
 // sines and weights loaded once for them.
 // False: more workgroups than a launch has.
@@ -506,7 +508,7 @@ bool plan_rows(RowsArgs& r, int ve, bool quant, int cus) {
     r.blocks[kind] = n == 0 ? 0 : static_cast<int>((static_cast<int64_t>(a.T) + r.tokens[kind] - 1) / r.tokens[kind]);
     all += r.blocks[kind];
   }
-  if (all >= (int64_t(1) << 31)) return false;
+  if (all >= kMostBlocks) return false;
   r.k_share = addr::spread_share(r.blocks[kKeys], r.blocks[kQueries] + r.blocks[kKeys] + r.blocks[kValues]);
   r.v_share = addr::spread_share(r.blocks[kValues], r.blocks[kQueries] + r.blocks[kValues]);
   r.page_magic = a.num_slots < (int64_t(1) << 31) ? addr::div_magic(a.page_size) : 0;
@@ -652,7 +654,8 @@ int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_ts, int64_t q_hs
   GS_CHECK_ARG(heads >= 0 && kv_heads > 0 && heads <= 4096 && kv_heads <= 4096, "%s: heads=%d kv_heads=%d", who, heads, kv_heads);
   GS_CHECK_ARG(head_dim > 0 && head_dim <= 512, "%s: head_dim=%d (1 .. 512)", who, head_dim);
   GS_CHECK_ARG(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, "%s: rot_dim=%d of head_dim=%d", who, rot_dim, head_dim);
-  GS_CHECK_ARG(page_size > 0 && num_pages > 0, "%s: page_size=%d num_pages=%lld", who, page_size, (long long)num_pages);
+  GS_CHECK_ARG(page_size > 0 && num_pages > 0 && num_pages < (int64_t(1) << 31), "%s: page_size=%d num_pages=%lld", who, page_size,
+               (long long)num_pages);
   GS_CHECK_ARG((q_norm == nullptr && k_norm == nullptr) || norm_dtype == dtype || norm_dtype == GS_DTYPE_FP32,
                "%s: norm_dtype=%d with dtype=%d", who, norm_dtype, dtype);
   GS_CHECK_ARG(eps >= 0.f, "%s: eps=%g", who, static_cast<double>(eps));
@@ -723,7 +726,8 @@ int gs_read_kv(int32_t dtype, int32_t cache_dtype, const void* k_cache, int64_t 
   GS_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t(1) << 31), "%s: num_tokens=%lld", who, (long long)num_tokens);
   GS_CHECK_ARG(kv_heads > 0 && kv_heads <= 4096 && head_dim > 0 && head_dim <= 512, "%s: kv_heads=%d head_dim=%d (1 .. 512)",
                who, kv_heads, head_dim);
-  GS_CHECK_ARG(page_size > 0 && num_pages > 0, "%s: page_size=%d num_pages=%lld", who, page_size, (long long)num_pages);
+  GS_CHECK_ARG(page_size > 0 && num_pages > 0 && num_pages < (int64_t(1) << 31), "%s: page_size=%d num_pages=%lld", who, page_size,
+               (long long)num_pages);
   if (num_tokens == 0) return GS_OK;
   const bool quant = cache_dtype == GS_DTYPE_E4M3;
   if (num_tokens == 1) ko_ts = vo_ts = 0;
@@ -752,7 +756,9 @@ int gs_read_kv(int32_t dtype, int32_t cache_dtype, const void* k_cache, int64_t 
   r.T = static_cast<int>(num_tokens);
   r.HK = kv_heads; r.D = head_dim;
   plan_read(r, vec ? ve : 1);
-  const dim3 grid(static_cast<unsigned>((num_tokens + r.tokens - 1) / r.tokens), 2);
+  const int64_t blocks = (num_tokens + r.tokens - 1) / r.tokens;
+  GS_CHECK_ARG(blocks < kMostBlocks, "%s: num_tokens=%lld with %d heads of %d are too many", who, (long long)num_tokens, kv_heads, head_dim);
+  const dim3 grid(static_cast<unsigned>(blocks), 2);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, r); };
   if (quant) {

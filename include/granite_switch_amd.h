@@ -562,7 +562,9 @@ int gs_append_kv(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q
  * head before the rotation, x rsqrt(mean(x^2) + eps) w over the head's columns
  * (q_norm, k_norm [head_dim] of norm_dtype -- dtype or fp32 -- or NULL: none),
  * and with a cache of dtype or quantised (scales: NULL unless it is).  In fp32
- * throughout, rounded once.  The rest as gs_append_kv. */
+ * throughout -- keys on their way into a quantised cache in fp64 -- and rounded
+ * once.  num_pages < 2^31, and less than 2^24 workgroups of 256 threads (refused
+ * otherwise: some 10^8 tokens).  The rest as gs_append_kv. */
 int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                         int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
                         int64_t v_head_stride, int64_t num_tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
@@ -578,7 +580,8 @@ int gs_append_kv_normed(int32_t dtype, const void* q, int64_t q_token_stride, in
 /* Rows of a cache by their slots: k_out and v_out [num_tokens, kv_heads,
  * head_dim] of dtype, with token and head strides; a slot outside the pool
  * gives zeros.  A quantised row's x = y 2^e is exact in either dtype from 2^-126
- * on, a cache that is not quantised has dtype.  A slot may come more than once. */
+ * on, a cache that is not quantised has dtype.  A slot may come more than once.
+ * num_pages < 2^31, and less than 2^24 workgroups of 256 threads. */
 int gs_read_kv(int32_t dtype, int32_t cache_dtype, const void* k_cache, int64_t kc_page_stride, int64_t kc_head_stride,
                int64_t kc_row_stride, const void* v_cache, int64_t vc_page_stride, int64_t vc_head_stride,
                int64_t vc_row_stride, const uint8_t* k_scales, int64_t ks_page_stride, int64_t ks_head_stride,

@@ -54,6 +54,13 @@ def test_append_arguments(change):
 def test_more_rows_than_a_launch_has():
     _refused("gs_append_kv_normed", APPEND, dict(num_tokens=2 ** 31 - 1, q_ts=4096, heads=32, head_dim=512, q_hs=512, k_hs=512,
                                                  v_hs=512, o_hs=512))
+    _refused("gs_append_kv_normed", APPEND, dict(num_tokens=2 ** 27))         # 2.5 x 2^23 workgroups of 256 threads
+    _refused("gs_read_kv", READ, dict(num_tokens=2 ** 25, kv_heads=16, ko_ts=2048, vo_ts=2048))
+
+
+def test_more_pages_than_an_id_counts():
+    for name, base in (("gs_append_kv_normed", APPEND), ("gs_read_kv", READ)):
+        _refused(name, base, dict(num_pages=2 ** 31))
 
 
 @pytest.mark.parametrize("change", [

@@ -5,7 +5,8 @@
 // two 2^e, x = y 2^e, with e the least integer that keeps the row's largest finite
 // magnitude within 448 2^e (e >= -126): the product with 2^-e is exact, so a value is
 // rounded once, by at most 2^-4 of itself down to 2^-6 2^e, and any factor between two
-// powers of two would leave it the same relative error.  e + 127 is the scale's byte.
+// powers of two would leave it the same relative error.  e + 127 is the scale's byte.  A
+// finite value stays finite (kMostHeld).
 //
 // gs_append_kv_normed: x rsqrt(mean(x^2) + eps) w over a head's columns, rotation, and for
 // keys and values the row's exponent and its e4m3 values.  A head's columns are held by 2^n
@@ -82,6 +83,14 @@ __device__ __forceinline__ T over_lanes(T x, int lanes, const F& f) {
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e+38f; }
+
+// The largest magnitude that a row holds: 240 2^120 = 1.875 2^127.  The next e4m3 value times
+// that power of two is 2^128, which neither type has; a larger x is kept as this one, off by
+// less than 2^-4 of itself.
+constexpr float kMostHeld = 0x1.ep127f;
+__device__ __forceinline__ float held_finite(float x) {
+  return !is_finite(x) ? __uint_as_float(0x7fc00000u) : fabsf(x) > kMostHeld ? copysignf(kMostHeld, x) : x;
+}
 
 // The partners x0 and x1 of a unit, turned: VE columns each of half-split pairs, or
 // VE / 2 side-by-side pairs each.
@@ -352,13 +361,13 @@ __device__ __forceinline__ void append_rows(const RowsArgs& r, int block) {
           return over_lanes(m, lanes, [](float x, float y) { return fmaxf(x, y); });
         };
         float m = largest();
-        if (!is_finite(m)) {                         // infinities become NaN, which e4m3 has
+        if (!(m <= kMostHeld)) {                     // infinities become NaN, which e4m3 has
 #pragma unroll
           for (int n = 0; n < NU; ++n)
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-              f0[n][i] = is_finite(f0[n][i]) ? f0[n][i] : __uint_as_float(0x7fc00000u);
-              f1[n][i] = is_finite(f1[n][i]) ? f1[n][i] : __uint_as_float(0x7fc00000u);
+              f0[n][i] = held_finite(f0[n][i]);
+              f1[n][i] = held_finite(f1[n][i]);
             }
           m = largest();
         }

@@ -58,7 +58,8 @@ class QuantizedCache(NamedTuple):
     ``append_kv_`` takes the smallest power of two (2^-126 at least) that keeps a row's
     largest magnitude within 448, the largest e4m3 value, and rounds to nearest, ties to
     even: a value is off by at most 2^-4 of itself, or 2^-10 of its scale where that is
-    more.  What is not finite becomes NaN, and the row's other values are kept.
+    more, and a finite one stays finite (magnitudes past 1.875 2^127 are kept as that).
+    What is not finite becomes NaN, and the row's other values are kept.
     """
 
     values: torch.Tensor

@@ -554,9 +554,10 @@ int gs_append_kv(int32_t dtype, const void* q, int64_t q_token_stride, int64_t q
  * value of one token -- as e4m3 values y, one byte each (sign, 4 bits of
  * exponent, 3 of mantissa, no infinities), and a scale 2^e, x = y 2^e, whose
  * byte is e + 127.  Storing takes the least e >= -126 with |x| <= 448 2^e for
- * the row's finite x, and rounds x 2^-e to nearest, ties to even; what is not
- * finite becomes NaN.  The scales are [num_pages, kv_heads, page_size] bytes
- * with page and head strides, a head's scales of a page side by side.
+ * the row's finite x, and rounds x 2^-e to nearest, ties to even; magnitudes past
+ * 240 2^120 (1.875 2^127) are kept as that, what is not finite becomes NaN.  The
+ * scales are [num_pages, kv_heads, page_size] bytes with page and head strides,
+ * a head's scales of a page side by side.
  *
  * gs_append_kv_normed: gs_append_kv with the norms of queries and keys for each
  * head before the rotation, x rsqrt(mean(x^2) + eps) w over the head's columns

@@ -1,0 +1,54 @@
+"""GPU parity of the quantised paged cache at its edges: the ends of the range, keys next to a border between e4m3
+values, scales with strides of their own, rows of values that are all tiny, how a ragged call's work is cut.
+
+References and tolerances are those of test_gpu_quantized.py, whose helpers these tests use; what a test adds to them
+stands beside it.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from granite_switch_amd import paged
+from test_gpu_quantized import BF16, FP32, _say, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Append and read
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [128, 33])
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("turned", [False, True])
+def test_the_largest_rows_stay_finite(dev, dtype, dim, turned):
+    """A finite row reads back finite, within 2^-4, up to the type's largest value: 256 2^120 is no number of either type."""
+    _say(f"the largest rows {dtype} {dim} turned={turned}")
+    big = torch.finfo(dtype).max
+    tops = [big, -big, 1.9375 * 2.0 ** 127, 1.875 * 2.0 ** 127, 1.75 * 2.0 ** 127, -1.90625 * 2.0 ** 127]
+    rows = [torch.full((dim,), t, dtype=torch.float64) for t in tops]
+    rows += [torch.linspace(-1, 1, dim, dtype=torch.float64) * abs(t) for t in tops]
+    k = torch.stack(rows).to(dtype)[:, None].to(dev)
+    assert bool(k.isfinite().all())
+    T = k.shape[0]
+    slots, caches = torch.arange(T, device=dev), [make_cache(dev, 2, 1, 16, dim) for _ in range(2)]
+    # position 0 turns by nothing, through the keys' own arithmetic
+    turn = (torch.zeros(T, dtype=torch.int64, device=dev), paged.rope_table(4, dim // 2 * 2, device=dev)) if turned else ()
+    paged.append_kv_(None, k, -k, *caches, slots, *turn)
+    for to in (BF16, FP32):
+        for got, want in zip(paged.read_kv(*caches, slots, to), (k, -k)):
+            off = (got.double() - want.double()).abs()
+            assert int((~got.isfinite()).sum()) == 0
+            assert bool((off <= want.double().abs() * 2.0 ** -4 + 2.0 ** 110).all())
+    # beside a value that is not finite, too
+    for bad in (math.nan, math.inf):
+        odd = k.clone()
+        odd[:, 0, 1] = bad
+        paged.append_kv_(None, odd, odd, *caches, slots)
+        got = paged.read_kv(*caches, slots)[0]
+        assert bool(got[:, 0, 1].isnan().all())
+        got[:, 0, 1] = 0
+        assert int((~got.isfinite()).sum()) == 0

@@ -356,10 +356,12 @@ GS_HD int row_part_units(int64_t U, int HK, int wgs) {
   const int64_t u = (U * HK + wgs - 1) / wgs;
   return u < 1 ? 1 : static_cast<int>(u);
 }
-// ... beside a quantised cache's chunk parts at least so many: shorter ones held places that
-// chunk parts wait for, with more start than work (8 chunks of 3 .. 64 rows over up to 16384
-// keys: 65.2 us without, 59.7 with 8 or 16).
-constexpr int kRaggedRowUnits = 8;
+// ... and at least so many in a ragged launch over a quantised cache.  Beside chunk parts
+// shorter ones held places that those wait for, with more start than work (8 chunks of 3 .. 64
+// rows over up to 16384 keys: 65.2 us without, 59.7 with 8 or 16).  Without any, 3 rows over 8192
+// keys take 20.7 us with 4, 21.5 with 1 and 23.3 with 8 (8 heads), 20.3, 26.7 and 23.1 (one
+// head, whose 64 parts cost their join more than they save).
+GS_HD int row_part_least(bool ragged, bool quantised, bool chunks) { return !ragged || !quantised ? 1 : chunks ? 8 : 4; }
 constexpr int kMostParts = 512;      // of an item
 GS_HD int row_parts(int units, int most, uint32_t magic) {
   uint32_t q, r;

@@ -117,8 +117,9 @@ void model_attention(PagedModel& m, const PagedArgs& a) {
   std::vector<char>& rows = m.rows;
   int64_t U = 0;
   for (int s = 0; s < a.B; ++s) U += addr::paged_seq_units(seq_of_form<false>(a, s), a.G, a.window, kUnit);
-  int most = addr::row_part_units(U, a.HK, a.row_wgs);
-  if (E4M3 && a.row_limit != INT32_MAX) most = std::max(most, addr::kRaggedRowUnits);
+  bool chunks = false;
+  for (int s = 0; s < a.B; ++s) chunks |= seq_of_form<true>(a, s).n > 0;
+  const int most = std::max(addr::row_part_units(U, a.HK, a.row_wgs), addr::row_part_least(a.row_limit != INT32_MAX, E4M3, chunks));
   const uint32_t magic = addr::div_magic(most);
   int64_t parts = 0, slot = 0;
   for (int s = 0; s < a.B && !m.bad; ++s) {

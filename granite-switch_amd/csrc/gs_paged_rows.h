@@ -267,7 +267,10 @@ struct RowOrder {
     uint64_t U = 0;
     each_seq<false>(a, q, [&](int, const addr::PagedSeq& sq) { U += addr::paged_seq_units(sq, a.G, a.window, kUnit); });
     most = addr::row_part_units(static_cast<int64_t>(of_lane(lane_sums(U), 63)), a.HK, a.row_wgs);
-    if (a.ks != nullptr && a.row_limit != INT32_MAX) most = max(most, addr::kRaggedRowUnits);
+    const bool ragged = a.row_limit != INT32_MAX;
+    bool chunks = false;
+    if (ragged && a.ks != nullptr) each_seq<true>(a, q, [&](int, const addr::PagedSeq&) { chunks = true; });
+    most = max(most, addr::row_part_least(ragged, a.ks != nullptr, __any(chunks)));
     magic = addr::div_magic(most);
     order = ClassOrder{0, 0, a.row_parts >= 65536};
     uint64_t sl = 0;

@@ -12,8 +12,8 @@ import math
 import pytest
 import torch
 
-from granite_switch_amd import paged
-from test_gpu_quantized import BF16, FP32, _say, make_cache
+from granite_switch_amd import _lib, paged
+from test_gpu_quantized import BF16, FP32, QBatch, _say, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,39 @@ def test_the_largest_rows_stay_finite(dev, dtype, dim, turned):
         assert bool(got[:, 0, 1].isnan().all())
         got[:, 0, 1] = 0
         assert int((~got.isfinite()).sum()) == 0
+
+
+# ---------------------------------------------------------------------------
+# How a call's work is cut
+# ---------------------------------------------------------------------------
+def _row_parts(b, **kw):
+    """Partial results of the row form that a call leaves for each key/value head, from its workspace."""
+    ws = torch.zeros(paged.workspace_bytes(b.dtype, b.heads, b.kv, b.dim, ragged=True), dtype=torch.uint8, device=b.q.device)
+    ws[_lib.GS_PAGED_HEAD_BYTES:] = 0xA5
+    b.check(b.run(workspace=ws, **kw))
+    cus = torch.cuda.get_device_properties(b.q.device).multi_processor_count
+    rows, width = min(16, max(n for n in b.n if n * b.heads // b.kv <= 16) * b.heads // b.kv), 64 if b.dim <= 64 else 128
+    most = (2 * 2 * cus + b.kv - 1) // b.kv + 1           # of a head
+    left = ws[_lib.GS_PAGED_HEAD_BYTES:].view(torch.int32)[: b.kv * most * (16 * width + 32)]
+    sums = left.view(b.kv, most, 16 * width + 32)[:, :, : rows * b.dim]
+    found = (sums != -0x5A5A5A5B).any(-1).sum(1)
+    assert int(found.min()) == int(found.max())
+    return int(found[0])
+
+
+@pytest.mark.parametrize("kv,n,cached", [(8, [3], [8189]), (8, [3, 1, 2], [4100, 9000, 16000]), (1, [5], [8187])])
+def test_short_rows_without_chunks_fill_the_card(dev, kv, n, cached):
+    """A batch that has row parts only is cut for the workgroups that there are, down to 4 units of 128 keys a part, also
+    where the caller does not know max_q."""
+    _say(f"row parts of a ragged call, {kv} heads, {n} over {cached}")
+    b = QBatch(dev, n, cached, kv, kv, 128, seed=kv)
+    known, unknown = _row_parts(b, max_q=max(n)), _row_parts(b)
+    units = sum(-(-x // 128) for x in b.len)
+    assert known > 8 and unknown >= min(known // 2, units // 4), (known, unknown)
+
+
+def test_short_rows_beside_chunks(dev):
+    """Beside chunk parts a row part has 8 units of 128 keys at least."""
+    _say("row parts beside chunk parts")
+    b = QBatch(dev, [3, 70], [8189, 500], 8, 8, 128, seed=1)
+    assert 2 <= _row_parts(b) <= 8192 // (8 * 128)

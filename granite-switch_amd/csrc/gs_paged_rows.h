@@ -93,6 +93,11 @@ struct VVec<4> {
 
 // The power of two of byte `at` of a word of scales; 0 for code 0.
 __device__ __forceinline__ float scale_of(uint32_t w, int at) { return __uint_as_float(((w >> (8 * at)) & 255u) << 23); }
+// The bytes of four scales that are less than 2^-63, as ones: those below 64.
+__device__ __forceinline__ uint32_t tiny_bytes(uint32_t w) {
+  const uint32_t t = ~(w | (w << 1)) & 0x80808080u;  // neither of a byte's upper two bits
+  return (t - (t >> 7)) | t;
+}
 
 // One 32-key (16-key, fp32) block's keys and values in a wave's registers.
 struct NoScales {};
@@ -625,10 +630,11 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
           for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
             for (int w = 0; w < F::kVW * F::kCS / 4; ++w) x.v[i][n][w] = 0;
-          if constexpr (E4M3) {                      // nor is 0 * inf: its scale is zero, too
-            const int at = (BF16 ? i : v_in + i);
-            x.s.v[0] = at < 4 ? x.s.v[0] & ~(255u << (8 * (at & 3))) : x.s.v[0];
-            x.s.v[1] = at < 4 ? x.s.v[1] : x.s.v[1] & ~(255u << (8 * (at & 3)));
+          if constexpr (E4M3) {                      // nor is 0 * inf: its scale is one
+            const int at = (BF16 ? i : v_in + i), sh = 8 * (at & 3);
+            const uint32_t one = (x.s.v[at >> 2] & ~(255u << sh)) | (127u << sh);
+            x.s.v[0] = at < 4 ? one : x.s.v[0];
+            x.s.v[1] = at < 4 ? x.s.v[1] : one;
           }
         }
       }
@@ -654,33 +660,56 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
     for (int i = 0; i < F::kKeys; ++i) {
       p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
       lsum += p[i];
-      if constexpr (E4M3) p[i] *= scale_of(BF16 ? x.s.v[i >> 2] : v_in == 0 ? x.s.v[0] : x.s.v[1], i & 3);
+      if constexpr (E4M3 && !BF16) p[i] *= scale_of(v_in == 0 ? x.s.v[0] : x.s.v[1], i & 3);
     }
     if constexpr (BF16 && E4M3) {
       // The values' scales are the probabilities', which then are rounded as below: a column's
       // bytes of two keys are brought together before they become bf16.
-      u32x4 pf;
+      const auto add = [&](u32x2 scales, float by, const auto& into) {
+        float w8[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) w8[i] = p[i] * (scale_of(scales[i >> 2], i & 3) * by);
+        u32x4 pf;
 #pragma unroll
-      for (int n = 0; n < F::kVN; ++n)
+        for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(w8[2 * i], w8[2 * i + 1]);
 #pragma unroll
-        for (int w = 0; w < F::kVW / 4; ++w)
+        for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
-          for (int up = 0; up < 2; ++up) {
-            u32x4 vf[2];
+          for (int w = 0; w < F::kVW / 4; ++w)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t y = __builtin_amdgcn_perm(x.v[2 * i + 1][n][w], x.v[2 * i][n][w], up ? 0x07030602u : 0x05010400u);
-              vf[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, false));
-              vf[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, true));
+            for (int up = 0; up < 2; ++up) {
+              u32x4 vf[2];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t y = __builtin_amdgcn_perm(x.v[2 * i + 1][n][w], x.v[2 * i][n][w], up ? 0x07030602u : 0x05010400u);
+                vf[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, false));
+                vf[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, true));
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e) into(o[n * F::kVW + 4 * w + 2 * up + e], vf[e], pf);
             }
+      };
+      // A probability times 2^-126, the least scale, has no bf16 digits left: scales below 2^-63
+      // count 2^96 times over, in sums of their own.
+      const u32x2 less = {tiny_bytes(x.s.v[0]), tiny_bytes(x.s.v[1])};
+      const bool tiny = __any((less[0] | less[1]) != 0);
+      u32x2 scales = x.s.v;
+      if (tiny) scales &= ~less;
+      add(scales, 1.f, [](f32x4& sum, u32x4 vf, u32x4 pf) { sum = mfma16_bf16(vf, pf, sum); });
+      if (tiny) {
+        // converted again, or all of them would be kept from the sums before
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int c = n * F::kVW + 4 * w + 2 * up + e;
-              o[c] = mfma16_bf16(vf[e], pf, o[c]);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int n = 0; n < F::kVN; ++n)
+#pragma unroll
+            for (int w = 0; w < F::kVW / 4; ++w) {
+              uint32_t y = x.v[i][n][w];
+              asm("" : "+v"(y));
+              x.v[i][n][w] = y;
             }
-          }
+        add(x.s.v & less, 0x1p96f, [](f32x4& sum, u32x4 vf, u32x4 pf) { sum += mfma16_bf16(vf, pf, f32x4{0, 0, 0, 0}) * 0x1p-96f; });
+      }
     } else if constexpr (BF16) {
       // Probabilities enter the product in bf16, their total stays in fp32.  Each is off by
       // up to 2^-8 of itself, as the values and the result are; with values of both signs a

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from granite_switch_amd import _lib, paged
-from test_gpu_quantized import BF16, FP32, QBatch, _say, make_cache
+from test_gpu_quantized import BF16, E4M3, E8M0, FP32, QBatch, _bytes, _say, held, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,57 @@ def test_short_rows_beside_chunks(dev):
     _say("row parts beside chunk parts")
     b = QBatch(dev, [3, 70], [8189, 500], 8, 8, 128, seed=1)
     assert 2 <= _row_parts(b) <= 8192 // (8 * 128)
+
+
+# ---------------------------------------------------------------------------
+# Attention
+# ---------------------------------------------------------------------------
+def _against_exact(b, out, rounding):
+    """``out`` against float64, within ``rounding`` beside what fp32 sums leave, all relative to A = sum_j p_j |v_j|.
+
+    Scores of D products are off by ds <= (D + 4) u scale sum |q||k|, a probability so by a factor within 1 +- 2 ds twice
+    over, sums of L terms by L u; bf16 subnormals by 2^-134 each.
+    """
+    G, t, scale = b.heads // b.kv, 0, b.dim ** -0.5
+    for n, L, k, v in zip(b.n, b.len, *b.rows):
+        if n and L > 0:
+            q = b.q[t:t + n].double().unflatten(1, (b.kv, G)).permute(1, 0, 2, 3).reshape(b.kv, n * G, b.dim)
+            k, v = k.double().transpose(0, 1).contiguous(), v.double().transpose(0, 1).contiguous()        # [kv, L, dim]
+            kt = k.transpose(1, 2).contiguous()
+            hide = torch.arange(L, device=q.device)[None] > (L - n + torch.arange(n, device=q.device)).repeat_interleave(G)[:, None]
+            sc = (torch.bmm(q, kt) * scale).masked_fill(hide, -math.inf)
+            ds = ((b.dim + 4) * 2.0 ** -24 * scale * torch.bmm(q.abs(), kt.abs())).masked_fill(hide, 0).amax(-1, keepdim=True)
+            p = torch.softmax(sc, -1).nan_to_num(0.0)
+            ref, A = torch.bmm(p, v), torch.bmm(p, v.abs())
+            got = out[t:t + n].double().unflatten(1, (b.kv, G)).permute(1, 0, 2, 3).reshape(b.kv, n * G, b.dim)
+            tol = (4 * ds + (L + 64) * 2.0 ** -24 + rounding) * A + 2.0 ** -133
+            worst = float(((got - ref).abs() / tol).nan_to_num(9e9).max())
+            assert worst <= 1, (n, L)
+        t += n
+
+
+def _put_value_scales(b, codes):
+    """Gives every value row of sequence s the scale bytes codes(s, number of tokens) [tokens, kv]."""
+    for s, L in enumerate(b.len):
+        j = torch.arange(max(L, 0), device=b.q.device)
+        at = (b.table[s].long()[j // b.page], slice(None), j % b.page)
+        code = codes(s, max(L, 0)).to(torch.uint8)
+        _bytes(b.v.scales)[at] = code
+        b.rows[1][s] = held(_bytes(b.v.values)[at].view(E4M3), code.view(E8M0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("decode", [True, False])
+def test_sequences_of_tiny_or_large_values(dev, dtype, dim, decode):
+    """One power of two for all of a sequence's values, from the least that append writes; then some of each in one."""
+    _say(f"tiny and large values {dtype} {dim} decode={decode}")
+    n = [1] * 7 if decode else [5, 1, 33, 20, 9, 70, 2]
+    b = QBatch(dev, n, [40, 100, 3, 0, 64, 200, 300], 4, 2, dim, dtype=dtype, seed=dim, decode=decode, spread=0.0)
+    g = torch.Generator(device=dev).manual_seed(1)
+    rounding = 2.0 ** -7 * 1.01 if dtype == BF16 else 0.0    # a probability's and the result's
+    for code in (1, 2, 6, 40, 63, 64, 130, 220):
+        _put_value_scales(b, lambda s, L: torch.full((L, b.kv), code, device=dev))
+        _against_exact(b, b.run(), rounding)
+    _put_value_scales(b, lambda s, L: torch.randint(1, 100, (L, b.kv), generator=g, device=dev))
+    _against_exact(b, b.run(), rounding)

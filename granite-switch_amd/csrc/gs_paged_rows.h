@@ -663,15 +663,20 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
       if constexpr (E4M3 && !BF16) p[i] *= scale_of(v_in == 0 ? x.s.v[0] : x.s.v[1], i & 3);
     }
     if constexpr (BF16 && E4M3) {
-      // The values' scales are the probabilities', which then are rounded as below: a column's
+      // The values' scales are the probabilities', which enter the product as two bf16 numbers,
+      // off by 2^-16 of themselves: the products are 6% of the kernel's cycles, and one number
+      // (2^-8) took 67.5 us where this takes 68.3 (256 sequences of 16 .. 2047 keys).  A column's
       // bytes of two keys are brought together before they become bf16.
       const auto add = [&](u32x2 scales, float by, const auto& into) {
         float w8[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w8[i] = p[i] * (scale_of(scales[i >> 2], i & 3) * by);
-        u32x4 pf;
+        u32x4 hi, lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pf[i] = pack_bf16x2(w8[2 * i], w8[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+          hi[i] = pack_bf16x2(w8[2 * i], w8[2 * i + 1]);
+          lo[i] = pack_bf16x2(w8[2 * i] - __uint_as_float(hi[i] << 16), w8[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
+        }
 #pragma unroll
         for (int n = 0; n < F::kVN; ++n)
 #pragma unroll
@@ -686,7 +691,7 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
                 vf[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, true));
               }
 #pragma unroll
-              for (int e = 0; e < 2; ++e) into(o[n * F::kVW + 4 * w + 2 * up + e], vf[e], pf);
+              for (int e = 0; e < 2; ++e) into(o[n * F::kVW + 4 * w + 2 * up + e], vf[e], hi, lo);
             }
       };
       // A probability times 2^-126, the least scale, has no bf16 digits left: scales below 2^-63
@@ -695,7 +700,7 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
       const bool tiny = __any((less[0] | less[1]) != 0);
       u32x2 scales = x.s.v;
       if (tiny) scales &= ~less;
-      add(scales, 1.f, [](f32x4& sum, u32x4 vf, u32x4 pf) { sum = mfma16_bf16(vf, pf, sum); });
+      add(scales, 1.f, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) { sum = mfma16_bf16(vf, hi, mfma16_bf16(vf, lo, sum)); });
       if (tiny) {
         // converted again, or all of them would be kept from the sums before
 #pragma unroll
@@ -708,7 +713,9 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
               asm("" : "+v"(y));
               x.v[i][n][w] = y;
             }
-        add(x.s.v & less, 0x1p96f, [](f32x4& sum, u32x4 vf, u32x4 pf) { sum += mfma16_bf16(vf, pf, f32x4{0, 0, 0, 0}) * 0x1p-96f; });
+        add(x.s.v & less, 0x1p96f, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) {
+          sum += mfma16_bf16(vf, hi, mfma16_bf16(vf, lo, f32x4{0, 0, 0, 0})) * 0x1p-96f;
+        });
       }
     } else if constexpr (BF16) {
       // Probabilities enter the product in bf16, their total stays in fp32.  Each is off by

@@ -93,8 +93,9 @@ def test_short_rows_beside_chunks(dev):
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
-def _against_exact(b, out, rounding):
-    """``out`` against float64, within ``rounding`` beside what fp32 sums leave, all relative to A = sum_j p_j |v_j|.
+def _against_exact(b, out, rounding, of_result=0.0):
+    """``out`` against float64, within ``rounding`` beside what fp32 sums leave, all relative to A = sum_j p_j |v_j|, and
+    within ``of_result`` relative to the result.
 
     Scores of D products are off by ds <= (D + 4) u scale sum |q||k|, a probability so by a factor within 1 +- 2 ds twice
     over, sums of L terms by L u; bf16 subnormals by 2^-134 each.
@@ -111,7 +112,7 @@ def _against_exact(b, out, rounding):
             p = torch.softmax(sc, -1).nan_to_num(0.0)
             ref, A = torch.bmm(p, v), torch.bmm(p, v.abs())
             got = out[t:t + n].double().unflatten(1, (b.kv, G)).permute(1, 0, 2, 3).reshape(b.kv, n * G, b.dim)
-            tol = (4 * ds + (L + 64) * 2.0 ** -24 + rounding) * A + 2.0 ** -133
+            tol = (4 * ds + (L + 64) * 2.0 ** -24 + rounding) * A + of_result * ref.abs() + 2.0 ** -133
             worst = float(((got - ref).abs() / tol).nan_to_num(9e9).max())
             assert worst <= 1, (n, L)
         t += n
@@ -142,3 +143,12 @@ def test_sequences_of_tiny_or_large_values(dev, dtype, dim, decode):
         _against_exact(b, b.run(), rounding)
     _put_value_scales(b, lambda s, L: torch.randint(1, 100, (L, b.kv), generator=g, device=dev))
     _against_exact(b, b.run(), rounding)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_row_form_rounds_its_result_only(dev, dim):
+    """Probabilities enter the row form's products as two bf16 numbers: off by 2^-16 of themselves, not 2^-8."""
+    _say(f"probabilities of the row form, {dim}")
+    for n, decode in (([1] * 6, True), ([3, 1, 2, 4, 1, 2], False)):
+        b = QBatch(dev, n, [40, 100, 3, 700, 64, 2000], 4, 2, dim, seed=dim, decode=decode)
+        _against_exact(b, b.run(), 2.0 ** -16 * 1.01, 2.0 ** -8 * 1.01)

@@ -91,7 +91,8 @@ struct VVec<4> {
   typedef uint32_t T __attribute__((ext_vector_type(1)));
 };
 
-// The power of two of byte `at` of a word of scales; 0 for code 0.
+// The power of two of byte `at` of a word of scales; for code 0 a float without exponent, which
+// conversions take for 2^-127 and products for 0.
 __device__ __forceinline__ float scale_of(uint32_t w, int at) { return __uint_as_float(((w >> (8 * at)) & 255u) << 23); }
 // The bytes of four scales that are less than 2^-63, as ones: those below 64.
 __device__ __forceinline__ uint32_t tiny_bytes(uint32_t w) {
@@ -660,17 +661,14 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
     for (int i = 0; i < F::kKeys; ++i) {
       p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
       lsum += p[i];
-      if constexpr (E4M3 && !BF16) p[i] *= scale_of(v_in == 0 ? x.s.v[0] : x.s.v[1], i & 3);
+      if constexpr (E4M3 && !BF16) p[i] *= e8m0_scale(((v_in == 0 ? x.s.v[0] : x.s.v[1]) >> (8 * i)) & 255u);
     }
     if constexpr (BF16 && E4M3) {
       // The values' scales are the probabilities', which enter the product as two bf16 numbers,
       // off by 2^-16 of themselves: the products are 6% of the kernel's cycles, and one number
       // (2^-8) took 67.5 us where this takes 68.3 (256 sequences of 16 .. 2047 keys).  A column's
       // bytes of two keys are brought together before they become bf16.
-      const auto add = [&](u32x2 scales, float by, const auto& into) {
-        float w8[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w8[i] = p[i] * (scale_of(scales[i >> 2], i & 3) * by);
+      const auto add = [&](const float (&w8)[8], const auto& into) {
         u32x4 hi, lo;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -700,7 +698,10 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
       const bool tiny = __any((less[0] | less[1]) != 0);
       u32x2 scales = x.s.v;
       if (tiny) scales &= ~less;
-      add(scales, 1.f, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) { sum = mfma16_bf16(vf, hi, mfma16_bf16(vf, lo, sum)); });
+      float w8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w8[i] = p[i] * scale_of(scales[i >> 2], i & 3);
+      add(w8, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) { sum = mfma16_bf16(vf, hi, mfma16_bf16(vf, lo, sum)); });
       if (tiny) {
         // converted again, or all of them would be kept from the sums before
 #pragma unroll
@@ -713,7 +714,12 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
               asm("" : "+v"(y));
               x.v[i][n][w] = y;
             }
-        add(x.s.v & less, 0x1p96f, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t code = (x.s.v[i >> 2] >> (8 * (i & 3))) & 255u;
+          w8[i] = code < 64 ? p[i] * __uint_as_float((code + 96) << 23) : 0.f;
+        }
+        add(w8, [](f32x4& sum, u32x4 vf, u32x4 hi, u32x4 lo) {
           sum += mfma16_bf16(vf, hi, mfma16_bf16(vf, lo, f32x4{0, 0, 0, 0})) * 0x1p-96f;
         });
       }

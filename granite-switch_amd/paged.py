@@ -59,7 +59,9 @@ class QuantizedCache(NamedTuple):
     largest magnitude within 448, the largest e4m3 value, and rounds to nearest, ties to
     even: a value is off by at most 2^-4 of itself, or 2^-10 of its scale where that is
     more, and a finite one stays finite (magnitudes past 1.875 2^127 are kept as that).
-    What is not finite becomes NaN, and the row's other values are kept.
+    What is not finite becomes NaN, and the row's other values are kept.  A scale's byte
+    is the power of two's exponent + 127: 0 is 2^-127 and 255 NaN, and ``append_kv_``
+    writes neither.
     """
 
     values: torch.Tensor

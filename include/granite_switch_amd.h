@@ -638,9 +638,9 @@ int gs_paged_attention(int32_t dtype, const void* q, int64_t q_token_stride, int
                        float* lse, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* gs_paged_attention over a quantised cache: k and v rows are y 2^e of the
- * cache's e4m3 values and scales, taken as they stand.  A scale byte of 0 counts as
- * zero for values; one of 255 (NaN), or a value that is NaN, is as a value that is not
- * finite above.
+ * cache's e4m3 values and scales, taken as they stand: a scale byte of 0 is 2^-127 (append
+ * writes none below 1), one of 255 is NaN.  A row with that scale, or a value that is NaN,
+ * is as one that is not finite above.
  * head_dim a multiple of 16 up to 256; caches 16-byte aligned with strides that
  * are multiples of 16, scales 8-byte aligned with strides that are multiples of
  * 8.  dtype is that of q and out; the workspace is gs_paged_attention's, and

@@ -54,6 +54,30 @@ def test_the_largest_rows_stay_finite(dev, dtype, dim, turned):
         assert int((~got.isfinite()).sum()) == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim", [128, 33])
+def test_read_of_every_scale(dev, dtype, dim):
+    """Every scale byte times every value: x = y 2^e to the nearest, NaN for 255, an infinity where the type ends."""
+    _say(f"read of every scale {dtype} {dim}")
+    kc, vc = (make_cache(dev, 16, 1, 16, dim) for _ in range(2))
+    for c, first in ((kc, 0), (vc, 128)):
+        _bytes(c.scales).copy_(torch.arange(256, device=dev).view(16, 1, 16))
+        _bytes(c.values).copy_((first + torch.arange(dim, device=dev) * 5) % 256)
+    got = paged.read_kv(kc, vc, torch.arange(256, device=dev), dtype)
+    for x, c in zip(got, (kc, vc)):
+        want = held(c.values.transpose(1, 2).flatten(0, 1), c.scales.transpose(1, 2).flatten(0, 1))
+        want[255] = math.nan
+        least = 2.0 ** -126                                # below it the conversion may leave nothing
+        x = x.double()
+        assert torch.equal(x.isnan(), want.isnan())
+        ends = want.abs() > torch.finfo(dtype).max
+        assert bool((x[ends].abs() == math.inf).all()) and torch.equal(x[ends].sign(), want[ends].sign())
+        exact = ~want.isnan() & ~ends & ((want.abs() >= least) | (want == 0))
+        assert torch.equal(x[exact], want[exact])
+        rest = ~want.isnan() & ~ends & ~exact
+        assert bool((x[rest].abs() <= least).all())
+
+
 # ---------------------------------------------------------------------------
 # How a call's work is cut
 # ---------------------------------------------------------------------------
@@ -152,3 +176,43 @@ def test_row_form_rounds_its_result_only(dev, dim):
     for n, decode in (([1] * 6, True), ([3, 1, 2, 4, 1, 2], False)):
         b = QBatch(dev, n, [40, 100, 3, 700, 64, 2000], 4, 2, dim, seed=dim, decode=decode)
         _against_exact(b, b.run(), 2.0 ** -16 * 1.01, 2.0 ** -8 * 1.01)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("decode", [True, False])
+def test_the_least_scale_byte(dev, dtype, dim, decode):
+    """Byte 0 is 2^-127, as in ``read_kv``: for a sequence's values, for some of them, and for its keys."""
+    _say(f"scale byte 0 {dtype} {dim} decode={decode}")
+    n = [1] * 5 if decode else [5, 1, 33, 20, 70]
+    b = QBatch(dev, n, [40, 100, 3, 64, 200], 4, 2, dim, dtype=dtype, seed=dim, decode=decode, spread=0.0)
+    g = torch.Generator(device=dev).manual_seed(1)
+    rounding = 2.0 ** -7 * 1.01 if dtype == BF16 else 0.0
+    _put_value_scales(b, lambda s, L: torch.zeros(L, b.kv, device=dev))
+    _against_exact(b, b.run(), rounding)
+    _put_value_scales(b, lambda s, L: 70 * torch.randint(0, 2, (L, b.kv), generator=g, device=dev))
+    _against_exact(b, b.run(), rounding)
+    # keys of 2^-127 times at most 448, queries past 2^100: scores of 0.0001 at most without the power of two
+    for s, L in enumerate(b.len):
+        j = torch.arange(L, device=dev)
+        at = (b.table[s].long()[j // b.page], slice(None), j % b.page)
+        _bytes(b.k.scales)[at] = 0
+        b.rows[0][s] = held(_bytes(b.k.values)[at].view(E4M3), _bytes(b.k.scales)[at].view(E8M0))
+    b.q = (b.q.float() * 2.0 ** 118).to(dtype)
+    _against_exact(b, b.run(), rounding)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_scales_that_are_nan(dev, dtype):
+    """Byte 255: the rows that see it are not finite, other sequences are as without it."""
+    _say(f"scale byte 255 {dtype}")
+    b = QBatch(dev, [3, 40, 1], [50, 30, 400], 4, 2, 64, dtype=dtype, seed=3)
+    want = b.run()
+    for c in (b.k, b.v):
+        kept = _bytes(c.scales).clone()
+        at = b.table[0].long()[0]
+        _bytes(c.scales)[at, :, 5] = 255
+        got = b.run()
+        assert int(got[:3].isfinite().all(-1).sum()) == 0
+        assert torch.equal(got[3:], want[3:])
+        _bytes(c.scales).copy_(kept)

@@ -12,7 +12,8 @@ import ctypes
 import os
 import threading
 
-import torch  # noqa: F401  -- must be imported before the HIP library is loaded
+import torch  # must be imported before the HIP library is loaded
+from torch.autograd import forward_ad
 
 from .build import LIB_PATH
 
@@ -211,7 +212,18 @@ def capture_id(stream: int) -> int:
 def no_gradients(who: str) -> RuntimeError:
     """For a call whose inputs autograd tracks: their gradients would be lost silently."""
     return RuntimeError(f"{who} computes no gradients: call it under torch.no_grad() / torch.inference_mode(), or with "
-                        "tensors that do not require grad")
+                        "tensors that do not require grad and have no forward-mode tangent")
+
+
+def has_tangent(*ts) -> bool:
+    """Whether one of the tensors (or None) is a dual one of forward-mode differentiation: ``requires_grad`` says nothing
+    of its tangent, and ``no_grad`` does not end it."""
+    if forward_ad._current_level < 0:
+        return False
+    # a registered op's body runs below autograd, where no tangent can be asked for: look from above it
+    with torch._C._ForceDispatchKeyGuard(torch._C._dispatch_tls_local_include_set(),
+                                         torch._C.DispatchKeySet(torch._C.DispatchKey.Undefined)):
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -21,7 +21,7 @@ the same; ``read_kv`` gives rows back.
 
 Everything is launched on torch's current stream without host synchronisation;
 bfloat16 or float32.  No gradients are computed: inputs that autograd tracks are
-refused where gradients are enabled.
+refused where gradients are enabled, and those with a forward-mode tangent everywhere.
 """
 
 from __future__ import annotations
@@ -249,9 +249,10 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
             return append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm, eps)
     if q_norm is not None or k_norm is not None or isinstance(k_cache, QuantizedCache) or isinstance(v_cache, QuantizedCache):
         return _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm, eps)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
-                                    or (q is not None and q.requires_grad)
-                                    or (cos_sin is not None and cos_sin.requires_grad)):
+    if (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                     or (q is not None and q.requires_grad)
+                                     or (cos_sin is not None and cos_sin.requires_grad))
+            or _lib.has_tangent(q, k, v, k_cache, v_cache, cos_sin)):
         raise _lib.no_gradients("append_kv_")
     dev = k.device
     key = (None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype, dev, v.shape,
@@ -279,11 +280,12 @@ def _append_rows(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, in
                  eps) -> torch.Tensor | None:
     """``append_kv_`` with norms of the heads, or into a quantised cache."""
     k_cache, v_cache, k_scales, v_scales = _parts("append_kv_", k_cache, v_cache)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)
-                                    or k_cache.requires_grad or v_cache.requires_grad
-                                    or (cos_sin is not None and cos_sin.requires_grad)
-                                    or (q_norm is not None and q_norm.requires_grad)
-                                    or (k_norm is not None and k_norm.requires_grad)):
+    if (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)
+                                     or k_cache.requires_grad or v_cache.requires_grad
+                                     or (cos_sin is not None and cos_sin.requires_grad)
+                                     or (q_norm is not None and q_norm.requires_grad)
+                                     or (k_norm is not None and k_norm.requires_grad))
+            or _lib.has_tangent(q, k, v, k_cache, v_cache, cos_sin, q_norm, k_norm)):
         raise _lib.no_gradients("append_kv_")
     interleaved, eps = bool(interleaved), float(eps)       # a tensor's value now, not the tensor
     key = (interleaved, eps, None if q is None else (q.shape, q.stride(), q.dtype, q.device), k.shape, k.stride(), k.dtype,
@@ -417,9 +419,10 @@ def read_kv(k_cache, v_cache, slots: torch.Tensor, dtype: torch.dtype | None = N
         with torch.cuda.device(slots.device):
             return read_kv(k_cache, v_cache, slots, dtype, k_out, v_out)
     k_cache, v_cache, k_scales, v_scales = _parts(who, k_cache, v_cache)
-    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad
-                                    or (k_out is not None and k_out.requires_grad)
-                                    or (v_out is not None and v_out.requires_grad)):
+    if (torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad
+                                     or (k_out is not None and k_out.requires_grad)
+                                     or (v_out is not None and v_out.requires_grad))
+            or _lib.has_tangent(k_cache, v_cache, k_out, v_out)):
         raise _lib.no_gradients(who)
     key = (dtype, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(),
            v_cache.dtype, v_cache.device,
@@ -558,7 +561,8 @@ def paged_attention(q: torch.Tensor, k_cache, v_cache, page_table: torch.Tensor,
             return paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, out, lse, max_q,
                                    workspace)
     k_cache, v_cache, k_scales, v_scales = _parts("paged_attention", k_cache, v_cache)
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+    if ((torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad))
+            or _lib.has_tangent(q, k_cache, v_cache)):
         raise _lib.no_gradients("paged_attention")
     key = (q.shape, q.stride(), q.dtype, dev, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
            v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device, page_table.shape, page_table.stride(),

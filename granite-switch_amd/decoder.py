@@ -49,7 +49,8 @@ class SwitchedDecoderLayer(nn.Module):
     ``qkv`` has three slices (heads * head_dim, kv_heads * head_dim twice),
     ``gate_up`` two with ``fuse_swiglu``; ``window`` > 0 is a sliding window.
     ``q_norm`` and ``k_norm`` [head_dim] norm each head before its rotation.  The
-    cache is a pair of tensors or of ``paged.QuantizedCache``.
+    cache is a pair of tensors or of ``paged.QuantizedCache``, of a head_dim and page
+    size that ``paged.paged_attention`` takes.
     """
 
     def __init__(self, qkv: SwitchedLoRALinear, o_proj: SwitchedLoRALinear, gate_up: SwitchedLoRALinear,
@@ -80,6 +81,7 @@ class SwitchedDecoderLayer(nn.Module):
     def forward(self, x: torch.Tensor | None, residual: torch.Tensor, step: PagedStep,
                 cache: tuple) -> tuple[torch.Tensor, torch.Tensor]:
         """``(x, residual)`` [T, hidden]: the block before and the stream (x None: the first layer), and after."""
+        paged.check_attended(*cache)                       # before a row is stored
         T, D = residual.shape[0], self.head_dim
         y, residual = norms.residual_norm(x, residual, self.input_norm, self.eps, self.residual_multiplier)
         qkv = self.qkv(y)[0]

@@ -70,7 +70,11 @@ class QuantizedCache(NamedTuple):
 
 def allocate_quantized_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int,
                              device="cuda") -> tuple[QuantizedCache, QuantizedCache]:
-    """A key and a value cache of e4m3 rows, laid out as ``allocate_cache`` has them; not initialised."""
+    """A key and a value cache of e4m3 rows, laid out as ``allocate_cache`` has them; not initialised.
+
+    ``append_kv_`` and ``read_kv`` take any page_size and a head_dim up to 512; ``paged_attention`` takes pages of a
+    multiple of 8 rows and a head_dim that is a multiple of 16 up to 256.
+    """
     one = lambda: QuantizedCache(  # noqa: E731
         torch.empty((num_pages, kv_heads, page_size, head_dim), dtype=torch.float8_e4m3fn, device=device),
         torch.empty((num_pages, kv_heads, page_size), dtype=torch.float8_e8m0fnu, device=device))
@@ -594,6 +598,16 @@ def paged_attention(q: torch.Tensor, k_cache, v_cache, page_table: torch.Tensor,
     return out
 
 
+def check_attended(k_cache, v_cache) -> None:
+    """Refuses caches that rows could be stored into but not attended over, by their head dimension or page size."""
+    k, _, scales, _ = _parts("paged_attention", k_cache, v_cache)
+    page, D = k.shape[2:]
+    of = 16 if scales is not None else 8 if k.dtype == torch.bfloat16 else 4
+    if D % of or not 0 < D <= 256 or page % 8:
+        raise ValueError(f"paged_attention: head_dim={D} must be a multiple of {of} up to 256 and page_size={page} one of 8 "
+                         f"(a cache of {'QuantizedCache' if scales is not None else k.dtype})")
+
+
 def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window, out, lse, max_q, workspace, k_scales,
                     v_scales) -> tuple:
     """The checks of a ``paged_attention`` call, and its arguments that are not addresses."""
@@ -638,5 +652,5 @@ def _attention_plan(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, window
             1.0 / math.sqrt(D))
 
 
-__all__ = ["QuantizedCache", "allocate_cache", "allocate_quantized_cache", "append_kv_", "cache_slots", "paged_attention",
-           "read_kv", "rope_table", "workspace_bytes"]
+__all__ = ["QuantizedCache", "allocate_cache", "allocate_quantized_cache", "append_kv_", "cache_slots", "check_attended",
+           "paged_attention", "read_kv", "rope_table", "workspace_bytes"]

@@ -1,4 +1,6 @@
-"""What the paged cache's and the norms' calls refuse, without a GPU: tangents of forward-mode differentiation."""
+"""What the paged cache's, the norms' and the decoder layer's calls refuse, without a GPU: tangents of forward-mode
+differentiation, caches that attention does not take.
+"""
 
 from __future__ import annotations
 
@@ -6,7 +8,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from granite_switch_amd import norms, ops, paged
+from granite_switch_amd import decoder, norms, ops, paged, vllm_layers
 
 
 def _cpu_call():
@@ -49,3 +51,20 @@ def test_tangents_are_refused(call):
                     run(**args)
     with forward_ad.dual_level(), pytest.raises(ValueError, match="on the GPU"):
         run(**t)                                           # inside a level, but without a tangent
+
+
+@pytest.mark.parametrize("dim,page,quant", [(40, 16, True), (72, 16, True), (272, 16, True), (64, 12, True), (4, 16, False),
+                                            (264, 16, False), (64, 12, False)])
+def test_a_layer_refuses_a_cache_that_it_could_not_attend_over(dim, page, quant):
+    """Before it stores a row there, not after."""
+    lin = lambda n_in, slices, **kw: vllm_layers.SwitchedLoRALinear(
+        torch.nn.Linear(n_in, sum(slices), bias=False), 1, 8, num_slices=len(slices), output_slices=slices, **kw)
+    one = torch.ones(64)
+    layer = decoder.SwitchedDecoderLayer(lin(64, (2 * dim, dim, dim)), lin(2 * dim, (64,)), lin(64, (128, 128), fuse_swiglu=True),
+                                         lin(128, (64,)), one, one, 2, 1, dim)
+    make = paged.allocate_quantized_cache if quant else paged.allocate_cache
+    cache = make(3, 1, page, dim, device="cpu")
+    with pytest.raises(ValueError, match=f"head_dim={dim} must be a multiple of {16 if quant else 8}"):
+        layer(None, torch.zeros(2, 64), None, cache)
+    with pytest.raises(ValueError, match="on the GPU"):
+        layer(None, torch.zeros(2, 64), None, make(3, 1, 16, 64, device="cpu"))

@@ -202,6 +202,11 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def elsewhere(dev: torch.device) -> bool:
+    """Whether ``dev`` is a GPU that is not the current one: a launch goes to the current one's queues."""
+    return dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device()
+
+
 def capture_id(stream: int) -> int:
     """The id of the graph capture that ``stream`` is part of; 0: none."""
     found = c_i64()

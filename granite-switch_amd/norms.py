@@ -64,6 +64,9 @@ def residual_norm(x: torch.Tensor | None, residual: torch.Tensor, weight: torch.
                                      or (post_weight is not None and post_weight.requires_grad))
             or _lib.has_tangent(x, residual, weight, gate, post_weight)):
         raise _lib.no_gradients("residual_norm")
+    if _lib.elsewhere(residual.device):
+        with torch.cuda.device(residual.device):
+            return residual_norm(x, residual, weight, eps, scale, gate, post_weight, gate_act, out, residual_out)
     if x is not None and x.dim() == 2 and residual.dim() == 2:
         key = (x.shape, x.stride(), x.dtype, x.device, residual.shape, residual.stride(), residual.dtype, residual.device,
                weight.shape, weight.stride(), weight.dtype, weight.device,

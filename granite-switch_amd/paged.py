@@ -181,11 +181,6 @@ _attention_plans: dict = {}
 _PLAN_CAP = 4096
 
 
-def _elsewhere(dev: torch.device) -> bool:
-    """Whether ``dev`` is a GPU that is not the current one: a launch goes to the current one's queues."""
-    return dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device()
-
-
 def _keep(plans: dict, key, plan):
     if len(plans) >= _PLAN_CAP:            # batch sizes vary per step: keep it bounded
         plans.clear()
@@ -207,6 +202,9 @@ def cache_slots(page_table: torch.Tensor, kv_lens: torch.Tensor, page_size: int,
     otherwise ``num_tokens`` is the packed batch's row count.
     """
     who = "cache_slots"
+    if _lib.elsewhere(kv_lens.device):
+        with torch.cuda.device(kv_lens.device):
+            return cache_slots(page_table, kv_lens, page_size, num_pages, cu_seqlens, num_tokens)
     B = kv_lens.shape[0]
     _on_gpu(who, kv_lens.device, page_table, cu_seqlens)
     _ints(who, "kv_lens", kv_lens, torch.int32, (B,))
@@ -248,7 +246,7 @@ def append_kv_(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache
     q_norm, k_norm [D], of q's type or float32: each head of q (k) is normed before its
               rotation, x / sqrt(mean(x^2) + eps) * weight, in the same pass
     """
-    if _elsewhere(k.device):
+    if _lib.elsewhere(k.device):
         with torch.cuda.device(k.device):
             return append_kv_(q, k, v, k_cache, v_cache, slots, positions, cos_sin, q_out, interleaved, q_norm, k_norm, eps)
     if q_norm is not None or k_norm is not None or isinstance(k_cache, QuantizedCache) or isinstance(v_cache, QuantizedCache):
@@ -419,7 +417,7 @@ def read_kv(k_cache, v_cache, slots: torch.Tensor, dtype: torch.dtype | None = N
     k_out, v_out receive the result (allocated when None): views with contiguous head rows
     """
     who = "read_kv"
-    if _elsewhere(slots.device):
+    if _lib.elsewhere(slots.device):
         with torch.cuda.device(slots.device):
             return read_kv(k_cache, v_cache, slots, dtype, k_out, v_out)
     k_cache, v_cache, k_scales, v_scales = _parts(who, k_cache, v_cache)
@@ -560,7 +558,7 @@ def paged_attention(q: torch.Tensor, k_cache, v_cache, page_table: torch.Tensor,
     not finite may also reach rows of its sequence that come before it.
     """
     dev = q.device
-    if _elsewhere(dev):
+    if _lib.elsewhere(dev):
         with torch.cuda.device(dev):
             return paged_attention(q, k_cache, v_cache, page_table, kv_lens, cu_seqlens, scale, window, out, lse, max_q,
                                    workspace)

@@ -6,9 +6,10 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
 from torch.autograd import forward_ad
 
-from granite_switch_amd import decoder, norms, ops, paged, vllm_layers
+from granite_switch_amd import _lib, decoder, norms, ops, paged, vllm_layers
 
 
 def _cpu_call():
@@ -68,3 +69,37 @@ def test_a_layer_refuses_a_cache_that_it_could_not_attend_over(dim, page, quant)
         layer(None, torch.zeros(2, 64), None, cache)
     with pytest.raises(ValueError, match="on the GPU"):
         layer(None, torch.zeros(2, 64), None, make(3, 1, 16, 64, device="cpu"))
+
+
+@pytest.mark.parametrize("call", ["cache_slots", "residual_norm"])
+def test_calls_on_another_device_make_it_the_current_one(monkeypatch, call):
+    """A launch, the default stream's among them, goes to the current device, wherever the tensors live."""
+    current, launched = [0], []
+
+    class On:
+        def __init__(self, device):
+            self.index = torch.device(device).index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.was
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda device=None: 0)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: launched.append((name, current[0])))
+    monkeypatch.setattr(torch.Tensor, "data_ptr", lambda self: 0)
+    monkeypatch.setattr(FakeTensor, "data_ptr", lambda self: 0, raising=False)
+    for device in (1, 0, 1):
+        with FakeTensorMode(), torch.no_grad():
+            t = lambda *s, dtype=torch.float32: torch.empty(s, dtype=dtype, device=f"cuda:{device}")  # noqa: E731
+            if call == "cache_slots":
+                paged.cache_slots(t(2, 3, dtype=torch.int32), t(2, dtype=torch.int32), 16, 8)
+            else:
+                norms.residual_norm(t(3, 64), t(3, 64), t(64))
+                norms.residual_norm(t(2, 3, 64), t(2, 3, 64), t(64))
+        assert launched and all(on == device for _, on in launched), launched
+        launched.clear()
+        assert current == [0]

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from granite_switch_amd import _lib, paged
-from test_gpu_quantized import BF16, E4M3, E8M0, FP32, QBatch, _bytes, _say, held, make_cache
+from test_gpu_quantized import BF16, E4M3, E8M0, FP32, QBatch, _bytes, _say, _turned, exponents, held, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -76,6 +76,103 @@ def test_read_of_every_scale(dev, dtype, dim):
         assert torch.equal(x[exact], want[exact])
         rest = ~want.isnan() & ~ends & ~exact
         assert bool((x[rest].abs() <= least).all())
+
+
+def _rounded(y):
+    """The e4m3 value nearest to float64 y (at most 448 + 16), ties to even, without a float32 between."""
+    step = torch.exp2((torch.frexp(y)[1] - 1).clamp(min=-6).double() - 3)
+    return torch.round(y / step) * step
+
+
+def _exact_bytes(rows):
+    """(values as float64, scale bytes) of float64 rows."""
+    e = exponents(rows)
+    return _rounded(rows * torch.exp2(-e.double())[..., None]), (e + 127).to(torch.uint8)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("turn", ["halves", "pairs", "norm only"])
+def test_keys_are_rounded_from_64_bits(dev, dtype, turn):
+    """Normed and rotated keys: the e4m3 values nearest to the exact ones, of 10^7 of which fp32 would move some ten.
+
+    Exact where 64-bit arithmetic leaves no doubt: sums, a root and products of it are within 10^-13 of the row's largest
+    value.
+    """
+    _say(f"keys from 64 bits {dtype} {turn}")
+    g = torch.Generator(device=dev).manual_seed(11)
+    T, HK, D, page = 10240, 8, 128, 64
+    k = torch.randn(T, HK, D, generator=g, device=dev).to(dtype)
+    w = (1 + 0.3 * torch.randn(D, generator=g, device=dev)).to(dtype)
+    pos, table = torch.randint(0, 4000, (T,), generator=g, device=dev), paged.rope_table(4000, D, device=dev)
+    caches, slots = [make_cache(dev, T // page, HK, page, D) for _ in range(2)], torch.arange(T, device=dev)
+    rope = () if turn == "norm only" else (pos, table)
+    paged.append_kv_(None, k, k, *caches, slots, *rope, interleaved=turn == "pairs", k_norm=w, eps=1e-5)
+    x = k.double()
+    x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + torch.tensor(1e-5).double()) * w.double()
+    if rope:
+        x = _turned(x, 0.0, table, pos, turn == "pairs")[0]
+    values, scales = (_bytes(c).transpose(1, 2).flatten(0, 1) for c in caches[0])
+    top = x.abs().amax(-1)
+    sure = exponents((top * (1 + 1e-13))[..., None]) == exponents((top * (1 - 1e-13))[..., None])
+    want, code = _exact_bytes(x)
+    assert int((scales != code)[sure].sum()) == 0
+    y = x * torch.exp2(127.0 - code.double())[..., None]
+    firm = sure[..., None] & (_rounded(y + 448e-13) == _rounded(y - 448e-13))
+    assert int((~firm).sum()) < 100
+    moved = int((values.view(E4M3).double() != want)[firm].sum())
+    assert moved == 0, moved
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_keys_next_to_a_border(dev, dtype):
+    """Rotated keys 2^-30 from a midpoint between e4m3 values, and from 448: fp32 holds none of these apart from it."""
+    _say(f"keys next to a border {dtype}")
+    rows = torch.zeros(4, 1, 128, dtype=torch.float64)      # pairs (j, j + 64), turned to (p + q, q - p)
+    p, q = rows[..., :64], rows[..., 64:]
+    p[:, 0, :] = 1.0
+    for r, tiny in enumerate((2.0 ** -30, -2.0 ** -30)):
+        p[r, 0, :6], q[r, 0, :6] = torch.tensor([17.0, 19, 34, 2.125, 300, 136]), tiny
+        p[2 + r, 0, :2], q[2 + r, 0, :2] = torch.tensor([448.0, 17]), tiny * 2 ** 5
+    k = rows.to(dtype).to(dev)
+    assert torch.equal(k.double().cpu(), rows)
+    table = torch.cat([torch.ones(1, 64), -torch.ones(1, 64)], 1).to(dev)
+    caches, slots = [make_cache(dev, 1, 1, 16, 128) for _ in range(2)], torch.arange(4, device=dev)
+    paged.append_kv_(None, k, k, *caches, slots, torch.zeros(4, dtype=torch.int64, device=dev), table)
+    want, code = _exact_bytes(torch.cat([p + q, q - p], -1).to(dev))
+    assert code.flatten().tolist() == [127, 127, 128, 128]
+    assert torch.equal(_bytes(caches[0].scales)[0, 0, :4], code.flatten())
+    assert torch.equal(caches[0].values[0, 0, :4].double(), want[:, 0])
+
+
+def test_scales_with_strides_of_their_own(dev):
+    """Keys' and values' scales apart from each other's, in append, read and attention of both forms."""
+    _say("strided scales")
+    b = QBatch(dev, [1, 60, 3], [30, 300, 0], 8, 2, 64, seed=4)
+    pages, kv, page = b.k.scales.shape
+    out, one = b.run(), (b.k, b.v)
+    big = [torch.full((pages + 1, kv + 1 + i, (2 + i) * page), 255, dtype=torch.uint8, device=dev) for i in range(2)]
+    two = []
+    for i, (c, x) in enumerate(zip(one, big)):
+        scales = x[i:, 1:][:pages, :kv, i * page:(i + 1) * page]
+        scales.copy_(_bytes(c.scales))
+        two.append(paged.QuantizedCache(c.values, scales.view(E8M0)))
+    assert two[0].scales.stride() != two[1].scales.stride()
+    n = b.len[1]
+    slots, _ = paged.cache_slots(b.table[1:2], b.lens[1:2], page, pages, torch.tensor([0, n], dtype=torch.int32, device=dev), n)
+    for x, y in zip(paged.read_kv(*one, slots), paged.read_kv(*two, slots)):
+        assert torch.equal(x, y)
+    assert not torch.equal(*paged.read_kv(*one, slots))
+    for kw in ({}, {"max_q": 60}):
+        assert torch.equal(paged.paged_attention(b.q, *two, b.table, b.lens, b.cu, **kw), out)
+    few = paged.paged_attention(b.q[:1], *one, b.table[:1], b.lens[:1])
+    assert torch.equal(paged.paged_attention(b.q[:1], *two, b.table[:1], b.lens[:1]), few)
+    k, v = (torch.randn(n, kv, 64, generator=torch.Generator(device=dev).manual_seed(i), device=dev).to(BF16) for i in (5, 6))
+    for cache in (one, two):
+        paged.append_kv_(None, k, 100 * v, *cache, slots)
+    for c, x, keep in zip(one, two, big):
+        assert torch.equal(_bytes(c.scales), _bytes(x.scales))
+    for x in (*paged.read_kv(*two, slots),):
+        assert int(x.isnan().sum()) == 0
 
 
 # ---------------------------------------------------------------------------

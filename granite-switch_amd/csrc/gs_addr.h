@@ -360,7 +360,10 @@ GS_HD int row_part_units(int64_t U, int HK, int wgs) {
 // shorter ones held places that those wait for, with more start than work (8 chunks of 3 .. 64
 // rows over up to 16384 keys: 65.2 us without, 59.7 with 8 or 16).  Without any, 3 rows over 8192
 // keys take 20.7 us with 4, 21.5 with 1 and 23.3 with 8 (8 heads), 20.3, 26.7 and 23.1 (one
-// head, whose 64 parts cost their join more than they save).
+// head, whose 64 parts cost their join more than they save).  A bf16 cache has no minimum: with
+// 8 beside chunk parts, 3, 3 and 64 rows over 8192 keys each would take 42.9 us for 46.3, the 8
+// chunks 3% less and a step of 48 decode rows and 16 chunks what it takes, but its sums would be
+// taken in another order.
 GS_HD int row_part_least(bool ragged, bool quantised, bool chunks) { return !ragged || !quantised ? 1 : chunks ? 8 : 4; }
 constexpr int kMostParts = 512;      // of an item
 GS_HD int row_parts(int units, int most, uint32_t magic) {

@@ -275,8 +275,10 @@ __device__ __forceinline__ void chunk_values(const PagedArgs& a, const ChunkRow&
       p[i] = __builtin_amdgcn_exp2f(fmaf(sc[g >> 1][8 * (g & 1) + i], a.scale_log2, -ms));
       sum.lsum += p[i];
     }
-    // bf16 probabilities with the error they have in the row form; two bf16 numbers for each
-    // are half as many products again, where instructions bound.  The total stays in fp32.
+    // Probabilities are rounded to bf16, each off by up to 2^-8 of itself; their total stays in
+    // fp32.  Two bf16 numbers for each, off by 2^-16, are half as many products again, where
+    // instructions bound: over a quantised cache 121 -> 143 us for 8192 rows of prompts, 90 -> 106
+    // for a step of 48 decode rows and 16 chunks, 58 -> 67 for 8 chunks of 3 .. 64 rows.
 #pragma unroll
     for (int i = 0; i < 4; ++i) pf[g][i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
   }

@@ -661,7 +661,7 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
     for (int i = 0; i < F::kKeys; ++i) {
       p[i] = __builtin_amdgcn_exp2f(sc[i] - ms);
       lsum += p[i];
-      if constexpr (E4M3 && !BF16) p[i] *= e8m0_scale(((v_in == 0 ? x.s.v[0] : x.s.v[1]) >> (8 * i)) & 255u);
+      if constexpr (E4M3 && !BF16) p[i] *= fmaxf(scale_of(v_in == 0 ? x.s.v[0] : x.s.v[1], i), 0x1p-127f);
     }
     if constexpr (BF16 && E4M3) {
       // The values' scales are the probabilities', which enter the product as two bf16 numbers,

@@ -8,8 +8,8 @@
 // for the keys: the matrix units hold those sums to 2^-11 of the largest product (measured,
 // 64 terms), bf16 ones to 2^-21.
 //
-// 8192 rows of 16 prompts (32 query, 8 key/value heads of 128): 118 us, 554 TFLOP/s of the
-// products that the mask leaves, 102 over a bf16 cache; vector instructions take 54% of the
+// 8192 rows of 16 prompts (32 query, 8 key/value heads of 128): 119 .. 122 us, 540 TFLOP/s of
+// the products that the mask leaves, 103 over a bf16 cache; vector instructions take 54% of the
 // SIMDs' cycles and the products 25%.  A step of 48 decode rows and 16 chunks of 256 over up to
 // 3839 keys: 92 us.  8 chunks of 3 .. 64 rows over up to 16384 keys: 58 us, where a part's
 // start (its schedule, its first tile) is a sixth of its time and the join 7.
@@ -158,7 +158,8 @@ __global__ __launch_bounds__(64 * kCWaves, 2) void ragged_attention_e4m3_kernel(
 void launch_ragged_e4m3(const PagedArgs& a, int DT, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(ragged_grid(a)));
   // a workgroup for an eighth of a tile up to 2 chunk_slots of them: with one chunk_slots the
-  // invocation chunks' join took some workgroups two turns (59.7 us for the call, 57.7 so)
+  // invocation chunks' join took some workgroups two turns (59.7 us for the call, 57.7 so; the
+  // bf16 cache's calls show no difference)
   const dim3 join(static_cast<unsigned>(2 * a.chunk_slots));
   if (DT == 64) {
     hipLaunchKernelGGL((ragged_attention_e4m3_kernel<64>), grid, dim3(64 * kCWaves), 0, st, a);

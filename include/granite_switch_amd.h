@@ -617,7 +617,7 @@ int gs_cache_slots(const int32_t* page_table, int64_t ld_table, int32_t max_page
  * A window no sequence is longer than is none; num_tokens and a narrower one
  * sum to less than 2^31.  Scores and sums are fp32: weights of up to 2^8 a key are
  * summed with their values before the division, so values past 2^120 over the
- * number of keys may give infinities.
+ * number of keys may give infinities or NaN.
  * kv_lens past the page table's reach are cut to it; page ids outside the
  * pool are read as page 0.  max_q: the most rows of a sequence where the caller
  * knows it (0: unknown), a choice of kernels only: a smaller value than the batch

@@ -694,7 +694,8 @@ __device__ __forceinline__ void row_part(const PagedArgs& a, const RowItem& it, 
             }
       };
       // A probability times 2^-126, the least scale, has no bf16 digits left: scales below 2^-63
-      // count 2^96 times over, in sums of their own.
+      // count 2^96 times over, in sums of their own.  Where every block has them (rows of zeros have
+      // that scale, too) 256 sequences' decode takes 5% more, elsewhere 0.4%.
       const u32x2 less = {tiny_bytes(x.s.v[0]), tiny_bytes(x.s.v[1])};
       const bool tiny = __any((less[0] | less[1]) != 0);
       u32x2 scales = x.s.v;
